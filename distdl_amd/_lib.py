@@ -140,6 +140,15 @@ SIGNATURES = {
     "ddl_transpose_2d": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "ddl_transpose_padded": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "ddl_pad_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "ddl_head_rotary": (c_int, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                c_void_p, c_void_p, c_int, c_float, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_int,
+                                c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p]),
+    "ddl_head_norm_rotary_backward_workspace": (c_int64, [c_int64]),
+    "ddl_head_norm_rotary_backward": (c_int, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p,
+                                              POINTER(c_int64), c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                              c_float, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_void_p,
+                                              POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_int64,
+                                              c_void_p]),
     "ddl_colsum_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

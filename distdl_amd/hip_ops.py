@@ -5,6 +5,7 @@ layers call step by step first offer their operands to their native counterpart
 (``_lib.front()``), which takes the usual forms and answers None to any other.
 """
 
+import contextlib
 import ctypes
 import functools
 import struct
@@ -1122,3 +1123,120 @@ def _linear_padded(a, b, m, n, k_padded, dt):
         return out.zero_()
     _gemm(a, a.stride(0) if m > 1 else k_padded, 1, b, b.stride(0) if n > 1 else k_padded, 1, None, out, dt, m, n, k_padded)
     return out
+
+
+# ---------------------------------------------------------------- heads of an attention block
+
+
+@contextlib.contextmanager
+def _on_device_of(t):
+    """The current device is that of ``t``, whose current stream ``_stream`` then gives."""
+    if t.device.index == torch.cuda.current_device():
+        yield
+    else:
+        with torch.cuda.device(t.device):
+            yield
+
+
+def _heads(t, name, like=None):
+    """``t`` as the head kernels take it: [batch, tokens, heads, head_dim] with unit stride of the last; a copy where it has another."""
+    if t.dim() != 4 or t.dtype not in _LN_DTYPES:
+        raise ValueError(f"{name}: need [batch, tokens, heads, head_dim] tensors of float32, bfloat16 or float16, got {tuple(t.shape)} {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name}: operands differ in type or device ({t.dtype} on {t.device}, {like.dtype} on {like.device})")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        t = contiguous(t)
+    return t
+
+
+def _strides3(t):
+    return None if t is None else _lib.i64_array(t.stride()[:3])
+
+
+def _rotary_arguments(q, k, frequencies, positions, name):
+    """Checked operands of a rotation: ``(first, rest)``, the tensor that sets the extents, and the arguments of the entry points
+    from the frequencies to the positions' pitch."""
+    first = q if q is not None else k
+    if first is None:
+        raise ValueError(f"{name}: neither queries nor keys")
+    _require_gpu(q, k, frequencies, positions)
+    for t in (q, k):
+        if t is not None and (t.shape[:2] != first.shape[:2] or t.shape[3] != first.shape[3]):
+            raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)} differ in batch, tokens or head_dim")
+    batch, tokens, _, dim = first.shape
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous() or 2 * frequencies.numel() > dim or \
+       frequencies.device != first.device:
+        raise ValueError(f"{name}: frequencies must be a contiguous float64 vector of at most head_dim / 2 = {dim // 2} elements on {first.device}, "
+                         f"got {tuple(frequencies.shape)} {frequencies.dtype} on {frequencies.device}")
+    pitch = width = 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != first.device or \
+           tuple(positions.shape) not in ((tokens,), (1, tokens), (batch, tokens)):
+            raise ValueError(f"{name}: positions must be int32 or int64, [{tokens}] or [{batch}, {tokens}], on {first.device}, "
+                             f"got {tuple(positions.shape)} {positions.dtype} on {positions.device}")
+        if tokens > 1 and positions.stride(-1) != 1:
+            positions = contiguous(positions)
+        width = positions.element_size()
+        pitch = positions.stride(0) if positions.dim() == 2 and positions.shape[0] == batch and batch > 1 else 0
+    return first, positions, (frequencies.data_ptr(), 2 * frequencies.numel(), _ptr(positions), width, pitch)
+
+
+def _head_weights(first, q, k, q_weight, k_weight, name):
+    _require_gpu(q_weight, k_weight)
+    for t, w in ((q, q_weight), (k, k_weight)):
+        if w is not None and (t is None or w.dtype != first.dtype or w.device != first.device or w.numel() != first.shape[3] or not w.is_contiguous()):
+            raise ValueError(f"{name}: weights must be contiguous, of the heads' type and device, with head_dim = {first.shape[3]} elements")
+
+
+def _empty_heads(t):
+    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def head_rotary(q, k, frequencies, positions=None, interleaved=False, amplitude=1.0, inverse=False, norm=False, q_weight=None, k_weight=None,
+                eps=1e-6):
+    """Queries and keys [batch, tokens, heads, head_dim] (either may be None) turned by their positions, behind a norm of each head
+    if ``norm``; ``inverse`` turns back (the adjoint).  New contiguous tensors."""
+    name = "head_rotary"
+    q, k = (None if t is None else _heads(t, name, q if q is not None else k) for t in (q, k))
+    first, positions, middle = _rotary_arguments(q, k, frequencies, positions, name)
+    _head_weights(first, q, k, q_weight, k_weight, name)
+    yq, yk = _empty_heads(q), _empty_heads(k)
+    batch, tokens, _, dim = first.shape
+    with _on_device_of(first):
+        rc = _lib.load().ddl_head_rotary(
+            _ptr(q), _strides3(q), _ptr(k), _strides3(k), _LN_DTYPES[first.dtype], batch, tokens, 0 if q is None else q.shape[2],
+            0 if k is None else k.shape[2], dim, _ptr(q_weight), _ptr(k_weight), int(norm), float(eps), *middle, int(interleaved), float(amplitude),
+            int(inverse), _ptr(yq), _strides3(yq), _ptr(yk), _strides3(yk), _stream())
+    _lib.check(rc, "ddl_head_rotary")
+    return yq, yk
+
+
+def head_norm_rotary_backward(dyq, dyk, q, k, q_weight, k_weight, frequencies, positions=None, interleaved=False, amplitude=1.0, eps=1e-6,
+                              want_q_weight=False, want_k_weight=False):
+    """Adjoint of ``head_rotary(..., norm=True)``: ``(dq, dk, dq_weight, dk_weight)``, None where there is no gradient coming or none wanted."""
+    name = "head_norm_rotary_backward"
+    q, k = (None if dy is None else _heads(t, name, q if q is not None else k) for t, dy in ((q, dyq), (k, dyk)))
+    dyq, dyk = (None if t is None else _heads(t, name, x) for t, x in ((dyq, q), (dyk, k)))
+    first, positions, middle = _rotary_arguments(q, k, frequencies, positions, name)
+    q_weight, k_weight = None if q is None else q_weight, None if k is None else k_weight
+    _head_weights(first, q, k, q_weight, k_weight, name)
+    _require_gpu(dyq, dyk)
+    for t, dy in ((q, dyq), (k, dyk)):
+        if t is not None and dy.shape != t.shape:
+            raise ValueError(f"{name}: gradients {tuple(dy.shape)} of heads {tuple(t.shape)}")
+    dq, dk = _empty_heads(q), _empty_heads(k)
+    batch, tokens, _, dim = first.shape
+    lib = _lib.load()
+    dqw, dkw = (torch.empty(dim, dtype=first.dtype, device=first.device) if want and t is not None else None
+                for want, t in ((want_q_weight, q), (want_k_weight, k)))
+    work, elems = None, 0
+    if dqw is not None or dkw is not None:
+        elems = lib.ddl_head_norm_rotary_backward_workspace(dim)
+        work = torch.empty(elems, dtype=torch.float32, device=first.device)
+    with _on_device_of(first):
+        rc = lib.ddl_head_norm_rotary_backward(
+            _ptr(dyq), _strides3(dyq), _ptr(dyk), _strides3(dyk), _ptr(q), _strides3(q), _ptr(k), _strides3(k), _LN_DTYPES[first.dtype], batch, tokens,
+            0 if q is None else q.shape[2], 0 if k is None else k.shape[2], dim, _ptr(q_weight), _ptr(k_weight), float(eps), *middle, int(interleaved),
+            float(amplitude), _ptr(dq), _strides3(dq), _ptr(dk), _strides3(dk), _ptr(dqw), _ptr(dkw), _ptr(work), elems, _stream())
+    _lib.check(rc, "ddl_head_norm_rotary_backward")
+    return dq, dk, dqw, dkw

@@ -19,6 +19,11 @@ from .linear_rs import DistributedLinearReduceScatter  # noqa: F401
 from .reduce_scatter import ReduceScatter  # noqa: F401
 from .module import Module  # noqa: F401
 from .repartition import Repartition  # noqa: F401
+from .rotary import DistributedHeadNormRotary  # noqa: F401
+from .rotary import DistributedRotary  # noqa: F401
+from .rotary import head_norm_rotary_shard  # noqa: F401
+from .rotary import rotary_frequencies  # noqa: F401
+from .rotary import rotary_shard  # noqa: F401
 from .sum_reduce import SumReduce  # noqa: F401
 from .transpose import DistributedTranspose  # noqa: F401
 
@@ -26,5 +31,6 @@ __all__ = [
     "AllGather", "AllSumReduce", "Broadcast", "DistributedConv1d", "DistributedConv2d", "DistributedConv3d",
     "DistributedFeatureConv1d", "DistributedFeatureConv2d", "DistributedFeatureConv3d", "DistributedEmbedding",
     "HaloExchange", "DistributedLayerNorm", "DistributedLinear", "DistributedLinearAllGather", "DistributedLinearReduceScatter", "Module", "ReduceScatter",
-    "Repartition", "SumReduce", "DistributedTranspose",
+    "Repartition", "SumReduce", "DistributedTranspose", "DistributedRotary", "DistributedHeadNormRotary", "rotary_frequencies",
+    "rotary_shard", "head_norm_rotary_shard",
 ]

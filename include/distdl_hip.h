@@ -596,6 +596,66 @@ int ddl_colsum_bf16(const void* a, int64_t rows, int64_t cols, int64_t ld,
                     void* out, float* workspace, int64_t workspace_elems,
                     void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Heads between the sharded projections of an attention block.  The reference
+ * shards those projections by heads (nn/linear_ag.py:46-60: num_heads,
+ * num_heads_kv, num_vars) and leaves what lies between them to its user: these
+ * have no counterpart there.  fp32, bf16 or fp16 elements, fp32 sums.
+ *
+ * Tensors are [batch, tokens, heads, head_dim] with `*_strides` = the strides
+ * of the first three dimensions (host arrays, elements); head_dim's is 1.
+ * ------------------------------------------------------------------------ */
+
+/* Queries and keys turned by their positions, one launch for both: with
+ * t = position * frequencies[p], p < rotated / 2,
+ *   y[p] = a (x[p] cos t - x[p'] sin t),  y[p'] = a (x[p'] cos t + x[p] sin t),
+ * a = amplitude and p' = p + rotated / 2, or, `neighbours` != 0, the pair of
+ * elements 2 p, 2 p + 1.  Elements from `rotated` (even) on pass through.
+ *   frequencies   device, rotated / 2 doubles, radians for each position; the
+ *                 angle is formed in 64 bits, so far positions lose nothing
+ *   positions     device, int32 or int64 (position_bytes 4, 8), one for each
+ *                 token, `position_batch` elements from one sequence's to the
+ *                 next's (0: all the same); position_bytes 0: 0, 1, 2, ...
+ *   norm != 0     every head is divided by sqrt(mean of its squares + eps) and
+ *                 multiplied by its weights [head_dim] (NULL: 1) first
+ *   inverse != 0  the angles with the other sign: the adjoint (norm = 0 only)
+ * k_heads (q_heads) may be 0, with k (q) NULL.  y may be x with its strides; else
+ * they must not overlap.  head_dim <= 512 (DDL_E_UNSUPP). */
+int ddl_head_rotary(const void* q, const int64_t* q_strides, const void* k,
+                    const int64_t* k_strides, int dtype, int64_t batch,
+                    int64_t tokens, int64_t q_heads, int64_t k_heads,
+                    int64_t head_dim, const void* q_weight, const void* k_weight,
+                    int norm, float eps, const double* frequencies,
+                    int64_t rotated, const void* positions, int position_bytes,
+                    int64_t position_batch, int neighbours, float amplitude,
+                    int inverse, void* yq, const int64_t* yq_strides, void* yk,
+                    const int64_t* yk_strides, void* stream);
+
+/* The adjoint of ddl_head_rotary with norm != 0.  With g = the inverse rotation
+ * of dy and xhat = x / sqrt(mean of squares + eps):
+ *   dx = rstd (w g - xhat mean(w g xhat)),  dw = sum over tokens and heads of g xhat.
+ * dq_weight / dk_weight may be NULL; where one is wanted, `workspace` is device
+ * memory of ddl_head_norm_rotary_backward_workspace(head_dim) floats, whose
+ * contents on entry do not matter.  Sums have one order, so equal calls give
+ * equal bits.  dq (dk) may be dyq (dyk) or q (k) with its strides. */
+int64_t ddl_head_norm_rotary_backward_workspace(int64_t head_dim);
+int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
+                                  const void* dyk, const int64_t* dyk_strides,
+                                  const void* q, const int64_t* q_strides,
+                                  const void* k, const int64_t* k_strides,
+                                  int dtype, int64_t batch, int64_t tokens,
+                                  int64_t q_heads, int64_t k_heads,
+                                  int64_t head_dim, const void* q_weight,
+                                  const void* k_weight, float eps,
+                                  const double* frequencies, int64_t rotated,
+                                  const void* positions, int position_bytes,
+                                  int64_t position_batch, int neighbours,
+                                  float amplitude, void* dq,
+                                  const int64_t* dq_strides, void* dk,
+                                  const int64_t* dk_strides, void* dq_weight,
+                                  void* dk_weight, float* workspace,
+                                  int64_t workspace_elems, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
