@@ -1,0 +1,371 @@
+// Attention of queries to keys and values of another (or the same) length, on heads that a worker holds whole, forward.
+//
+//   out[i] = sum over the keys j that query i sees of p_ij v_j,   p_ij = exp(scale q_i . k_j) / sum over j of the same
+//
+// in one pass over the keys with the running maximum and sum of the softmax (fp32); 2^x takes the place of e^x, log2(e) goes
+// into the scale.  A query that sees no key gives zeros.  Kept for the adjoint: log2 of each row's sum (+inf for a row
+// without keys, so that its probabilities come out as zero there).
+//
+// Two forms, attention_rows and attention_split below; what they are made of is in attention_parts.h.
+#include "ddl_common.h"
+
+#include "attention_parts.h"
+
+namespace ddl {
+namespace {
+
+constexpr float kSlack = 8.f;           // the running maximum is moved when it lags by more than this (in powers of two)
+
+// The softmax of a wavefront's columns as far as it has come.
+template <int BLOCKS>
+struct Running {
+    floatx16 acc[BLOCKS];
+    float top = -INFINITY, total = 0.f;      // of this lane's column; the total of this lane's half of the rows
+
+    __device__ Running() {
+#pragma unroll
+        for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    }
+    // Scores to probabilities relative to `top`, which follows the scores.  `rest`: rows of the first block that this lane's
+    // column sees, from this lane's half's first one on; MASKED: they may end here.
+    template <int NS, bool MASKED>
+    __device__ void take(floatx16 (&s)[NS], float scale, int rest) {
+        if (MASKED) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * n + (r & 3) + 8 * (r >> 2) >= rest) s[n][r] = -INFINITY;
+        }
+        float m = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][r]);
+        m = max_halves(m) * scale;
+        // Moved only where it lags by a factor of 2^8: the sums have room for that, and most tiles leave them alone.
+        if (__any(m > top + kSlack)) {
+            const float moved = fmaxf(top, m), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
+            top = moved;
+            total *= factor;
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= factor;
+        }
+        const float from = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], scale, -from));
+                sum += s[n][r];
+            }
+        total += sum;
+    }
+};
+
+template <typename T>
+constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
+
+// One wavefront, 32 queries of one head; a workgroup, 128 of them, walks over the keys tile by tile through LDS, two tiles deep,
+// the tile after the next in registers on its way.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 2) void attention_rows(const AttnArgs a) {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    constexpr int KEYS = keys_of_tile<T>(), NS = KEYS / 32, kTileBytes = KEYS * Tile::kRowBytes;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    int bh, block;
+    block_of(blockIdx.x, a.batch * a.heads, a.blocks, bh, block);     // the last rows, which see most keys in the causal form, first
+    const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
+    const int length = sequence_keys(a, batch);
+    const int first_row = block * kRows * kWaves, my_row = first_row + wave * kRows + (lane & 31);
+    const int seen = keys_seen(a, my_row, length);
+    const int end = keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length);            // most that a row of the workgroup sees
+    const int wave_most = keys_seen(a, min(first_row + (wave + 1) * kRows, a.tokens) - 1, length);  // rows of a wavefront: most,
+    const int wave_least = first_row + wave * kRows < a.tokens ? keys_seen(a, first_row + wave * kRows, length) : 0;   // and least
+    const bool wave_has_rows = first_row + wave * kRows < a.tokens;
+    const T* q = static_cast<const T*>(a.q) + batch * a.q_at.batch + head * a.q_at.head;
+    const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
+    const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
+
+    const Tile tile(lane);
+    Frag column[Tile::kSteps];
+#pragma unroll
+    for (int s = 0; s < Tile::kSteps; ++s) {
+        Frag f = {};
+        if (my_row < a.tokens && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + my_row * a.q_at.token + (2 * s + half) * Tile::kPerChunk);
+        column[s] = f;
+    }
+    Running<Tile::kBlocks> run;
+    const int tiles = (end + KEYS - 1) / KEYS;
+    AttnStage<T, DP, KEYS, kThreads> k_next, v_next;
+    if (tiles > 0) {
+        k_next.load(k, a.k_at.token, 0, end, a.chunks, tid), v_next.load(v, a.v_at.token, 0, end, a.chunks, tid);
+        k_next.store(lds, tid), v_next.store(lds + 2 * kTileBytes, tid);
+        if (tiles > 1) k_next.load(k, a.k_at.token, KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, KEYS, end, a.chunks, tid);
+    }
+    lds_barrier();
+    for (int t = 0; t < tiles; ++t) {
+        const char *kt = lds + (t & 1) * kTileBytes, *vt = kt + 2 * kTileBytes;
+        if (t + 1 < tiles) {
+            char* to = lds + ((t + 1) & 1) * kTileBytes;
+            k_next.store(to, tid), v_next.store(to + 2 * kTileBytes, tid);
+            if (t + 2 < tiles) k_next.load(k, a.k_at.token, (t + 2) * KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, (t + 2) * KEYS, end, a.chunks, tid);
+        }
+        if (wave_has_rows && t * KEYS < wave_most) {
+            floatx16 s[NS];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+                tile.straight(s[n], kt, n, column);
+            }
+            const int rest = seen - t * KEYS - 4 * half;
+            if ((t + 1) * KEYS > wave_least) run.template take<NS, true>(s, a.scale_log2, rest);
+            else run.template take<NS, false>(s, a.scale_log2, rest);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) tile.transposed(run.acc, vt, n, s[n]);
+        }
+        lds_barrier();
+    }
+    const float total = add_halves(run.total);
+    if (a.lse && half == 0 && my_row < a.tokens)
+        a.lse[static_cast<int64_t>(bh) * a.tokens + my_row] = total > 0.f ? run.top + __builtin_amdgcn_logf(total) : INFINITY;
+    typedef AttnOut<T, DP> Out;
+    char* room = lds + wave * Out::kRoom;
+    Out::park(room, run.acc, total > 0.f ? 1.0f / total : 0.f, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    T* out = static_cast<T*>(a.out) + batch * a.out_at.batch + head * a.out_at.head;
+    Out::write(room, a.chunks, lane, [&](int col) -> T* {
+        const int row = first_row + wave * kRows + col;
+        return row < a.tokens ? out + row * a.out_at.token : nullptr;
+    });
+}
+
+template <typename T, int DP>
+constexpr int rows_lds() {
+    typedef AttnTile<T, DP> Tile;
+    constexpr int tiles = 4 * keys_of_tile<T>() * Tile::kRowBytes, out = kWaves * AttnOut<T, DP>::kRoom;
+    return tiles > out ? tiles : out;
+}
+
+// Few queries, many keys: the queries of all heads that share a key head (row = token x group + head in the group) in one
+// wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with a tile of its own
+// and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).
+// (Rows of more than 256 bytes fill the registers of a SIMD with one wavefront: 128 of them for the tiles on their way.)
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_split(const AttnArgs a) {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    constexpr int KEYS = 32, kTileBytes = KEYS * Tile::kRowBytes;
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
+    const int pairs = a.batch * a.kv_heads;
+    const int bk = blockIdx.x % pairs, rest_id = blockIdx.x / pairs, split = rest_id % a.splits, block = rest_id / a.splits;
+    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    const int length = sequence_keys(a, batch);
+    const int rows = a.tokens * a.group, first_row = block * kRows, my_row = first_row + (lane & 31);
+    const int token = my_row / a.group, head = kv_head * a.group + my_row - token * a.group;
+    const int seen = my_row < rows ? keys_seen(a, token, length) : 0;
+    const int most = keys_seen(a, (min(first_row + kRows, rows) - 1) / a.group, length), least = keys_seen(a, first_row / a.group, length);
+    // This split's keys, of those that there are: whole tiles, shared evenly.
+    const int tiles = (most + KEYS - 1) / KEYS;
+    const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
+    const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
+    const Tile tile(lane);
+    AttnStage<T, DP, KEYS, kWave> k_next, v_next;
+    int t = t0 + wave;
+    if (t < t1) k_next.load(k, a.k_at.token, t * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, t * KEYS, most, a.chunks, lane);
+    Frag column[Tile::kSteps];
+    const T* q = static_cast<const T*>(a.q) + batch * a.q_at.batch;
+#pragma unroll
+    for (int s = 0; s < Tile::kSteps; ++s) {
+        Frag f = {};
+        if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
+        column[s] = f;
+    }
+    Running<Tile::kBlocks> run;
+    char *kt = lds + wave * 2 * kTileBytes, *vt = kt + kTileBytes;
+    for (; t < t1; t += kWaves) {
+        k_next.store(kt, lane), v_next.store(vt, lane);
+        if (t + kWaves < t1) k_next.load(k, a.k_at.token, (t + kWaves) * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, (t + kWaves) * KEYS, most, a.chunks, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        floatx16 s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        tile.straight(s[0], kt, 0, column);
+        const int rest = seen - t * KEYS - 4 * half;
+        if ((t + 1) * KEYS > least) run.template take<1, true>(s, a.scale_log2, rest);
+        else run.template take<1, false>(s, a.scale_log2, rest);
+        tile.transposed(run.acc, vt, 0, s[0]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    // Joined: every wavefront's maximum and total, then its sums relative to the common maximum, added in the wavefronts' order.
+    __shared__ float tops[kWaves][kRows], totals[kWaves][kRows];
+    const float own_total = add_halves(run.total);
+    if (half == 0) tops[wave][lane] = run.top, totals[wave][lane] = own_total;
+    __syncthreads();
+    const int col = lane & 31;
+    float top = tops[0][col];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, tops[w][col]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += totals[w][col] * __builtin_amdgcn_exp2f(tops[w][col] - from);
+    const bool whole = a.splits == 1;
+    const float factor = __builtin_amdgcn_exp2f(run.top - from) * (whole ? (total > 0.f ? 1.0f / total : 0.f) : 1.f);
+    typedef AttnOut<float, DP> Out;
+    Out::park(lds + wave * Out::kRoom, run.acc, factor, lane);
+    __syncthreads();
+    const int dim = a.chunks * Tile::kPerChunk;
+    float* partial = a.partial + (static_cast<int64_t>(split) * pairs + bk) * rows * (DP + 2);
+    for (int i = threadIdx.x; i < kRows * (DP / 4); i += kThreads) {
+        const int c = i / (DP / 4), d = 4 * (i % (DP / 4)), row = first_row + c;
+        if (row >= rows || d >= dim) continue;
+        float4 sum = *reinterpret_cast<const float4*>(lds + c * Out::kPitch + 4 * d);
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            const float4 more = *reinterpret_cast<const float4*>(lds + w * Out::kRoom + c * Out::kPitch + 4 * d);
+            sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+        }
+        if (whole) {
+            const int tk = row / a.group, hd = kv_head * a.group + row - tk * a.group;
+            store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + tk * a.out_at.token + hd * a.out_at.head + d, sum);
+        } else {
+            *reinterpret_cast<float2*>(partial + row * (DP + 2) + d) = make_float2(sum.x, sum.y);
+            *reinterpret_cast<float2*>(partial + row * (DP + 2) + d + 2) = make_float2(sum.z, sum.w);
+        }
+    }
+    if (wave == 0 && half == 0 && my_row < rows) {
+        if (whole) {
+            if (a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+        } else {
+            partial[my_row * (DP + 2) + DP] = top;
+            partial[my_row * (DP + 2) + DP + 1] = total;
+        }
+    }
+}
+
+// The splits of a row, in their order.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
+    constexpr int kLanes = DP / 4;      // of a row, four elements each
+    const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group;
+    const int64_t lane = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, at = lane / kLanes;
+    const int d = 4 * static_cast<int>(lane % kLanes);
+    if (at >= static_cast<int64_t>(pairs) * rows) return;
+    const int bk = static_cast<int>(at / rows), row = static_cast<int>(at - static_cast<int64_t>(bk) * rows);
+    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    const int64_t pitch = static_cast<int64_t>(pairs) * rows * (DP + 2);
+    const float* p = a.partial + at * (DP + 2);
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * pitch + DP]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool there = d < a.chunks * AttnElem<T>::kPerChunk;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 m = *reinterpret_cast<const float2*>(p + s * pitch + DP);
+        const float factor = __builtin_amdgcn_exp2f(m.x - from);
+        total += m.y * factor;
+        if (there) {
+            const float2 lo = *reinterpret_cast<const float2*>(p + s * pitch + d), hi = *reinterpret_cast<const float2*>(p + s * pitch + d + 2);
+            sum.x += lo.x * factor, sum.y += lo.y * factor, sum.z += hi.x * factor, sum.w += hi.y * factor;
+        }
+    }
+    const float inv = total > 0.f ? 1.0f / total : 0.f;
+    const int token = row / a.group, head = kv_head * a.group + row - token * a.group;
+    if (there)
+        store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + token * a.out_at.token + head * a.out_at.head + d,
+                          make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    if (d == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+}
+
+template <typename T, int DP>
+constexpr int split_lds() {
+    typedef AttnTile<T, DP> Tile;
+    constexpr int tiles = kWaves * 2 * 32 * Tile::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
+    return tiles > out ? tiles : out;
+}
+
+int padded_dim(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+
+// Into how many parts the keys are split; 0: attention_rows.
+int splits_for(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
+    if (tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1 || batch < 1) return 0;
+    int dev;
+    const int64_t cus = compute_units(dev);
+    const int64_t rows = tokens * (heads / kv_heads), row_blocks = (rows + kRows - 1) / kRows;
+    const int64_t whole = batch * heads * ((tokens + kRows * kWaves - 1) / (kRows * kWaves));
+    if (rows > 4 * kRows || (whole >= 2 * cus && tokens >= kRows)) return 0;
+    // Two workgroups a CU, each with at least four tiles of 32 keys for each of its wavefronts.
+    const int64_t units = batch * kv_heads * row_blocks, most = (keys + 511) / 512;
+    int64_t splits = (2 * cus + units - 1) / units;
+    if (splits > most) splits = most;
+    return static_cast<int>(splits < 1 ? 1 : splits);
+}
+
+}  // namespace
+}  // namespace ddl
+
+extern "C" {
+
+int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    using namespace ddl;
+    if (dim < 1 || dim > 128) return 0;
+    const int splits = splits_for(batch, tokens, keys, heads, kv_heads);
+    return splits > 1 ? static_cast<int64_t>(splits) * batch * tokens * heads * (padded_dim(dim) + 2) : 0;
+}
+
+int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
+                  int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, const int32_t* lengths, int causal,
+                  float scale, void* out, const int64_t* out_strides, float* lse, float* workspace, int64_t workspace_elems, void* stream) {
+    using namespace ddl;
+    AttnArgs a{};
+    bool nothing;
+    if (const int rc = fill_attention(a, nothing, "ddl_attention", {{q, q_strides}, {k, k_strides}, {v, v_strides}, {out, out_strides}}, dtype, batch, tokens, keys, heads,
+                                      kv_heads, dim, lengths, causal, scale))
+        return rc;
+    if (nothing || tokens == 0) return 0;
+    a.out = out, a.out_at = place_of(out_strides), a.lse = lse;
+    a.splits = splits_for(batch, tokens, keys, heads, kv_heads);
+    const int64_t need = ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim);
+    if (need && (!workspace || workspace_elems < need))
+        return fail(DDL_E_ARG, "ddl_attention: workspace of %lld floats, %lld are needed", static_cast<long long>(workspace ? workspace_elems : 0), static_cast<long long>(need));
+    if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention: workspace is not 16-byte aligned");
+    a.partial = workspace;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) {
+        typedef std::remove_pointer_t<decltype(e)> T;
+        constexpr int DP = decltype(dp)::value;
+        if (a.splits == 0) {
+            if (const int rc = grant_lds<attention_rows<T, DP>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
+            a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+            const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
+            if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
+            hipLaunchKernelGGL((attention_rows<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (rows_lds<T, DP>()), s, a);
+            return check_launch("ddl_attention");
+        }
+        if (const int rc = grant_lds<attention_split<T, DP>>(split_lds<T, DP>(), "ddl_attention")) return rc;
+        const int64_t rows = static_cast<int64_t>(a.tokens) * a.group, pairs = static_cast<int64_t>(a.batch) * a.kv_heads;
+        a.blocks = static_cast<int>((rows + kRows - 1) / kRows);
+        const int64_t grid = pairs * a.splits * a.blocks;
+        if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
+        hipLaunchKernelGGL((attention_split<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
+        if (const int rc = check_launch("ddl_attention")) return rc;
+        if (a.splits == 1) return 0;
+        const int64_t lanes = pairs * rows * (DP / 4);
+        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>((lanes + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+        return check_launch("ddl_attention");
+    });
+}
+
+}  // extern "C"

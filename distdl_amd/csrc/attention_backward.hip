@@ -1,0 +1,373 @@
+// Adjoint of attention.hip: with p_ij of the forward (formed anew from the scores and each row's sum), dO the gradient of out and
+//   D_i = sum of dO_i out_i,   dS_ij = p_ij (dO_i . v_j - D_i):
+//   dq_i = scale sum over j of dS_ij k_j,   dk_j = scale sum over i of dS_ij q_i,   dv_j = sum over i of p_ij dO_i
+//
+// Two kernels, so that every sum has one owner and one order and nothing is added atomically, at the price of forming the
+// scores and dO . v twice (seven products instead of five): attention_backward_rows, a wavefront for 32 queries that walks over
+// the keys, and attention_backward_keys, a wavefront for 32 keys that walks over the queries of all heads that share
+// them -- the gradient of a shared key head is summed there, in registers.
+#include "ddl_common.h"
+
+#include "attention_parts.h"
+
+namespace ddl {
+namespace {
+
+template <typename T>
+constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+template <int N>
+__device__ inline void clear(floatx16 (&acc)[N]) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+}
+
+__device__ inline float chunk_dot(const floatx4v& a, const floatx4v& b, const float*) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
+template <typename T>
+__device__ inline float chunk_dot(const shortx8& a, const shortx8& b, const T*) {
+    float s = 0.f;
+    T x[8], y[8];
+    __builtin_memcpy(x, &a, 16);
+    __builtin_memcpy(y, &b, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += load1(&x[i]) * load1(&y[i]);
+    return s;
+}
+
+// A column's row of a tensor as the straight product takes it; zeros where `there` is false.
+template <typename T, int DP, typename Frag>
+__device__ inline void load_column(Frag* column, const T* row, bool there, int chunks, int side) {
+    typedef AttnTile<T, DP> Tile;
+#pragma unroll
+    for (int s = 0; s < Tile::kSteps; ++s) {
+        Frag f = {};
+        if (there && 2 * s + side < chunks) f = *reinterpret_cast<const Frag*>(row + (2 * s + side) * Tile::kPerChunk);
+        column[s] = f;
+    }
+}
+
+// dq of 32 queries a wavefront, 128 a workgroup, tiles of keys and values through LDS as in attention_rows; and their D.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_backward_rows(const AttnArgs a) {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    constexpr int KEYS = tile_rows<T>(), NS = KEYS / 32, kTileBytes = KEYS * Tile::kRowBytes;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    int bh, block;
+    block_of(blockIdx.x, a.batch * a.heads, a.blocks, bh, block);
+    const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
+    const int length = sequence_keys(a, batch);
+    const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
+    const bool mine = my_row < a.tokens;
+    const int seen = keys_seen(a, my_row, length);
+    const int end = keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length);
+    const int wave_most = wave_row < a.tokens ? keys_seen(a, min(wave_row + kRows, a.tokens) - 1, length) : 0;
+    const int wave_least = keys_seen(a, wave_row, length);
+    const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
+    const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
+    const Tile tile(lane);
+    const int tiles = (end + KEYS - 1) / KEYS;
+    AttnStage<T, DP, KEYS, kThreads> k_next, v_next;
+    if (tiles > 0) k_next.load(k, a.k_at.token, 0, end, a.chunks, tid), v_next.load(v, a.v_at.token, 0, end, a.chunks, tid);
+    Frag q_column[Tile::kSteps], g_column[Tile::kSteps];
+    load_column<T, DP>(q_column, static_cast<const T*>(a.q) + batch * a.q_at.batch + my_row * a.q_at.token + head * a.q_at.head, mine, a.chunks, half);
+    load_column<T, DP>(g_column, static_cast<const T*>(a.dout) + batch * a.dout_at.batch + my_row * a.dout_at.token + head * a.dout_at.head, mine, a.chunks, half);
+    float delta = 0.f, lse = INFINITY;
+    {
+        Frag o_column[Tile::kSteps];
+        load_column<T, DP>(o_column, static_cast<const T*>(a.out) + batch * a.out_at.batch + my_row * a.out_at.token + head * a.out_at.head, mine, a.chunks, half);
+#pragma unroll
+        for (int s = 0; s < Tile::kSteps; ++s) delta += chunk_dot(g_column[s], o_column[s], static_cast<const T*>(nullptr));
+        delta = add_halves(delta);
+        const int64_t at = static_cast<int64_t>(bh) * a.tokens + my_row;
+        if (mine) {
+            lse = a.lse[at];
+            if (half == 0) a.delta[at] = delta;
+        }
+    }
+    if (!a.dq) return;      // D alone
+    floatx16 acc[Tile::kBlocks];
+    clear(acc);
+    if (tiles > 0) {
+        k_next.store(lds, tid), v_next.store(lds + 2 * kTileBytes, tid);
+        if (tiles > 1) k_next.load(k, a.k_at.token, KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, KEYS, end, a.chunks, tid);
+    }
+    lds_barrier();
+    for (int t = 0; t < tiles; ++t) {
+        const char *kt = lds + (t & 1) * kTileBytes, *vt = kt + 2 * kTileBytes;
+        if (t + 1 < tiles) {
+            char* to = lds + ((t + 1) & 1) * kTileBytes;
+            k_next.store(to, tid), v_next.store(to + 2 * kTileBytes, tid);
+            if (t + 2 < tiles) k_next.load(k, a.k_at.token, (t + 2) * KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, (t + 2) * KEYS, end, a.chunks, tid);
+        }
+        if (t * KEYS < wave_most) {
+            const bool masked = (t + 1) * KEYS > wave_least;
+            const int rest = seen - t * KEYS - 4 * half;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                floatx16 s[2];
+                clear(s);
+                tile.straight(s[0], kt, n, q_column);
+                tile.straight(s[1], vt, n, g_column);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.scale_log2, -lse));
+                    if (masked) p = 32 * n + (r & 3) + 8 * (r >> 2) < rest ? p : 0.f;
+                    s[0][r] = p * (s[1][r] - delta);
+                }
+                tile.transposed(acc, kt, n, s[0]);
+            }
+        }
+        lds_barrier();
+    }
+    typedef AttnOut<T, DP> Out;
+    char* room = lds + wave * Out::kRoom;
+    Out::park(room, acc, a.scale, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    T* dq = static_cast<T*>(a.dq) + batch * a.dq_at.batch + head * a.dq_at.head;
+    Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_row + col < a.tokens ? dq + (wave_row + col) * a.dq_at.token : nullptr; });
+}
+
+template <typename T, int DP>
+constexpr int query_tile() { return AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32; }
+
+// dk and dv of 32 keys a wavefront, 128 a workgroup; 32 or 64 queries of one head at a time through LDS, with their sums and D.  Where
+// there are few blocks of keys, `splits` workgroups share the queries of one and leave sums in fp32.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attention_backward_keys(const AttnArgs a) {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    constexpr int ROWS = query_tile<T, DP>(), NS = ROWS / 32, kTileBytes = ROWS * Tile::kRowBytes, kSetBytes = 2 * kTileBytes + 2 * ROWS * 4;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    const int pairs = a.batch * a.kv_heads;
+    int bk, unit;
+    block_of(blockIdx.x, pairs, a.blocks * a.splits, bk, unit);
+    unit = a.blocks * a.splits - 1 - unit;      // the first keys, which most queries see in the causal form, first
+    const int block = unit / a.splits, split = unit - block * a.splits;
+    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    const int length = sequence_keys(a, batch);
+    const int first_key = block * kRows * kWaves, wave_key = first_key + wave * kRows, my_key = wave_key + (lane & 31);
+    // Query i sees key j from i = j - shift on.
+    const int shift = a.causal ? a.keys - a.tokens : 0x3FFFFFFF;
+    const int need = my_key < length ? max(my_key - shift, 0) : 0x7FFFFFFF;      // first query that sees this lane's key
+    const int block_need = first_key < length ? max(first_key - shift, 0) : a.tokens;
+    const int wave_need = wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF;
+    const int wave_all = wave_key + kRows <= length ? max(wave_key + kRows - 1 - shift, 0) : 0x7FFFFFFF;   // from here on queries see all of the wavefront's keys
+    const int first_tile = min(block_need, a.tokens) / ROWS, head_tiles = block_need < a.tokens ? (a.tokens + ROWS - 1) / ROWS - first_tile : 0;
+    const int64_t all = static_cast<int64_t>(head_tiles) * a.group;
+    const int it0 = static_cast<int>(all * split / a.splits), it1 = static_cast<int>(all * (split + 1) / a.splits);
+    const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
+    const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
+    const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
+    const Tile tile(lane);
+    AttnStage<T, DP, ROWS, kThreads> q_next, g_next;
+    float row_next = 0.f;
+    auto load = [&](int it) {
+        const int in_group = it / head_tiles, first = (first_tile + it - in_group * head_tiles) * ROWS;
+        q_next.load(q0 + in_group * a.q_at.head, a.q_at.token, first, a.tokens, a.chunks, tid);
+        g_next.load(g0 + in_group * a.dout_at.head, a.dout_at.token, first, a.tokens, a.chunks, tid);
+        if (tid < 2 * ROWS) {
+            const int row = first + (tid & (ROWS - 1));
+            const int64_t at = row0 + static_cast<int64_t>(in_group) * a.tokens + row;
+            row_next = tid < ROWS ? (row < a.tokens ? a.lse[at] : INFINITY) : (row < a.tokens ? a.delta[at] : 0.f);
+        }
+    };
+    auto store = [&](char* set) {
+        q_next.store(set, tid), g_next.store(set + kTileBytes, tid);
+        if (tid < 2 * ROWS) reinterpret_cast<float*>(set + 2 * kTileBytes)[tid] = row_next;
+    };
+    if (it0 < it1) load(it0);
+    Frag k_column[Tile::kSteps], v_column[Tile::kSteps];
+    const bool mine = my_key < length;
+    load_column<T, DP>(k_column, static_cast<const T*>(a.k) + batch * a.k_at.batch + my_key * a.k_at.token + kv_head * a.k_at.head, mine, a.chunks, half);
+    load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
+    floatx16 dk[Tile::kBlocks], dv[Tile::kBlocks];
+    clear(dk), clear(dv);
+    if (it0 < it1) {
+        store(lds);
+        if (it0 + 1 < it1) load(it0 + 1);
+    }
+    lds_barrier();
+    for (int it = it0; it < it1; ++it) {
+        const char* set = lds + ((it - it0) & 1) * kSetBytes;
+        if (it + 1 < it1) {
+            store(lds + ((it + 1 - it0) & 1) * kSetBytes);
+            if (it + 2 < it1) load(it + 2);
+        }
+        const int first = (first_tile + it % head_tiles) * ROWS;
+        if (first + ROWS > wave_need) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                if (NS > 1 && first + 32 * (n + 1) <= wave_need) continue;
+                floatx16 s[2];
+                clear(s);
+                tile.straight(s[0], set, n, k_column);
+                tile.straight(s[1], set + kTileBytes, n, v_column);
+                const float* rows = reinterpret_cast<const float*>(set + 2 * kTileBytes) + 32 * n + 4 * half;
+                const bool masked = first + 32 * n < wave_all;
+                floatx16 p;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 8 * g), delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 8 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 4 * g + i;
+                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.scale_log2, -lse[i]));
+                        if (masked) p[r] = first + 32 * n + 4 * half + i + 8 * g >= need ? p[r] : 0.f;
+                        s[0][r] = p[r] * (s[1][r] - delta[i]);
+                    }
+                }
+                tile.transposed(dv, set + kTileBytes, n, p);
+                tile.transposed(dk, set, n, s[0]);
+            }
+        }
+        lds_barrier();
+    }
+    if (a.splits == 1) {
+        typedef AttnOut<T, DP> Out;
+        char* room = lds + wave * Out::kRoom;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const HeadsAt& at = which ? a.dv_at : a.dk_at;
+            T* to = static_cast<T*>(which ? a.dv : a.dk);
+            if (!to) continue;
+            to += batch * at.batch + kv_head * at.head;
+            if (which) Out::park(room, dv, 1.f, lane);
+            else Out::park(room, dk, a.scale, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_key + col < a.keys ? to + (wave_key + col) * at.token : nullptr; });
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    } else {
+        typedef AttnOut<float, DP> Out;
+        char* room = lds + wave * Out::kRoom;
+        const int dim = a.chunks * Tile::kPerChunk;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
+            if (which) Out::park(room, dv, 1.f, lane);
+            else Out::park(room, dk, a.scale, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_key + col < a.keys ? to + static_cast<int64_t>(wave_key + col) * dim : nullptr; });
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+}
+
+// dk and dv from the splits' sums, in their order: four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_backward_join(const AttnArgs a) {
+    const int quads = a.chunks * AttnElem<T>::kPerChunk / 4, pairs = a.batch * a.kv_heads;
+    const int64_t one = static_cast<int64_t>(pairs) * a.keys * quads, at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (at >= 2 * one) return;
+    const int which = at >= one;
+    const int64_t in = at - which * one;
+    const float4* p = reinterpret_cast<const float4*>(a.partial) + at;
+    float4 sum = p[0];
+    for (int s = 1; s < a.splits; ++s) {
+        const float4 more = p[2 * one * s];
+        sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+    }
+    const int64_t row = in / quads;
+    const int d = 4 * static_cast<int>(in - row * quads), bk = static_cast<int>(row / a.keys), key = static_cast<int>(row - static_cast<int64_t>(bk) * a.keys);
+    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    const HeadsAt& to = which ? a.dv_at : a.dk_at;
+    T* base = static_cast<T*>(which ? a.dv : a.dk);
+    if (base) store_piece<true>(base + batch * to.batch + key * to.token + kv_head * to.head + d, sum);
+}
+
+template <typename T, int DP>
+constexpr int backward_rows_lds() {
+    constexpr int tiles = 4 * tile_rows<T>() * AttnTile<T, DP>::kRowBytes, out = kWaves * AttnOut<T, DP>::kRoom;
+    return tiles > out ? tiles : out;
+}
+template <typename T, int DP>
+constexpr int backward_keys_lds() {
+    constexpr int tiles = 2 * query_tile<T, DP>() * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4), out = kWaves * AttnOut<float, DP>::kRoom;
+    return tiles > out ? tiles : out;
+}
+
+// Workgroups that share the queries of a block of keys.
+int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
+    if (batch < 1 || tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1) return 1;
+    int dev;
+    const int64_t units = batch * kv_heads * ((keys + kRows * kWaves - 1) / (kRows * kWaves)), tiles = heads / kv_heads * ((tokens + 31) / 32);
+    int64_t splits = (2 * static_cast<int64_t>(compute_units(dev)) + units - 1) / units;
+    if (splits > tiles / 8) splits = tiles / 8;
+    return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+}
+
+int64_t rounded4(int64_t n) { return (n + 3) / 4 * 4; }
+
+}  // namespace
+}  // namespace ddl
+
+extern "C" {
+
+int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    using namespace ddl;
+    if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || dim < 1 || keys < 0) return 0;
+    const int64_t splits = key_splits(batch, tokens, keys, heads, kv_heads);
+    return rounded4(batch * heads * tokens) + (splits > 1 ? splits * 2 * batch * kv_heads * keys * dim : 0);
+}
+
+int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                           const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides, const float* lse, int dtype, int64_t batch,
+                           int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, const int32_t* lengths, int causal, float scale,
+                           void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides, float* workspace,
+                           int64_t workspace_elems, void* stream) {
+    using namespace ddl;
+    AttnArgs a{};
+    bool nothing;
+    if (const int rc = fill_attention(a, nothing, "ddl_attention_backward", {{q, q_strides}, {k, k_strides}, {v, v_strides}, {out, out_strides}, {dout, dout_strides}}, dtype,
+                                      batch, tokens, keys, heads, kv_heads, dim, lengths, causal, scale))
+        return rc;
+    if (nothing || (!dq && !dk && !dv)) return 0;
+    const struct { void* p; const int64_t* s; } results[3] = {{dq, dq_strides}, {dk, dk_strides}, {dv, dv_strides}};
+    for (const auto& r : results) {
+        if (!r.p) continue;
+        const int per = dtype == DDL_DT_F32 ? 4 : 8;
+        if (!r.s) return fail(DDL_E_ARG, "ddl_attention_backward: no strides");
+        if (!aligned_to(r.p, 16) || r.s[0] % per || r.s[1] % per || r.s[2] % per) return fail(DDL_E_ALIGN, "ddl_attention_backward: gradients are not 16-byte aligned");
+    }
+    if (tokens && !lse) return fail(DDL_E_ARG, "ddl_attention_backward: no row sums");
+    const int64_t need = ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim);
+    if (need && (!workspace || workspace_elems < need))
+        return fail(DDL_E_ARG, "ddl_attention_backward: workspace of %lld floats, %lld are needed", static_cast<long long>(workspace ? workspace_elems : 0), static_cast<long long>(need));
+    if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention_backward: workspace is not 16-byte aligned");
+    a.dout = dout, a.dout_at = place_of(dout_strides), a.out = const_cast<void*>(out), a.out_at = place_of(out_strides), a.lse = const_cast<float*>(lse);
+    a.dq = dq, a.dk = dk, a.dv = dv, a.dq_at = place_of(dq_strides), a.dk_at = place_of(dk_strides), a.dv_at = place_of(dv_strides);
+    a.delta = workspace, a.partial = workspace + rounded4(batch * heads * tokens);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) {
+        typedef std::remove_pointer_t<decltype(e)> T;
+        constexpr int DP = decltype(dp)::value;
+        constexpr int kRowsLds = backward_rows_lds<T, DP>(), kKeysLds = backward_keys_lds<T, DP>();
+        if (a.tokens) {
+            if (const int rc = grant_lds<attention_backward_rows<T, DP>>(kRowsLds, "ddl_attention_backward")) return rc;
+            a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+            const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
+            if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
+            hipLaunchKernelGGL((attention_backward_rows<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kRowsLds, s, a);
+            if (const int rc = check_launch("ddl_attention_backward")) return rc;
+        }
+        if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
+        if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kKeysLds, "ddl_attention_backward")) return rc;
+        a.splits = key_splits(batch, tokens, keys, heads, kv_heads);
+        a.blocks = (a.keys + kRows * kWaves - 1) / (kRows * kWaves);
+        const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads, grid = pairs * a.blocks * a.splits;
+        if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
+        hipLaunchKernelGGL((attention_backward_keys<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kKeysLds, s, a);
+        if (const int rc = check_launch("ddl_attention_backward")) return rc;
+        if (a.splits == 1) return 0;
+        const int64_t threads = 2 * pairs * a.keys * (dim / 4);
+        hipLaunchKernelGGL((attention_backward_join<T>), dim3(static_cast<uint32_t>((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+        return check_launch("ddl_attention_backward");
+    });
+}
+
+}  // extern "C"

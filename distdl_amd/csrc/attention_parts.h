@@ -1,0 +1,367 @@
+// What the attention kernels share: tiles of rows in LDS, and the two products that all of them are made of.
+//
+// A wavefront owns 32 columns (queries forward, keys in the gradients of keys and values), one a lane, lanes l and l + 32
+// the same one, and walks over tiles of 32 rows of the other side:
+//
+//   straight    S[row, column]    = sum over d of tile[row, d] column[d]       scores, and dP from values or gradients
+//   transposed  acc[d, column]   += sum over rows of tile[row, d] P[row, column]
+//
+// with v_mfma_f32_32x32x16 (16-bit types) or v_mfma_f32_32x32x2_f32.  A lane's sixteen results of the first are rows
+//   (r & 3) + 8 (r >> 2) + 4 (l >> 5),  r = 0 .. 15,
+// of its own column, so a column's maximum and sum need one exchange between the lanes' halves, and the second product
+// takes them back as they lie: which row a reduction index stands for is free as long as both operands agree, so the tile is
+// read for the rows that each lane happens to hold (16-bit: ds_read_b64_tr_b16, four rows of one column; fp32: a word a row).
+// Nothing of P goes through LDS.
+//
+// A tile's rows are DP elements of ROWB bytes, a power of two, in chunks of 16 bytes; chunk c of row r lies at c ^ swizzle(r), a
+// permutation of r's low four bits that gives 16 rows of one chunk different banks (straight reads), and the four rows
+// of 64 bytes of a transposing read as well.
+#ifndef DDL_ATTENTION_PARTS_H
+#define DDL_ATTENTION_PARTS_H
+#include "ddl_common.h"
+
+#include "ln_elements.h"
+
+#include <initializer_list>
+
+namespace ddl {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4v __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) shortx4* lds_shortx4;
+
+template <typename T>
+struct AttnElem {
+    typedef shortx8 Frag;                 // 16 bytes of a row
+    static constexpr int kPerChunk = 8;
+};
+template <>
+struct AttnElem<float> {
+    typedef floatx4v Frag;
+    static constexpr int kPerChunk = 4;
+};
+
+__device__ inline void mfma_chunk(floatx16& acc, const floatx4v& a, const floatx4v& b, const float*) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
+}
+__device__ inline void mfma_chunk(floatx16& acc, const shortx8& a, const shortx8& b, const bf16_t*) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), acc, 0, 0, 0);
+}
+__device__ inline void mfma_chunk(floatx16& acc, const shortx8& a, const shortx8& b, const __half*) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), acc, 0, 0, 0);
+}
+
+// Eight values rounded to the 16-bit type (half a step each: 2^-9 of a probability in bf16, 2^-12 in fp16; sums of
+// many of them average it out).
+__device__ inline shortx8 pack8(const floatx16& v, int first, const bf16_t*) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = f32x2_to_bf16(v[first + 2 * i], v[first + 2 * i + 1]);
+    shortx8 o;
+    __builtin_memcpy(&o, w, 16);
+    return o;
+}
+__device__ inline shortx8 pack8(const floatx16& v, int first, const __half*) {
+    halfx8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = static_cast<_Float16>(v[first + i]);
+    return __builtin_bit_cast(shortx8, o);
+}
+
+// Rows of DP elements of type T in LDS.
+template <typename T, int DP>
+struct AttnTile {
+    typedef typename AttnElem<T>::Frag Frag;
+    static constexpr int kPerChunk = AttnElem<T>::kPerChunk;
+    static constexpr int kBytes = DP * static_cast<int>(sizeof(T));
+    static constexpr int kRowBytes = kBytes <= 64 ? 64 : kBytes <= 128 ? 128 : kBytes <= 256 ? 256 : 512;
+    static constexpr int kSteps = kBytes / 32;         // of the straight product: a chunk from either half of the lanes
+    static constexpr int kBlocks = DP / 32;            // of the transposed product
+    static constexpr int kChunks = kBytes / 16;        // of a row
+    static_assert(DP % 32 == 0 && kBytes <= 512, "rows of 32 to 128 elements");
+
+    // Linear over exclusive or, so that the parts of a row number that the compiler knows and those of a lane can be permuted apart.
+    static constexpr __device__ int swizzle(int row) {
+        if (kRowBytes == 64) return (row >> 2) & 3;
+        if (kRowBytes == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        if (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+        return (((row >> 2) & 1) << 3) | (row & 3) | (((row >> 3) & 1) << 2);
+    }
+
+    int straight_row, straight_x;     // of this lane: byte offset of its row, its part of the chunk number
+    int trans_row, trans_x, trans_byte;
+
+    __device__ explicit AttnTile(int lane) {
+        const int half = lane >> 5, col = lane & 31;
+        straight_row = col * kRowBytes, straight_x = half ^ swizzle(col);
+        if constexpr (sizeof(T) == 2) {   // lane i of 16 points at row i / 4, columns 4 (i % 4) .. + 3 of 16, and receives column i of the four rows
+            const int i = lane & 15, row = 4 * half + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            trans_row = row * kRowBytes, trans_x = chunk ^ swizzle(row), trans_byte = 8 * (i & 1);
+        } else {
+            trans_row = 4 * half * kRowBytes, trans_x = (col >> 2) ^ swizzle(4 * half), trans_byte = 4 * (col & 3);
+        }
+    }
+
+    // acc[r] += the product of rows 32 block .. + 31 of the tile with this lane's column.
+    __device__ void straight(floatx16& acc, const char* tile, int block, const Frag (&column)[kSteps]) const {
+        const char* base = tile + block * 32 * kRowBytes + straight_row;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const Frag a = *reinterpret_cast<const Frag*>(base + (((2 * s) ^ straight_x) << 4));
+            mfma_chunk(acc, a, column[s], static_cast<const T*>(nullptr));
+        }
+    }
+
+    // acc[d block] += tile rows 32 block .. + 31, transposed, times p of this lane's column.
+    __device__ void transposed(floatx16 (&acc)[kBlocks], const char* tile, int block, const floatx16& p) const {
+        const char* base = tile + block * 32 * kRowBytes + trans_row + trans_byte;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const shortx8 b = pack8(p, 8 * k, static_cast<const T*>(nullptr));
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)(base + 16 * k * kRowBytes + (((4 * d) ^ trans_x) << 4)));
+                    const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)(base + (16 * k + 8) * kRowBytes + (((4 * d) ^ swizzle(8) ^ trans_x) << 4)));
+                    mfma_chunk(acc[d], __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, static_cast<const T*>(nullptr));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = (r & 3) + 8 * (r >> 2);
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const float a = *reinterpret_cast<const float*>(base + row * kRowBytes + (((8 * d) ^ swizzle(row) ^ trans_x) << 4));
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[d], 0, 0, 0);
+                }
+            }
+        }
+    }
+};
+
+// ROWS rows of a tensor on their way through the registers of THREADS threads into a tile.  A thread has one chunk of every
+// kStep-th row, so its addresses are one 32-bit offset from places that are the same for all threads.
+constexpr int64_t kMaxPitch = 1 << 22;      // elements from row to row: 64 rows of 4 bytes each stay below 2^31
+template <typename T, int DP, int ROWS, int THREADS>
+struct AttnStage {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    static constexpr int kSlots = Tile::kRowBytes / 16, kStep = THREADS / kSlots, kPieces = ROWS / kStep;
+    static_assert(THREADS % kSlots == 0 && ROWS % kStep == 0, "whole rows for the threads");
+    Frag piece[kPieces];
+
+    // Rows first .. first + ROWS of `base` (row r at base + r * pitch elements); zeros from row `end` and chunk `chunks` on.
+    // `tid`: of the THREADS.
+    __device__ void load(const T* base, int64_t pitch, int first, int end, int chunks, int tid) {
+        const int row = tid / kSlots, c = tid % kSlots;
+        const uint32_t offset = (static_cast<uint32_t>(row) * static_cast<uint32_t>(pitch) + c * Tile::kPerChunk) * static_cast<uint32_t>(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const char* from = reinterpret_cast<const char*>(base + (first + i * kStep) * pitch);
+            Frag v = {};
+            if (first + i * kStep + row < end && c < chunks) v = *reinterpret_cast<const Frag*>(from + offset);
+            piece[i] = v;
+        }
+    }
+    __device__ void store(char* tile, int tid) const {
+        const int row = tid / kSlots, c = tid % kSlots;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int r = row + i * kStep;
+            if (kSlots == Tile::kChunks || c < Tile::kChunks) *reinterpret_cast<Frag*>(tile + r * Tile::kRowBytes + ((c ^ Tile::swizzle(r)) << 4)) = piece[i];
+        }
+    }
+};
+
+// The value of lane l ^ 32 and this lane's, combined.
+template <typename Fn>
+__device__ inline float both_halves(float v, Fn&& fn) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fn(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float add_halves(float v) {
+    return both_halves(v, [](float a, float b) { return a + b; });
+}
+__device__ inline float max_halves(float v) {
+    return both_halves(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// Barrier of a workgroup whose wavefronts share LDS only: global loads stay in flight across it.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A wavefront's 32 columns of acc[d block][r] (d = 32 block + (r & 3) + 8 (r >> 2) + 4 half), times `factor`, as rows of DP elements
+// in its own room of LDS, kPitch bytes apart.
+template <typename T, int DP>
+struct AttnOut {
+    static constexpr int kPitch = DP * static_cast<int>(sizeof(T)) + 16;
+    static constexpr int kRoom = 32 * kPitch;      // bytes for a wavefront
+    static constexpr int kBlocks = DP / 32;
+    static __device__ void park(char* room, const floatx16 (&acc)[kBlocks], float factor, int lane) {
+        char* row = room + (lane & 31) * kPitch;
+        const int half = lane >> 5;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                T* at = reinterpret_cast<T*>(row) + 32 * d + 8 * q + 4 * half;
+                const float a = acc[d][4 * q] * factor, b = acc[d][4 * q + 1] * factor, c = acc[d][4 * q + 2] * factor, e = acc[d][4 * q + 3] * factor;
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(at) = make_float4(a, b, c, e);
+                } else if constexpr (std::is_same_v<T, bf16_t>) {
+                    *reinterpret_cast<uint2*>(at) = make_uint2(f32x2_to_bf16(a, b), f32x2_to_bf16(c, e));
+                } else {
+                    const __half2 lo = __floats2half2_rn(a, b), hi = __floats2half2_rn(c, e);
+                    *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                }
+            }
+    }
+    // Row by row to memory: `place(column)` is where a column's first element goes, null for none; `chunks` of 16 bytes each.
+    template <typename Fn>
+    static __device__ void write(const char* room, int chunks, int lane, Fn&& place) {
+        typedef typename AttnElem<T>::Frag Frag;
+        const int all = 32 * chunks;
+        for (int i = lane; i < all; i += 64) {
+            const int col = i / chunks, c = i - col * chunks;
+            T* to = place(col);
+            if (to) *reinterpret_cast<Frag*>(to + c * AttnElem<T>::kPerChunk) = *reinterpret_cast<const Frag*>(room + col * kPitch + (c << 4));
+        }
+    }
+};
+
+// ------------------------------------------------------------- arguments --
+
+constexpr int kWave = 64;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWave * kWaves;
+constexpr int kRows = 32;               // columns of a wavefront: rows of the tensor that it works for
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct HeadsAt {                        // of a [batch, tokens, heads, head_dim] tensor: strides in elements
+    int64_t batch, token, head;
+};
+inline HeadsAt place_of(const int64_t* s) { return s ? HeadsAt{s[0], s[1], s[2]} : HeadsAt{0, 0, 0}; }
+
+struct AttnArgs {
+    const void *q, *k, *v, *dout;
+    void *out, *dq, *dk, *dv;
+    HeadsAt q_at, k_at, v_at, out_at, dout_at, dq_at, dk_at, dv_at;
+    float* lse;                         // [batch][heads][tokens], log2
+    float* delta;                       // the same, sum of dout out
+    const int32_t* lengths;             // [batch] or null
+    int tokens, keys, heads, kv_heads, group, batch;
+    int chunks;                         // of 16 bytes of a head
+    int causal;
+    float scale, scale_log2;
+    int blocks;                         // of rows (or keys) of a head
+    int splits;                         // of the keys (adjoint of keys: of the queries)
+    float* partial;                     // sums of the splits
+};
+
+// Keys that the query at `token` sees of a sequence of `length`.
+__device__ inline int keys_seen(const AttnArgs& a, int token, int length) {
+    if (token >= a.tokens) return 0;
+    if (!a.causal) return length;
+    const int own = token + 1 + a.keys - a.tokens;
+    return min(length, max(own, 0));
+}
+
+__device__ inline int sequence_keys(const AttnArgs& a, int batch) {
+    if (!a.lengths) return a.keys;
+    const int n = a.lengths[batch];
+    return n < 0 ? 0 : n < a.keys ? n : a.keys;
+}
+
+// Workgroup `id` of `blocks` x `heads`: neighbouring numbers go to different XCDs, each of which takes its own share of the heads,
+// so that what they have in common stays in its L2.  Blocks come in descending order.
+__device__ inline void block_of(int id, int heads, int blocks, int& head, int& block) {
+    if (heads % 8 == 0) {
+        const int share = heads / 8, slot = id >> 3;
+        head = (id & 7) * share + slot % share, block = slot / share;
+    } else {
+        head = id % heads, block = id / heads;
+    }
+    block = blocks - 1 - block;
+}
+
+// More LDS than a kernel gets unasked: set once for each kernel and device.
+template <auto kernel>
+int grant_lds(int bytes, const char* what) {
+    static std::atomic<uint64_t> granted{0};   // one bit a device
+    int dev;
+    compute_units(dev);
+    if (granted.load(std::memory_order_relaxed) >> dev & 1) return 0;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(static_cast<int>(e), "%s: %s", what, hipGetErrorString(e));
+    granted.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return 0;
+}
+
+
+struct HeadsOperand {
+    const void* p;
+    const int64_t* strides;
+};
+
+// The checks and arguments that the entry points share: `operands` are q, k, v and others like q.  0 or a refusal;
+// `nothing`: there are no queries to work for.
+inline int fill_attention(AttnArgs& a, bool& nothing, const char* what, std::initializer_list<HeadsOperand> operands, int dtype, int64_t batch, int64_t tokens,
+                          int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, const int32_t* lengths, int causal, float scale) {
+    if (batch < 0 || tokens < 0 || keys < 0 || heads < 0 || kv_heads < 0 || dim < 1) return fail(DDL_E_ARG, "%s: negative extent or empty heads", what);
+    if (dtype != DDL_DT_F32 && dtype != DDL_DT_BF16 && dtype != DDL_DT_F16) return fail(DDL_E_ARG, "%s: dtype %d", what, dtype);
+    if (dim > 128) return fail(DDL_E_UNSUPP, "%s: heads of %lld elements (at most 128)", what, static_cast<long long>(dim));
+    const int per = dtype == DDL_DT_F32 ? 4 : 8;
+    if (dim % per) return fail(DDL_E_ALIGN, "%s: heads of %lld elements are no multiple of 16 bytes", what, static_cast<long long>(dim));
+    if (!(scale > 0.f && scale <= 3.0e38f)) return fail(DDL_E_ARG, "%s: scale %g is not positive", what, static_cast<double>(scale));
+    if (heads && (kv_heads == 0 || heads % kv_heads))
+        return fail(DDL_E_SHAPE, "%s: %lld heads cannot share %lld key heads", what, static_cast<long long>(heads), static_cast<long long>(kv_heads));
+    if ((heads && (tokens > 0x3FFFFFFF / heads || batch > 0x3FFFFFFF / heads)) || keys > 0x3FFFFFFF || heads > 0x3FFFFFFF)
+        return fail(DDL_E_UNSUPP, "%s: 2^30 rows or keys", what);
+    nothing = batch == 0 || heads == 0 || (tokens == 0 && keys == 0);
+    if (nothing) return 0;
+    int i = 0;
+    for (const HeadsOperand& o : operands) {
+        const bool of_keys = i == 1 || i == 2;
+        if ((of_keys ? keys : tokens) && (!o.p || !o.strides)) return fail(DDL_E_ARG, "%s: null tensor", what);
+        if (o.p && o.strides) {
+            if (o.strides[0] % per || o.strides[1] % per || o.strides[2] % per) return fail(DDL_E_ALIGN, "%s: strides are no multiples of 16 bytes", what);
+            if (!aligned_to(o.p, 16)) return fail(DDL_E_ALIGN, "%s: operands are not 16-byte aligned", what);
+            if (o.strides[1] < 0 || o.strides[1] >= kMaxPitch) return fail(DDL_E_UNSUPP, "%s: rows 2^22 elements apart", what);
+        }
+        const HeadsAt at = place_of(o.strides);
+        if (i == 0) a.q = o.p, a.q_at = at;
+        if (i == 1) a.k = o.p, a.k_at = at;
+        if (i == 2) a.v = o.p, a.v_at = at;
+        ++i;
+    }
+    a.lengths = lengths;
+    a.tokens = static_cast<int>(tokens), a.keys = static_cast<int>(keys), a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
+    a.group = static_cast<int>(heads / kv_heads), a.batch = static_cast<int>(batch), a.chunks = static_cast<int>(dim / per), a.causal = causal != 0;
+    a.scale = scale, a.scale_log2 = scale * kLog2e;
+    return 0;
+}
+
+// Calls fn(element, head size): the element type that `dtype` names and the smallest supported row of at least `dim`.
+template <typename Fn>
+inline int with_attention_kernel(int dtype, int64_t dim, Fn&& fn) {
+    int rc = DDL_E_ARG;
+    with_ln_element(dtype, [&](auto* e) {
+        if (dim <= 32) rc = fn(e, std::integral_constant<int, 32>{});
+        else if (dim <= 64) rc = fn(e, std::integral_constant<int, 64>{});
+        else if (dim <= 96) rc = fn(e, std::integral_constant<int, 96>{});
+        else rc = fn(e, std::integral_constant<int, 128>{});
+    });
+    return rc;
+}
+
+}  // namespace ddl
+#endif  // DDL_ATTENTION_PARTS_H

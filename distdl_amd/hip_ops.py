@@ -1240,3 +1240,100 @@ def head_norm_rotary_backward(dyq, dyk, q, k, q_weight, k_weight, frequencies, p
             float(amplitude), _ptr(dq), _strides3(dq), _ptr(dk), _strides3(dk), _ptr(dqw), _ptr(dkw), _ptr(work), elems, _stream())
     _lib.check(rc, "ddl_head_norm_rotary_backward")
     return dq, dk, dqw, dkw
+
+
+def _aligned_heads(t, dim):
+    """``t`` as the attention kernels take it: 16-byte aligned rows of ``dim`` elements, a multiple of 16 bytes; else a copy, with zeros behind
+    the head's own elements."""
+    per = 16 // t.element_size()
+    if t.shape[3] == dim and t.data_ptr() % 16 == 0 and all(s % per == 0 or n <= 1 for s, n in zip(t.stride()[:3], t.shape[:3])):
+        return t
+    if t.shape[3] == dim:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    else:
+        out = torch.zeros(t.shape[:3] + (dim,), dtype=t.dtype, device=t.device)
+    if t.numel():
+        full = [slice(0, int(n)) for n in t.shape]
+        copy_box(t, full, out, full)
+    return out
+
+
+def _attention_strides(t):
+    """Strides of the first three dimensions, 0 where there is one element (whatever the tensor says: nothing is ever a stride away)."""
+    return _lib.i64_array([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])])
+
+
+def _attention_operands(q, k, v, lengths, scale, name):
+    """Checked operands: ``(q, k, v, lengths, scale, dim)``, heads padded to ``dim``, a multiple of 16 bytes."""
+    _require_gpu(q, k, v, lengths)
+    q = _heads(q, name)
+    k, v = _heads(k, name, q), _heads(v, name, q)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"{name}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit")
+    if q.shape[2] and (k.shape[2] == 0 or q.shape[2] % k.shape[2]):
+        raise ValueError(f"{name}: {q.shape[2]} heads cannot share {k.shape[2]} key heads")
+    if not 1 <= q.shape[3] <= 128:
+        raise ValueError(f"{name}: heads of {q.shape[3]} elements (1 to 128 are supported)")
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],) or lengths.device != q.device):
+        raise ValueError(f"{name}: lengths must be int32 [{q.shape[0]}] on {q.device}, got {tuple(lengths.shape)} {lengths.dtype} on {lengths.device}")
+    if lengths is not None and not lengths.is_contiguous():
+        lengths = contiguous(lengths)
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    if not 0 < scale <= 3e38:
+        raise ValueError(f"{name}: scale {scale} is not positive")
+    per = 16 // q.element_size()
+    dim = -(-q.shape[3] // per) * per
+    with _on_device_of(q):
+        q, k, v = (_aligned_heads(t, dim) for t in (q, k, v))
+    return q, k, v, lengths, scale, dim
+
+
+def attention(q, k, v, lengths=None, causal=False, scale=None, want_lse=False):
+    """Attention of ``q`` [batch, tokens, heads, head_dim] to ``k``, ``v`` [batch, keys, kv_heads, head_dim], see ``ddl_attention``: a new
+    tensor like ``q``, and with ``want_lse`` what the adjoint needs."""
+    head_dim = q.shape[-1] if q.dim() else 0
+    q, k, v, lengths, scale, dim = _attention_operands(q, k, v, lengths, scale, "attention")
+    batch, tokens, heads, _ = q.shape
+    keys, kv_heads = k.shape[1:3]
+    lib = _lib.load()
+    with _on_device_of(q):
+        out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
+        lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if want_lse else None
+        elems = lib.ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim)
+        work = torch.empty(elems, dtype=torch.float32, device=q.device) if elems else None
+        rc = lib.ddl_attention(q.data_ptr(), _attention_strides(q), k.data_ptr(), _attention_strides(k), v.data_ptr(), _attention_strides(v),
+                               _LN_DTYPES[q.dtype], batch, tokens, keys, heads, kv_heads, dim, _ptr(lengths), int(causal), scale, out.data_ptr(),
+                               _attention_strides(out), _ptr(lse), _ptr(work), elems, _stream())
+        _lib.check(rc, "ddl_attention")
+        if dim != head_dim:
+            out = contiguous(out[..., :head_dim])
+    return (out, lse) if want_lse else out
+
+
+def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scale=None, want_q=True, want_k=True, want_v=True):
+    """Adjoint of ``attention``: ``(dq, dk, dv)``, None where not wanted."""
+    name = "attention_backward"
+    head_dim = q.shape[-1]
+    q, k, v, lengths, scale, dim = _attention_operands(q, k, v, lengths, scale, name)
+    batch, tokens, heads, _ = q.shape
+    keys, kv_heads = k.shape[1:3]
+    _require_gpu(dout, out, lse)
+    for t in (dout, out):
+        if t.shape[:3] != q.shape[:3] or t.shape[3] != head_dim:
+            raise ValueError(f"{name}: {tuple(t.shape)} does not fit queries {tuple(q.shape[:3]) + (head_dim,)}")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (batch, heads, tokens) or not lse.is_contiguous() or lse.device != q.device:
+        raise ValueError(f"{name}: lse must be contiguous float32 [{batch}, {heads}, {tokens}] on {q.device}")
+    lib = _lib.load()
+    with _on_device_of(q):
+        dout, out = (_aligned_heads(_heads(t, name, q), dim) for t in (dout, out))
+        grads = [torch.empty(t.shape, dtype=q.dtype, device=q.device) if want else None for t, want in ((q, want_q), (k, want_k), (v, want_v))]
+        elems = lib.ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim)
+        work = torch.empty(max(elems, 1), dtype=torch.float32, device=q.device)
+        arguments = [a for t in (dout, q, k, v, out) for a in (t.data_ptr(), _attention_strides(t))]
+        results = [a for t in grads for a in ((None, None) if t is None else (t.data_ptr(), _attention_strides(t)))]
+        rc = lib.ddl_attention_backward(*arguments, lse.data_ptr(), _LN_DTYPES[q.dtype], batch, tokens, keys, heads, kv_heads, dim, _ptr(lengths),
+                                        int(causal), scale, *results, work.data_ptr(), elems, _stream())
+        _lib.check(rc, "ddl_attention_backward")
+        if dim != head_dim:
+            grads = [None if t is None else contiguous(t[..., :head_dim]) for t in grads]
+    return tuple(grads)

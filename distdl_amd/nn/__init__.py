@@ -3,6 +3,8 @@
 
 from .all_gather import AllGather  # noqa: F401
 from .all_sum_reduce import AllSumReduce  # noqa: F401
+from .attention import DistributedAttention  # noqa: F401
+from .attention import attention_shard  # noqa: F401
 from .broadcast import Broadcast  # noqa: F401
 from .conv import DistributedConv1d  # noqa: F401
 from .conv import DistributedConv2d  # noqa: F401
@@ -32,5 +34,5 @@ __all__ = [
     "DistributedFeatureConv1d", "DistributedFeatureConv2d", "DistributedFeatureConv3d", "DistributedEmbedding",
     "HaloExchange", "DistributedLayerNorm", "DistributedLinear", "DistributedLinearAllGather", "DistributedLinearReduceScatter", "Module", "ReduceScatter",
     "Repartition", "SumReduce", "DistributedTranspose", "DistributedRotary", "DistributedHeadNormRotary", "rotary_frequencies",
-    "rotary_shard", "head_norm_rotary_shard",
+    "rotary_shard", "head_norm_rotary_shard", "DistributedAttention", "attention_shard",
 ]

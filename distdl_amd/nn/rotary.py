@@ -59,7 +59,7 @@ class _RotaryShard(torch.autograd.Function):
     def forward(ctx, q, k, frequencies, positions, interleaved, amplitude):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(frequencies, positions)
-        ctx.how, ctx.dtype = (interleaved, amplitude), q.dtype
+        ctx.how, ctx.dtype = (interleaved, amplitude), (q if q is not None else k).dtype
         return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude)
 
     @staticmethod
@@ -89,9 +89,9 @@ class _HeadNormRotaryShard(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, q_weight, k_weight, frequencies, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dyq = _as(dyq, q.dtype) if need[0] or need[2] else None
-        dyk = _as(dyk, q.dtype) if need[1] or need[3] else None
+        need, dtype = ctx.needs_input_grad, (q if q is not None else k).dtype
+        dyq = _as(dyq, dtype) if need[0] or need[2] else None
+        dyk = _as(dyk, dtype) if need[1] or need[3] else None
         if dyq is None and dyk is None:
             return (None,) * 9
         dq, dk, dqw, dkw = hip_ops.head_norm_rotary_backward(dyq, dyk, q, k, _row(q_weight), _row(k_weight), frequencies, positions, *ctx.how,
@@ -111,7 +111,7 @@ def _records(*tensors):
 def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplitude=1.0):
     """``(q, k)`` turned by their positions: pair p of a head by ``position * frequencies[p]``, with ``amplitude``.
 
-    q, k: [batch, tokens, heads, head_dim] (k may be None).  A pair is the elements p and p + len(frequencies) of a head, or
+    q, k: [batch, tokens, heads, head_dim] (either may be None).  A pair is the elements p and p + len(frequencies) of a head, or
     2 p and 2 p + 1 if ``interleaved``; elements behind the pairs stay.  ``positions``: integers, [tokens] or [batch, tokens];
     None counts from 0."""
     if _records(q, k):
@@ -122,8 +122,6 @@ def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplit
 def head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions=None, *, eps=1e-6, interleaved=False, amplitude=1.0):
     """``rotary_shard`` of heads that are divided by ``sqrt(mean of their squares + eps)`` and multiplied by their weights
     (``head_dim`` elements of the heads' type, or None) first, in the same pass."""
-    if k is None and k_weight is not None:
-        raise ValueError("head_norm_rotary_shard: weights of keys that are not there")
     if _records(q, k, q_weight, k_weight):
         return _HeadNormRotaryShard.apply(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(interleaved), float(amplitude))
     return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude, norm=True, q_weight=_row(q_weight), k_weight=_row(k_weight), eps=eps)

@@ -656,6 +656,57 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
                                   void* dk_weight, float* workspace,
                                   int64_t workspace_elems, void* stream);
 
+/* Attention of queries to keys and values of another (or the same) length:
+ *   out[i] = sum over j of p_ij v_j,   p_ij = exp(scale q_i . k_j) / sum over j
+ * over the keys j < lengths[batch] (device, int32, values outside 0 .. keys
+ * count as those; NULL: all), and with causal != 0 over those with
+ * j <= i + keys - tokens of them.  A query without keys gives zeros.  Keys and
+ * values from a sequence's length on are not read.
+ *   q, out   [batch, tokens, heads, head_dim]
+ *   k, v     [batch, keys, kv_heads, head_dim], heads a multiple of kv_heads:
+ *            head h uses key head h * kv_heads / heads
+ *   lse      [batch, heads, tokens] floats or NULL: log2 of a query's sum of
+ *            exp(scale q . k) (+inf without keys), for the adjoint
+ *   workspace  device memory of ddl_attention_workspace(...) floats, 16-byte
+ *            aligned (few queries: the keys are split over workgroups)
+ * scale > 0.  16-byte aligned tensors with strides and head_dim that are multiples
+ * of 16 bytes (DDL_E_ALIGN; zeros behind a head's elements change nothing),
+ * head_dim <= 128 (DDL_E_UNSUPP).  Probabilities are rounded to the element
+ * type for the product with the values. */
+int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys,
+                                int64_t heads, int64_t kv_heads, int64_t head_dim);
+int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                  int dtype, int64_t batch, int64_t tokens, int64_t keys,
+                  int64_t heads, int64_t kv_heads, int64_t head_dim,
+                  const int32_t* lengths, int causal, float scale, void* out,
+                  const int64_t* out_strides, float* lse, float* workspace,
+                  int64_t workspace_elems, void* stream);
+
+/* The adjoint of ddl_attention: with dS_ij = p_ij (dout_i . v_j - dout_i . out_i),
+ *   dq_i = scale sum dS_ij k_j,  dk_j = scale sum dS_ij q_i,  dv_j = sum p_ij dout_i,
+ * summed over all heads that share a key head; zeros for queries and keys that
+ * nothing is summed for.  out and lse as ddl_attention returned them; dq, dk or
+ * dv may be NULL; `workspace`: device memory of
+ * ddl_attention_backward_workspace(...) floats, 16-byte aligned.  Nothing is added
+ * atomically: equal calls give equal bits.  Probabilities and dS are rounded to
+ * the element type for their products.  Limits as ddl_attention's. */
+int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens,
+                                         int64_t keys, int64_t heads,
+                                         int64_t kv_heads, int64_t head_dim);
+int ddl_attention_backward(const void* dout, const int64_t* dout_strides,
+                           const void* q, const int64_t* q_strides, const void* k,
+                           const int64_t* k_strides, const void* v,
+                           const int64_t* v_strides, const void* out,
+                           const int64_t* out_strides, const float* lse, int dtype,
+                           int64_t batch, int64_t tokens, int64_t keys,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim,
+                           const int32_t* lengths, int causal, float scale,
+                           void* dq, const int64_t* dq_strides, void* dk,
+                           const int64_t* dk_strides, void* dv,
+                           const int64_t* dv_strides, float* workspace,
+                           int64_t workspace_elems, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -258,3 +258,23 @@ def test_layers_broadcast_their_weights_and_take_views():
     assert layer.q_weight.grad.shape == layer.q_weight.shape and layer.k_weight.grad is not None
     plain = nn.DistributedRotary(P, 32, amplitude=1.5).to(torch.float16)       # moves between types leave the angles' 64 bits
     assert torch.equal(plain(q)[0], nn.rotary_shard(q, None, nn.rotary_frequencies(32, device="cuda"), amplitude=1.5)[0])
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_keys_alone(norm):
+    from distdl_amd import nn
+    _, q, k = _case(torch.float16, 2, 9, 2, 3, 24, seed=11)
+    freq = nn.rotary_frequencies(24, device="cuda")
+    w = torch.full((24,), 1.5, dtype=torch.float16, device="cuda").requires_grad_()
+
+    def call(a, b):
+        return nn.head_norm_rotary_shard(a, b, w if a is not None else None, w, freq) if norm else nn.rotary_shard(a, b, freq)
+
+    k.requires_grad_()
+    none, alone = call(None, k)
+    _, both = call(q, k)
+    assert none is None and torch.equal(alone, both)
+    for leaf in [k] + ([w] if norm else []):
+        assert torch.equal(torch.autograd.grad(alone, [leaf], k.detach(), retain_graph=True)[0], torch.autograd.grad(both, [leaf], k.detach(), retain_graph=True)[0])
+    with pytest.raises(ValueError, match="neither"):
+        nn.rotary_shard(None, None, freq)

@@ -99,3 +99,75 @@ def test_rotation_of_the_oracle_keeps_lengths_and_turns_back():
         y = o_heads.rotate(x, f, p, interleaved)
         assert np.allclose((y * y).sum(-1), (x * x).sum(-1)) and np.array_equal(y[..., 12:], x[..., 12:])
         assert np.allclose(o_heads.rotate(y, f, p, interleaved, inverse=True), x)
+
+
+def _attention(lib, **change):
+    st = _i64(64, 64, 64)
+    a = dict(q=16, qs=st, k=16, ks=st, v=16, vs=st, dtype=_lib.DDL_DT_BF16, batch=1, tokens=1, keys=1, heads=2, kv=1, dim=64, lengths=None, causal=0,
+             scale=0.125, out=16, outs=st, lse=None, work=None, elems=0, stream=None)
+    assert set(change) <= set(a)
+    a.update(change)
+    return lib.ddl_attention(*a.values())
+
+
+ATTENTION_REFUSALS = [
+    (dict(dtype=_lib.DDL_DT_I32), -1, "dtype"), (dict(tokens=-1), -1, "negative"), (dict(dim=136), -5, "at most 128"), (dict(dim=60), -3, "16 bytes"),
+    (dict(kv=0), -4, "cannot share"), (dict(heads=3, kv=2), -4, "cannot share"), (dict(scale=0.0), -1, "positive"), (dict(scale=-1.0), -1, "positive"),
+    (dict(scale=float("nan")), -1, "positive"), (dict(scale=float("inf")), -1, "positive"), (dict(q=None), -1, "null"), (dict(v=None), -1, "null"),
+    (dict(outs=None), -1, "null"), (dict(k=8), -3, "aligned"), (dict(ks=_i64(64, 60, 64)), -3, "multiples"), (dict(ks=_i64(64, 1 << 22, 64)), -5, "2^22"),
+    (dict(vs=_i64(64, -64, 64)), -5, "2^22"), (dict(tokens=1 << 30), -5, "2^30"), (dict(keys=1 << 30), -5, "2^30"),
+]
+
+
+@pytest.mark.parametrize("change,code,what", ATTENTION_REFUSALS)
+def test_attention_refuses(change, code, what):
+    lib = _lib.load()
+    assert _attention(lib, **change) == code
+    assert what in lib.ddl_last_error().decode()
+
+
+def test_attention_of_nothing_is_no_launch():
+    lib = _lib.load()
+    assert _attention(lib, tokens=0, q=None, out=None) == 0
+    assert _attention(lib, batch=0) == 0
+
+
+def test_attention_asks_for_its_workspaces():
+    lib = _lib.load()
+    need = lib.ddl_attention_workspace(1, 1, 65536, 2, 1, 64)
+    assert need >= 2 * 2 * 64
+    assert _attention(lib, keys=65536, elems=need - 1, work=16) == -1 and "workspace" in lib.ddl_last_error().decode()
+    assert _attention(lib, keys=65536, elems=need, work=8) == -3
+    assert lib.ddl_attention_workspace(1, 4096, 4096, 64, 8, 128) == 0
+    need = lib.ddl_attention_backward_workspace(2, 5, 7, 4, 2, 64)
+    assert need >= 2 * 5 * 4
+    st = _i64(64, 64, 64)
+    call = [16, st] * 5 + [16, _lib.DDL_DT_BF16, 2, 5, 7, 4, 2, 64, None, 0, 0.125] + [16, st] * 3
+    assert lib.ddl_attention_backward(*call, 16, need - 1, None) == -1 and "workspace" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:10], None, *call[11:], 16, need, None) == -1 and "row sums" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:22], None, *call[23:], 16, need, None) == -1 and "no strides" in lib.ddl_last_error().decode()
+
+
+def test_attention_layers_and_functions_refuse():
+    from distdl_amd.backends.stub_hip import SimWorld
+    q = torch.zeros(1, 1, 2, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        nn.attention_shard(q, q, q)
+    P = SimWorld(2).partition(0).create_partition_inclusive([0, 1])
+    for shape in ([1, 2, 1, 1], [1, 1, 1, 2]):
+        with pytest.raises(ValueError, match="whole sequences"):
+            nn.DistributedAttention(P.create_cartesian_topology_partition(shape))
+    with pytest.raises(ValueError, match="positive"):
+        nn.DistributedAttention(P.create_cartesian_topology_partition([1, 1, 2, 1]), scale=-1.0)
+
+
+def test_attention_of_the_oracle_against_its_softmax():
+    rng = np.random.default_rng(1)
+    q, k, v = rng.standard_normal((1, 3, 2, 4)), rng.standard_normal((1, 5, 1, 4)), rng.standard_normal((1, 5, 1, 4))
+    out, lse = o_heads.attention(q, k, v, [4])
+    for i in range(3):
+        for h in range(2):
+            s = k[0, :4, 0] @ q[0, i, h] / 2
+            assert np.allclose(out[0, i, h], (np.exp(s)[:, None] * v[0, :4, 0]).sum(0) / np.exp(s).sum()) and np.isclose(lse[0, i, h], np.log(np.exp(s).sum()))
+    out, lse = o_heads.attention(rng.standard_normal((1, 4, 1, 4)), k[:, :2], v[:, :2], causal=True)
+    assert not out[0, :2].any() and np.isinf(lse[0, :2]).all() and np.allclose(out[0, 2], v[0, 0])
