@@ -183,14 +183,18 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     AttnStage<T, DP, KEYS, kWave> k_next, v_next;
     int t = t0 + wave;
     if (t < t1) k_next.load(k, a.k_at.token, t * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, t * KEYS, most, a.chunks, lane);
-    Frag column[Tile::kSteps];
-    const T* q = static_cast<const T*>(a.q) + batch * a.q_at.batch;
-#pragma unroll
-    for (int s = 0; s < Tile::kSteps; ++s) {
+    // The queries wait in LDS, as a tile of their own: in registers they would be an eighth of what a wavefront has.
+    char* q_tile = lds + kWaves * 2 * kTileBytes;
+    for (int i = threadIdx.x; i < kRows * Tile::kChunks; i += kThreads) {
+        const int r = i / Tile::kChunks, c = i - r * Tile::kChunks, row = first_row + r;
         Frag f = {};
-        if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
-        column[s] = f;
+        if (row < rows && c < a.chunks) {
+            const int tk = row / a.group, hd = kv_head * a.group + row - tk * a.group;
+            f = *reinterpret_cast<const Frag*>(static_cast<const T*>(a.q) + batch * a.q_at.batch + tk * a.q_at.token + hd * a.q_at.head + c * Tile::kPerChunk);
+        }
+        *reinterpret_cast<Frag*>(q_tile + r * Tile::kRowBytes + ((c ^ Tile::swizzle(r)) << 4)) = f;
     }
+    lds_barrier();
     Running<Tile::kBlocks> run;
     char *kt = lds + wave * 2 * kTileBytes, *vt = kt + kTileBytes;
     for (; t < t1; t += kWaves) {
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         floatx16 s[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
-        tile.straight(s[0], kt, 0, column);
+        tile.straight(s[0], kt, q_tile);
         const int rest = seen - t * KEYS - 4 * half;
         if ((t + 1) * KEYS > least) run.template take<1, true>(s, a.scale_log2, rest);
         else run.template take<1, false>(s, a.scale_log2, rest);
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const bool whole = a.splits == 1;
     const float factor = __builtin_amdgcn_exp2f(run.top - from) * (whole ? (total > 0.f ? 1.0f / total : 0.f) : 1.f);
     typedef AttnOut<float, DP> Out;
-    Out::park(lds + wave * Out::kRoom, run.acc, factor, lane);
+    if (my_row < rows) Out::park(lds + wave * Out::kRoom, run.acc, factor, lane);
     __syncthreads();
     const int dim = a.chunks * Tile::kPerChunk;
     float* partial = a.partial + (static_cast<int64_t>(split) * pairs + bk) * rows * (DP + 2);
@@ -254,45 +258,62 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     }
 }
 
-// The splits of a row, in their order.
+// The splits of a row, a workgroup for each row: groups of DP / 4 lanes take a share of the splits each (four of them in flight), in
+// one pass with a running maximum, and are joined in their order.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
-    constexpr int kLanes = DP / 4;      // of a row, four elements each
-    const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group;
-    const int64_t lane = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, at = lane / kLanes;
-    const int d = 4 * static_cast<int>(lane % kLanes);
-    if (at >= static_cast<int64_t>(pairs) * rows) return;
-    const int bk = static_cast<int>(at / rows), row = static_cast<int>(at - static_cast<int64_t>(bk) * rows);
-    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    constexpr int kLanes = DP == 96 ? 32 : DP / 4, kGroups = kThreads / kLanes;    // of a split's row, four elements each; rows of 96 leave 8 idle
+    __shared__ float tops[kGroups], totals[kGroups];
+    __shared__ float4 sums[kGroups][kLanes];
+    const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group, at = blockIdx.x;
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, d = 4 * lane;
     const int64_t pitch = static_cast<int64_t>(pairs) * rows * (DP + 2);
-    const float* p = a.partial + at * (DP + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * pitch + DP]);
-    const float from = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* p = a.partial + static_cast<int64_t>(at) * (DP + 2);
     const bool there = d < a.chunks * AttnElem<T>::kPerChunk;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 m = *reinterpret_cast<const float2*>(p + s * pitch + DP);
-        const float factor = __builtin_amdgcn_exp2f(m.x - from);
-        total += m.y * factor;
-        if (there) {
-            const float2 lo = *reinterpret_cast<const float2*>(p + s * pitch + d), hi = *reinterpret_cast<const float2*>(p + s * pitch + d + 2);
-            sum.x += lo.x * factor, sum.y += lo.y * factor, sum.z += hi.x * factor, sum.w += hi.y * factor;
+    float top = -INFINITY, total = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto join = [&](float2 m, float4 v) {
+        const float both = fmaxf(top, m.x), from = both == -INFINITY ? 0.f : both;
+        const float f = __builtin_amdgcn_exp2f(top - from), g = __builtin_amdgcn_exp2f(m.x - from);
+        top = both, total = total * f + m.y * g;
+        sum.x = sum.x * f + v.x * g, sum.y = sum.y * f + v.y * g, sum.z = sum.z * f + v.z * g, sum.w = sum.w * f + v.w * g;
+    };
+    for (int s0 = group; s0 < a.splits; s0 += 4 * kGroups) {
+        float2 m[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * kGroups;
+            m[i] = make_float2(-INFINITY, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (s < a.splits) {
+                m[i] = *reinterpret_cast<const float2*>(p + s * pitch + DP);
+                if (there) {
+                    const float2 lo = *reinterpret_cast<const float2*>(p + s * pitch + d), hi = *reinterpret_cast<const float2*>(p + s * pitch + d + 2);
+                    v[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+                }
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) join(m[i], v[i]);
     }
+    if (lane == 0) tops[group] = top, totals[group] = total;
+    sums[group][lane] = sum;
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < kGroups && g < a.splits; ++g) join(make_float2(tops[g], totals[g]), sums[g][lane]);
     const float inv = total > 0.f ? 1.0f / total : 0.f;
+    const int bk = at / rows, row = at - bk * rows, batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int token = row / a.group, head = kv_head * a.group + row - token * a.group;
     if (there)
         store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + token * a.out_at.token + head * a.out_at.head + d,
                           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-    if (d == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+    if (lane == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
 }
 
 template <typename T, int DP>
 constexpr int split_lds() {
     typedef AttnTile<T, DP> Tile;
-    constexpr int tiles = kWaves * 2 * 32 * Tile::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
+    constexpr int tiles = (kWaves * 2 + 1) * 32 * Tile::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
 }
 
@@ -362,8 +383,7 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
         hipLaunchKernelGGL((attention_split<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
         if (const int rc = check_launch("ddl_attention")) return rc;
         if (a.splits == 1) return 0;
-        const int64_t lanes = pairs * rows * (DP / 4);
-        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>((lanes + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>(pairs * rows)), dim3(kThreads), 0, s, a);
         return check_launch("ddl_attention");
     });
 }

@@ -297,7 +297,7 @@ int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64
     int dev;
     const int64_t units = batch * kv_heads * ((keys + kRows * kWaves - 1) / (kRows * kWaves)), tiles = heads / kv_heads * ((tokens + 31) / 32);
     int64_t splits = (2 * static_cast<int64_t>(compute_units(dev)) + units - 1) / units;
-    if (splits > tiles / 8) splits = tiles / 8;
+    if (splits > tiles / 2) splits = tiles / 2;
     return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
 }
 

@@ -117,6 +117,15 @@ struct AttnTile {
         }
     }
 
+    // The same with the columns in a tile of their own.
+    __device__ void straight(floatx16& acc, const char* tile, const char* columns) const {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int at = straight_row + (((2 * s) ^ straight_x) << 4);
+            mfma_chunk(acc, *reinterpret_cast<const Frag*>(tile + at), *reinterpret_cast<const Frag*>(columns + at), static_cast<const T*>(nullptr));
+        }
+    }
+
     // acc[d block] += tile rows 32 block .. + 31, transposed, times p of this lane's column.
     __device__ void transposed(floatx16 (&acc)[kBlocks], const char* tile, int block, const floatx16& p) const {
         const char* base = tile + block * 32 * kRowBytes + trans_row + trans_byte;

@@ -10,6 +10,10 @@
 // interpreter lock is released while a function runs.
 #include "front.h"
 
+#include <c10/hip/HIPFunctions.h>
+
+#include <cmath>
+
 namespace ddl_front {
 
 int float_code(const Tensor& t) {   // 0: none of the three
@@ -215,6 +219,160 @@ MaybeTensor embedding_backward(const Tensor& dy, const Tensor& ids, int64_t lo, 
                                  dim, work.data_ptr<int32_t>(), elems, current_stream()),
           "ddl_embedding_backward");
     return dw;
+}
+
+// ----------------------------------------------------------------- heads --
+
+namespace {
+
+// [batch, tokens, heads, head_dim] on the current device, the last dimension's elements side by side.
+bool heads_tensor(const Tensor& t, const Tensor& like) {
+    return t.is_cuda() && t.dim() == 4 && float_code(t) && t.scalar_type() == like.scalar_type() && t.device() == like.device() &&
+           t.device().index() == c10::hip::current_device() && (t.size(3) <= 1 || t.stride(3) == 1);
+}
+const int64_t* strides(const MaybeTensor& t) { return t ? t->strides().data() : nullptr; }
+int64_t heads_of(const MaybeTensor& t) { return t ? t->size(2) : 0; }
+MaybeTensor like_heads(const MaybeTensor& t) { return t ? MaybeTensor(at::empty(t->sizes(), t->options())) : std::nullopt; }
+void* target(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
+
+bool weight_of_heads(const MaybeTensor& w, const MaybeTensor& of, const Tensor& first) {
+    return !w || (of && plain(*w) && w->scalar_type() == first.scalar_type() && w->device() == first.device() && w->numel() == first.size(3));
+}
+
+// Do the operands of a rotation fit?  `first` is the one of q and k that is there.
+bool rotation_operands(const MaybeTensor& q, const MaybeTensor& k, const Rotation& r, const Tensor& first) {
+    if (!heads_tensor(first, first) || first.size(3) < 1 || (q && k && (!heads_tensor(*k, *q) || k->size(0) != q->size(0) || k->size(1) != q->size(1) || k->size(3) != q->size(3))))
+        return false;
+    const Tensor& f = r.frequencies;
+    if (!plain(f) || f.scalar_type() != at::kDouble || f.dim() != 1 || f.device() != first.device() || 2 * f.numel() > first.size(3)) return false;
+    if (!r.positions) return true;
+    const Tensor& p = *r.positions;
+    const int64_t batch = first.size(0), tokens = first.size(1);
+    return p.is_cuda() && p.device() == first.device() && (p.scalar_type() == at::kLong || p.scalar_type() == at::kInt) && p.dim() >= 1 && p.dim() <= 2 &&
+           p.size(-1) == tokens && (p.dim() == 1 || p.size(0) == 1 || p.size(0) == batch) && (tokens <= 1 || p.stride(-1) == 1);
+}
+int64_t position_pitch(const Rotation& r, const Tensor& first) {
+    return r.positions && r.positions->dim() == 2 && r.positions->size(0) == first.size(0) && first.size(0) > 1 ? r.positions->stride(0) : 0;
+}
+int position_bytes(const Rotation& r) { return r.positions ? static_cast<int>(r.positions->element_size()) : 0; }
+
+std::optional<Two> turned_heads(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight, const Rotation& r, bool norm,
+                                double eps, bool inverse) {
+    if (!q && !k) return std::nullopt;
+    const Tensor& first = q ? *q : *k;
+    if (!rotation_operands(q, k, r, first) || !weight_of_heads(q_weight, q, first) || !weight_of_heads(k_weight, k, first)) return std::nullopt;
+    const MaybeTensor yq = like_heads(q), yk = like_heads(k);
+    check(ddl_head_rotary(pointer(q), strides(q), pointer(k), strides(k), float_code(first), first.size(0), first.size(1), heads_of(q), heads_of(k), first.size(3),
+                          pointer(q_weight), pointer(k_weight), norm, static_cast<float>(eps), static_cast<const double*>(r.frequencies.data_ptr()),
+                          2 * r.frequencies.numel(), pointer(r.positions), position_bytes(r), position_pitch(r, first), r.neighbours,
+                          static_cast<float>(r.amplitude), inverse, target(yq), strides(yq), target(yk), strides(yk), current_stream()),
+          "ddl_head_rotary");
+    return Two(yq, yk);
+}
+
+}  // namespace
+
+std::optional<Two> head_rotary(const MaybeTensor& q, const MaybeTensor& k, const Rotation& r, bool inverse) {
+    return turned_heads(q, k, std::nullopt, std::nullopt, r, false, 0.0, inverse);
+}
+
+std::optional<Two> head_norm_rotary(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight, const Rotation& r, double eps) {
+    return turned_heads(q, k, q_weight, k_weight, r, true, eps, false);
+}
+
+std::optional<Four> head_norm_rotary_backward(const MaybeTensor& dyq, const MaybeTensor& dyk, const MaybeTensor& q_all, const MaybeTensor& k_all,
+                                              const MaybeTensor& q_weight_all, const MaybeTensor& k_weight_all, const Rotation& r, double eps, bool want_q_weight,
+                                              bool want_k_weight) {
+    const MaybeTensor q = dyq ? q_all : std::nullopt, k = dyk ? k_all : std::nullopt;
+    if (!q && !k) return std::nullopt;
+    const Tensor& first = q ? *q : *k;
+    const MaybeTensor q_weight = q ? q_weight_all : std::nullopt, k_weight = k ? k_weight_all : std::nullopt;
+    if (!rotation_operands(q, k, r, first) || !weight_of_heads(q_weight, q, first) || !weight_of_heads(k_weight, k, first)) return std::nullopt;
+    if ((q && (!heads_tensor(*dyq, first) || dyq->sizes() != q->sizes())) || (k && (!heads_tensor(*dyk, first) || dyk->sizes() != k->sizes()))) return std::nullopt;
+    const MaybeTensor dq = like_heads(q), dk = like_heads(k);
+    const MaybeTensor dqw = want_q_weight && q_weight ? MaybeTensor(at::empty(q_weight->sizes(), q_weight->options())) : std::nullopt;
+    const MaybeTensor dkw = want_k_weight && k_weight ? MaybeTensor(at::empty(k_weight->sizes(), k_weight->options())) : std::nullopt;
+    Tensor work;
+    const int64_t elems = dqw || dkw ? ddl_head_norm_rotary_backward_workspace(first.size(3)) : 0;
+    if (elems) work = floats(first, {elems});
+    check(ddl_head_norm_rotary_backward(pointer(dyq), strides(dyq), pointer(dyk), strides(dyk), pointer(q), strides(q), pointer(k), strides(k), float_code(first),
+                                        first.size(0), first.size(1), heads_of(q), heads_of(k), first.size(3), pointer(q_weight), pointer(k_weight),
+                                        static_cast<float>(eps), static_cast<const double*>(r.frequencies.data_ptr()), 2 * r.frequencies.numel(),
+                                        pointer(r.positions), position_bytes(r), position_pitch(r, first), r.neighbours, static_cast<float>(r.amplitude),
+                                        target(dq), strides(dq), target(dk), strides(dk), target(dqw), target(dkw), static_cast<float*>(pointer(work)), elems,
+                                        current_stream()),
+          "ddl_head_norm_rotary_backward");
+    return Four(dq, dk, dqw, dkw);
+}
+
+namespace {
+
+constexpr int64_t kMaxAttentionPitch = int64_t{1} << 22;
+
+// What ddl_attention takes as it lies.
+bool attention_tensor(const Tensor& t, const Tensor& like) {
+    const int64_t per = 16 / t.element_size();
+    if (!heads_tensor(t, like) || t.size(3) != like.size(3) || t.size(3) % per != 0 || t.size(3) < 1 || t.size(3) > 128 || !multiple(t.data_ptr(), 16)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > 1 && t.stride(i) % per != 0) return false;
+    return t.size(1) <= 1 || (t.stride(1) >= 0 && t.stride(1) < kMaxAttentionPitch);
+}
+
+struct Strides3 {   // 0 where there is one element, whatever the tensor says
+    int64_t of[3];
+    explicit Strides3(const Tensor& t) {
+        for (int i = 0; i < 3; ++i) of[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    }
+    operator const int64_t*() const { return of; }
+};
+
+bool attention_operands(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, const std::optional<double>& scale) {
+    if (q.dim() != 4 || !attention_tensor(q, q) || !attention_tensor(k, q) || !attention_tensor(v, q) || k.sizes() != v.sizes() || k.size(0) != q.size(0)) return false;
+    if (q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2) != 0 || (scale && !(*scale > 0 && *scale <= 3e38))) return false;
+    return !lengths || (plain(*lengths) && lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->device() == q.device());
+}
+float scale_of(const Tensor& q, const std::optional<double>& scale) {
+    return static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))));
+}
+const int32_t* length_pointer(const MaybeTensor& t) { return static_cast<const int32_t*>(pointer(t)); }
+
+}  // namespace
+
+std::optional<std::tuple<Tensor, Tensor>> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal,
+                                                    const std::optional<double>& scale, bool want_lse) {
+    if (!attention_operands(q, k, v, lengths, scale)) return std::nullopt;
+    const int64_t batch = q.size(0), tokens = q.size(1), keys = k.size(1), heads = q.size(2), kv_heads = k.size(2), dim = q.size(3);
+    Tensor out = at::empty(q.sizes(), q.options()), lse, work;
+    if (want_lse) lse = floats(q, {batch, heads, tokens});
+    const int64_t elems = ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim);
+    if (elems) work = floats(q, {elems});
+    check(ddl_attention(q.data_ptr(), Strides3(q), k.data_ptr(), Strides3(k), v.data_ptr(), Strides3(v), float_code(q), batch, tokens, keys, heads, kv_heads, dim,
+                        length_pointer(lengths), causal, scale_of(q, scale), out.data_ptr(), Strides3(out), static_cast<float*>(pointer(lse)),
+                        static_cast<float*>(pointer(work)), elems, current_stream()),
+          "ddl_attention");
+    return std::make_tuple(out, lse);
+}
+
+std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal,
+                                                                                   const std::optional<double>& scale, bool want_q, bool want_k, bool want_v) {
+    if (!attention_operands(q, k, v, lengths, scale) || dout.dim() != 4 || dout.sizes() != q.sizes() || out.sizes() != q.sizes() || !attention_tensor(dout, q) ||
+        !attention_tensor(out, q))
+        return std::nullopt;
+    const int64_t batch = q.size(0), tokens = q.size(1), keys = k.size(1), heads = q.size(2), kv_heads = k.size(2), dim = q.size(3);
+    if (!plain(lse) || lse.scalar_type() != at::kFloat || lse.device() != q.device() || lse.numel() != batch * heads * tokens) return std::nullopt;
+    auto result = [](const Tensor& t, bool want) { return want ? MaybeTensor(at::empty(t.sizes(), t.options())) : std::nullopt; };
+    const MaybeTensor dq = result(q, want_q), dk = result(k, want_k), dv = result(v, want_v);
+    Tensor work;
+    const int64_t elems = ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim);
+    if (elems) work = floats(q, {elems});
+    auto at_rest = [](const MaybeTensor& t, const Tensor& like) { return Strides3(t ? *t : like); };
+    check(ddl_attention_backward(dout.data_ptr(), Strides3(dout), q.data_ptr(), Strides3(q), k.data_ptr(), Strides3(k), v.data_ptr(), Strides3(v), out.data_ptr(),
+                                 Strides3(out), lse.data_ptr<float>(), float_code(q), batch, tokens, keys, heads, kv_heads, dim, length_pointer(lengths), causal,
+                                 scale_of(q, scale), target(dq), at_rest(dq, q), target(dk), at_rest(dk, k), target(dv), at_rest(dv, v),
+                                 static_cast<float*>(pointer(work)), elems, current_stream()),
+          "ddl_attention_backward");
+    return std::make_tuple(dq, dk, dv);
 }
 
 // ----------------------------------------------------------------- boxes --

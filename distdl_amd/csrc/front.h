@@ -45,6 +45,27 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> ln_backward_input_params(const
 MaybeTensor embedding_gather(const Tensor& weight, const Tensor& ids, int64_t lo, int64_t hi);
 MaybeTensor embedding_backward(const Tensor& dy, const Tensor& ids, int64_t lo, int64_t hi, int64_t padding_idx, bool by_freq);
 
+// Heads of an attention block, [batch, tokens, heads, head_dim].
+struct Rotation {
+    Tensor frequencies;
+    MaybeTensor positions;
+    bool neighbours = false;
+    double amplitude = 1.0;
+};
+typedef std::tuple<MaybeTensor, MaybeTensor> Two;
+typedef std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> Four;
+std::optional<Two> head_rotary(const MaybeTensor& q, const MaybeTensor& k, const Rotation& rotation, bool inverse);
+std::optional<Two> head_norm_rotary(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight, const Rotation& rotation,
+                                    double eps);
+std::optional<Four> head_norm_rotary_backward(const MaybeTensor& dyq, const MaybeTensor& dyk, const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight,
+                                              const MaybeTensor& k_weight, const Rotation& rotation, double eps, bool want_q_weight, bool want_k_weight);
+// The result and, if asked for, each query's sum (else undefined).
+std::optional<std::tuple<Tensor, Tensor>> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal,
+                                                    const std::optional<double>& scale, bool want_lse);
+std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal,
+                                                                                   const std::optional<double>& scale, bool want_q, bool want_k, bool want_v);
+
 // The boxes of one launch with everything but the base addresses: a call adds those
 // of the slots.  Calls only read the object.
 class Boxes {

@@ -18,6 +18,7 @@
 #include <ATen/core/PythonFallbackKernel.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -25,6 +26,7 @@
 #include <torch/csrc/dynamo/compiled_autograd.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/util/bit_cast.h>
 
 #include <atomic>
 
@@ -114,6 +116,25 @@ private:
     std::string bytes_;
 };
 
+// An adjoint of several results takes all their gradients, undefined where none came; the others take the one, zeros if there is none.
+template <typename A, typename = void>
+struct Results {
+    static constexpr int kCount = 1;
+};
+template <typename A>
+struct Results<A, std::void_t<decltype(A::kResults)>> {
+    static constexpr int kCount = A::kResults;
+};
+template <typename A>
+variable_list run_adjoint(const A& adjoint, const std::vector<Tensor>& kept, const variable_list& grads, const Asked& asked, const torch::autograd::InputMetadata& meta) {
+    if constexpr (Results<A>::kCount > 1) {
+        (void)meta;
+        return adjoint.run(kept, grads, asked);
+    } else {
+        return adjoint.run(kept, grads[0].defined() ? grads[0] : meta.zeros_like(), asked);
+    }
+}
+
 // The node of an adjoint A: `A::run(saved tensors, gradient, asked)` computes the gradients, `A::identify(key)` adds all that A
 // holds.  Unpacking runs hooks on saved tensors under the lock, as torch's nodes do; the adjoint runs without it.
 //
@@ -134,14 +155,16 @@ struct ShardNode final : Node {
         for (SavedVariable& s : saved) s.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
-        return adjoint.run(unpacked(), grads[0].defined() ? grads[0] : input_metadata(0).zeros_like(), asked());
+        return run_adjoint(adjoint, unpacked(), grads, asked(), input_metadata(0));
     }
     void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
-        const auto& meta = input_metadata(0);
         Key key;
         key(int64_t{present})(int64_t{asked().now})(int64_t{asked().ever});
-        key(static_cast<int64_t>(c10::typeMetaToScalarType(meta.dtype())))(int64_t{meta.device().index()});
-        for (const c10::SymInt& n : meta.shape_as_dim_vector()) key(n.expect_int());
+        for (uint32_t i = 0; i < num_inputs(); ++i) {
+            const auto& meta = input_metadata(i);
+            key(static_cast<int64_t>(c10::typeMetaToScalarType(meta.dtype())))(int64_t{meta.device().index()});
+            for (const c10::SymInt& n : meta.shape_as_dim_vector()) key(n.expect_int());
+        }
         adjoint.identify(key);
         args.collect(key.bytes());
         for (const SavedVariable& s : saved) args.collect(s, false);
@@ -161,7 +184,7 @@ struct ShardNode final : Node {
             std::vector<Tensor> kept(count);
             for (size_t i = 0, k = 0; i < count; ++i)
                 if (has(present, static_cast<int>(i))) kept[i] = tensors.at(k++);
-            return adjoint.run(kept, given[0].defined() ? given[0] : meta.zeros_like(), asked);
+            return run_adjoint(adjoint, kept, given, asked, meta);
         };
         const auto& compiler = compiled::getPyCompilerInterface();
         const std::string bound = compiler->bind_function(swap.get_py_compiler(), name(), std::move(call), {compiled::IValuePacker<std::vector<Tensor>>::packed_type()},
@@ -333,6 +356,151 @@ MaybeTensor embedding_shard(const Tensor& weight, const Tensor& ids, int64_t lo,
     return y;
 }
 
+// ----------------------------------------------------------------- heads --
+
+// These adjoints have no history, and say so: what a pass that records one differentiates further is an error there, not a zero.
+variable_list final_gradients(variable_list grads, const char* name) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads) {
+        if (!g.defined()) continue;
+        g = g.detach().set_requires_grad(true);
+        auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + ": trying to differentiate twice a layer whose adjoint has no derivative", 1);
+        g = (*error)({g})[0];
+    }
+    return grads;
+}
+
+variable_list gradients(std::initializer_list<MaybeTensor> grads) {
+    variable_list list;
+    for (const MaybeTensor& g : grads) list.push_back(g ? *g : Tensor());
+    return list;
+}
+
+// The gradients of two results, those that some asked input depends on.
+MaybeTensor arrived(const Tensor& grad, bool needed) { return grad.defined() && needed ? MaybeTensor(grad.detach()) : std::nullopt; }
+
+struct RotaryShard {
+    static constexpr const char* kName = "RotaryShardBackward";
+    static constexpr int kResults = 2;
+    bool neighbours = false, queries = true, keys = true;    // which of the two there are: the results are these
+    double amplitude = 1.0;
+    Shared general;
+    void identify(Key& key) const { key(int64_t{neighbours})(int64_t{queries})(int64_t{keys})(static_cast<int64_t>(c10::bit_cast<int64_t>(amplitude)))(general); }
+    variable_list run(const std::vector<Tensor>& kept, const variable_list& grads, const Asked& asked) const {
+        const MaybeTensor dyq = queries ? arrived(grads[0], has(asked.now, 0)) : std::nullopt, dyk = keys ? arrived(grads[queries ? 1 : 0], has(asked.now, 1)) : std::nullopt;
+        if (!dyq && !dyk) return {Tensor(), Tensor()};
+        const Rotation rotation{kept[0], defined(kept[1]), neighbours, amplitude};
+        std::optional<Two> res;
+        {
+            at::NoGradGuard no_grad;
+            res = head_rotary(dyq, dyk, rotation, true);
+            if (!res) res = general->call<Two>(dyq, dyk, rotation.frequencies, rotation.positions, neighbours, amplitude);
+        }
+        return final_gradients(gradients({std::get<0>(*res), std::get<1>(*res)}), kName);
+    }
+};
+
+std::optional<Two> rotary_shard(const MaybeTensor& q, const MaybeTensor& k, const Tensor& frequencies, const MaybeTensor& positions, bool neighbours, double amplitude,
+                                const Shared& general) {
+    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(frequencies) || !ordinary(positions)) return std::nullopt;
+    std::optional<Two> y;
+    {
+        at::NoGradGuard no_grad;
+        y = head_rotary(q, k, Rotation{frequencies, positions, neighbours, amplitude}, false);
+    }
+    if (!y || !at::GradMode::is_enabled() || !(wanted(q) || wanted(k))) return y;
+    auto node = make_node(RotaryShard{neighbours, q.has_value(), k.has_value(), amplitude, general}, {q, k});
+    node->save(frequencies);
+    node->save(positions ? *positions : Tensor());
+    if (q) torch::autograd::create_gradient_edge(*std::get<0>(*y), node);
+    if (k) torch::autograd::create_gradient_edge(*std::get<1>(*y), node);
+    return y;
+}
+
+struct HeadNormRotaryShard {
+    static constexpr const char* kName = "HeadNormRotaryShardBackward";
+    static constexpr int kResults = 2;
+    bool neighbours = false;
+    double amplitude = 1.0, eps = 0.0;
+    Shared general;
+    void identify(Key& key) const { key(int64_t{neighbours})(c10::bit_cast<int64_t>(amplitude))(c10::bit_cast<int64_t>(eps))(general); }
+    variable_list run(const std::vector<Tensor>& kept, const variable_list& grads, const Asked& asked) const {
+        const MaybeTensor q = defined(kept[0]), k = defined(kept[1]), q_weight = defined(kept[2]), k_weight = defined(kept[3]);
+        const MaybeTensor dyq = q ? arrived(grads[0], has(asked.now, 0) || has(asked.now, 2)) : std::nullopt;
+        const MaybeTensor dyk = k ? arrived(grads[q ? 1 : 0], has(asked.now, 1) || has(asked.now, 3)) : std::nullopt;
+        if (!dyq && !dyk) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const Rotation rotation{kept[4], defined(kept[5]), neighbours, amplitude};
+        const bool want_qw = has(asked.now, 2), want_kw = has(asked.now, 3);
+        std::optional<Four> res;
+        {
+            at::NoGradGuard no_grad;
+            res = head_norm_rotary_backward(dyq, dyk, q, k, q_weight, k_weight, rotation, eps, want_qw, want_kw);
+            if (!res) res = general->call<Four>(dyq, dyk, q, k, q_weight, k_weight, rotation.frequencies, rotation.positions, neighbours, amplitude, eps, want_qw, want_kw);
+        }
+        const MaybeTensor none;
+        return final_gradients(gradients({has(asked.now, 0) ? std::get<0>(*res) : none, has(asked.now, 1) ? std::get<1>(*res) : none, std::get<2>(*res), std::get<3>(*res)}),
+                               kName);
+    }
+};
+
+std::optional<Two> head_norm_rotary_shard(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight, const Tensor& frequencies,
+                                          const MaybeTensor& positions, double eps, bool neighbours, double amplitude, const Shared& general) {
+    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(q_weight) || !ordinary(k_weight) || !ordinary(frequencies) || !ordinary(positions)) return std::nullopt;
+    std::optional<Two> y;
+    {
+        at::NoGradGuard no_grad;
+        y = head_norm_rotary(q, k, q_weight, k_weight, Rotation{frequencies, positions, neighbours, amplitude}, eps);
+    }
+    if (!y || !at::GradMode::is_enabled() || !(wanted(q) || wanted(k) || wanted(q_weight) || wanted(k_weight))) return y;
+    auto node = make_node(HeadNormRotaryShard{neighbours, amplitude, eps, general}, {q, k, q_weight, k_weight});
+    for (const MaybeTensor& t : {q, k, q_weight, k_weight, MaybeTensor(frequencies), positions}) node->save(t ? *t : Tensor());
+    if (q) torch::autograd::create_gradient_edge(*std::get<0>(*y), node);
+    if (k) torch::autograd::create_gradient_edge(*std::get<1>(*y), node);
+    return y;
+}
+
+struct AttentionShard {
+    static constexpr const char* kName = "AttentionShardBackward";
+    bool causal = false;
+    std::optional<double> scale;
+    Shared general;
+    void identify(Key& key) const { key(int64_t{causal})(int64_t{scale.has_value()})(c10::bit_cast<int64_t>(scale.value_or(0.0)))(general); }
+    variable_list run(const std::vector<Tensor>& kept, const Tensor& dy_given, const Asked& asked) const {
+        const Tensor dy = dy_given.detach();
+        const MaybeTensor lengths = defined(kept[5]);
+        const bool need_q = has(asked.now, 0), need_k = has(asked.now, 1), need_v = has(asked.now, 2);
+        std::optional<Three> res;
+        {
+            at::NoGradGuard no_grad;
+            res = attention_backward(dy, kept[0], kept[1], kept[2], kept[3], kept[4], lengths, causal, scale, need_q, need_k, need_v);
+            if (!res) res = general->call<Three>(dy, kept[0], kept[1], kept[2], kept[3], kept[4], lengths, causal, scale, need_q, need_k, need_v);
+        }
+        return final_gradients(listed(*res), kName);
+    }
+};
+
+MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, std::optional<double> scale, const Shared& general) {
+    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(v) || !ordinary(lengths)) return std::nullopt;
+    const bool graph = at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v));
+    std::optional<std::tuple<Tensor, Tensor>> res;
+    {
+        at::NoGradGuard no_grad;
+        res = attention(q, k, v, lengths, causal, scale, graph);
+    }
+    if (!res) return std::nullopt;
+    Tensor out = std::get<0>(*res);
+    if (!graph) return out;
+    auto node = make_node(AttentionShard{causal, scale, general}, {q, k, v});
+    node->save(q);
+    node->save(k);
+    node->save(v);
+    node->save(out.detach());      // the same memory and version, without this node
+    node->save(std::get<1>(*res));
+    node->save(lengths ? *lengths : Tensor());
+    torch::autograd::create_gradient_edge(out, node);
+    return out;
+}
+
 // ----------------------------------------------------------------- moves --
 
 // Pooled communication buffers that have been reallocated since this extension was loaded.
@@ -458,6 +626,9 @@ void define_nodes(py::module_& m) {
     m.def("layer_norm_shard", &layer_norm_shard, unlocked());
     m.def("layer_norm_node", &layer_norm_node, unlocked());
     m.def("embedding_shard", &embedding_shard, unlocked());
+    m.def("rotary_shard", &rotary_shard, unlocked());
+    m.def("head_norm_rotary_shard", &head_norm_rotary_shard, unlocked());
+    m.def("attention_shard", &attention_shard, unlocked());
     m.def("move", &move, unlocked());
     m.def("alias", &alias, unlocked());
     m.def("attachable", &attachable);

@@ -1243,10 +1243,11 @@ def head_norm_rotary_backward(dyq, dyk, q, k, q_weight, k_weight, frequencies, p
 
 
 def _aligned_heads(t, dim):
-    """``t`` as the attention kernels take it: 16-byte aligned rows of ``dim`` elements, a multiple of 16 bytes; else a copy, with zeros behind
-    the head's own elements."""
+    """``t`` as the attention kernels take it: 16-byte aligned rows of ``dim`` elements, a multiple of 16 bytes, less than 2^22 elements
+    apart; else a copy, with zeros behind the head's own elements."""
     per = 16 // t.element_size()
-    if t.shape[3] == dim and t.data_ptr() % 16 == 0 and all(s % per == 0 or n <= 1 for s, n in zip(t.stride()[:3], t.shape[:3])):
+    if t.shape[3] == dim and t.data_ptr() % 16 == 0 and all(s % per == 0 or n <= 1 for s, n in zip(t.stride()[:3], t.shape[:3])) and \
+       (t.shape[1] <= 1 or t.stride(1) < 1 << 22):
         return t
     if t.shape[3] == dim:
         out = torch.empty(t.shape, dtype=t.dtype, device=t.device)

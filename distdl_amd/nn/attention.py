@@ -7,6 +7,7 @@ float32, bfloat16 and float16, forward and backward; scores, softmax statistics 
 
 import torch
 
+from .. import _lib
 from .. import hip_ops
 from .module import Module
 
@@ -30,6 +31,11 @@ class _AttentionShard(torch.autograd.Function):
         return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, *ctx.how, *ctx.needs_input_grad[:3]) + (None, None, None)
 
 
+def _general_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v):
+    """The adjoint for what its native form does not take."""
+    return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v)
+
+
 def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None):
     """``softmax(scale q k^T) v`` for each head.
 
@@ -38,6 +44,9 @@ def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None):
     (None: all); what lies behind them is not read and gets zero gradients.  ``causal``: query i sees keys up to
     ``i + keys - tokens``, so the last query sees all.  A query that sees no key gives zeros.  ``scale`` defaults to
     ``head_dim ** -0.5`` and has to be positive."""
+    out = _lib.front().attention_shard(q, k, v, lengths, causal, scale, _lib.callback(_general_backward))
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionShard.apply(q, k, v, lengths, bool(causal), scale)
     return hip_ops.attention(q, k, v, lengths, causal, scale)

@@ -11,6 +11,7 @@ import math
 
 import torch
 
+from .. import _lib
 from .. import hip_ops
 from ..utilities.slicing import worker_layout
 from ..utilities.torch import zero_volume_tensor
@@ -100,6 +101,17 @@ class _HeadNormRotaryShard(torch.autograd.Function):
                 None if dkw is None else dkw.view(k_weight.shape), None, None, None, None, None)
 
 
+def _general_rotary_backward(dyq, dyk, frequencies, positions, interleaved, amplitude):
+    """The adjoint for what its native form does not take."""
+    return hip_ops.head_rotary(dyq, dyk, frequencies, positions, interleaved, amplitude, inverse=True)
+
+
+def _general_head_norm_backward(dyq, dyk, q, k, q_weight, k_weight, frequencies, positions, interleaved, amplitude, eps, want_q_weight, want_k_weight):
+    dq, dk, dqw, dkw = hip_ops.head_norm_rotary_backward(dyq, dyk, q, k, _row(q_weight), _row(k_weight), frequencies, positions, interleaved, amplitude,
+                                                         eps, want_q_weight, want_k_weight)
+    return dq, dk, None if dqw is None else dqw.view(q_weight.shape), None if dkw is None else dkw.view(k_weight.shape)
+
+
 def _row(weight):
     return None if weight is None else weight.detach().reshape(-1)
 
@@ -114,6 +126,9 @@ def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplit
     q, k: [batch, tokens, heads, head_dim] (either may be None).  A pair is the elements p and p + len(frequencies) of a head, or
     2 p and 2 p + 1 if ``interleaved``; elements behind the pairs stay.  ``positions``: integers, [tokens] or [batch, tokens];
     None counts from 0."""
+    res = _lib.front().rotary_shard(q, k, frequencies, positions, interleaved, amplitude, _lib.callback(_general_rotary_backward))
+    if res is not None:
+        return res
     if _records(q, k):
         return _RotaryShard.apply(q, k, frequencies, positions, bool(interleaved), float(amplitude))
     return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude)
@@ -122,6 +137,10 @@ def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplit
 def head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions=None, *, eps=1e-6, interleaved=False, amplitude=1.0):
     """``rotary_shard`` of heads that are divided by ``sqrt(mean of their squares + eps)`` and multiplied by their weights
     (``head_dim`` elements of the heads' type, or None) first, in the same pass."""
+    res = _lib.front().head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions, eps, interleaved, amplitude,
+                                              _lib.callback(_general_head_norm_backward))
+    if res is not None:
+        return res
     if _records(q, k, q_weight, k_weight):
         return _HeadNormRotaryShard.apply(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(interleaved), float(amplitude))
     return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude, norm=True, q_weight=_row(q_weight), k_weight=_row(k_weight), eps=eps)
