@@ -11,6 +11,8 @@
 
 #include "attention_parts.h"
 
+#include <utility>
+
 namespace ddl {
 namespace {
 
@@ -28,53 +30,59 @@ struct Running {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     }
-    // Scores to probabilities relative to `top`, which follows the scores.  `rest`: rows of the first block that this lane's
-    // column sees, from this lane's half's first one on; MASKED: they may end here.
-    template <int NS, bool MASKED>
-    __device__ void take(floatx16 (&s)[NS], float scale, int rest) {
-        if (MASKED) {
+    // The maximum follows the scores of 32 keys, which this looks at: only where it lags by a factor of 2^8, since the sums have room for that
+    // and most blocks then leave them alone, and to a whole power of two, so that what has been summed (and `before`, what waits to
+    // be) moves without a rounding.
+    template <typename Tile>
+    __device__ void follow(const floatx16& s, float scale, const Tile&, typename Tile::Packed* before) {
+        float m = fmaxf(s[0], s[1]);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (32 * n + (r & 3) + 8 * (r >> 2) >= rest) s[n][r] = -INFINITY;
-        }
-        float m = s[0][0];
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][r]);
+        for (int r = 2; r < 16; ++r) m = fmaxf(m, s[r]);
         m = max_halves(m) * scale;
-        // Moved only where it lags by a factor of 2^8: the sums have room for that, and most tiles leave them alone.
         if (__any(m > top + kSlack)) {
-            const float moved = fmaxf(top, m), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
+            const float moved = fmaxf(top, ceilf(m)), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
             top = moved;
             total *= factor;
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= factor;
+            if (before) Tile::scale_packed(*before, factor);
         }
-        const float from = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
+    }
+    __device__ float from() const { return top == -INFINITY ? 0.f : top; }
+    // Scores to probabilities relative to the maximum, packed and added to the total.
+    template <typename Tile>
+    __device__ typename Tile::Packed take(floatx16& s, float scale, const Tile&) {
+        const float base = from();
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], scale, -from));
-                sum += s[n][r];
-            }
-        total += sum;
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
+        const typename Tile::Packed p = Tile::pack(s);
+        total = Tile::add_packed(total, p);
+        return p;
     }
 };
+
+// `rest`: keys of these 32 that this lane's column sees, from this lane's half's first one on.
+__device__ inline void mask_scores(floatx16& s, int rest) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if ((r & 3) + 8 * (r >> 2) >= rest) s[r] = -INFINITY;
+}
 
 template <typename T>
 constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
 
-// One wavefront, 32 queries of one head; a workgroup, 128 of them, walks over the keys tile by tile through LDS, two tiles deep,
-// the tile after the next in registers on its way.
+// One wavefront, 32 queries of one head; a workgroup, 128 of them, walks over the keys tile by tile through LDS, each tile on its way from
+// memory while those before are worked on.
+//
+// Steps of 32 keys.  Step s has three parts that do not wait for each other, so that the matrix cores and the vector
+// units both have work: the scores of block s + 1, the softmax of block s, and the product of block s - 1 with its values.
+// With tiles of NS blocks, keys are read up to one block before and values one block after the softmax: one barrier a tile, in
+// front of its last block, is then enough for two buffers of each.  What follows it is copied to where
+// everybody has just finished reading: keys two tiles ahead, values NS - 1 blocks ahead.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 2) void attention_rows(const AttnArgs a) {
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
     constexpr int KEYS = keys_of_tile<T>(), NS = KEYS / 32, kTileBytes = KEYS * Tile::kRowBytes;
@@ -84,17 +92,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(const AttnArgs a) 
     block_of(blockIdx.x, a.batch * a.heads, a.blocks, bh, block);     // the last rows, which see most keys in the causal form, first
     const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
     const int length = sequence_keys(a, batch);
-    const int first_row = block * kRows * kWaves, my_row = first_row + wave * kRows + (lane & 31);
+    const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
     const int seen = keys_seen(a, my_row, length);
-    const int end = keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length);            // most that a row of the workgroup sees
-    const int wave_most = keys_seen(a, min(first_row + (wave + 1) * kRows, a.tokens) - 1, length);  // rows of a wavefront: most,
-    const int wave_least = first_row + wave * kRows < a.tokens ? keys_seen(a, first_row + wave * kRows, length) : 0;   // and least
-    const bool wave_has_rows = first_row + wave * kRows < a.tokens;
+    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int end = scalar(keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length));    // most that a row of the workgroup sees
+    const int wave_most = scalar(wave_row < a.tokens ? keys_seen(a, min(wave_row + kRows, a.tokens) - 1, length) : 0);   // rows of a wavefront: most,
+    const int wave_least = scalar(keys_seen(a, wave_row, length));                                  // and least
     const T* q = static_cast<const T*>(a.q) + batch * a.q_at.batch + head * a.q_at.head;
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
 
-    const Tile tile(lane);
+    const Tile tile(lds, lane);
+    const int tiles = (end + KEYS - 1) / KEYS, steps = (wave_most + 31) / 32;
+    constexpr int kPhases = 2 * NS;      // steps after which the tiles' places come again
+    auto k_tile = [](int t) { return (t & 1) * kTileBytes; };
+    auto v_tile = [](int t) { return (2 + (t & 1)) * kTileBytes; };
+    auto k_block = [&](int s) { return k_tile(s / NS) + s % NS * (32 * Tile::kRowBytes); };
+    auto v_block = [&](int s) { return v_tile(s / NS) + s % NS * (32 * Tile::kRowBytes); };
+    const AttnCopy<T, DP, KEYS, kWaves> k_copy(k, a.k_at.token, a.chunks, wave, lane), v_copy(v, a.v_at.token, a.chunks, wave, lane);
+    k_copy.request(lds + k_tile(0), 0, end), k_copy.request(lds + k_tile(1), KEYS, end);
+    if (NS > 1) v_copy.request(lds + v_tile(0), 0, end);
     Frag column[Tile::kSteps];
 #pragma unroll
     for (int s = 0; s < Tile::kSteps; ++s) {
@@ -102,38 +119,113 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(const AttnArgs a) 
         if (my_row < a.tokens && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + my_row * a.q_at.token + (2 * s + half) * Tile::kPerChunk);
         column[s] = f;
     }
-    Running<Tile::kBlocks> run;
-    const int tiles = (end + KEYS - 1) / KEYS;
-    AttnStage<T, DP, KEYS, kThreads> k_next, v_next;
-    if (tiles > 0) {
-        k_next.load(k, a.k_at.token, 0, end, a.chunks, tid), v_next.load(v, a.v_at.token, 0, end, a.chunks, tid);
-        k_next.store(lds, tid), v_next.store(lds + 2 * kTileBytes, tid);
-        if (tiles > 1) k_next.load(k, a.k_at.token, KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, KEYS, end, a.chunks, tid);
-    }
+    wait_for_copies();
     lds_barrier();
-    for (int t = 0; t < tiles; ++t) {
-        const char *kt = lds + (t & 1) * kTileBytes, *vt = kt + 2 * kTileBytes;
-        if (t + 1 < tiles) {
-            char* to = lds + ((t + 1) & 1) * kTileBytes;
-            k_next.store(to, tid), v_next.store(to + 2 * kTileBytes, tid);
-            if (t + 2 < tiles) k_next.load(k, a.k_at.token, (t + 2) * KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, (t + 2) * KEYS, end, a.chunks, tid);
-        }
-        if (wave_has_rows && t * KEYS < wave_most) {
-            floatx16 s[NS];
+    Running<Tile::kBlocks> run;
+    floatx16 scores;
+    typename Tile::Packed before;
+    auto score = [&](floatx16& to, int s) {
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
+        for (int r = 0; r < 16; ++r) to[r] = 0.f;
+        tile.straight(to, k_block(s), 0, column);
+    };
+    auto values = [&](int s) { tile.transposed(run.acc, v_block(s), 0, before); };
+    auto step = [&](int s, auto ahead, auto behind) {
+        if (32 * (s + 1) > wave_least) mask_scores(scores, seen - 32 * s - 4 * half);
+        run.follow(scores, a.scale_log2, tile, behind ? &before : nullptr);
+        floatx16 next;
+        if constexpr (ahead) score(next, s + 1);
+        if constexpr (behind) values(s - 1);
+        before = run.take(scores, a.scale_log2, tile);
+        if constexpr (ahead) scores = next;
+    };
+    // The same in full, 16-bit types: after every matrix instruction (32 cycles) an LDS read for the one after the next two and a share of the
+    // sixteen exponentials, in this order -- left to itself the compiler puts one part behind the other.  `phase`: s modulo kPhases.
+    auto full_step = [&](int s, auto phase) {
+        if (32 * (s + 1) > wave_least) mask_scores(scores, seen - 32 * s - 4 * half);
+        run.follow(scores, a.scale_log2, tile, &before);
+        if constexpr (sizeof(T) == 2) {
+            constexpr int kPhase = decltype(phase)::value, kSlots = 2 * Tile::kSteps;
+            const uint32_t kb = k_block((kPhase + 1) % kPhases), vb = v_block((kPhase + kPhases - 1) % kPhases);
+            const float base = run.from();
+            floatx16 next;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-                tile.straight(s[n], kt, n, column);
+            for (int r = 0; r < 16; ++r) next[r] = 0.f;
+            Frag kf[Tile::kSteps], vf[Tile::kSteps];
+            auto read = [&](int i) {
+                if (i >= Tile::kSteps) return;
+                kf[i] = tile.read_straight(kb, i), vf[i] = tile.read_transposed(vb, i / Tile::kBlocks, i % Tile::kBlocks);
+            };
+            auto share = [&](int slot) {
+#pragma unroll
+                for (int r = 16 * slot / kSlots; r < 16 * (slot + 1) / kSlots; ++r) {
+                    scores[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], a.scale_log2, -base));
+                    asm volatile("" : "+v"(scores[r]));      // here and not where it is used
+                }
+            };
+            read(0), read(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < Tile::kSteps; ++i) {
+                mfma_chunk(next, kf[i], column[i], static_cast<const T*>(nullptr));
+                if (i + 2 < Tile::kSteps) kf[i + 2] = tile.read_straight(kb, i + 2);
+                share(2 * i);
+                __builtin_amdgcn_sched_barrier(0);
+                mfma_chunk(run.acc[i % Tile::kBlocks], vf[i], i / Tile::kBlocks ? before.hi : before.lo, static_cast<const T*>(nullptr));
+                if (i + 2 < Tile::kSteps) vf[i + 2] = tile.read_transposed(vb, (i + 2) / Tile::kBlocks, (i + 2) % Tile::kBlocks);
+                share(2 * i + 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const int rest = seen - t * KEYS - 4 * half;
-            if ((t + 1) * KEYS > wave_least) run.template take<NS, true>(s, a.scale_log2, rest);
-            else run.template take<NS, false>(s, a.scale_log2, rest);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) tile.transposed(run.acc, vt, n, s[n]);
+            before = Tile::pack(scores);
+            run.total = Tile::add_packed(run.total, before);
+            scores = next;
+        } else {
+            floatx16 next;
+            score(next, s + 1);
+            values(s - 1);
+            before = run.take(scores, a.scale_log2, tile);
+            scores = next;
         }
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    auto turn = [&](int s) {
+        if (s % NS != NS - 1) return;
+        wait_for_copies();
         lds_barrier();
+        const int kt = s / NS + 2, vt = (s + NS - 1) / NS;
+        k_copy.request(lds + k_tile(kt), kt * KEYS, end), v_copy.request(lds + v_tile(vt), vt * KEYS, end);
+    };
+    int s = 0;      // (a wavefront whose rows see fewer keys than others' still takes its part in the copies and barriers)
+    if (steps > 0) {
+        score(scores, 0);
+        turn(0);
+        if (steps == 1) {
+            step(0, no, no);
+        } else {
+            step(0, yes, no);
+            for (s = 1; s + kPhases < steps; s += kPhases) {      // always from phase 1 on
+                turn(s), full_step(s, std::integral_constant<int, 1>{});
+                if constexpr (NS == 2) {
+                    turn(s + 1), full_step(s + 1, std::integral_constant<int, 2>{});
+                    turn(s + 2), full_step(s + 2, std::integral_constant<int, 3>{});
+                }
+                turn(s + kPhases - 1), full_step(s + kPhases - 1, std::integral_constant<int, 0>{});
+            }
+            for (; s + 1 < steps; ++s) {
+                turn(s);
+                step(s, yes, yes);
+            }
+            turn(s);
+            step(s, no, yes);
+        }
+        turn(++s);
+        values(s - 1);
+        ++s;
     }
+    for (; s <= tiles * NS; ++s) turn(s);
+    wait_for_copies();
+    lds_barrier();
     const float total = add_halves(run.total);
     if (a.lse && half == 0 && my_row < a.tokens)
         a.lse[static_cast<int64_t>(bh) * a.tokens + my_row] = total > 0.f ? run.top + __builtin_amdgcn_logf(total) : INFINITY;
@@ -179,7 +271,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
-    const Tile tile(lane);
+    const Tile tile(lds, lane);
     AttnStage<T, DP, KEYS, kWave> k_next, v_next;
     int t = t0 + wave;
     if (t < t1) k_next.load(k, a.k_at.token, t * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, t * KEYS, most, a.chunks, lane);
@@ -196,19 +288,18 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     }
     lds_barrier();
     Running<Tile::kBlocks> run;
-    char *kt = lds + wave * 2 * kTileBytes, *vt = kt + kTileBytes;
+    const int kt = wave * 2 * kTileBytes, vt = kt + kTileBytes;
     for (; t < t1; t += kWaves) {
-        k_next.store(kt, lane), v_next.store(vt, lane);
+        k_next.store(lds + kt, lane), v_next.store(lds + vt, lane);
         if (t + kWaves < t1) k_next.load(k, a.k_at.token, (t + kWaves) * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, (t + kWaves) * KEYS, most, a.chunks, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        floatx16 s[1];
+        floatx16 s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
-        tile.straight(s[0], kt, q_tile);
-        const int rest = seen - t * KEYS - 4 * half;
-        if ((t + 1) * KEYS > least) run.template take<1, true>(s, a.scale_log2, rest);
-        else run.template take<1, false>(s, a.scale_log2, rest);
-        tile.transposed(run.acc, vt, 0, s[0]);
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        tile.straight(s, kt, static_cast<uint32_t>(q_tile - lds));
+        if ((t + 1) * KEYS > least) mask_scores(s, seen - t * KEYS - 4 * half);
+        run.follow(s, a.scale_log2, tile, nullptr);
+        tile.transposed(run.acc, vt, 0, run.take(s, a.scale_log2, tile));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     // Joined: every wavefront's maximum and total, then its sums relative to the common maximum, added in the wavefronts' order.

@@ -63,15 +63,20 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
     const bool mine = my_row < a.tokens;
     const int seen = keys_seen(a, my_row, length);
-    const int end = keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length);
-    const int wave_most = wave_row < a.tokens ? keys_seen(a, min(wave_row + kRows, a.tokens) - 1, length) : 0;
-    const int wave_least = keys_seen(a, wave_row, length);
+    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int end = scalar(keys_seen(a, min(first_row + kRows * kWaves, a.tokens) - 1, length));
+    const int wave_most = scalar(wave_row < a.tokens ? keys_seen(a, min(wave_row + kRows, a.tokens) - 1, length) : 0);
+    const int wave_least = scalar(keys_seen(a, wave_row, length));
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
-    const Tile tile(lane);
+    const Tile tile(lds, lane);
     const int tiles = (end + KEYS - 1) / KEYS;
-    AttnStage<T, DP, KEYS, kThreads> k_next, v_next;
-    if (tiles > 0) k_next.load(k, a.k_at.token, 0, end, a.chunks, tid), v_next.load(v, a.v_at.token, 0, end, a.chunks, tid);
+    const AttnCopy<T, DP, KEYS, kWaves> k_copy(k, a.k_at.token, a.chunks, wave, lane), v_copy(v, a.v_at.token, a.chunks, wave, lane);
+    auto request = [&](int t) {
+        const char* to = lds + (t & 1) * kTileBytes;
+        k_copy.request(to, t * KEYS, end), v_copy.request(to + 2 * kTileBytes, t * KEYS, end);
+    };
+    if (a.dq) request(0);
     Frag q_column[Tile::kSteps], g_column[Tile::kSteps];
     load_column<T, DP>(q_column, static_cast<const T*>(a.q) + batch * a.q_at.batch + my_row * a.q_at.token + head * a.q_at.head, mine, a.chunks, half);
     load_column<T, DP>(g_column, static_cast<const T*>(a.dout) + batch * a.dout_at.batch + my_row * a.dout_at.token + head * a.dout_at.head, mine, a.chunks, half);
@@ -91,18 +96,11 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     if (!a.dq) return;      // D alone
     floatx16 acc[Tile::kBlocks];
     clear(acc);
-    if (tiles > 0) {
-        k_next.store(lds, tid), v_next.store(lds + 2 * kTileBytes, tid);
-        if (tiles > 1) k_next.load(k, a.k_at.token, KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, KEYS, end, a.chunks, tid);
-    }
-    lds_barrier();
     for (int t = 0; t < tiles; ++t) {
-        const char *kt = lds + (t & 1) * kTileBytes, *vt = kt + 2 * kTileBytes;
-        if (t + 1 < tiles) {
-            char* to = lds + ((t + 1) & 1) * kTileBytes;
-            k_next.store(to, tid), v_next.store(to + 2 * kTileBytes, tid);
-            if (t + 2 < tiles) k_next.load(k, a.k_at.token, (t + 2) * KEYS, end, a.chunks, tid), v_next.load(v, a.v_at.token, (t + 2) * KEYS, end, a.chunks, tid);
-        }
+        wait_for_copies();
+        lds_barrier();
+        request(t + 1);
+        const int kt = (t & 1) * kTileBytes, vt = kt + 2 * kTileBytes;
         if (t * KEYS < wave_most) {
             const bool masked = (t + 1) * KEYS > wave_least;
             const int rest = seen - t * KEYS - 4 * half;
@@ -118,11 +116,12 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
                     if (masked) p = 32 * n + (r & 3) + 8 * (r >> 2) < rest ? p : 0.f;
                     s[0][r] = p * (s[1][r] - delta);
                 }
-                tile.transposed(acc, kt, n, s[0]);
+                tile.transposed(acc, kt, n, Tile::pack(s[0]));
             }
         }
-        lds_barrier();
     }
+    wait_for_copies();
+    lds_barrier();
     typedef AttnOut<T, DP> Out;
     char* room = lds + wave * Out::kRoom;
     Out::park(room, acc, a.scale, lane);
@@ -136,13 +135,24 @@ constexpr int query_tile() { return AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32;
 
 // dk and dv of 32 keys a wavefront, 128 a workgroup; 32 or 64 queries of one head at a time through LDS, with their sums and D.  Where
 // there are few blocks of keys, `splits` workgroups share the queries of one and leave sums in fp32.
+//
+// 16-bit rows of more than 128 bytes: keys and values, both sums and both products of a step are more than the 256 registers with which
+// two wavefronts fit on a SIMD, and one alone leaves the matrix cores idle while it forms probabilities.  There a second set of four
+// wavefronts takes half of the work: the first four keep dk, the others dv, and both form the probabilities, five
+// products instead of four.  ([4,4096,16,128] bf16, both sums in one wavefront: 2460 us.)
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attention_backward_keys(const AttnArgs a) {
+constexpr bool two_roles() { return sizeof(T) == 2 && DP > 64; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!two_roles<T, DP>() && DP * sizeof(T) > 128 ? 1 : 2)) void attention_backward_keys(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
-    constexpr int ROWS = query_tile<T, DP>(), NS = ROWS / 32, kTileBytes = ROWS * Tile::kRowBytes, kSetBytes = 2 * kTileBytes + 2 * ROWS * 4;
+    constexpr bool ROLES = two_roles<T, DP>();
+    constexpr int WAVES = ROLES ? 2 * kWaves : kWaves, ROWS = query_tile<T, DP>(), NS = ROWS / 32;
+    constexpr int kTileBytes = ROWS * Tile::kRowBytes, kSetBytes = 2 * kTileBytes + 2 * ROWS * 4;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    const bool for_k = !ROLES || wave < kWaves, for_v = !ROLES || wave >= kWaves;
     const int pairs = a.batch * a.kv_heads;
     int bk, unit;
     block_of(blockIdx.x, pairs, a.blocks * a.splits, bk, unit);
@@ -150,88 +160,112 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
     const int block = unit / a.splits, split = unit - block * a.splits;
     const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
-    const int first_key = block * kRows * kWaves, wave_key = first_key + wave * kRows, my_key = wave_key + (lane & 31);
+    const int first_key = block * kRows * kWaves, wave_key = first_key + wave % kWaves * kRows, my_key = wave_key + (lane & 31);
     // Query i sees key j from i = j - shift on.
     const int shift = a.causal ? a.keys - a.tokens : 0x3FFFFFFF;
     const int need = my_key < length ? max(my_key - shift, 0) : 0x7FFFFFFF;      // first query that sees this lane's key
-    const int block_need = first_key < length ? max(first_key - shift, 0) : a.tokens;
-    const int wave_need = wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF;
-    const int wave_all = wave_key + kRows <= length ? max(wave_key + kRows - 1 - shift, 0) : 0x7FFFFFFF;   // from here on queries see all of the wavefront's keys
+    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int block_need = scalar(first_key < length ? max(first_key - shift, 0) : a.tokens);
+    const int wave_need = scalar(wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF);
+    const int wave_all = scalar(wave_key + kRows <= length ? max(wave_key + kRows - 1 - shift, 0) : 0x7FFFFFFF);   // from here on queries see all of the wavefront's keys
     const int first_tile = min(block_need, a.tokens) / ROWS, head_tiles = block_need < a.tokens ? (a.tokens + ROWS - 1) / ROWS - first_tile : 0;
     const int64_t all = static_cast<int64_t>(head_tiles) * a.group;
     const int it0 = static_cast<int>(all * split / a.splits), it1 = static_cast<int>(all * (split + 1) / a.splits);
     const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
     const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
     const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
-    const Tile tile(lane);
-    AttnStage<T, DP, ROWS, kThreads> q_next, g_next;
-    float row_next = 0.f;
-    auto load = [&](int it) {
-        const int in_group = it / head_tiles, first = (first_tile + it - in_group * head_tiles) * ROWS;
-        q_next.load(q0 + in_group * a.q_at.head, a.q_at.token, first, a.tokens, a.chunks, tid);
-        g_next.load(g0 + in_group * a.dout_at.head, a.dout_at.token, first, a.tokens, a.chunks, tid);
-        if (tid < 2 * ROWS) {
-            const int row = first + (tid & (ROWS - 1));
-            const int64_t at = row0 + static_cast<int64_t>(in_group) * a.tokens + row;
-            row_next = tid < ROWS ? (row < a.tokens ? a.lse[at] : INFINITY) : (row < a.tokens ? a.delta[at] : 0.f);
-        }
+    const Tile tile(lds, lane);
+    AttnCopy<T, DP, ROWS, WAVES> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
+    // Where an iteration's queries are: the head of the group and its first query.
+    struct At {
+        int head, tile;
     };
-    auto store = [&](char* set) {
-        q_next.store(set, tid), g_next.store(set + kTileBytes, tid);
-        if (tid < 2 * ROWS) reinterpret_cast<float*>(set + 2 * kTileBytes)[tid] = row_next;
+    auto after = [&](At at) {
+        if (++at.tile == head_tiles) at.tile = 0, ++at.head;
+        return at;
     };
-    if (it0 < it1) load(it0);
+    auto set_of = [&](int it) { return ((it - it0) & 1) * kSetBytes; };
+    auto request = [&](int it, At at) {
+        if (it >= it1) return;
+        char* to = lds + set_of(it);
+        q_copy.base = reinterpret_cast<const char*>(q0 + at.head * a.q_at.head), g_copy.base = reinterpret_cast<const char*>(g0 + at.head * a.dout_at.head);
+        const int first = (first_tile + at.tile) * ROWS;
+        q_copy.request(to, first, a.tokens), g_copy.request(to + kTileBytes, first, a.tokens);
+    };
+    float row_next = 0.f;       // of the queries on their way: threads 0 .. ROWS - 1 their sums, the next as many their D
+    auto load_rows = [&](int it, At at) {
+        if (it >= it1 || tid >= 2 * ROWS) return;
+        const int row = (first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
+        const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
+        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
+    };
+    auto store_rows = [&](int it) {
+        if (it < it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + set_of(it) + 2 * kTileBytes)[tid] = row_next;
+    };
+    At next{0, 0};
+    if (it0 < it1) next.head = it0 / head_tiles, next.tile = it0 - next.head * head_tiles;
+    At now = next;
+    request(it0, next);
+    load_rows(it0, next), store_rows(it0);
+    next = after(next);
+    load_rows(it0 + 1, next);
     Frag k_column[Tile::kSteps], v_column[Tile::kSteps];
     const bool mine = my_key < length;
     load_column<T, DP>(k_column, static_cast<const T*>(a.k) + batch * a.k_at.batch + my_key * a.k_at.token + kv_head * a.k_at.head, mine, a.chunks, half);
-    load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
-    floatx16 dk[Tile::kBlocks], dv[Tile::kBlocks];
+    if (for_k) load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
+    floatx16 sums[ROLES ? 1 : 2][Tile::kBlocks];      // two roles: one sum a wavefront
+    floatx16(&dk)[Tile::kBlocks] = sums[0], (&dv)[Tile::kBlocks] = sums[ROLES ? 0 : 1];
     clear(dk), clear(dv);
-    if (it0 < it1) {
-        store(lds);
-        if (it0 + 1 < it1) load(it0 + 1);
-    }
-    lds_barrier();
     for (int it = it0; it < it1; ++it) {
-        const char* set = lds + ((it - it0) & 1) * kSetBytes;
-        if (it + 1 < it1) {
-            store(lds + ((it + 1 - it0) & 1) * kSetBytes);
-            if (it + 2 < it1) load(it + 2);
-        }
-        const int first = (first_tile + it % head_tiles) * ROWS;
-        if (first + ROWS > wave_need) {
+        wait_for_copies();
+        lds_barrier();
+        // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
+        request(it + 1, next), store_rows(it + 1);
+        const int first = (first_tile + now.tile) * ROWS, set = set_of(it);
+        now = next, next = after(next);
+        load_rows(it + 2, next);
+        if (first + ROWS <= wave_need) continue;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                if (NS > 1 && first + 32 * (n + 1) <= wave_need) continue;
-                floatx16 s[2];
-                clear(s);
-                tile.straight(s[0], set, n, k_column);
-                tile.straight(s[1], set + kTileBytes, n, v_column);
-                const float* rows = reinterpret_cast<const float*>(set + 2 * kTileBytes) + 32 * n + 4 * half;
-                const bool masked = first + 32 * n < wave_all;
-                floatx16 p;
+        for (int n = 0; n < NS; ++n) {
+            if (NS > 1 && first + 32 * (n + 1) <= wave_need) continue;
+            floatx16 s[2];
+            clear(s);
+            tile.straight(s[0], set, n, k_column);
+            const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 32 * n + 4 * half;
+            const bool masked = first + 32 * n < wave_all;
+            floatx16 p;
+            if (for_k) tile.straight(s[1], set + kTileBytes, n, v_column);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 8 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + i], a.scale_log2, -lse[i]));
+            }
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = first + 32 * n + 4 * half + (r & 3) + 8 * (r >> 2) >= need ? p[r] : 0.f;
+            }
+            if (for_v) tile.transposed(dv, set + kTileBytes, n, Tile::pack(p));
+            if (for_k) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 8 * g), delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 8 * g);
+                    const floatx4v delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 8 * g);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 4 * g + i;
-                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.scale_log2, -lse[i]));
-                        if (masked) p[r] = first + 32 * n + 4 * half + i + 8 * g >= need ? p[r] : 0.f;
-                        s[0][r] = p[r] * (s[1][r] - delta[i]);
-                    }
+                    for (int i = 0; i < 4; ++i) p[4 * g + i] *= s[1][4 * g + i] - delta[i];
                 }
-                tile.transposed(dv, set + kTileBytes, n, p);
-                tile.transposed(dk, set, n, s[0]);
+                tile.transposed(dk, set, n, Tile::pack(p));
             }
         }
-        lds_barrier();
     }
-    if (a.splits == 1) {
-        typedef AttnOut<T, DP> Out;
-        char* room = lds + wave * Out::kRoom;
+    wait_for_copies();
+    lds_barrier();
+    const int dim = a.chunks * Tile::kPerChunk;
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
+    for (int which = 0; which < 2; ++which) {
+        if (!(which ? for_v : for_k)) continue;
+        if (a.splits == 1) {
+            typedef AttnOut<T, DP> Out;
+            char* room = lds + wave * Out::kRoom;
             const HeadsAt& at = which ? a.dv_at : a.dk_at;
             T* to = static_cast<T*>(which ? a.dv : a.dk);
             if (!to) continue;
@@ -240,21 +274,16 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
             else Out::park(room, dk, a.scale, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_key + col < a.keys ? to + (wave_key + col) * at.token : nullptr; });
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-    } else {
-        typedef AttnOut<float, DP> Out;
-        char* room = lds + wave * Out::kRoom;
-        const int dim = a.chunks * Tile::kPerChunk;
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
+        } else {
+            typedef AttnOut<float, DP> Out;
+            char* room = lds + wave * Out::kRoom;
             float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
             if (which) Out::park(room, dv, 1.f, lane);
             else Out::park(room, dk, a.scale, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_key + col < a.keys ? to + static_cast<int64_t>(wave_key + col) * dim : nullptr; });
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -287,7 +316,7 @@ constexpr int backward_rows_lds() {
 }
 template <typename T, int DP>
 constexpr int backward_keys_lds() {
-    constexpr int tiles = 2 * query_tile<T, DP>() * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4), out = kWaves * AttnOut<float, DP>::kRoom;
+    constexpr int tiles = 2 * query_tile<T, DP>() * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4), out = (two_roles<T, DP>() ? 2 : 1) * kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
 }
 
@@ -361,7 +390,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         a.blocks = (a.keys + kRows * kWaves - 1) / (kRows * kWaves);
         const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads, grid = pairs * a.blocks * a.splits;
         if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
-        hipLaunchKernelGGL((attention_backward_keys<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kKeysLds, s, a);
+        hipLaunchKernelGGL((attention_backward_keys<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(two_roles<T, DP>() ? 2 * kThreads : kThreads), kKeysLds, s, a);
         if (const int rc = check_launch("ddl_attention_backward")) return rc;
         if (a.splits == 1) return 0;
         const int64_t threads = 2 * pairs * a.keys * (dim / 4);

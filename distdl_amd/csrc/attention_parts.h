@@ -20,6 +20,7 @@
 #define DDL_ATTENTION_PARTS_H
 #include "ddl_common.h"
 
+#include "gemm_tiles.h"
 #include "ln_elements.h"
 
 #include <initializer_list>
@@ -34,14 +35,25 @@ typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) shortx4* lds_shortx4;
 
+// Byte address of a place in LDS: what the reads add their immediate offsets to.
+__device__ inline uint32_t lds_address(const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); }
+template <typename V>
+__device__ inline V lds_read(uint32_t at) {
+    return *(const __attribute__((address_space(3))) V*)static_cast<uintptr_t>(at);
+}
+
 template <typename T>
 struct AttnElem {
     typedef shortx8 Frag;                 // 16 bytes of a row
+    struct Packed {                       // 32 values of a column, for the rows that either half of the lanes holds
+        shortx8 lo, hi;
+    };
     static constexpr int kPerChunk = 8;
 };
 template <>
 struct AttnElem<float> {
     typedef floatx4v Frag;
+    typedef floatx16 Packed;
     static constexpr int kPerChunk = 4;
 };
 
@@ -73,10 +85,46 @@ __device__ inline shortx8 pack8(const floatx16& v, int first, const __half*) {
     return __builtin_bit_cast(shortx8, o);
 }
 
+// total + eight packed values, rounded as they are: a weighted mean's weights then add up to what it is divided by, and a single large one
+// comes out as exactly 1.  (Half as many instructions as the sum of the unrounded ones, too.)
+__device__ inline float add8(float total, const shortx8& v, const bf16_t*) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    pair p[4];
+    const pair one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+    __builtin_memcpy(p, &v, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total = __builtin_amdgcn_fdot2_f32_bf16(p[i], one, total, false);
+    return total;
+}
+__device__ inline float add8(float total, const shortx8& v, const __half*) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    pair p[4];
+    const pair one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
+    __builtin_memcpy(p, &v, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total = __builtin_amdgcn_fdot2(p[i], one, total, false);
+    return total;
+}
+
+// Eight values of the 16-bit type times a power of two.
+__device__ inline shortx8 scale8(const shortx8& v, float factor, const bf16_t*) {
+    shortx8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = static_cast<short>(f32_to_bf16(bf16_to_f32(static_cast<uint16_t>(v[i])) * factor));
+    return o;
+}
+__device__ inline shortx8 scale8(const shortx8& v, float factor, const __half*) {
+    halfx8 o = __builtin_bit_cast(halfx8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = static_cast<_Float16>(static_cast<float>(o[i]) * factor);
+    return __builtin_bit_cast(shortx8, o);
+}
+
 // Rows of DP elements of type T in LDS.
 template <typename T, int DP>
 struct AttnTile {
     typedef typename AttnElem<T>::Frag Frag;
+    typedef typename AttnElem<T>::Packed Packed;
     static constexpr int kPerChunk = AttnElem<T>::kPerChunk;
     static constexpr int kBytes = DP * static_cast<int>(sizeof(T));
     static constexpr int kRowBytes = kBytes <= 64 ? 64 : kBytes <= 128 ? 128 : kBytes <= 256 ? 256 : 512;
@@ -93,60 +141,88 @@ struct AttnTile {
         return (((row >> 2) & 1) << 3) | (row & 3) | (((row >> 3) & 1) << 2);
     }
 
-    int straight_row, straight_x;     // of this lane: byte offset of its row, its part of the chunk number
-    int trans_row, trans_x, trans_byte;
+    // Of this lane, LDS addresses in the block of 32 rows at `base`: its chunk of every straight step; for every 32 columns of the transposed
+    // product the first four rows of a lane's half (16-bit), and those eight further down, or its row 0 (fp32).
+    static constexpr int kHigh = sizeof(T) == 2 ? kBlocks : 1;
+    uint32_t straight_at[kSteps], trans_at[kBlocks], trans_high[kHigh];
 
-    __device__ explicit AttnTile(int lane) {
+    __device__ AttnTile(const char* lds, int lane) {
+        const uint32_t base = lds_address(lds);      // of all tiles, which the products name by their byte offsets from here
         const int half = lane >> 5, col = lane & 31;
-        straight_row = col * kRowBytes, straight_x = half ^ swizzle(col);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) straight_at[s] = base + col * kRowBytes + (((2 * s + half) ^ swizzle(col)) << 4);
         if constexpr (sizeof(T) == 2) {   // lane i of 16 points at row i / 4, columns 4 (i % 4) .. + 3 of 16, and receives column i of the four rows
             const int i = lane & 15, row = 4 * half + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-            trans_row = row * kRowBytes, trans_x = chunk ^ swizzle(row), trans_byte = 8 * (i & 1);
-        } else {
-            trans_row = 4 * half * kRowBytes, trans_x = (col >> 2) ^ swizzle(4 * half), trans_byte = 4 * (col & 3);
-        }
-    }
-
-    // acc[r] += the product of rows 32 block .. + 31 of the tile with this lane's column.
-    __device__ void straight(floatx16& acc, const char* tile, int block, const Frag (&column)[kSteps]) const {
-        const char* base = tile + block * 32 * kRowBytes + straight_row;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const Frag a = *reinterpret_cast<const Frag*>(base + (((2 * s) ^ straight_x) << 4));
-            mfma_chunk(acc, a, column[s], static_cast<const T*>(nullptr));
-        }
-    }
-
-    // The same with the columns in a tile of their own.
-    __device__ void straight(floatx16& acc, const char* tile, const char* columns) const {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int at = straight_row + (((2 * s) ^ straight_x) << 4);
-            mfma_chunk(acc, *reinterpret_cast<const Frag*>(tile + at), *reinterpret_cast<const Frag*>(columns + at), static_cast<const T*>(nullptr));
-        }
-    }
-
-    // acc[d block] += tile rows 32 block .. + 31, transposed, times p of this lane's column.
-    __device__ void transposed(floatx16 (&acc)[kBlocks], const char* tile, int block, const floatx16& p) const {
-        const char* base = tile + block * 32 * kRowBytes + trans_row + trans_byte;
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const shortx8 b = pack8(p, 8 * k, static_cast<const T*>(nullptr));
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)(base + 16 * k * kRowBytes + (((4 * d) ^ trans_x) << 4)));
-                    const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)(base + (16 * k + 8) * kRowBytes + (((4 * d) ^ swizzle(8) ^ trans_x) << 4)));
-                    mfma_chunk(acc[d], __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, static_cast<const T*>(nullptr));
-                }
+            for (int d = 0; d < kBlocks; ++d) {
+                trans_at[d] = base + row * kRowBytes + (((4 * d + chunk) ^ swizzle(row)) << 4) + 8 * (i & 1);
+                trans_high[d] = base + (row + 8) * kRowBytes + (((4 * d + chunk) ^ swizzle(row + 8)) << 4) + 8 * (i & 1);
             }
         } else {
 #pragma unroll
+            for (int d = 0; d < kBlocks; ++d) trans_at[d] = base + 4 * half * kRowBytes + (((8 * d + (col >> 2)) ^ swizzle(4 * half)) << 4) + 4 * (col & 3);
+        }
+    }
+
+    __device__ Frag read_straight(uint32_t block, int s) const { return lds_read<Frag>(straight_at[s] + block); }
+    // 16-bit: what the transposed product of rows 16 k .. + 15 with 32 columns takes.
+    __device__ shortx8 read_transposed(uint32_t block, int k, int d) const {
+        const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)static_cast<uintptr_t>((trans_at[d] + block) + 16 * k * kRowBytes));
+        const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4)static_cast<uintptr_t>((trans_high[d] + block) + 16 * k * kRowBytes));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+
+    // acc[r] += the product of rows 32 block .. + 31 of the tile with this lane's column.
+    __device__ void straight(floatx16& acc, uint32_t tile, int block, const Frag (&column)[kSteps]) const {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) mfma_chunk(acc, read_straight(tile + block * 32 * kRowBytes, s), column[s], static_cast<const T*>(nullptr));
+    }
+
+    // The same with the columns in a tile of their own.
+    __device__ void straight(floatx16& acc, uint32_t tile, uint32_t columns) const {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) mfma_chunk(acc, read_straight(tile, s), read_straight(columns, s), static_cast<const T*>(nullptr));
+    }
+
+    // A column's 32 values as the transposed product takes them.
+    static __device__ Packed pack(const floatx16& p) {
+        Packed o;
+        if constexpr (sizeof(T) == 2) o.lo = pack8(p, 0, static_cast<const T*>(nullptr)), o.hi = pack8(p, 8, static_cast<const T*>(nullptr));
+        else o = p;
+        return o;
+    }
+
+    // total + the values as packed.
+    static __device__ float add_packed(float total, const Packed& p) {
+        if constexpr (sizeof(T) == 2) {
+            return add8(add8(total, p.lo, static_cast<const T*>(nullptr)), p.hi, static_cast<const T*>(nullptr));
+        } else {
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += p[r];
+            return total + sum;
+        }
+    }
+    static __device__ void scale_packed(Packed& p, float factor) {
+        if constexpr (sizeof(T) == 2) p.lo = scale8(p.lo, factor, static_cast<const T*>(nullptr)), p.hi = scale8(p.hi, factor, static_cast<const T*>(nullptr));
+        else p *= factor;
+    }
+
+    // acc[d block] += tile rows 32 block .. + 31, transposed, times p of this lane's column.
+    __device__ void transposed(floatx16 (&acc)[kBlocks], uint32_t tile, int block, const Packed& p) const {
+        const uint32_t base = tile + block * 32 * kRowBytes;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) mfma_chunk(acc[d], read_transposed(base, k, d), k ? p.hi : p.lo, static_cast<const T*>(nullptr));
+        } else {
+#pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int row = (r & 3) + 8 * (r >> 2);
+                const int row = (r & 3) + 8 * (r >> 2);      // its part of the swizzle reaches chunks by exclusive or
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
-                    const float a = *reinterpret_cast<const float*>(base + row * kRowBytes + (((8 * d) ^ swizzle(row) ^ trans_x) << 4));
+                    const float a = lds_read<float>(((trans_at[d] ^ (swizzle(row) << 4)) + base) + row * kRowBytes);
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[d], 0, 0, 0);
                 }
             }
@@ -187,6 +263,43 @@ struct AttnStage {
         }
     }
 };
+
+// ROWS rows of a tensor straight from memory into a tile, by the WAVES wavefronts of a workgroup, without passing registers: every copy instruction
+// fills 1 KiB of the tile, lane after lane, so a lane takes the chunk that belongs where it writes.  Rows from the end on and chunks
+// behind the head's own lie outside the buffer that the copies are told of, which gives zeros.
+template <typename T, int DP, int ROWS, int WAVES>
+struct AttnCopy {
+    typedef AttnTile<T, DP> Tile;
+    static constexpr int kSlots = Tile::kRowBytes / 16, kPieces = ROWS * kSlots / (64 * WAVES);
+    static_assert(ROWS * kSlots % (64 * WAVES) == 0, "whole instructions for every wavefront");
+    const char* base;
+    int64_t pitch;             // bytes
+    int row_bytes, wave;
+    uint32_t offset[kPieces];
+
+    __device__ AttnCopy(const T* tensor, int64_t pitch_elems, int chunks, int wave, int lane)
+        : base(reinterpret_cast<const char*>(tensor)), pitch(pitch_elems * static_cast<int>(sizeof(T))), row_bytes(16 * chunks), wave(wave) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int at = (i * WAVES + wave) * 64 + lane, row = at / kSlots, c = (at % kSlots) ^ Tile::swizzle(row);
+            offset[i] = c < chunks ? static_cast<uint32_t>(row) * static_cast<uint32_t>(pitch) + 16 * c : 0x7FFFFFF0u;
+        }
+    }
+    // Rows first .. first + ROWS of the tensor, which ends with row `end`.
+    __device__ void request(const char* tile, int first, int end) const {
+        const int rows = end - first;
+        u32x4 buffer = raw_buffer(base + first * pitch);
+        buffer[2] = rows > 0 ? static_cast<uint32_t>((rows < ROWS ? rows - 1 : ROWS - 1) * static_cast<uint32_t>(pitch) + row_bytes) : 0u;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) buffer[i] = __builtin_amdgcn_readfirstlane(buffer[i]);     // the same in all lanes, as the instruction wants it
+        const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tile)));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) dma16(buffer, offset[i], 0, reinterpret_cast<const char*>(static_cast<uintptr_t>(to + (i * WAVES + wave) * 1024)));
+    }
+};
+
+// All requested copies of this wavefront have landed; with a barrier behind it, those of the workgroup.
+__device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // The value of lane l ^ 32 and this lane's, combined.
 template <typename Fn>
@@ -286,7 +399,7 @@ __device__ inline int keys_seen(const AttnArgs& a, int token, int length) {
 
 __device__ inline int sequence_keys(const AttnArgs& a, int batch) {
     if (!a.lengths) return a.keys;
-    const int n = a.lengths[batch];
+    const int n = __builtin_amdgcn_readfirstlane(a.lengths[batch]);     // the same in all lanes: into a scalar register
     return n < 0 ? 0 : n < a.keys ? n : a.keys;
 }
 
@@ -346,7 +459,10 @@ inline int fill_attention(AttnArgs& a, bool& nothing, const char* what, std::ini
             if (!aligned_to(o.p, 16)) return fail(DDL_E_ALIGN, "%s: operands are not 16-byte aligned", what);
             if (o.strides[1] < 0 || o.strides[1] >= kMaxPitch) return fail(DDL_E_UNSUPP, "%s: rows 2^22 elements apart", what);
         }
-        const HeadsAt at = place_of(o.strides);
+        HeadsAt at = place_of(o.strides);
+        const int64_t rows = of_keys ? keys : tokens;
+        if (rows <= 1) at.token = dim;      // nothing is ever that far away
+        else if (o.p && at.token < dim) return fail(DDL_E_UNSUPP, "%s: rows that overlap", what);
         if (i == 0) a.q = o.p, a.q_at = at;
         if (i == 1) a.k = o.p, a.k_at = at;
         if (i == 2) a.v = o.p, a.v_at = at;
