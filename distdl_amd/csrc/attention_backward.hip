@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
     int bh, block;
-    block_of(blockIdx.x, a.batch * a.heads, a.blocks, bh, block);
+    block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, bh, block);
     const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
     const int length = sequence_keys(a, batch);
     const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
 }
 
 template <typename T, int DP>
-constexpr int query_tile() { return AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32; }
+constexpr int query_tile() { return sizeof(T) == 2 || AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32; }
 
 // dk and dv of 32 keys a wavefront, 128 a workgroup; 32 or 64 queries of one head at a time through LDS, with their sums and D.  Where
 // there are few blocks of keys, `splits` workgroups share the queries of one and leave sums in fp32.
@@ -155,7 +155,7 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     const bool for_k = !ROLES || wave < kWaves, for_v = !ROLES || wave >= kWaves;
     const int pairs = a.batch * a.kv_heads;
     int bk, unit;
-    block_of(blockIdx.x, pairs, a.blocks * a.splits, bk, unit);
+    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, bk, unit);
     unit = a.blocks * a.splits - 1 - unit;      // the first keys, which most queries see in the causal form, first
     const int block = unit / a.splits, split = unit - block * a.splits;
     const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
@@ -381,6 +381,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
             a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
             const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
             if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
+            a.folded = folds(a.causal, grid);
             hipLaunchKernelGGL((attention_backward_rows<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kRowsLds, s, a);
             if (const int rc = check_launch("ddl_attention_backward")) return rc;
         }

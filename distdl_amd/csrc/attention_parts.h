@@ -385,6 +385,7 @@ struct AttnArgs {
     int causal;
     float scale, scale_log2;
     int blocks;                         // of rows (or keys) of a head
+    int folded;                         // order of the blocks, see block_of
     int splits;                         // of the keys (adjoint of keys: of the queries)
     float* partial;                     // sums of the splits
 };
@@ -404,15 +405,17 @@ __device__ inline int sequence_keys(const AttnArgs& a, int batch) {
 }
 
 // Workgroup `id` of `blocks` x `heads`: neighbouring numbers go to different XCDs, each of which takes its own share of the heads,
-// so that what they have in common stays in its L2.  Blocks come in descending order.
-__device__ inline void block_of(int id, int heads, int blocks, int& head, int& block) {
+// so that what they have in common stays in its L2.  Blocks come in descending order, the longest first where a row sees the keys before it;
+// `folded`: the second half of them in ascending order.
+__device__ inline void block_of(int id, int heads, int blocks, bool folded, int& head, int& block) {
     if (heads % 8 == 0) {
         const int share = heads / 8, slot = id >> 3;
         head = (id & 7) * share + slot % share, block = slot / share;
     } else {
         head = id % heads, block = id / heads;
     }
-    block = blocks - 1 - block;
+    const int down = blocks / 2;
+    block = folded && block >= down ? block - down : blocks - 1 - block;
 }
 
 // More LDS than a kernel gets unasked: set once for each kernel and device.
@@ -428,6 +431,13 @@ int grant_lds(int bytes, const char* what) {
     return 0;
 }
 
+
+// Where all workgroups of a causal launch are resident at once, two on a CU, the second one on a CU is one of the short half that goes with
+// the long one there; with more of them than that, longest first is what levels them.
+inline bool folds(int causal, int64_t grid) {
+    int dev;
+    return causal && grid <= 2 * static_cast<int64_t>(compute_units(dev));
+}
 
 struct HeadsOperand {
     const void* p;
