@@ -174,8 +174,21 @@ struct AttnTile {
 
     // acc[r] += the product of rows 32 block .. + 31 of the tile with this lane's column.
     __device__ void straight(floatx16& acc, uint32_t tile, int block, const Frag (&column)[kSteps]) const {
+        const uint32_t base = tile + block * 32 * kRowBytes;
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) mfma_chunk(acc, read_straight(tile + block * 32 * kRowBytes, s), column[s], static_cast<const T*>(nullptr));
+            for (int s = 0; s < kSteps; ++s) mfma_chunk(acc, read_straight(base, s), column[s], static_cast<const T*>(nullptr));
+        } else {      // four matrix instructions of 64 cycles a read: the next two reads go out in front of them
+            Frag a[kSteps];
+            a[0] = read_straight(base, 0), a[1] = read_straight(base, 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (s + 2 < kSteps) a[s + 2] = read_straight(base, s + 2);
+                mfma_chunk(acc, a[s], column[s], static_cast<const T*>(nullptr));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
 
     // The same with the columns in a tile of their own.
@@ -217,14 +230,20 @@ struct AttnTile {
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) mfma_chunk(acc[d], read_transposed(base, k, d), k ? p.hi : p.lo, static_cast<const T*>(nullptr));
         } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            float v[16][kBlocks];
+            auto read = [&](int r) {
                 const int row = (r & 3) + 8 * (r >> 2);      // its part of the swizzle reaches chunks by exclusive or
 #pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const float a = lds_read<float>(((trans_at[d] ^ (swizzle(row) << 4)) + base) + row * kRowBytes);
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[d], 0, 0, 0);
-                }
+                for (int d = 0; d < kBlocks; ++d) v[r][d] = lds_read<float>(((trans_at[d] ^ (swizzle(row) << 4)) + base) + row * kRowBytes);
+            };
+            read(0), read(1), read(2), read(3);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (r + 4 < 16) read(r + 4);
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][d], p[r], acc[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
