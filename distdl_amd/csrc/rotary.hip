@@ -26,7 +26,7 @@ constexpr int kWave = 64;
 constexpr int kBlock = 256;
 constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kMaxHeadDim = 512;      // 64 lanes of eight elements
-constexpr int kGradBlocks = 512;      // workgroups of the norm's adjoint at most, each with a partial sum of dw
+constexpr int kGradBlocks = 1024;     // workgroups of the norm's adjoint at most, each with a partial sum of dw
 
 struct Place {   // of a [batch, tokens, heads, head_dim] tensor: strides in elements, head_dim's is 1
     int64_t batch, token, head;
@@ -304,23 +304,23 @@ __global__ __launch_bounds__(kBlock) void rotary_heads(const RotaryArgs arg) {
     }
 }
 
-// dw[e] = sum over the workgroups' partial sums, in their order: 16 columns x 16 rows at a time.
+// dw[e] = sum over the workgroups' partial sums, in one order: 16 columns x 64 rows at a time.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void weight_grads(const float* __restrict__ partial, int blocks, int dim, T* dwq, T* dwk) {
-    __shared__ float sums[16][17];
+__global__ __launch_bounds__(1024) void weight_grads(const float* __restrict__ partial, int blocks, int dim, T* dwq, T* dwk) {
+    __shared__ float sums[64][17];
     const int col = threadIdx.x & 15, lane = threadIdx.x >> 4;
     const int e = blockIdx.x * 16 + col;
     float t = 0.f;
     if (e < 2 * dim) {
 #pragma unroll 8
-        for (int b = lane; b < blocks; b += 16) t += partial[static_cast<int64_t>(b) * 2 * dim + e];
+        for (int b = lane; b < blocks; b += 64) t += partial[static_cast<int64_t>(b) * 2 * dim + e];
     }
     sums[lane][col] = t;
     __syncthreads();
     if (lane == 0 && e < 2 * dim) {
         float all = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) all += sums[k][col];
+        for (int k = 0; k < 64; ++k) all += sums[k][col];
         T* out = e < dim ? dwq : dwk;
         if (out) store1(out + (e < dim ? e : e - dim), all);
     }
@@ -434,7 +434,7 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides, c
         a.x_at[0] = place_of(q_strides), a.x_at[1] = place_of(k_strides), a.dy_at[0] = place_of(dyq_strides), a.dy_at[1] = place_of(dyk_strides);
         a.y_at[0] = place_of(dq_strides), a.y_at[1] = place_of(dk_strides);
         a.partial = sums ? workspace : nullptr;
-        grid = grid_for(a, 8);
+        grid = grid_for(a, 4);
         if (grid > kGradBlocks) grid = kGradBlocks;
         const int rc = with_element(dtype, [&](auto* e) {
             return launch_pairs<std::remove_pointer_t<decltype(e)>>(a, neighbours != 0, kNormRotateBackward, grid, static_cast<hipStream_t>(stream));
@@ -444,7 +444,7 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides, c
     if (!sums) return 0;
     return with_element(dtype, [&](auto* e) {
         typedef std::remove_pointer_t<decltype(e)> T;
-        hipLaunchKernelGGL((weight_grads<T>), dim3((2 * static_cast<int>(dim) + 15) / 16), dim3(kBlock), 0, static_cast<hipStream_t>(stream), workspace, grid,
+        hipLaunchKernelGGL((weight_grads<T>), dim3((2 * static_cast<int>(dim) + 15) / 16), dim3(1024), 0, static_cast<hipStream_t>(stream), workspace, grid,
                            static_cast<int>(dim), static_cast<T*>(dq_weight), static_cast<T*>(dk_weight));
         return check_launch("ddl_head_norm_rotary_backward");
     });
