@@ -248,7 +248,7 @@ constexpr int rows_lds() {
 }
 
 // Few queries, many keys: the queries of all heads that share a key head (row = token x group + head in the group) in one
-// wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with a tile of its own
+// wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with tiles of its own
 // and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).
 // (Rows of more than 256 bytes fill the registers of a SIMD with one wavefront: 128 of them for the tiles on their way.)
 template <typename T, int DP>
@@ -265,43 +265,63 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const int rows = a.tokens * a.group, first_row = block * kRows, my_row = first_row + (lane & 31);
     const int token = my_row / a.group, head = kv_head * a.group + my_row - token * a.group;
     const int seen = my_row < rows ? keys_seen(a, token, length) : 0;
-    const int most = keys_seen(a, (min(first_row + kRows, rows) - 1) / a.group, length), least = keys_seen(a, first_row / a.group, length);
+    const int most = __builtin_amdgcn_readfirstlane(keys_seen(a, (min(first_row + kRows, rows) - 1) / a.group, length));
+    const int least = __builtin_amdgcn_readfirstlane(keys_seen(a, first_row / a.group, length));
     // This split's keys, of those that there are: whole tiles, shared evenly.
     const int tiles = (most + KEYS - 1) / KEYS;
+    constexpr bool kEarly = sizeof(T) == 2;      // of the values, too
     const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
     const Tile tile(lds, lane);
-    AttnStage<T, DP, KEYS, kWave> k_next, v_next;
-    int t = t0 + wave;
-    if (t < t1) k_next.load(k, a.k_at.token, t * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, t * KEYS, most, a.chunks, lane);
-    // The queries wait in LDS, as a tile of their own: in registers they would be an eighth of what a wavefront has.
-    char* q_tile = lds + kWaves * 2 * kTileBytes;
-    for (int i = threadIdx.x; i < kRows * Tile::kChunks; i += kThreads) {
-        const int r = i / Tile::kChunks, c = i - r * Tile::kChunks, row = first_row + r;
-        Frag f = {};
-        if (row < rows && c < a.chunks) {
-            const int tk = row / a.group, hd = kv_head * a.group + row - tk * a.group;
-            f = *reinterpret_cast<const Frag*>(static_cast<const T*>(a.q) + batch * a.q_at.batch + tk * a.q_at.token + hd * a.q_at.head + c * Tile::kPerChunk);
-        }
-        *reinterpret_cast<Frag*>(q_tile + r * Tile::kRowBytes + ((c ^ Tile::swizzle(r)) << 4)) = f;
-    }
-    lds_barrier();
-    Running<Tile::kBlocks> run;
     const int kt = wave * 2 * kTileBytes, vt = kt + kTileBytes;
+    const AttnCopy<T, DP, KEYS, 1> k_copy(k, a.k_at.token, a.chunks, 0, lane), v_copy(v, a.v_at.token, a.chunks, 0, lane);
+    int t = t0 + wave;
+    if (t < t1) k_copy.request(lds + kt, t * KEYS, most), v_copy.request(lds + vt, t * KEYS, most);
+    Frag column[Tile::kSteps];
+    const T* q = static_cast<const T*>(a.q) + batch * a.q_at.batch;
+#pragma unroll
+    for (int s = 0; s < Tile::kSteps; ++s) {
+        Frag f = {};
+        if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
+        column[s] = f;
+    }
+    Running<Tile::kBlocks> run;
     for (; t < t1; t += kWaves) {
-        k_next.store(lds + kt, lane), v_next.store(lds + vt, lane);
-        if (t + kWaves < t1) k_next.load(k, a.k_at.token, (t + kWaves) * KEYS, most, a.chunks, lane), v_next.load(v, a.v_at.token, (t + kWaves) * KEYS, most, a.chunks, lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int after = t + kWaves;
+        wait_for_copies();
+        // What the products take is read out of the tiles at once, so that the next ones can come in while this one is worked on.
+        Frag kf[Tile::kSteps];
+#pragma unroll
+        for (int s = 0; s < Tile::kSteps; ++s) kf[s] = tile.read_straight(kt, s);
+        shortx8 vf[kEarly ? 2 * Tile::kBlocks : 1];
+        if constexpr (kEarly) {
+#pragma unroll
+            for (int i = 0; i < 2 * Tile::kBlocks; ++i) vf[i] = tile.read_transposed(vt, i / Tile::kBlocks, i % Tile::kBlocks);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (after < t1) {
+            k_copy.request(lds + kt, after * KEYS, most);
+            if constexpr (kEarly) v_copy.request(lds + vt, after * KEYS, most);
+        }
         floatx16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        tile.straight(s, kt, static_cast<uint32_t>(q_tile - lds));
+#pragma unroll
+        for (int i = 0; i < Tile::kSteps; ++i) mfma_chunk(s, kf[i], column[i], static_cast<const T*>(nullptr));
         if ((t + 1) * KEYS > least) mask_scores(s, seen - t * KEYS - 4 * half);
         run.follow(s, a.scale_log2, tile, nullptr);
-        tile.transposed(run.acc, vt, 0, run.take(s, a.scale_log2, tile));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const typename Tile::Packed p = run.take(s, a.scale_log2, tile);
+        if constexpr (kEarly) {
+#pragma unroll
+            for (int i = 0; i < 2 * Tile::kBlocks; ++i) mfma_chunk(run.acc[i % Tile::kBlocks], vf[i], i / Tile::kBlocks ? p.hi : p.lo, static_cast<const T*>(nullptr));
+        } else {
+            tile.transposed(run.acc, vt, 0, p);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (after < t1) v_copy.request(lds + vt, after * KEYS, most);
+        }
     }
+    wait_for_copies();
     // Joined: every wavefront's maximum and total, then its sums relative to the common maximum, added in the wavefronts' order.
     __shared__ float tops[kWaves][kRows], totals[kWaves][kRows];
     const float own_total = add_halves(run.total);
@@ -349,7 +369,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     }
 }
 
-// The splits of a row, a workgroup for each row: groups of DP / 4 lanes take a share of the splits each (four of them in flight), in
+// The splits of a row, a workgroup for each row: groups of DP / 4 lanes take a share of the splits each (eight of them in flight), in
 // one pass with a running maximum, and are joined in their order.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
@@ -369,11 +389,12 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
         top = both, total = total * f + m.y * g;
         sum.x = sum.x * f + v.x * g, sum.y = sum.y * f + v.y * g, sum.z = sum.z * f + v.z * g, sum.w = sum.w * f + v.w * g;
     };
-    for (int s0 = group; s0 < a.splits; s0 += 4 * kGroups) {
-        float2 m[4];
-        float4 v[4];
+    constexpr int kFlight = 8;
+    for (int s0 = group; s0 < a.splits; s0 += kFlight * kGroups) {
+        float2 m[kFlight];
+        float4 v[kFlight];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kFlight; ++i) {
             const int s = s0 + i * kGroups;
             m[i] = make_float2(-INFINITY, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (s < a.splits) {
@@ -385,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) join(m[i], v[i]);
+        for (int i = 0; i < kFlight; ++i) join(m[i], v[i]);
     }
     if (lane == 0) tops[group] = top, totals[group] = total;
     sums[group][lane] = sum;
@@ -404,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
 template <typename T, int DP>
 constexpr int split_lds() {
     typedef AttnTile<T, DP> Tile;
-    constexpr int tiles = (kWaves * 2 + 1) * 32 * Tile::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
+    constexpr int tiles = kWaves * 2 * 32 * Tile::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
 }
 

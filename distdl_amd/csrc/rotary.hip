@@ -234,12 +234,14 @@ __global__ __launch_bounds__(kBlock) void rotary_heads(const RotaryArgs arg) {
                 float v[UN][8], g[UN][8];
 #pragma unroll
                 for (int u = 0; u < UN; ++u) {
+                    if (u > 0 && h0 + u * step >= hi) continue;      // for all lanes
                     const int h = h0 + u * step + sub;
                     piece.load(x + h * xa.head, h < hi, v[u]);
                     if (MODE == kNormRotateBackward) piece.load(dy + h * da.head, h < hi, g[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < UN; ++u) {
+                    if (u > 0 && h0 + u * step >= hi) continue;
                     const int h = h0 + u * step + sub;
                     if (MODE != kRotate) {
                         float q = 0.f;
@@ -338,7 +340,7 @@ int launch(const RotaryArgs& a, int mode, int grid, hipStream_t s) {
     switch (mode) {
         case kRotate: hipLaunchKernelGGL((rotary_heads<T, VP, NEIGHBOURS, kRotate, 4>), dim3(grid), dim3(kBlock), 0, s, a); break;
         case kNormRotate: hipLaunchKernelGGL((rotary_heads<T, VP, NEIGHBOURS, kNormRotate, 4>), dim3(grid), dim3(kBlock), 0, s, a); break;
-        default: hipLaunchKernelGGL((rotary_heads<T, VP, NEIGHBOURS, kNormRotateBackward, 2>), dim3(grid), dim3(kBlock), 0, s, a); break;
+        default: hipLaunchKernelGGL((rotary_heads<T, VP, NEIGHBOURS, kNormRotateBackward, 1>), dim3(grid), dim3(kBlock), 0, s, a); break;
     }
     return check_launch("ddl_rotary");
 }
