@@ -158,10 +158,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             };
             auto share = [&](int slot) {
 #pragma unroll
-                for (int r = 16 * slot / kSlots; r < 16 * (slot + 1) / kSlots; ++r) {
-                    scores[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], a.scale_log2, -base));
-                    asm volatile("" : "+v"(scores[r]));      // here and not where it is used
-                }
+                for (int r = 16 * slot / kSlots; r < 16 * (slot + 1) / kSlots; ++r) scores[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], a.scale_log2, -base)));
             };
             read(0), read(1);
             __builtin_amdgcn_sched_barrier(0);

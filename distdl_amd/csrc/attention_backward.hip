@@ -174,7 +174,7 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
     const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
     const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
-    const Tile tile(lds, lane);
+    Tile tile(lds, lane);
     AttnCopy<T, DP, ROWS, WAVES> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
     // Where an iteration's queries are: the head of the group and its first query.
     struct At {
@@ -216,47 +216,148 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     floatx16 sums[ROLES ? 1 : 2][Tile::kBlocks];      // two roles: one sum a wavefront
     floatx16(&dk)[Tile::kBlocks] = sums[0], (&dv)[Tile::kBlocks] = sums[ROLES ? 0 : 1];
     clear(dk), clear(dv);
-    for (int it = it0; it < it1; ++it) {
-        wait_for_copies();
-        lds_barrier();
-        // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
-        request(it + 1, next), store_rows(it + 1);
-        const int first = (first_tile + now.tile) * ROWS, set = set_of(it);
-        now = next, next = after(next);
-        load_rows(it + 2, next);
-        if (first + ROWS <= wave_need) continue;
+    constexpr int kS = Tile::kSteps, kT = 2 * Tile::kBlocks;
+    const std::integral_constant<int, 16> all16{};
+    const std::integral_constant<int, 0> none{};
+    auto nothing = [](int) {};
+    // Scores or dO . v of 32 queries, and the sums' share of them, with `count` calls of `vector` between the matrix instructions.
+    auto chain = [&](floatx16& to, uint32_t from, const Frag (&column)[kS], auto count, auto&& vector) {
+        if constexpr (sizeof(T) == 2) {
+            Frag f[kS];
+            f[0] = tile.read_straight(from, 0), f[1] = tile.read_straight(from, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            weave<kS, decltype(count)::value>(
+                [&](int i) {
+                    if (i + 2 < kS) f[i + 2] = tile.read_straight(from, i + 2);
+                    mfma_chunk(to, f[i], column[i], static_cast<const T*>(nullptr));
+                },
+                vector);
+        } else {
+            tile.straight(to, from, 0, column);
+        }
+    };
+    auto sum = [&](floatx16 (&to)[Tile::kBlocks], uint32_t from, const typename Tile::Packed& p, auto count, auto&& vector) {
+        if constexpr (sizeof(T) == 2) {
+            shortx8 f[kT];
+            f[0] = tile.read_transposed(from, 0, 0), f[1] = tile.read_transposed(from, 1 / Tile::kBlocks, 1 % Tile::kBlocks);
+            __builtin_amdgcn_sched_barrier(0);
+            weave<kT, decltype(count)::value>(
+                [&](int i) {
+                    if (i + 2 < kT) f[i + 2] = tile.read_transposed(from, (i + 2) / Tile::kBlocks, (i + 2) % Tile::kBlocks);
+                    mfma_chunk(to[i % Tile::kBlocks], f[i], i / Tile::kBlocks ? p.hi : p.lo, static_cast<const T*>(nullptr));
+                },
+                vector);
+        } else {
+            tile.transposed(to, from, 0, p);
+        }
+    };
+    // Row values (sums or D) of the rows that this half of the lanes holds, four at a time, the next four on their way.
+    struct OfRows {
+        const float* at;
+        floatx4v now, next;
+        __device__ explicit OfRows(const float* rows) : at(rows), next(*reinterpret_cast<const floatx4v*>(rows)) {}
+        __device__ float operator()(int r) {
+            if (r % 4 == 0) {
+                now = next;
+                if (r < 12) next = *reinterpret_cast<const floatx4v*>(at + 2 * (r + 4));
+            }
+            return now[r % 4];
+        }
+    };
+    auto exponential = [&](floatx16& p, OfRows& lse) {
+        return [&](int r) { p[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, -lse(r)))); };
+    };
+    auto difference = [&](floatx16& d, const floatx16& p, OfRows& delta) {
+        return [&](int r) { d[r] = pinned(p[r] * (d[r] - delta(r))); };
+    };
+    constexpr uint32_t kQ = 0, kG = kTileBytes, kNext = 32 * Tile::kRowBytes;
+    auto zero = [](floatx16& v) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            if (NS > 1 && first + 32 * (n + 1) <= wave_need) continue;
-            floatx16 s[2];
-            clear(s);
-            tile.straight(s[0], set, n, k_column);
-            const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 32 * n + 4 * half;
-            const bool masked = first + 32 * n < wave_all;
-            floatx16 p;
-            if (for_k) tile.straight(s[1], set + kTileBytes, n, v_column);
+        for (int r = 0; r < 16; ++r) v[r] = 0.f;
+    };
+    // 32 queries, some of which (`masked`) may not see some of the wavefront's keys.
+    auto block_step = [&](int n, int first, const float* rows, bool masked, auto fk, auto fv) {
+        floatx16 p, d;
+        zero(p), zero(d);
+        tile.straight(p, kQ, n, k_column);
+        if constexpr (fk) tile.straight(d, kG, n, v_column);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 32 * n + 8 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[4 * g + i], a.scale_log2, -lse[i]));
+        }
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = first + 32 * n + 4 * half + (r & 3) + 8 * (r >> 2) >= need ? p[r] : 0.f;
+        }
+        if constexpr (fv) tile.transposed(dv, kG, n, Tile::pack(p));
+        if constexpr (fk) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 8 * g);
+                const floatx4v delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 32 * n + 8 * g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + i], a.scale_log2, -lse[i]));
+                for (int i = 0; i < 4; ++i) d[4 * g + i] = p[4 * g + i] * (d[4 * g + i] - delta[i]);
             }
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] = first + 32 * n + 4 * half + (r & 3) + 8 * (r >> 2) >= need ? p[r] : 0.f;
-            }
-            if (for_v) tile.transposed(dv, set + kTileBytes, n, Tile::pack(p));
-            if (for_k) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const floatx4v delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 8 * g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[4 * g + i] *= s[1][4 * g + i] - delta[i];
-                }
-                tile.transposed(dk, set, n, Tile::pack(p));
-            }
+            tile.transposed(dk, kQ, n, Tile::pack(d));
         }
-    }
+    };
+    // 64 queries that see all of the wavefront's keys: while the vector units are at the first 32, the matrix cores form the scores of the
+    // others, and while they are at those, the sums of the first.
+    auto pair_step = [&](const float* rows, auto fk, auto fv) {
+        floatx16 p0, p1, d0, d1;
+        zero(p0), zero(p1), zero(d0), zero(d1);
+        OfRows lse0(rows);
+        chain(p0, kQ, k_column, none, nothing);
+        if constexpr (fk) {
+            chain(d0, kG, v_column, all16, exponential(p0, lse0));
+            const typename Tile::Packed b0 = Tile::pack(p0);
+            OfRows delta0(rows + ROWS);
+            chain(p1, kQ + kNext, k_column, all16, difference(d0, p0, delta0));
+            const typename Tile::Packed a0 = Tile::pack(d0);
+            OfRows lse1(rows + 32);
+            chain(d1, kG + kNext, v_column, all16, exponential(p1, lse1));
+            const typename Tile::Packed b1 = Tile::pack(p1);
+            OfRows delta1(rows + ROWS + 32);
+            if constexpr (fv) sum(dv, kG, b0, none, nothing);
+            sum(dk, kQ, a0, all16, difference(d1, p1, delta1));
+            if constexpr (fv) sum(dv, kG + kNext, b1, none, nothing);
+            sum(dk, kQ + kNext, Tile::pack(d1), none, nothing);
+        } else {
+            chain(p1, kQ + kNext, k_column, all16, exponential(p0, lse0));
+            OfRows lse1(rows + 32);
+            sum(dv, kG, Tile::pack(p0), all16, exponential(p1, lse1));
+            sum(dv, kG + kNext, Tile::pack(p1), none, nothing);
+        }
+    };
+    auto walk = [&](auto fk, auto fv) {
+        for (int it = it0; it < it1; ++it) {
+            wait_for_copies();
+            lds_barrier();
+            // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
+            request(it + 1, next), store_rows(it + 1);
+            const int first = (first_tile + now.tile) * ROWS, set = set_of(it);
+            now = next, next = after(next);
+            load_rows(it + 2, next);
+            const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 4 * half;
+            bool done = false;
+            if constexpr (sizeof(T) == 2 && NS == 2 && !(ROLES && fk)) {      // (the two columns and dk leave no registers for 64 at a time)
+                done = first >= wave_all;
+                if (done) pair_step(rows, fk, fv);
+            }
+            if (!done) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+                    if (first + 32 * (n + 1) > wave_need) block_step(n, first, rows, first + 32 * n < wave_all, fk, fv);
+            }
+            tile.shift(set ? -kSetBytes : kSetBytes);
+        }
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    if constexpr (!ROLES) walk(yes, yes);
+    else if (for_k) walk(yes, no);
+    else walk(no, yes);
     wait_for_copies();
     lds_barrier();
     const int dim = a.chunks * Tile::kPerChunk;

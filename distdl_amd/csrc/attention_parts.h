@@ -164,6 +164,17 @@ struct AttnTile {
         }
     }
 
+    // All places `bytes` further on: to another set of tiles, whose reads then keep their immediate offsets.
+    __device__ void shift(int bytes) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) straight_at[s] += bytes;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) {
+            trans_at[d] += bytes;
+            if (sizeof(T) == 2) trans_high[d % kHigh] += bytes;
+        }
+    }
+
     __device__ Frag read_straight(uint32_t block, int s) const { return lds_read<Frag>(straight_at[s] + block); }
     // 16-bit: what the transposed product of rows 16 k .. + 15 with 32 columns takes.
     __device__ shortx8 read_transposed(uint32_t block, int k, int d) const {
@@ -319,6 +330,24 @@ struct AttnCopy {
 
 // All requested copies of this wavefront have landed; with a barrier behind it, those of the workgroup.
 __device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// `N` matrix instructions, behind each of which a share of other work is issued: matrix(i), then the parts of vector(r), r < COUNT, that fall to
+// it, in this order -- left to itself the compiler puts one kind behind the other, and then one kind of unit waits.
+template <int N, int COUNT, typename M, typename V>
+__device__ inline void weave(M&& matrix, V&& vector) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        matrix(i);
+#pragma unroll
+        for (int r = COUNT * i / N; r < COUNT * (i + 1) / N; ++r) vector(r);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// A value that is computed here and not where it is used.
+__device__ inline float pinned(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // The value of lane l ^ 32 and this lane's, combined.
 template <typename Fn>
