@@ -16,13 +16,18 @@
 namespace ddl {
 namespace {
 
+constexpr int kStats = 4;               // behind the sums of a row over a split's keys: its maximum, its two totals, nothing
 constexpr float kSlack = 8.f;           // the running maximum is moved when it lags by more than this (in powers of two)
 
 // The softmax of a wavefront's columns as far as it has come.
-template <int BLOCKS>
+//
+// Two totals: of the probabilities as they are rounded for the product, which is what the result is divided by (the weights of a mean add
+// up to one then, and a single large one is exact), and, EXACT, of the unrounded ones, from which the adjoint forms them anew:
+// divided by the other one they would all be off by its rounding, up to half a step where one key has most of the weight.
+template <int BLOCKS, bool EXACT>
 struct Running {
     floatx16 acc[BLOCKS];
-    float top = -INFINITY, total = 0.f;      // of this lane's column; the total of this lane's half of the rows
+    float top = -INFINITY, total = 0.f, exact = 0.f;      // of this lane's column; the totals of this lane's half of the rows
 
     __device__ Running() {
 #pragma unroll
@@ -43,6 +48,7 @@ struct Running {
             const float moved = fmaxf(top, ceilf(m)), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
             top = moved;
             total *= factor;
+            if (EXACT) exact *= factor;
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
@@ -59,8 +65,18 @@ struct Running {
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
         const typename Tile::Packed p = Tile::pack(s);
         total = Tile::add_packed(total, p);
+        add_exact(s);
         return p;
     }
+    __device__ void add_exact(const floatx16& p) {
+        if constexpr (EXACT) {
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += p[r];
+            exact += sum;
+        }
+    }
+    __device__ float exact_total() const { return EXACT ? exact : total; }
 };
 
 // `rest`: keys of these 32 that this lane's column sees, from this lane's half's first one on.
@@ -81,7 +97,7 @@ constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // With tiles of NS blocks, keys are read up to one block before and values one block after the softmax: one barrier a tile, in
 // front of its last block, is then enough for two buffers of each.  What follows it is copied to where
 // everybody has just finished reading: keys two tiles ahead, values NS - 1 blocks ahead.
-template <typename T, int DP>
+template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
@@ -121,7 +137,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     }
     wait_for_copies();
     lds_barrier();
-    Running<Tile::kBlocks> run;
+    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run;
     floatx16 scores;
     typename Tile::Packed before;
     auto score = [&](floatx16& to, int s) {
@@ -175,6 +191,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             }
             before = Tile::pack(scores);
             run.total = Tile::add_packed(run.total, before);
+            run.add_exact(scores);
             scores = next;
         } else {
             floatx16 next;
@@ -224,8 +241,10 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     wait_for_copies();
     lds_barrier();
     const float total = add_halves(run.total);
-    if (a.lse && half == 0 && my_row < a.tokens)
-        a.lse[static_cast<int64_t>(bh) * a.tokens + my_row] = total > 0.f ? run.top + __builtin_amdgcn_logf(total) : INFINITY;
+    if constexpr (LSE) {
+        const float exact = add_halves(run.exact_total());
+        if (half == 0 && my_row < a.tokens) a.lse[static_cast<int64_t>(bh) * a.tokens + my_row] = exact > 0.f ? run.top + __builtin_amdgcn_logf(exact) : INFINITY;
+    }
     typedef AttnOut<T, DP> Out;
     char* room = lds + wave * Out::kRoom;
     Out::park(room, run.acc, total > 0.f ? 1.0f / total : 0.f, lane);
@@ -248,7 +267,7 @@ constexpr int rows_lds() {
 // wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with tiles of its own
 // and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).
 // (Rows of more than 256 bytes fill the registers of a SIMD with one wavefront: 128 of them for the tiles on their way.)
-template <typename T, int DP>
+template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_split(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
@@ -283,7 +302,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
         column[s] = f;
     }
-    Running<Tile::kBlocks> run;
+    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run;
     for (; t < t1; t += kWaves) {
         const int after = t + kWaves;
         wait_for_copies();
@@ -320,25 +339,28 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     }
     wait_for_copies();
     // Joined: every wavefront's maximum and total, then its sums relative to the common maximum, added in the wavefronts' order.
-    __shared__ float tops[kWaves][kRows], totals[kWaves][kRows];
-    const float own_total = add_halves(run.total);
-    if (half == 0) tops[wave][lane] = run.top, totals[wave][lane] = own_total;
+    __shared__ float tops[kWaves][kRows], totals[kWaves][kRows], exacts[kWaves][kRows];
+    const float own_total = add_halves(run.total), own_exact = add_halves(run.exact_total());
+    if (half == 0) tops[wave][lane] = run.top, totals[wave][lane] = own_total, exacts[wave][lane] = own_exact;
     __syncthreads();
     const int col = lane & 31;
     float top = tops[0][col];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) top = fmaxf(top, tops[w][col]);
     const float from = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
+    float total = 0.f, exact = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += totals[w][col] * __builtin_amdgcn_exp2f(tops[w][col] - from);
+    for (int w = 0; w < kWaves; ++w) {
+        const float part = __builtin_amdgcn_exp2f(tops[w][col] - from);
+        total += totals[w][col] * part, exact += exacts[w][col] * part;
+    }
     const bool whole = a.splits == 1;
     const float factor = __builtin_amdgcn_exp2f(run.top - from) * (whole ? (total > 0.f ? 1.0f / total : 0.f) : 1.f);
     typedef AttnOut<float, DP> Out;
     if (my_row < rows) Out::park(lds + wave * Out::kRoom, run.acc, factor, lane);
     __syncthreads();
     const int dim = a.chunks * Tile::kPerChunk;
-    float* partial = a.partial + (static_cast<int64_t>(split) * pairs + bk) * rows * (DP + 2);
+    float* partial = a.partial + (static_cast<int64_t>(split) * pairs + bk) * rows * (DP + kStats);
     for (int i = threadIdx.x; i < kRows * (DP / 4); i += kThreads) {
         const int c = i / (DP / 4), d = 4 * (i % (DP / 4)), row = first_row + c;
         if (row >= rows || d >= dim) continue;
@@ -352,16 +374,14 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
             const int tk = row / a.group, hd = kv_head * a.group + row - tk * a.group;
             store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + tk * a.out_at.token + hd * a.out_at.head + d, sum);
         } else {
-            *reinterpret_cast<float2*>(partial + row * (DP + 2) + d) = make_float2(sum.x, sum.y);
-            *reinterpret_cast<float2*>(partial + row * (DP + 2) + d + 2) = make_float2(sum.z, sum.w);
+            *reinterpret_cast<float4*>(partial + row * (DP + kStats) + d) = sum;
         }
     }
     if (wave == 0 && half == 0 && my_row < rows) {
         if (whole) {
-            if (a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+            if (LSE) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = exact > 0.f ? top + __builtin_amdgcn_logf(exact) : INFINITY;
         } else {
-            partial[my_row * (DP + 2) + DP] = top;
-            partial[my_row * (DP + 2) + DP + 1] = total;
+            *reinterpret_cast<float4*>(partial + my_row * (DP + kStats) + DP) = make_float4(top, total, exact, 0.f);
         }
     }
 }
@@ -371,52 +391,48 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
     constexpr int kLanes = DP == 96 ? 32 : DP / 4, kGroups = kThreads / kLanes;    // of a split's row, four elements each; rows of 96 leave 8 idle
-    __shared__ float tops[kGroups], totals[kGroups];
+    __shared__ float4 stats[kGroups];      // maximum, total, exact total
     __shared__ float4 sums[kGroups][kLanes];
     const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group, at = blockIdx.x;
     const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, d = 4 * lane;
-    const int64_t pitch = static_cast<int64_t>(pairs) * rows * (DP + 2);
-    const float* p = a.partial + static_cast<int64_t>(at) * (DP + 2);
+    const int64_t pitch = static_cast<int64_t>(pairs) * rows * (DP + kStats);
+    const float* p = a.partial + static_cast<int64_t>(at) * (DP + kStats);
     const bool there = d < a.chunks * AttnElem<T>::kPerChunk;
-    float top = -INFINITY, total = 0.f;
+    float top = -INFINITY, total = 0.f, exact = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto join = [&](float2 m, float4 v) {
+    auto join = [&](float4 m, float4 v) {
         const float both = fmaxf(top, m.x), from = both == -INFINITY ? 0.f : both;
         const float f = __builtin_amdgcn_exp2f(top - from), g = __builtin_amdgcn_exp2f(m.x - from);
-        top = both, total = total * f + m.y * g;
+        top = both, total = total * f + m.y * g, exact = exact * f + m.z * g;
         sum.x = sum.x * f + v.x * g, sum.y = sum.y * f + v.y * g, sum.z = sum.z * f + v.z * g, sum.w = sum.w * f + v.w * g;
     };
     constexpr int kFlight = 8;
     for (int s0 = group; s0 < a.splits; s0 += kFlight * kGroups) {
-        float2 m[kFlight];
-        float4 v[kFlight];
+        float4 m[kFlight], v[kFlight];
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
             const int s = s0 + i * kGroups;
-            m[i] = make_float2(-INFINITY, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            m[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (s < a.splits) {
-                m[i] = *reinterpret_cast<const float2*>(p + s * pitch + DP);
-                if (there) {
-                    const float2 lo = *reinterpret_cast<const float2*>(p + s * pitch + d), hi = *reinterpret_cast<const float2*>(p + s * pitch + d + 2);
-                    v[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
-                }
+                m[i] = *reinterpret_cast<const float4*>(p + s * pitch + DP);
+                if (there) v[i] = *reinterpret_cast<const float4*>(p + s * pitch + d);
             }
         }
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) join(m[i], v[i]);
     }
-    if (lane == 0) tops[group] = top, totals[group] = total;
+    if (lane == 0) stats[group] = make_float4(top, total, exact, 0.f);
     sums[group][lane] = sum;
     __syncthreads();
     if (group) return;
-    for (int g = 1; g < kGroups && g < a.splits; ++g) join(make_float2(tops[g], totals[g]), sums[g][lane]);
+    for (int g = 1; g < kGroups && g < a.splits; ++g) join(stats[g], sums[g][lane]);
     const float inv = total > 0.f ? 1.0f / total : 0.f;
     const int bk = at / rows, row = at - bk * rows, batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int token = row / a.group, head = kv_head * a.group + row - token * a.group;
     if (there)
         store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + token * a.out_at.token + head * a.out_at.head + d,
                           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-    if (lane == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+    if (lane == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = exact > 0.f ? top + __builtin_amdgcn_logf(exact) : INFINITY;
 }
 
 template <typename T, int DP>
@@ -452,7 +468,7 @@ int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys, int
     using namespace ddl;
     if (dim < 1 || dim > 128) return 0;
     const int splits = splits_for(batch, tokens, keys, heads, kv_heads);
-    return splits > 1 ? static_cast<int64_t>(splits) * batch * tokens * heads * (padded_dim(dim) + 2) : 0;
+    return splits > 1 ? static_cast<int64_t>(splits) * batch * tokens * heads * (padded_dim(dim) + kStats) : 0;
 }
 
 int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
@@ -476,24 +492,29 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
     return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr int DP = decltype(dp)::value;
-        if (a.splits == 0) {
-            if (const int rc = grant_lds<attention_rows<T, DP>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
-            a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
-            const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
+        const auto launch = [&](auto with_lse) {
+            constexpr bool LSE = decltype(with_lse)::value;
+            if (a.splits == 0) {
+                if (const int rc = grant_lds<attention_rows<T, DP, LSE>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
+                a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+                const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
+                if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
+                a.folded = folds(a.causal, grid);
+                hipLaunchKernelGGL((attention_rows<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (rows_lds<T, DP>()), s, a);
+                return check_launch("ddl_attention");
+            }
+            if (const int rc = grant_lds<attention_split<T, DP, LSE>>(split_lds<T, DP>(), "ddl_attention")) return rc;
+            const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
+            a.blocks = static_cast<int>((rows + kRows - 1) / kRows);
+            const int64_t grid = static_cast<int64_t>(a.batch) * a.kv_heads * a.splits * a.blocks;
             if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
-            a.folded = folds(a.causal, grid);
-            hipLaunchKernelGGL((attention_rows<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (rows_lds<T, DP>()), s, a);
+            hipLaunchKernelGGL((attention_split<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
             return check_launch("ddl_attention");
-        }
-        if (const int rc = grant_lds<attention_split<T, DP>>(split_lds<T, DP>(), "ddl_attention")) return rc;
-        const int64_t rows = static_cast<int64_t>(a.tokens) * a.group, pairs = static_cast<int64_t>(a.batch) * a.kv_heads;
-        a.blocks = static_cast<int>((rows + kRows - 1) / kRows);
-        const int64_t grid = pairs * a.splits * a.blocks;
-        if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
-        hipLaunchKernelGGL((attention_split<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
-        if (const int rc = check_launch("ddl_attention")) return rc;
-        if (a.splits == 1) return 0;
-        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>(pairs * rows)), dim3(kThreads), 0, s, a);
+        };
+        if (const int rc = lse ? launch(std::true_type{}) : launch(std::false_type{})) return rc;
+        if (a.splits <= 1) return 0;
+        const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
+        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, s, a);
         return check_launch("ddl_attention");
     });
 }

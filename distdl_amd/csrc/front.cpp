@@ -309,13 +309,13 @@ namespace {
 
 constexpr int64_t kMaxAttentionPitch = int64_t{1} << 22;
 
-// What ddl_attention takes as it lies.
-bool attention_tensor(const Tensor& t, const Tensor& like) {
+// Does ddl_attention take this as it lies, with heads of `dim` elements?
+bool read_in_place(const Tensor& t, int64_t dim) {
     const int64_t per = 16 / t.element_size();
-    if (!heads_tensor(t, like) || t.size(3) != like.size(3) || t.size(3) % per != 0 || t.size(3) < 1 || t.size(3) > 128 || !multiple(t.data_ptr(), 16)) return false;
+    if (t.size(3) != dim || (dim > 1 && t.stride(3) != 1) || !multiple(t.data_ptr(), 16)) return false;
     for (int i = 0; i < 3; ++i)
         if (t.size(i) > 1 && t.stride(i) % per != 0) return false;
-    return t.size(1) <= 1 || (t.stride(1) >= 0 && t.stride(1) < kMaxAttentionPitch);
+    return t.size(1) <= 1 || (t.stride(1) >= dim && t.stride(1) < kMaxAttentionPitch);
 }
 
 struct Strides3 {   // 0 where there is one element, whatever the tensor says
@@ -326,53 +326,116 @@ struct Strides3 {   // 0 where there is one element, whatever the tensor says
     operator const int64_t*() const { return of; }
 };
 
-bool attention_operands(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, const std::optional<double>& scale) {
-    if (q.dim() != 4 || !attention_tensor(q, q) || !attention_tensor(k, q) || !attention_tensor(v, q) || k.sizes() != v.sizes() || k.size(0) != q.size(0)) return false;
-    if (q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2) != 0 || (scale && !(*scale > 0 && *scale <= 3e38))) return false;
-    return !lengths || (plain(*lengths) && lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->device() == q.device());
+ddl_box_t heads_box(const Tensor& src, const Tensor& dst, int64_t extent) {
+    ddl_box_t box{};
+    box.src = src.data_ptr(), box.dst = dst.data_ptr(), box.ndim = 4;
+    for (int i = 0; i < 4; ++i) box.shape[i] = src.size(i), box.src_stride[i] = src.stride(i), box.dst_stride[i] = dst.stride(i);
+    box.shape[3] = extent;
+    return box;
 }
-float scale_of(const Tensor& q, const std::optional<double>& scale) {
-    return static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))));
+void copy_heads(const std::vector<ddl_box_t>& boxes, const Tensor& like) {
+    if (!boxes.empty())
+        check(ddl_copy_boxes(boxes.data(), static_cast<int>(boxes.size()), static_cast<int>(like.element_size()), DDL_OP_COPY, DDL_DT_BITS, current_stream()), "ddl_copy_boxes");
+}
+
+// The tensors that ddl_attention does not take as they lie become copies, with zeros behind the heads' own elements: one launch, and one for the zero.
+void lay_out(std::initializer_list<Tensor*> tensors, int64_t dim) {
+    std::vector<ddl_box_t> boxes;
+    Tensor zero;
+    std::vector<Tensor> originals;
+    for (Tensor* t : tensors) {
+        if (t->numel() == 0 ? t->size(3) == dim : read_in_place(*t, dim)) continue;
+        const Tensor from = *t;
+        originals.push_back(from);
+        *t = at::empty({from.size(0), from.size(1), from.size(2), dim}, from.options());
+        if (from.numel() == 0) continue;
+        boxes.push_back(heads_box(from, *t, from.size(3)));
+        if (from.size(3) == dim) continue;
+        if (!zero.defined()) zero = at::zeros({1}, from.options());
+        ddl_box_t box = heads_box(from, *t, dim - from.size(3));
+        box.src = zero.data_ptr(), box.dst = static_cast<char*>(t->data_ptr()) + from.size(3) * from.element_size();
+        for (int i = 0; i < 4; ++i) box.src_stride[i] = 0;
+        boxes.push_back(box);
+    }
+    if (!originals.empty()) copy_heads(boxes, originals[0]);
+}
+
+// The heads' own elements of results with padded ones.
+void crop(std::initializer_list<Tensor*> tensors, int64_t dim) {
+    std::vector<ddl_box_t> boxes;
+    std::vector<Tensor> padded;
+    for (Tensor* t : tensors) {
+        if (!t->defined() || t->size(3) == dim) continue;
+        padded.push_back(*t);
+        *t = at::empty({t->size(0), t->size(1), t->size(2), dim}, t->options());
+        if (t->numel()) boxes.push_back(heads_box(padded.back(), *t, dim));
+    }
+    if (!padded.empty()) copy_heads(boxes, padded[0]);
+}
+
+bool attention_operands(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, const std::optional<double>& scale) {
+    auto heads = [&](const Tensor& t) {
+        return t.is_cuda() && t.dim() == 4 && t.scalar_type() == q.scalar_type() && t.device() == q.device() && t.device().index() == c10::hip::current_device();
+    };
+    if (!float_code(q) || !heads(q) || !heads(k) || !heads(v) || k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3)) return false;
+    if (q.size(3) < 1 || q.size(3) > 128 || q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2) != 0 || (scale && !(*scale > 0 && *scale <= 3e38))) return false;
+    return !lengths || (plain(*lengths) && lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->device() == q.device());
 }
 const int32_t* length_pointer(const MaybeTensor& t) { return static_cast<const int32_t*>(pointer(t)); }
 
 }  // namespace
 
-std::optional<std::tuple<Tensor, Tensor>> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal,
-                                                    const std::optional<double>& scale, bool want_lse) {
-    if (!attention_operands(q, k, v, lengths, scale)) return std::nullopt;
-    const int64_t batch = q.size(0), tokens = q.size(1), keys = k.size(1), heads = q.size(2), kv_heads = k.size(2), dim = q.size(3);
-    Tensor out = at::empty(q.sizes(), q.options()), lse, work;
-    if (want_lse) lse = floats(q, {batch, heads, tokens});
+double attention_scale(const Tensor& q, const std::optional<double>& scale) { return scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))); }
+
+std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, const Tensor& v_given, const MaybeTensor& lengths, bool causal,
+                                  const std::optional<double>& scale, bool want_lse) {
+    if (!attention_operands(q_given, k_given, v_given, lengths, scale)) return std::nullopt;
+    const int64_t per = 16 / q_given.element_size(), own = q_given.size(3), dim = (own + per - 1) / per * per;
+    Attended r;
+    r.q = q_given, r.k = k_given, r.v = v_given;
+    lay_out({&r.q, &r.k, &r.v}, dim);
+    const int64_t batch = r.q.size(0), tokens = r.q.size(1), keys = r.k.size(1), heads = r.q.size(2), kv_heads = r.k.size(2);
+    Tensor work;
+    r.out = at::empty({batch, tokens, heads, dim}, r.q.options());
+    if (want_lse) r.lse = floats(r.q, {batch, heads, tokens});
     const int64_t elems = ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim);
-    if (elems) work = floats(q, {elems});
-    check(ddl_attention(q.data_ptr(), Strides3(q), k.data_ptr(), Strides3(k), v.data_ptr(), Strides3(v), float_code(q), batch, tokens, keys, heads, kv_heads, dim,
-                        length_pointer(lengths), causal, scale_of(q, scale), out.data_ptr(), Strides3(out), static_cast<float*>(pointer(lse)),
-                        static_cast<float*>(pointer(work)), elems, current_stream()),
+    if (elems) work = floats(r.q, {elems});
+    check(ddl_attention(r.q.data_ptr(), Strides3(r.q), r.k.data_ptr(), Strides3(r.k), r.v.data_ptr(), Strides3(r.v), float_code(r.q), batch, tokens, keys, heads, kv_heads,
+                        dim, length_pointer(lengths), causal, static_cast<float>(attention_scale(q_given, scale)), r.out.data_ptr(), Strides3(r.out),
+                        static_cast<float*>(pointer(r.lse)), static_cast<float*>(pointer(work)), elems, current_stream()),
           "ddl_attention");
-    return std::make_tuple(out, lse);
+    r.padded_out = r.out;
+    crop({&r.out}, own);
+    return r;
 }
 
-std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal,
-                                                                                   const std::optional<double>& scale, bool want_q, bool want_k, bool want_v) {
-    if (!attention_operands(q, k, v, lengths, scale) || dout.dim() != 4 || dout.sizes() != q.sizes() || out.sizes() != q.sizes() || !attention_tensor(dout, q) ||
-        !attention_tensor(out, q))
-        return std::nullopt;
+std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout_given, const Tensor& q, const Tensor& k, const Tensor& v,
+                                                                                   const Tensor& out, const Tensor& lse, const MaybeTensor& lengths, bool causal,
+                                                                                   double scale, bool want_q, bool want_k, bool want_v) {
+    if (!attention_operands(q, k, v, lengths, scale) || out.sizes() != q.sizes()) return std::nullopt;
     const int64_t batch = q.size(0), tokens = q.size(1), keys = k.size(1), heads = q.size(2), kv_heads = k.size(2), dim = q.size(3);
+    for (const Tensor& t : {q, k, v, out})
+        if (t.numel() && !read_in_place(t, dim)) return std::nullopt;
+    if (!dout_given.is_cuda() || dout_given.dim() != 4 || dout_given.scalar_type() != q.scalar_type() || dout_given.device() != q.device() || dout_given.size(3) > dim ||
+        dout_given.size(3) < 1 || dout_given.sizes().slice(0, 3) != q.sizes().slice(0, 3))
+        return std::nullopt;
     if (!plain(lse) || lse.scalar_type() != at::kFloat || lse.device() != q.device() || lse.numel() != batch * heads * tokens) return std::nullopt;
-    auto result = [](const Tensor& t, bool want) { return want ? MaybeTensor(at::empty(t.sizes(), t.options())) : std::nullopt; };
-    const MaybeTensor dq = result(q, want_q), dk = result(k, want_k), dv = result(v, want_v);
-    Tensor work;
+    Tensor dout = dout_given, dq, dk, dv, work;
+    lay_out({&dout}, dim);
+    if (want_q) dq = at::empty(q.sizes(), q.options());
+    if (want_k) dk = at::empty(k.sizes(), k.options());
+    if (want_v) dv = at::empty(v.sizes(), v.options());
     const int64_t elems = ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim);
     if (elems) work = floats(q, {elems});
-    auto at_rest = [](const MaybeTensor& t, const Tensor& like) { return Strides3(t ? *t : like); };
+    auto at_rest = [](const Tensor& t, const Tensor& like) { return Strides3(t.defined() ? t : like); };
     check(ddl_attention_backward(dout.data_ptr(), Strides3(dout), q.data_ptr(), Strides3(q), k.data_ptr(), Strides3(k), v.data_ptr(), Strides3(v), out.data_ptr(),
                                  Strides3(out), lse.data_ptr<float>(), float_code(q), batch, tokens, keys, heads, kv_heads, dim, length_pointer(lengths), causal,
-                                 scale_of(q, scale), target(dq), at_rest(dq, q), target(dk), at_rest(dk, k), target(dv), at_rest(dv, v),
+                                 static_cast<float>(scale), pointer(dq), at_rest(dq, q), pointer(dk), at_rest(dk, k), pointer(dv), at_rest(dv, v),
                                  static_cast<float*>(pointer(work)), elems, current_stream()),
           "ddl_attention_backward");
-    return std::make_tuple(dq, dk, dv);
+    crop({&dq, &dk, &dv}, dout_given.size(3));
+    auto maybe = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; };
+    return std::make_tuple(maybe(dq), maybe(dk), maybe(dv));
 }
 
 // ----------------------------------------------------------------- boxes --

@@ -59,12 +59,17 @@ std::optional<Two> head_norm_rotary(const MaybeTensor& q, const MaybeTensor& k, 
                                     double eps);
 std::optional<Four> head_norm_rotary_backward(const MaybeTensor& dyq, const MaybeTensor& dyk, const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight,
                                               const MaybeTensor& k_weight, const Rotation& rotation, double eps, bool want_q_weight, bool want_k_weight);
-// The result and, if asked for, each query's sum (else undefined).
-std::optional<std::tuple<Tensor, Tensor>> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal,
-                                                    const std::optional<double>& scale, bool want_lse);
+// Attention's result, each query's sum if that was asked for, and what the adjoint takes: the operands (copies with padded heads where the kernels
+// do not read them as they lie) and the result with heads as long as theirs.
+struct Attended {
+    Tensor out, lse, q, k, v, padded_out;
+};
+std::optional<Attended> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, const std::optional<double>& scale,
+                                  bool want_lse);
+double attention_scale(const Tensor& q, const std::optional<double>& scale);
 std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal,
-                                                                                   const std::optional<double>& scale, bool want_q, bool want_k, bool want_v);
+                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal, double scale,
+                                                                                   bool want_q, bool want_k, bool want_v);
 
 // The boxes of one launch with everything but the base addresses: a call adds those
 // of the slots.  Calls only read the object.

@@ -462,9 +462,9 @@ std::optional<Two> head_norm_rotary_shard(const MaybeTensor& q, const MaybeTenso
 struct AttentionShard {
     static constexpr const char* kName = "AttentionShardBackward";
     bool causal = false;
-    std::optional<double> scale;
+    double scale = 1.0;
     Shared general;
-    void identify(Key& key) const { key(int64_t{causal})(int64_t{scale.has_value()})(c10::bit_cast<int64_t>(scale.value_or(0.0)))(general); }
+    void identify(Key& key) const { key(int64_t{causal})(c10::bit_cast<int64_t>(scale))(general); }
     variable_list run(const std::vector<Tensor>& kept, const Tensor& dy_given, const Asked& asked) const {
         const Tensor dy = dy_given.detach();
         const MaybeTensor lengths = defined(kept[5]);
@@ -482,23 +482,21 @@ struct AttentionShard {
 MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, std::optional<double> scale, const Shared& general) {
     if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(v) || !ordinary(lengths)) return std::nullopt;
     const bool graph = at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v));
-    std::optional<std::tuple<Tensor, Tensor>> res;
+    std::optional<Attended> res;
     {
         at::NoGradGuard no_grad;
         res = attention(q, k, v, lengths, causal, scale, graph);
     }
-    if (!res) return std::nullopt;
-    Tensor out = std::get<0>(*res);
-    if (!graph) return out;
-    auto node = make_node(AttentionShard{causal, scale, general}, {q, k, v});
-    node->save(q);
-    node->save(k);
-    node->save(v);
-    node->save(out.detach());      // the same memory and version, without this node
-    node->save(std::get<1>(*res));
+    if (!res || !graph) return res ? MaybeTensor(res->out) : std::nullopt;
+    auto node = make_node(AttentionShard{causal, attention_scale(q, scale), general}, {q, k, v});
+    node->save(res->q);
+    node->save(res->k);
+    node->save(res->v);
+    node->save(res->padded_out.is_same(res->out) ? res->out.detach() : res->padded_out);      // the result: the same memory and version, without this node
+    node->save(res->lse);
     node->save(lengths ? *lengths : Tensor());
-    torch::autograd::create_gradient_edge(out, node);
-    return out;
+    torch::autograd::create_gradient_edge(res->out, node);
+    return res->out;
 }
 
 // ----------------------------------------------------------------- moves --

@@ -32,7 +32,9 @@ class _AttentionShard(torch.autograd.Function):
 
 
 def _general_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v):
-    """The adjoint for what its native form does not take."""
+    """The adjoint for what its native form does not take.  ``q``, ``k``, ``v`` and ``out`` may be copies whose heads are padded with zeros."""
+    own = grad_output.shape[-1]
+    q, k, v, out = (t[..., :own] for t in (q, k, v, out))
     return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v)
 
 
