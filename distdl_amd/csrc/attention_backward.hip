@@ -69,9 +69,9 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const int wave_least = scalar(keys_seen(a, wave_row, length));
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
-    const Tile tile(lds, lane);
+    Tile tile(lds, lane);
     const int tiles = (end + KEYS - 1) / KEYS;
-    const AttnCopy<T, DP, KEYS, kWaves> k_copy(k, a.k_at.token, a.chunks, wave, lane), v_copy(v, a.v_at.token, a.chunks, wave, lane);
+    const AttnCopy<T, DP, KEYS, kWaves, (DP > 96)> k_copy(k, a.k_at.token, a.chunks, wave, lane), v_copy(v, a.v_at.token, a.chunks, wave, lane);
     auto request = [&](int t) {
         const char* to = lds + (t & 1) * kTileBytes;
         k_copy.request(to, t * KEYS, end), v_copy.request(to + 2 * kTileBytes, t * KEYS, end);
@@ -100,25 +100,49 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         wait_for_copies();
         lds_barrier();
         request(t + 1);
-        const int kt = (t & 1) * kTileBytes, vt = kt + 2 * kTileBytes;
-        if (t * KEYS < wave_most) {
+        constexpr uint32_t kK = 0, kV = 2 * kTileBytes, kNext = 32 * Tile::kRowBytes;
+        bool done = t * KEYS >= wave_most;
+        if constexpr (sizeof(T) == 2 && NS == 2) {
+            if (!done && (t + 1) * KEYS <= wave_least) {     // 64 keys that all see: the vector units are at 32 of them while the matrix cores are at others
+                done = true;
+                floatx16 p0, p1, d0, d1;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p0[r] = p1[r] = d0[r] = d1[r] = 0.f;
+                auto exponential = [&](floatx16& p) {
+                    return [&](int r) { p[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, -lse))); };
+                };
+                auto difference = [&](floatx16& d, const floatx16& p) {
+                    return [&](int r) { d[r] = pinned(p[r] * (d[r] - delta)); };
+                };
+                auto nothing = [](int) {};
+                tile.template straight_woven<0>(p0, kK, q_column, nothing);
+                tile.template straight_woven<16>(d0, kV, g_column, exponential(p0));
+                tile.template straight_woven<16>(p1, kK + kNext, q_column, difference(d0, p0));
+                const typename Tile::Packed first = Tile::pack(d0);
+                tile.template straight_woven<16>(d1, kV + kNext, g_column, exponential(p1));
+                tile.template transposed_woven<16>(acc, kK, first, difference(d1, p1));
+                tile.template transposed_woven<0>(acc, kK + kNext, Tile::pack(d1), nothing);
+            }
+        }
+        if (!done) {
             const bool masked = (t + 1) * KEYS > wave_least;
             const int rest = seen - t * KEYS - 4 * half;
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 floatx16 s[2];
                 clear(s);
-                tile.straight(s[0], kt, n, q_column);
-                tile.straight(s[1], vt, n, g_column);
+                tile.straight(s[0], kK, n, q_column);
+                tile.straight(s[1], kV, n, g_column);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.scale_log2, -lse));
                     if (masked) p = 32 * n + (r & 3) + 8 * (r >> 2) < rest ? p : 0.f;
                     s[0][r] = p * (s[1][r] - delta);
                 }
-                tile.transposed(acc, kt, n, Tile::pack(s[0]));
+                tile.transposed(acc, kK, n, Tile::pack(s[0]));
             }
         }
+        tile.shift(t & 1 ? -kTileBytes : kTileBytes);
     }
     wait_for_copies();
     lds_barrier();
@@ -216,41 +240,7 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     floatx16 sums[ROLES ? 1 : 2][Tile::kBlocks];      // two roles: one sum a wavefront
     floatx16(&dk)[Tile::kBlocks] = sums[0], (&dv)[Tile::kBlocks] = sums[ROLES ? 0 : 1];
     clear(dk), clear(dv);
-    constexpr int kS = Tile::kSteps, kT = 2 * Tile::kBlocks;
-    const std::integral_constant<int, 16> all16{};
-    const std::integral_constant<int, 0> none{};
     auto nothing = [](int) {};
-    // Scores or dO . v of 32 queries, and the sums' share of them, with `count` calls of `vector` between the matrix instructions.
-    auto chain = [&](floatx16& to, uint32_t from, const Frag (&column)[kS], auto count, auto&& vector) {
-        if constexpr (sizeof(T) == 2) {
-            Frag f[kS];
-            f[0] = tile.read_straight(from, 0), f[1] = tile.read_straight(from, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            weave<kS, decltype(count)::value>(
-                [&](int i) {
-                    if (i + 2 < kS) f[i + 2] = tile.read_straight(from, i + 2);
-                    mfma_chunk(to, f[i], column[i], static_cast<const T*>(nullptr));
-                },
-                vector);
-        } else {
-            tile.straight(to, from, 0, column);
-        }
-    };
-    auto sum = [&](floatx16 (&to)[Tile::kBlocks], uint32_t from, const typename Tile::Packed& p, auto count, auto&& vector) {
-        if constexpr (sizeof(T) == 2) {
-            shortx8 f[kT];
-            f[0] = tile.read_transposed(from, 0, 0), f[1] = tile.read_transposed(from, 1 / Tile::kBlocks, 1 % Tile::kBlocks);
-            __builtin_amdgcn_sched_barrier(0);
-            weave<kT, decltype(count)::value>(
-                [&](int i) {
-                    if (i + 2 < kT) f[i + 2] = tile.read_transposed(from, (i + 2) / Tile::kBlocks, (i + 2) % Tile::kBlocks);
-                    mfma_chunk(to[i % Tile::kBlocks], f[i], i / Tile::kBlocks ? p.hi : p.lo, static_cast<const T*>(nullptr));
-                },
-                vector);
-        } else {
-            tile.transposed(to, from, 0, p);
-        }
-    };
     // Row values (sums or D) of the rows that this half of the lanes holds, four at a time, the next four on their way.
     struct OfRows {
         const float* at;
@@ -308,26 +298,26 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
         floatx16 p0, p1, d0, d1;
         zero(p0), zero(p1), zero(d0), zero(d1);
         OfRows lse0(rows);
-        chain(p0, kQ, k_column, none, nothing);
+        tile.template straight_woven<0>(p0, kQ, k_column, nothing);
         if constexpr (fk) {
-            chain(d0, kG, v_column, all16, exponential(p0, lse0));
+            tile.template straight_woven<16>(d0, kG, v_column, exponential(p0, lse0));
             const typename Tile::Packed b0 = Tile::pack(p0);
             OfRows delta0(rows + ROWS);
-            chain(p1, kQ + kNext, k_column, all16, difference(d0, p0, delta0));
+            tile.template straight_woven<16>(p1, kQ + kNext, k_column, difference(d0, p0, delta0));
             const typename Tile::Packed a0 = Tile::pack(d0);
             OfRows lse1(rows + 32);
-            chain(d1, kG + kNext, v_column, all16, exponential(p1, lse1));
+            tile.template straight_woven<16>(d1, kG + kNext, v_column, exponential(p1, lse1));
             const typename Tile::Packed b1 = Tile::pack(p1);
             OfRows delta1(rows + ROWS + 32);
-            if constexpr (fv) sum(dv, kG, b0, none, nothing);
-            sum(dk, kQ, a0, all16, difference(d1, p1, delta1));
-            if constexpr (fv) sum(dv, kG + kNext, b1, none, nothing);
-            sum(dk, kQ + kNext, Tile::pack(d1), none, nothing);
+            if constexpr (fv) tile.template transposed_woven<0>(dv, kG, b0, nothing);
+            tile.template transposed_woven<16>(dk, kQ, a0, difference(d1, p1, delta1));
+            if constexpr (fv) tile.template transposed_woven<0>(dv, kG + kNext, b1, nothing);
+            tile.template transposed_woven<0>(dk, kQ + kNext, Tile::pack(d1), nothing);
         } else {
-            chain(p1, kQ + kNext, k_column, all16, exponential(p0, lse0));
+            tile.template straight_woven<16>(p1, kQ + kNext, k_column, exponential(p0, lse0));
             OfRows lse1(rows + 32);
-            sum(dv, kG, Tile::pack(p0), all16, exponential(p1, lse1));
-            sum(dv, kG + kNext, Tile::pack(p1), none, nothing);
+            tile.template transposed_woven<16>(dv, kG, Tile::pack(p0), exponential(p1, lse1));
+            tile.template transposed_woven<0>(dv, kG + kNext, Tile::pack(p1), nothing);
         }
     };
     auto walk = [&](auto fk, auto fv) {

@@ -120,6 +120,24 @@ __device__ inline shortx8 scale8(const shortx8& v, float factor, const __half*) 
     return __builtin_bit_cast(shortx8, o);
 }
 
+// `N` matrix instructions, behind each of which a share of other work is issued: matrix(i), then the parts of vector(r), r < COUNT, that fall to
+// it, in this order -- left to itself the compiler puts one kind behind the other, and then one kind of unit waits.
+template <int N, int COUNT, typename M, typename V>
+__device__ inline void weave(M&& matrix, V&& vector) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        matrix(i);
+#pragma unroll
+        for (int r = COUNT * i / N; r < COUNT * (i + 1) / N; ++r) vector(r);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// A value that is computed here and not where it is used.
+__device__ inline float pinned(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Rows of DP elements of type T in LDS.
 template <typename T, int DP>
 struct AttnTile {
@@ -202,6 +220,22 @@ struct AttnTile {
         }
     }
 
+    // The same for the block at `from`, woven with COUNT calls of `vector`; nothing to weave in fp32, whose matrix instructions take most of the time.
+    template <int COUNT, typename V>
+    __device__ void straight_woven(floatx16& acc, uint32_t from, const Frag (&column)[kSteps], V&& vector) const {
+        if constexpr (sizeof(T) == 2) {
+            Frag f[kSteps];
+            f[0] = read_straight(from, 0), f[1] = read_straight(from, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            weave<kSteps, COUNT>(
+                [&](int i) {
+                    if (i + 2 < kSteps) f[i + 2] = read_straight(from, i + 2);
+                    mfma_chunk(acc, f[i], column[i], static_cast<const T*>(nullptr));
+                },
+                vector);
+        }
+    }
+
     // The same with the columns in a tile of their own.
     __device__ void straight(floatx16& acc, uint32_t tile, uint32_t columns) const {
 #pragma unroll
@@ -230,6 +264,22 @@ struct AttnTile {
     static __device__ void scale_packed(Packed& p, float factor) {
         if constexpr (sizeof(T) == 2) p.lo = scale8(p.lo, factor, static_cast<const T*>(nullptr)), p.hi = scale8(p.hi, factor, static_cast<const T*>(nullptr));
         else p *= factor;
+    }
+
+    template <int COUNT, typename V>
+    __device__ void transposed_woven(floatx16 (&acc)[kBlocks], uint32_t from, const Packed& p, V&& vector) const {
+        if constexpr (sizeof(T) == 2) {
+            constexpr int kReads = 2 * kBlocks;
+            shortx8 f[kReads];
+            f[0] = read_transposed(from, 0, 0), f[1] = read_transposed(from, 1 / kBlocks, 1 % kBlocks);
+            __builtin_amdgcn_sched_barrier(0);
+            weave<kReads, COUNT>(
+                [&](int i) {
+                    if (i + 2 < kReads) f[i + 2] = read_transposed(from, (i + 2) / kBlocks, (i + 2) % kBlocks);
+                    mfma_chunk(acc[i % kBlocks], f[i], i / kBlocks ? p.hi : p.lo, static_cast<const T*>(nullptr));
+                },
+                vector);
+        }
     }
 
     // acc[d block] += tile rows 32 block .. + 31, transposed, times p of this lane's column.
@@ -297,57 +347,54 @@ struct AttnStage {
 // ROWS rows of a tensor straight from memory into a tile, by the WAVES wavefronts of a workgroup, without passing registers: every copy instruction
 // fills 1 KiB of the tile, lane after lane, so a lane takes the chunk that belongs where it writes.  Rows from the end on and chunks
 // behind the head's own lie outside the buffer that the copies are told of, which gives zeros.
-template <typename T, int DP, int ROWS, int WAVES>
+//
+// LEAN: one offset a lane and a base for every instruction, scalar work instead of registers.
+template <typename T, int DP, int ROWS, int WAVES, bool LEAN = false>
 struct AttnCopy {
     typedef AttnTile<T, DP> Tile;
     static constexpr int kSlots = Tile::kRowBytes / 16, kPieces = ROWS * kSlots / (64 * WAVES);
     static_assert(ROWS * kSlots % (64 * WAVES) == 0, "whole instructions for every wavefront");
+    // Rows from one instruction of a wavefront to its next; where the swizzle does not change over them, all can have one offset.
+    static constexpr int kStep = 64 * WAVES / kSlots;
+    static constexpr bool kSame = LEAN && kStep % 16 == 0;
     const char* base;
     int64_t pitch;             // bytes
     int row_bytes, wave;
-    uint32_t offset[kPieces];
+    uint32_t offset[kSame ? 1 : kPieces];
 
     __device__ AttnCopy(const T* tensor, int64_t pitch_elems, int chunks, int wave, int lane)
         : base(reinterpret_cast<const char*>(tensor)), pitch(pitch_elems * static_cast<int>(sizeof(T))), row_bytes(16 * chunks), wave(wave) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
+        for (int i = 0; i < (kSame ? 1 : kPieces); ++i) {
             const int at = (i * WAVES + wave) * 64 + lane, row = at / kSlots, c = (at % kSlots) ^ Tile::swizzle(row);
             offset[i] = c < chunks ? static_cast<uint32_t>(row) * static_cast<uint32_t>(pitch) + 16 * c : 0x7FFFFFF0u;
         }
     }
     // Rows first .. first + ROWS of the tensor, which ends with row `end`.
     __device__ void request(const char* tile, int first, int end) const {
-        const int rows = end - first;
-        u32x4 buffer = raw_buffer(base + first * pitch);
-        buffer[2] = rows > 0 ? static_cast<uint32_t>((rows < ROWS ? rows - 1 : ROWS - 1) * static_cast<uint32_t>(pitch) + row_bytes) : 0u;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile));
+        auto buffer_from = [&](int row) {     // a tile's rows from there on; the same in all lanes, as the instruction wants it
+            const int rows = end - row;
+            u32x4 buffer = raw_buffer(base + row * pitch);
+            buffer[2] = rows > 0 ? static_cast<uint32_t>((rows < ROWS ? rows - 1 : ROWS - 1) * static_cast<uint32_t>(pitch) + row_bytes) : 0u;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) buffer[i] = __builtin_amdgcn_readfirstlane(buffer[i]);     // the same in all lanes, as the instruction wants it
-        const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tile)));
+            for (int i = 0; i < 3; ++i) buffer[i] = __builtin_amdgcn_readfirstlane(buffer[i]);
+            return buffer;
+        };
+        auto place = [&](int i) { return reinterpret_cast<const char*>(static_cast<uintptr_t>(to + (i * WAVES + wave) * 1024)); };
+        if constexpr (kSame) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) dma16(buffer, offset[i], 0, reinterpret_cast<const char*>(static_cast<uintptr_t>(to + (i * WAVES + wave) * 1024)));
+            for (int i = 0; i < kPieces; ++i) dma16(buffer_from(first + i * kStep), offset[0], 0, place(i));
+        } else {
+            const u32x4 buffer = buffer_from(first);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) dma16(buffer, offset[i], 0, place(i));
+        }
     }
 };
 
 // All requested copies of this wavefront have landed; with a barrier behind it, those of the workgroup.
 __device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// `N` matrix instructions, behind each of which a share of other work is issued: matrix(i), then the parts of vector(r), r < COUNT, that fall to
-// it, in this order -- left to itself the compiler puts one kind behind the other, and then one kind of unit waits.
-template <int N, int COUNT, typename M, typename V>
-__device__ inline void weave(M&& matrix, V&& vector) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        matrix(i);
-#pragma unroll
-        for (int r = COUNT * i / N; r < COUNT * (i + 1) / N; ++r) vector(r);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-}
-// A value that is computed here and not where it is used.
-__device__ inline float pinned(float v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
 
 // The value of lane l ^ 32 and this lane's, combined.
 template <typename Fn>
