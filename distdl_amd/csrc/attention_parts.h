@@ -85,24 +85,23 @@ __device__ inline shortx8 pack8(const floatx16& v, int first, const __half*) {
     return __builtin_bit_cast(shortx8, o);
 }
 
-// total + eight packed values, rounded as they are: a weighted mean's weights then add up to what it is divided by, and a single large one
-// comes out as exactly 1.  (Half as many instructions as the sum of the unrounded ones, too.)
-__device__ inline float add8(float total, const shortx8& v, const bf16_t*) {
+// total + two packed values, rounded as they are: a weighted mean's weights then add up to what it is divided by, and a single large one comes
+// out as exactly 1.  (Half as many instructions as the sum of the unrounded ones, too.)
+__device__ inline float add2(float total, uint32_t v, const bf16_t*) {
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
-    pair p[4];
-    const pair one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
-    __builtin_memcpy(p, &v, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) total = __builtin_amdgcn_fdot2_f32_bf16(p[i], one, total, false);
-    return total;
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, v), pair{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, total, false);
 }
-__device__ inline float add8(float total, const shortx8& v, const __half*) {
+__device__ inline float add2(float total, uint32_t v, const __half*) {
     typedef _Float16 pair __attribute__((ext_vector_type(2)));
-    pair p[4];
-    const pair one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
-    __builtin_memcpy(p, &v, 16);
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, v), pair{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, total, false);
+}
+
+template <typename T>
+__device__ inline float add8(float total, const shortx8& v, const T* type) {
+    uint32_t w[4];
+    __builtin_memcpy(w, &v, 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) total = __builtin_amdgcn_fdot2(p[i], one, total, false);
+    for (int i = 0; i < 4; ++i) total = add2(total, w[i], type);
     return total;
 }
 
@@ -548,11 +547,12 @@ inline int fill_attention(AttnArgs& a, bool& nothing, const char* what, std::ini
     if (dim > 128) return fail(DDL_E_UNSUPP, "%s: heads of %lld elements (at most 128)", what, static_cast<long long>(dim));
     const int per = dtype == DDL_DT_F32 ? 4 : 8;
     if (dim % per) return fail(DDL_E_ALIGN, "%s: heads of %lld elements are no multiple of 16 bytes", what, static_cast<long long>(dim));
-    if (!(scale > 0.f && scale <= 3.0e38f)) return fail(DDL_E_ARG, "%s: scale %g is not positive", what, static_cast<double>(scale));
+    if (!(scale > 0.f && scale <= 1.0e38f)) return fail(DDL_E_ARG, "%s: scale %g is not positive", what, static_cast<double>(scale));
     if (heads && (kv_heads == 0 || heads % kv_heads))
         return fail(DDL_E_SHAPE, "%s: %lld heads cannot share %lld key heads", what, static_cast<long long>(heads), static_cast<long long>(kv_heads));
     if ((heads && (tokens > 0x3FFFFFFF / heads || batch > 0x3FFFFFFF / heads)) || keys > 0x3FFFFFFF || heads > 0x3FFFFFFF)
         return fail(DDL_E_UNSUPP, "%s: 2^30 rows or keys", what);
+    if (heads == 0 && kv_heads) return fail(DDL_E_SHAPE, "%s: key heads without heads", what);
     nothing = batch == 0 || heads == 0 || (tokens == 0 && keys == 0);
     if (nothing) return 0;
     int i = 0;

@@ -378,7 +378,7 @@ bool attention_operands(const Tensor& q, const Tensor& k, const Tensor& v, const
         return t.is_cuda() && t.dim() == 4 && t.scalar_type() == q.scalar_type() && t.device() == q.device() && t.device().index() == c10::hip::current_device();
     };
     if (!float_code(q) || !heads(q) || !heads(k) || !heads(v) || k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3)) return false;
-    if (q.size(3) < 1 || q.size(3) > 128 || q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2) != 0 || (scale && !(*scale > 0 && *scale <= 3e38))) return false;
+    if (q.size(3) < 1 || q.size(3) > 128 || q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2) != 0 || (scale && !(*scale > 0 && *scale <= 1e38))) return false;
     return !lengths || (plain(*lengths) && lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->device() == q.device());
 }
 const int32_t* length_pointer(const MaybeTensor& t) { return static_cast<const int32_t*>(pointer(t)); }

@@ -1280,7 +1280,7 @@ def _attention_operands(q, k, v, lengths, scale, name):
     if lengths is not None and not lengths.is_contiguous():
         lengths = contiguous(lengths)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    if not 0 < scale <= 3e38:
+    if not 0 < scale <= 1e38:
         raise ValueError(f"{name}: scale {scale} is not positive")
     per = 16 // q.element_size()
     dim = -(-q.shape[3] // per) * per
@@ -1297,6 +1297,9 @@ def attention(q, k, v, lengths=None, causal=False, scale=None, want_lse=False):
     batch, tokens, heads, _ = q.shape
     keys, kv_heads = k.shape[1:3]
     lib = _lib.load()
+    if heads == 0:
+        out = torch.empty(q.shape[:3] + (head_dim,), dtype=q.dtype, device=q.device)
+        return (out, torch.empty((batch, 0, tokens), dtype=torch.float32, device=q.device)) if want_lse else out
     with _on_device_of(q):
         out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
         lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if want_lse else None
@@ -1325,6 +1328,9 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scal
     if lse.dtype != torch.float32 or tuple(lse.shape) != (batch, heads, tokens) or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError(f"{name}: lse must be contiguous float32 [{batch}, {heads}, {tokens}] on {q.device}")
     lib = _lib.load()
+    if heads == 0:
+        return tuple(torch.zeros(t.shape[:3] + (head_dim,), dtype=q.dtype, device=q.device) if want else None
+                     for t, want in ((q, want_q), (k, want_k), (v, want_v)))
     with _on_device_of(q):
         dout, out = (_aligned_heads(_heads(t, name, q), dim) for t in (dout, out))
         grads = [torch.empty(t.shape, dtype=q.dtype, device=q.device) if want else None for t, want in ((q, want_q), (k, want_k), (v, want_v))]

@@ -669,7 +669,9 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  *            exp(scale q . k) (+inf without keys), for the adjoint
  *   workspace  device memory of ddl_attention_workspace(...) floats, 16-byte
  *            aligned (few queries: the keys are split over workgroups)
- * scale > 0.  16-byte aligned tensors with strides and head_dim that are multiples
+ * 0 < scale <= 1e38.  Values of keys that some query of a sequence sees are to be
+ * finite (a zero probability times an infinite one is not a number).  16-byte
+ * aligned tensors with strides and head_dim that are multiples
  * of 16 bytes (DDL_E_ALIGN; zeros behind a head's elements change nothing),
  * head_dim <= 128 (DDL_E_UNSUPP).  Probabilities are rounded to the element
  * type for the product with the values. */
@@ -690,7 +692,8 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
  * dv may be NULL; `workspace`: device memory of
  * ddl_attention_backward_workspace(...) floats, 16-byte aligned.  Nothing is added
  * atomically: equal calls give equal bits.  Probabilities and dS are rounded to
- * the element type for their products.  Limits as ddl_attention's. */
+ * the element type for their products: in fp16, dS beyond 65504 is infinite.
+ * Limits as ddl_attention's. */
 int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens,
                                          int64_t keys, int64_t heads,
                                          int64_t kv_heads, int64_t head_dim);

@@ -196,6 +196,15 @@ def test_nothing_to_attend(shape):
         assert grad.shape == leaf.shape and not grad.any()
 
 
+def test_key_heads_without_heads():
+    from distdl_amd import nn
+    k = torch.randn(2, 5, 2, 16, device="cuda", requires_grad=True)
+    q = torch.randn(2, 3, 0, 16, device="cuda", requires_grad=True)
+    out = nn.attention_shard(q, k, k)
+    assert out.shape == q.shape
+    assert not torch.autograd.grad(out.sum(), [k])[0].any()
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("slope", [0.02, 0.3, -0.3])
 def test_maxima_that_rise_and_fall_along_the_keys(dt, slope):
@@ -359,3 +368,40 @@ def test_block_of_an_attention_layer(causal):
     for a, b in zip([got] + list(grads), [want] + list(torch.autograd.grad(want, [copies[t] for t in leaves], dy.double().cpu()))):
         a, b = _f64(a), b.detach().numpy()
         assert np.abs(a - b).max() <= 2.0 ** -10 * np.abs(b).max()
+
+
+def test_layers_over_batch_and_heads_of_four_workers():
+    """Head norms with positions and attention on a 2 x 2 partition of batch and heads, every worker a thread: the workers' results are the whole
+    tensor's, bit for bit, and the norms' weights, which live on the first worker, get the gradient of all tokens and heads (sums of another order:
+    2^-17 of the magnitude that a single worker's would be off by, as for the head norms alone)."""
+    from distdl_amd import nn
+    from distdl_amd.backends.stub_hip import SimWorld
+    g = torch.Generator().manual_seed(13)
+    batch, tokens, heads, kv, dim = 4, 21, 4, 2, 32
+    q, k, v, dy = (torch.randn(batch, tokens, h, dim, generator=g) for h in (heads, kv, kv, heads))
+    lengths = torch.tensor([21, 7, 0, 20], dtype=torch.int32)
+
+    def body(P_world, P_shape):
+        P = P_world.create_partition_inclusive(list(range(int(np.prod(P_shape))))).create_cartesian_topology_partition(P_shape)
+        if not P.active:
+            return None
+        norm, attend = nn.DistributedHeadNormRotary(P, dim, rotated=16), nn.DistributedAttention(P, causal=True)
+
+        def own(t):
+            for d in (0, 2) if t.dim() == 4 else (0,):
+                t = t.chunk(P_shape[d], d)[P.index[d]]
+            return t.contiguous().cuda()
+
+        a, b = own(q).requires_grad_(), own(k).requires_grad_()
+        y = attend(*norm(a, b), own(v), own(lengths))
+        y.backward(own(dy))
+        grads = [w.grad for w in (norm.q_weight, norm.k_weight)]
+        return tuple(P.index), y.detach().cpu(), a.grad.cpu(), b.grad.cpu(), [None if w is None else w.cpu() for w in grads]
+
+    whole = SimWorld(1).run(lambda P: body(P, [1, 1, 1, 1]))[0]
+    parts = SimWorld(4).run(lambda P: body(P, [2, 1, 2, 1]))
+    for index, y, dq, dk, _ in parts:
+        for mine, all_ in ((y, whole[1]), (dq, whole[2]), (dk, whole[3])):
+            assert torch.equal(mine, all_.chunk(2, 0)[index[0]].chunk(2, 2)[index[2]])
+    for got, want in zip(parts[0][4], whole[4]):
+        assert (got - want).abs().max() <= 2.0 ** -17 * batch * tokens * heads * want.abs().max()

@@ -113,7 +113,7 @@ def _attention(lib, **change):
 ATTENTION_REFUSALS = [
     (dict(dtype=_lib.DDL_DT_I32), -1, "dtype"), (dict(tokens=-1), -1, "negative"), (dict(dim=136), -5, "at most 128"), (dict(dim=60), -3, "16 bytes"),
     (dict(kv=0), -4, "cannot share"), (dict(heads=3, kv=2), -4, "cannot share"), (dict(scale=0.0), -1, "positive"), (dict(scale=-1.0), -1, "positive"),
-    (dict(scale=float("nan")), -1, "positive"), (dict(scale=float("inf")), -1, "positive"), (dict(q=None), -1, "null"), (dict(v=None), -1, "null"),
+    (dict(scale=float("nan")), -1, "positive"), (dict(scale=float("inf")), -1, "positive"), (dict(scale=2e38), -1, "positive"), (dict(heads=0), -4, "without heads"), (dict(q=None), -1, "null"), (dict(v=None), -1, "null"),
     (dict(outs=None), -1, "null"), (dict(k=8), -3, "aligned"), (dict(ks=_i64(64, 60, 64)), -3, "multiples"), (dict(ks=_i64(64, 1 << 22, 64)), -5, "2^22"),
     (dict(vs=_i64(64, -64, 64)), -5, "2^22"), (dict(tokens=1 << 30), -5, "2^30"), (dict(keys=1 << 30), -5, "2^30"),
 ]
