@@ -97,6 +97,10 @@ constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // With tiles of NS blocks, keys are read up to one block before and values one block after the softmax: one barrier a tile, in
 // front of its last block, is then enough for two buffers of each.  What follows it is copied to where
 // everybody has just finished reading: keys two tiles ahead, values NS - 1 blocks ahead.
+//
+// [4,4096,16,128] bf16, all keys: 624 us (881 TFLOP/s; 754 with the parts one behind the other and tiles through registers); head size
+// 64: 303 us, causal: 273 us (1000), fp32 [2,2048,8,64] 159 us (108).  Bound by issue: the exponentials and the softmax's other
+// vector work next to the matrix instructions, of which each pipe is busy about half of the time.
 template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
@@ -265,7 +269,9 @@ constexpr int rows_lds() {
 
 // Few queries, many keys: the queries of all heads that share a key head (row = token x group + head in the group) in one
 // wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with tiles of its own
-// and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).
+// and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).  Bound by memory where
+// there are enough tiles ([64,1,32,128] bf16, 8 key heads of 2048: 76 us, 4.7 TB/s), by the latency of a few tiles and the join's
+// launch where there are not ([1,1,8,128], 65536 keys of one head: 18.9 us).
 // (Rows of more than 256 bytes fill the registers of a SIMD with one wavefront: 128 of them for the tiles on their way.)
 template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_split(const AttnArgs a) {
@@ -275,7 +281,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
     const int pairs = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % pairs, rest_id = blockIdx.x / pairs, split = rest_id % a.splits, block = rest_id / a.splits;
+    const int bk = blockIdx.x % pairs, rest_id = blockIdx.x / pairs, split = rest_id % a.splits;
+    const int block = a.blocks - 1 - rest_id / a.splits;      // the last rows, which see most keys in the causal form, first
     const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
     const int rows = a.tokens * a.group, first_row = block * kRows, my_row = first_row + (lane & 31);
@@ -386,15 +393,19 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     }
 }
 
-// The splits of a row, a workgroup for each row: groups of DP / 4 lanes take a share of the splits each (eight of them in flight), in
-// one pass with a running maximum, and are joined in their order.
-template <typename T, int DP>
+// The splits of a row: groups of DP / 4 lanes take every GROUPS-th of them (eight in flight), in one pass with a running maximum, and are
+// joined in their order.  GROUPS = 1, for up to eight splits: a group has a row to itself ([1,512,8,128] bf16 to 1024 keys, two splits:
+// 15.3 us for both kernels, with a workgroup for each row 20).
+constexpr int kSplitsInFlight = 8;
+template <int DP>
+constexpr int join_lanes() { return DP == 96 ? 32 : DP / 4; }      // of a split's row, four elements each; rows of 96 leave 8 idle
+template <typename T, int DP, int GROUPS>
 __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
-    constexpr int kLanes = DP == 96 ? 32 : DP / 4, kGroups = kThreads / kLanes;    // of a split's row, four elements each; rows of 96 leave 8 idle
-    __shared__ float4 stats[kGroups];      // maximum, total, exact total
-    __shared__ float4 sums[kGroups][kLanes];
-    const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group, at = blockIdx.x;
-    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, d = 4 * lane;
+    constexpr int kLanes = join_lanes<DP>(), kAtOnce = kThreads / kLanes / GROUPS;      // rows of a workgroup
+    const int pairs = a.batch * a.kv_heads, rows = a.tokens * a.group;
+    const int place = threadIdx.x / kLanes, group = GROUPS == 1 ? 0 : place, lane = threadIdx.x % kLanes, d = 4 * lane;
+    const int at = static_cast<int>(blockIdx.x) * kAtOnce + (GROUPS == 1 ? place : 0);
+    if (GROUPS == 1 && at >= pairs * rows) return;
     const int64_t pitch = static_cast<int64_t>(pairs) * rows * (DP + kStats);
     const float* p = a.partial + static_cast<int64_t>(at) * (DP + kStats);
     const bool there = d < a.chunks * AttnElem<T>::kPerChunk;
@@ -406,12 +417,11 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
         top = both, total = total * f + m.y * g, exact = exact * f + m.z * g;
         sum.x = sum.x * f + v.x * g, sum.y = sum.y * f + v.y * g, sum.z = sum.z * f + v.z * g, sum.w = sum.w * f + v.w * g;
     };
-    constexpr int kFlight = 8;
-    for (int s0 = group; s0 < a.splits; s0 += kFlight * kGroups) {
-        float4 m[kFlight], v[kFlight];
+    for (int s0 = group; s0 < a.splits; s0 += kSplitsInFlight * GROUPS) {
+        float4 m[kSplitsInFlight], v[kSplitsInFlight];
 #pragma unroll
-        for (int i = 0; i < kFlight; ++i) {
-            const int s = s0 + i * kGroups;
+        for (int i = 0; i < kSplitsInFlight; ++i) {
+            const int s = s0 + i * GROUPS;
             m[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (s < a.splits) {
                 m[i] = *reinterpret_cast<const float4*>(p + s * pitch + DP);
@@ -419,13 +429,17 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < kFlight; ++i) join(m[i], v[i]);
+        for (int i = 0; i < kSplitsInFlight; ++i) join(m[i], v[i]);
     }
-    if (lane == 0) stats[group] = make_float4(top, total, exact, 0.f);
-    sums[group][lane] = sum;
-    __syncthreads();
-    if (group) return;
-    for (int g = 1; g < kGroups && g < a.splits; ++g) join(stats[g], sums[g][lane]);
+    if constexpr (GROUPS > 1) {
+        __shared__ float4 stats[GROUPS];      // maximum, total, exact total
+        __shared__ float4 sums[GROUPS][kLanes];
+        if (lane == 0) stats[group] = make_float4(top, total, exact, 0.f);
+        sums[group][lane] = sum;
+        __syncthreads();
+        if (group) return;
+        for (int g = 1; g < GROUPS && g < a.splits; ++g) join(stats[g], sums[g][lane]);
+    }
     const float inv = total > 0.f ? 1.0f / total : 0.f;
     const int bk = at / rows, row = at - bk * rows, batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int token = row / a.group, head = kv_head * a.group + row - token * a.group;
@@ -444,19 +458,34 @@ constexpr int split_lds() {
 
 int padded_dim(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
-// Into how many parts the keys are split; 0: attention_rows.
-int splits_for(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
-    if (tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1 || batch < 1) return 0;
+// Row blocks of attention_split, times sequences and key heads.
+int64_t split_units(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
+    return batch * kv_heads * ((tokens * (heads / kv_heads) + kRows - 1) / kRows);
+}
+
+// Does attention_split take it?  A wavefront's 32 rows cost it about twice as much as attention_rows, which has 128 in a workgroup walk over the same
+// tile and overlaps the parts of a step; but its workgroups share the keys, while attention_rows takes the longest row's time however few
+// workgroups there are.  So: where attention_rows would mostly have rows that do not exist, or where there are not enough workgroups to be worth it
+// (measured: [1,512,16,128] bf16 to 4096 keys 41 us here and 70 there, [4,256,16,128] 80 and 81, [16,100,16,128] to 1500 115 and 46; head size 64:
+// 31 and 53, 36 and 54, 48 and 29; fp32, whose matrix instructions leave little to overlap: 101 and 311, 156 and 314, 136 and 125).
+bool takes_split(const AttnArgs& a, bool wide) {
     int dev;
-    const int64_t cus = compute_units(dev);
-    const int64_t rows = tokens * (heads / kv_heads), row_blocks = (rows + kRows - 1) / kRows;
-    const int64_t whole = batch * heads * ((tokens + kRows * kWaves - 1) / (kRows * kWaves));
-    if (rows > 4 * kRows || (whole >= 2 * cus && tokens >= kRows)) return 0;
-    // Two workgroups a CU, each with at least four tiles of 32 keys for each of its wavefronts.
-    const int64_t units = batch * kv_heads * row_blocks, most = (keys + 511) / 512;
-    int64_t splits = (2 * cus + units - 1) / units;
-    if (splits > most) splits = most;
-    return static_cast<int>(splits < 1 ? 1 : splits);
+    const int64_t cus = compute_units(dev), units = split_units(a.batch, a.tokens, a.heads, a.kv_heads);
+    const int64_t whole = static_cast<int64_t>(a.batch) * a.heads * ((a.tokens + kRows * kWaves - 1) / (kRows * kWaves));
+    const int64_t mean = a.causal ? a.keys - (a.tokens < a.keys ? a.tokens : a.keys) / 2 : a.keys;      // keys of a row
+    return units < 2 * whole || 2 * units * mean < (!wide ? 6 : 2 * whole <= cus ? 5 : 3) * cus * a.keys;
+}
+
+// Into how many parts it splits the keys: a workgroup for each CU, with at least 256 keys (two tiles of 32 for each of its wavefronts); up to 512 stay
+// together, the join costs more (2 x 512 keys, 16 heads of 64: 7.3 us, in two parts 8.5).  [16,1,8,128] bf16 to 4096 keys of one head: 13.5 us, with at
+// least 512 keys 16, with 128 13.4 (but one sequence of 65536 keys 22.7 instead of 18.9: the join); two workgroups for each CU:
+// [8,1,32,128] to 2048 keys 43 us instead of 39.
+int splits_for(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
+    if (tokens < 1 || keys <= 512 || heads < 1 || kv_heads < 1 || batch < 1) return 1;
+    int dev;
+    const int64_t units = split_units(batch, tokens, heads, kv_heads), most = (keys + 255) / 256;
+    const int64_t splits = (compute_units(dev) + units - 1) / units;
+    return static_cast<int>(splits < most ? splits : most);
 }
 
 }  // namespace
@@ -489,12 +518,12 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
     if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention: workspace is not 16-byte aligned");
     a.partial = workspace;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) {
+    return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) -> int {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr int DP = decltype(dp)::value;
         const auto launch = [&](auto with_lse) {
             constexpr bool LSE = decltype(with_lse)::value;
-            if (a.splits == 0) {
+            if (!takes_split(a, sizeof(T) == 2 && DP > 64)) {
                 if (const int rc = grant_lds<attention_rows<T, DP, LSE>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
                 a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
                 const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
@@ -514,7 +543,11 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
         if (const int rc = lse ? launch(std::true_type{}) : launch(std::false_type{})) return rc;
         if (a.splits <= 1) return 0;
         const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
-        hipLaunchKernelGGL((attention_join<T, DP>), dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, s, a);
+        constexpr int kGroups = kThreads / join_lanes<DP>();
+        if (a.splits <= kSplitsInFlight)
+            hipLaunchKernelGGL((attention_join<T, DP, 1>), dim3(static_cast<uint32_t>((rows + kGroups - 1) / kGroups)), dim3(kThreads), 0, s, a);
+        else
+            hipLaunchKernelGGL((attention_join<T, DP, kGroups>), dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, s, a);
         return check_launch("ddl_attention");
     });
 }

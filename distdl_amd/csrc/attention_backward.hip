@@ -49,6 +49,7 @@ __device__ inline void load_column(Frag* column, const T* row, bool there, int c
 }
 
 // dq of 32 queries a wavefront, 128 a workgroup, tiles of keys and values through LDS as in attention_rows; and their D.
+// [4,4096,16,128] bf16, all keys: 755 us (1093 TFLOP/s for three products; 782 before its two kinds of work were woven), head size 64: 407.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_backward_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
@@ -163,7 +164,10 @@ constexpr int query_tile() { return sizeof(T) == 2 || AttnTile<T, DP>::kRowBytes
 // 16-bit rows of more than 128 bytes: keys and values, both sums and both products of a step are more than the 256 registers with which
 // two wavefronts fit on a SIMD, and one alone leaves the matrix cores idle while it forms probabilities.  There a second set of four
 // wavefronts takes half of the work: the first four keep dk, the others dv, and both form the probabilities, five
-// products instead of four.  ([4,4096,16,128] bf16, both sums in one wavefront: 2460 us.)
+// products instead of four.  [4,4096,16,128] bf16: 1409 us (976 TFLOP/s for the five), both sums in one wavefront 2460.  Head size 64, one
+// role: 545 us, before its two kinds of work were woven 703.
+//
+// 64 queries at a time where LDS has room for two workgroups' (32: 1916 us with two roles then, 64: 1641).
 template <typename T, int DP>
 constexpr bool two_roles() { return sizeof(T) == 2 && DP > 64; }
 
@@ -411,15 +415,20 @@ constexpr int backward_keys_lds() {
     return tiles > out ? tiles : out;
 }
 
-// Workgroups that share the queries of a block of keys.
-int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
+// Workgroups that share the queries of a block of keys: as many as the chip has CUs in all, twice that where the blocks' lengths differ (causal), and
+// with at least `least` times 32 queries.  (dk and dv of [2,448,16,64] bf16, 1500 keys, in one part 22 us, in two 43: the sums' way through memory;
+// [2,2048,8,128] in one part each 84 us, in two 120; [4,2048,8,128] causal, one key head, eight parts each 113 us, four 154, sixteen 140.
+// fp32 [3,333,8,40], 77 keys, at least 64 queries each: 16 us, 256: 43.)
+int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, bool causal, int least) {
     if (batch < 1 || tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1) return 1;
     int dev;
     const int64_t units = batch * kv_heads * ((keys + kRows * kWaves - 1) / (kRows * kWaves)), tiles = heads / kv_heads * ((tokens + 31) / 32);
-    int64_t splits = (2 * static_cast<int64_t>(compute_units(dev)) + units - 1) / units;
-    if (splits > tiles / 2) splits = tiles / 2;
+    int64_t splits = (causal ? 2 : 1) * static_cast<int64_t>(compute_units(dev)) / units;
+    if (splits > tiles / least) splits = tiles / least;
     return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
 }
+template <typename T>
+constexpr int least_of_split() { return sizeof(T) == 2 ? 8 : 2; }
 
 int64_t rounded4(int64_t n) { return (n + 3) / 4 * 4; }
 
@@ -431,7 +440,7 @@ extern "C" {
 int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
     using namespace ddl;
     if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || dim < 1 || keys < 0) return 0;
-    const int64_t splits = key_splits(batch, tokens, keys, heads, kv_heads);
+    const int64_t splits = key_splits(batch, tokens, keys, heads, kv_heads, true, least_of_split<float>());      // the most that a call takes
     return rounded4(batch * heads * tokens) + (splits > 1 ? splits * 2 * batch * kv_heads * keys * dim : 0);
 }
 
@@ -478,7 +487,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         }
         if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
         if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kKeysLds, "ddl_attention_backward")) return rc;
-        a.splits = key_splits(batch, tokens, keys, heads, kv_heads);
+        a.splits = key_splits(batch, tokens, keys, heads, kv_heads, a.causal, least_of_split<T>());
         a.blocks = (a.keys + kRows * kWaves - 1) / (kRows * kWaves);
         const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads, grid = pairs * a.blocks * a.splits;
         if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");

@@ -402,7 +402,8 @@ struct RotaryShard {
 
 std::optional<Two> rotary_shard(const MaybeTensor& q, const MaybeTensor& k, const Tensor& frequencies, const MaybeTensor& positions, bool neighbours, double amplitude,
                                 const Shared& general) {
-    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(frequencies) || !ordinary(positions)) return std::nullopt;
+    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(frequencies) || !ordinary(positions) || (at::GradMode::is_enabled() && frequencies.requires_grad()))
+        return std::nullopt;
     std::optional<Two> y;
     {
         at::NoGradGuard no_grad;
@@ -445,7 +446,8 @@ struct HeadNormRotaryShard {
 
 std::optional<Two> head_norm_rotary_shard(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight, const Tensor& frequencies,
                                           const MaybeTensor& positions, double eps, bool neighbours, double amplitude, const Shared& general) {
-    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(q_weight) || !ordinary(k_weight) || !ordinary(frequencies) || !ordinary(positions)) return std::nullopt;
+    if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(q_weight) || !ordinary(k_weight) || !ordinary(frequencies) || !ordinary(positions) || (at::GradMode::is_enabled() && frequencies.requires_grad()))
+        return std::nullopt;
     std::optional<Two> y;
     {
         at::NoGradGuard no_grad;

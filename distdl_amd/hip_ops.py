@@ -1145,7 +1145,9 @@ def _heads(t, name, like=None):
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise ValueError(f"{name}: operands differ in type or device ({t.dtype} on {t.device}, {like.dtype} on {like.device})")
     if t.shape[3] > 1 and t.stride(3) != 1:
-        t = contiguous(t)
+        _require_gpu(t)
+        with _on_device_of(t):
+            t = contiguous(t)
     return t
 
 
@@ -1175,7 +1177,8 @@ def _rotary_arguments(q, k, frequencies, positions, name):
             raise ValueError(f"{name}: positions must be int32 or int64, [{tokens}] or [{batch}, {tokens}], on {first.device}, "
                              f"got {tuple(positions.shape)} {positions.dtype} on {positions.device}")
         if tokens > 1 and positions.stride(-1) != 1:
-            positions = contiguous(positions)
+            with _on_device_of(positions):
+                positions = contiguous(positions)
         width = positions.element_size()
         pitch = positions.stride(0) if positions.dim() == 2 and positions.shape[0] == batch and batch > 1 else 0
     return first, positions, (frequencies.data_ptr(), 2 * frequencies.numel(), _ptr(positions), width, pitch)
@@ -1247,7 +1250,7 @@ def _aligned_heads(t, dim):
     apart; else a copy, with zeros behind the head's own elements."""
     per = 16 // t.element_size()
     if t.shape[3] == dim and t.data_ptr() % 16 == 0 and all(s % per == 0 or n <= 1 for s, n in zip(t.stride()[:3], t.shape[:3])) and \
-       (t.shape[1] <= 1 or t.stride(1) < 1 << 22):
+       (t.shape[1] <= 1 or dim <= t.stride(1) < 1 << 22):
         return t
     if t.shape[3] == dim:
         out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
@@ -1278,7 +1281,8 @@ def _attention_operands(q, k, v, lengths, scale, name):
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],) or lengths.device != q.device):
         raise ValueError(f"{name}: lengths must be int32 [{q.shape[0]}] on {q.device}, got {tuple(lengths.shape)} {lengths.dtype} on {lengths.device}")
     if lengths is not None and not lengths.is_contiguous():
-        lengths = contiguous(lengths)
+        with _on_device_of(lengths):
+            lengths = contiguous(lengths)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not 0 < scale <= 1e38:
         raise ValueError(f"{name}: scale {scale} is not positive")

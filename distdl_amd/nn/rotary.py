@@ -116,7 +116,9 @@ def _row(weight):
     return None if weight is None else weight.detach().reshape(-1)
 
 
-def _records(*tensors):
+def _records(frequencies, *tensors):
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary frequencies have no gradient: detach them")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -129,7 +131,7 @@ def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplit
     res = _lib.front().rotary_shard(q, k, frequencies, positions, interleaved, amplitude, _lib.callback(_general_rotary_backward))
     if res is not None:
         return res
-    if _records(q, k):
+    if _records(frequencies, q, k):
         return _RotaryShard.apply(q, k, frequencies, positions, bool(interleaved), float(amplitude))
     return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude)
 
@@ -141,7 +143,7 @@ def head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions=None
                                               _lib.callback(_general_head_norm_backward))
     if res is not None:
         return res
-    if _records(q, k, q_weight, k_weight):
+    if _records(frequencies, q, k, q_weight, k_weight):
         return _HeadNormRotaryShard.apply(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(interleaved), float(amplitude))
     return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude, norm=True, q_weight=_row(q_weight), k_weight=_row(k_weight), eps=eps)
 

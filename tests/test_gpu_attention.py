@@ -7,9 +7,12 @@ the second product, fp32 keeps them) and e = 2^-24:
 * a score is a sum of head_dim <= 128 products in 32 bits, off by at most (128 + 2) e sum |q k| scale, which p turns into as large a
   relative error; with the exponential and the running sums (n terms of one sign) p is off by  c = 131 e A + 2^-21 + n e  of itself,
   A = the largest sum |q k| scale of the case (2^-21: exponential, its argument's rounding for scores up to A is in the first term);
-* out: u |out| for the result, (u + 2 c) sum p |v| before it (the error of the total is another c);
+* out: u |out| for the result, (u + 2 c) sum p |v| before it (the error of the total is another c), and u |out| more for the total, which is the
+  sum of the probabilities as rounded: with p (1 + d), |d| <= u, for p, sum p (1 + d) v / sum p (1 + d) is sum p d (v - out) off to first
+  order, at most u sum p |v - out| <= u (sum p |v| + |out|).  (With values of 0 and one of 1 that has little weight the sum is twice
+  u sum p |v|, so the second term is needed.)  The adjoint's probabilities come from the unrounded total;
 * gradients: dv as out, with sums over queries of p |dy|; dS = p (dP - D), dP and D off by 130 e sum |dy v| each (D: from `out`, which
-  is off by its own tolerance: u sum |dy out| + (u + 2 c) sum |dy| (p |v|) more), so dS is off by
+  is off by its own tolerance: 2 u sum |dy out| + (u + 2 c) sum |dy| (p |v|) more), so dS is off by
   p ((u + 2 c) (|dP| + |D|) + 260 e sum |dy v| + D's), and dq, dk sum that times |k|, |q|; sums of n terms add n e of their magnitude.
 The sums of magnitudes are formed in 64 bits with absolute values.  float16 loses 2^-25 next to zero for every rounding (a probability,
 a result) on top.
@@ -48,13 +51,13 @@ def _bounds(q, k, v, lengths, causal, scale, u, tiny, dy=None, rounded=True):
             c = 131 * e * big + 2.0 ** -21 + n * e
             o = p @ vb
             room = p + tiny * see
-            out[b, :, h] = u * np.abs(o) + (up + 2 * c) * (room @ np.abs(vb)) + tiny * (see @ np.abs(vb)) + tiny
+            out[b, :, h] = (u + up) * np.abs(o) + (up + 2 * c) * (room @ np.abs(vb)) + tiny * (see @ np.abs(vb)) + tiny
             if dy is None:
                 continue
             g = dy[b, :, h]
             dp, dd = g @ vb.T, (g * o).sum(-1)[:, None]
             mag, mago, magp = np.abs(g) @ np.abs(vb).T, (np.abs(g) * np.abs(o)).sum(-1)[:, None], (np.abs(g) * (p @ np.abs(vb))).sum(-1)[:, None]
-            off = p * ((up + 2 * c) * (np.abs(dp) + np.abs(dd)) + 260 * e * mag + u * mago + (up + 2 * c) * magp) + tiny * see
+            off = p * ((up + 2 * c) * (np.abs(dp) + np.abs(dd)) + 260 * e * mag + (u + up) * mago + (up + 2 * c) * magp) + tiny * see
             ds = p * (dp - dd)
             e_sum = (tokens + keys) * e
             dq[b, :, h] = u * np.abs(scale * ds @ kb) + scale * (off + e_sum * np.abs(ds)) @ np.abs(kb) + tiny
@@ -127,6 +130,34 @@ def test_adjoint(dt, case):
     _check(dt, q, k, v, None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda"), causal, dy=dy)
 
 
+# Enough rows for every workgroup to take whole ranges of keys (at least 3 blocks of 32 rows for each of 256 CUs, and at most half as many of 128;
+# causal ones count by the keys that they see).
+MANY = [
+    (20, 130, 70, 8, 8, 40, [70, 0, 33, 64, 1], False), (24, 200, 257, 8, 8, 72, [257, 250, 129], True), (50, 100, 33, 4, 4, 128, None, False),
+    (12, 300, 300, 8, 2, 64, None, True), (3, 520, 200, 16, 1, 24, [200, 0, 97], True), (26, 257, 64, 4, 2, 96, [64, 63], False), (10, 513, 97, 16, 2, 128, [97, 65, 0, 32, 31], True),
+    (16, 129, 1, 16, 16, 16, [1, 0], False),
+]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("case", MANY)
+def test_many_rows(dt, case):
+    batch, tokens, keys, heads, kv_heads, dim, lengths, causal = case
+    q, k, v, dy = _inputs(dt, batch, tokens, keys, heads, kv_heads, dim, seed=14)
+    n = None if lengths is None else torch.tensor((batch * lengths)[:batch], dtype=torch.int32, device="cuda")
+    _check(dt, q, k, v, n, causal)
+    _check(dt, q, k, v, n, causal, dy=dy)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("case", [(1, 300, 1000, 4, 2, 128, None, True), (2, 70, 1300, 4, 4, 64, [1300, 70], True), (1, 130, 2100, 2, 2, 32, None, False),
+                                  (1, 900, 700, 2, 1, 96, [650], True), (3, 9, 5000, 8, 1, 16, [5000, 0, 513], True)])
+def test_splits_of_several_blocks_of_rows(dt, case):
+    """The keys of 2 to 20 splits, whose sums are joined; causal ones end inside them."""
+    test_forward(dt, case)
+    test_adjoint(dt, case)
+
+
 @pytest.mark.parametrize("layout", ["packed", "heads_first", "shared_sequences", "unaligned", "strided_features"])
 @pytest.mark.parametrize("tokens", [1, 50])
 def test_layouts(layout, tokens):
@@ -157,14 +188,14 @@ def test_layouts(layout, tokens):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("tokens,keys", [(1, 300), (70, 130)])
-def test_what_lies_behind_a_sequence_is_not_looked_at(dt, tokens, keys):
+@pytest.mark.parametrize("tokens,keys,times", [(1, 300, 1), (70, 130, 1), (130, 130, 40), (20, 1300, 1)])
+def test_what_lies_behind_a_sequence_is_not_looked_at(dt, tokens, keys, times):
     """NaN and infinities in the padding: same bits as zeros there, zero gradients of the padding; a sequence without keys gives zeros."""
     from distdl_amd import nn
-    lengths = torch.tensor([keys - 37, 0, 1], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor(times * [keys - 37, 0, 1], dtype=torch.int32, device="cuda")
     results = []
     for filler in (0.0, float("nan"), float("inf"), -torch.finfo(dt).max):
-        q, k, v, dy = _inputs(dt, 3, tokens, keys, 4, 2, 40, seed=3)
+        q, k, v, dy = _inputs(dt, 3 * times, tokens, keys, 4, 2, 40, seed=3)
         for b, n in enumerate(lengths.tolist()):
             k[b, n:], v[b, n:] = filler, filler
         leaves = [t.requires_grad_() for t in (q, k, v)]
@@ -207,38 +238,42 @@ def test_key_heads_without_heads():
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("slope", [0.02, 0.3, -0.3])
-def test_maxima_that_rise_and_fall_along_the_keys(dt, slope):
+@pytest.mark.parametrize("batch,tokens", [(1, 40), (160, 130)])
+def test_maxima_that_rise_and_fall_along_the_keys(dt, slope, batch, tokens):
     """Scores that climb (by less and by more than the running maximum's slack from tile to tile) or fall along 400 keys."""
-    q, k, v, dy = _inputs(dt, 1, 40, 400, 1, 1, 16, seed=5)
+    q, k, v, dy = _inputs(dt, batch, tokens, 400, 1, 1, 16, seed=5)
     k.zero_()
-    k[0, :, 0, 0] = slope * torch.arange(400, device="cuda")
+    k[:, :, 0, 0] = slope * torch.arange(400, device="cuda")
     q[..., 0] = 2.0
     _check(dt, q, k, v, scale=1.0, dy=dy)
     _check(dt, q.detach()[:, :1], k.detach(), v.detach(), scale=1.0)
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
-def test_large_scores_and_other_scales(dt):
+@pytest.mark.parametrize("batch,tokens", [(1, 33), (160, 130)])
+def test_large_scores_and_other_scales(dt, batch, tokens):
     """Scores of some thousands: one key takes all.  In powers of two they stay below 2^13, where the maximum is rounded by up to 2^-11: the
     probability of the best key comes out as 1 within 2^-11, as does the total, whose rounded one is divided by the unrounded one."""
     from distdl_amd import nn
-    q, k, v, _ = _inputs(dt, 1, 33, 70, 1, 1, 64, seed=6)
+    q, k, v, _ = _inputs(dt, batch, tokens, 70, 1, 1, 64, seed=6)
     out = nn.attention_shard(q, k, v, scale=100.0)
-    best = (_f64(q)[0, :, 0] @ _f64(k)[0, :, 0].T).argsort(-1)
-    s = np.sort(_f64(q)[0, :, 0] @ _f64(k)[0, :, 0].T, -1)
-    clear = s[:, -1] - s[:, -2] > 1.0      # e^-100 and less for all others
-    assert clear.sum() > 20 and s.max() * 100 * np.log2(np.e) < 2 ** 13
-    want = _f64(v)[0, best[clear, -1], 0]
-    assert (np.abs(_f64(out)[0, clear, 0] - want) <= (torch.finfo(dt).eps / 2 + 2.0 ** -10) * np.abs(want)).all()
+    s = _f64(q)[:, :, 0] @ _f64(k)[:, :, 0].transpose(0, 2, 1)
+    best = s.argmax(-1)
+    s = np.sort(s, -1)
+    clear = (s[..., -1] - s[..., -2] > 1.0) & (s[..., -1] * 100 * np.log2(np.e) < 2 ** 13)      # e^-100 and less for all others
+    assert clear.sum() > 20 * batch
+    want = np.take_along_axis(_f64(v)[:, :, 0], best[..., None], 1)[clear]
+    assert (np.abs(_f64(out)[:, :, 0][clear] - want) <= (torch.finfo(dt).eps / 2 + 2.0 ** -10) * np.abs(want)).all()
 
 
-def test_strides_beyond_32_bits():
+@pytest.mark.parametrize("tokens,heads", [(33, 2), (1600, 16)])
+def test_strides_beyond_32_bits(tokens, heads):
     """Two sequences 2^31 elements apart."""
     from distdl_amd import nn
     far = 1 << 31
     base = torch.empty(far + 40 * 2 * 64, dtype=torch.bfloat16, device="cuda")
     k, v = (base.as_strided((2, 40, 1, 64), (far, 128, 64, 1), 64 * i) for i in (0, 1))
-    q, kk, vv, dy = _inputs(torch.bfloat16, 2, 33, 40, 2, 1, 64, seed=7)
+    q, kk, vv, dy = _inputs(torch.bfloat16, 2, tokens, 40, heads, 1, 64, seed=7)
     k.copy_(kk), v.copy_(vv)
     results = []
     for a, b in ((k, v), (kk, vv)):
@@ -280,12 +315,12 @@ def test_gradients_against_differences():
             assert abs((ends[0] - ends[1]) / (2 * h) - float(grad[at])) <= 2.0 ** -14 * (1 + np.abs(_f64(dy)).max())
 
 
-@pytest.mark.parametrize("tokens", [1, 96])
-def test_equal_calls_give_equal_bits_and_replay_from_a_graph(tokens):
+@pytest.mark.parametrize("tokens,times", [(1, 1), (96, 1), (300, 6)])
+def test_equal_calls_give_equal_bits_and_replay_from_a_graph(tokens, times):
     """Captured together with the adjoint, replayed with eager calls on the same leaves between, against the eager results."""
     from distdl_amd import nn
-    q, k, v, dy = _inputs(torch.bfloat16, 2, tokens, 3000, 8, 1, 64, seed=10)
-    lengths = torch.tensor([2999, 64], dtype=torch.int32, device="cuda")
+    q, k, v, dy = _inputs(torch.bfloat16, 2 * times, tokens, 3000, 8, 1, 64, seed=10)
+    lengths = torch.tensor(times * [2999, 64], dtype=torch.int32, device="cuda")
     leaves = [t.requires_grad_() for t in (q, k, v)]
 
     def step():

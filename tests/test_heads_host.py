@@ -76,6 +76,13 @@ def test_frequencies_and_their_scalings():
             nn.rotary_frequencies(**bad)
 
 
+def test_frequencies_take_no_gradient():
+    q, f = torch.zeros(1, 2, 1, 8), torch.ones(2, dtype=torch.float64, requires_grad=True)
+    for call in (lambda: nn.rotary_shard(q, None, f), lambda: nn.head_norm_rotary_shard(q, None, None, None, f)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+
+
 def test_layers_refuse_partitions_that_split_heads_and_positions_they_cannot_know():
     from distdl_amd.backends.stub_hip import SimWorld
     P_world = SimWorld(2).partition(0)
