@@ -152,9 +152,9 @@ SIGNATURES = {
     "ddl_attention_workspace": (c_int64, [c_int64] * 6),
     "ddl_attention": (c_int, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_int, c_int64, c_int64,
                               c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p, POINTER(c_int64), c_void_p, c_void_p,
-                              c_int64, c_void_p]),
+                              c_void_p, c_int64, c_void_p]),
     "ddl_attention_backward_workspace": (c_int64, [c_int64] * 6),
-    "ddl_attention_backward": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p, c_int] + [c_int64] * 6 + [c_void_p, c_int, c_float] +
+    "ddl_attention_backward": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p, c_void_p, c_int] + [c_int64] * 6 + [c_void_p, c_int, c_float] +
                                [c_void_p, POINTER(c_int64)] * 3 + [c_void_p, c_int64, c_void_p]),
     "ddl_colsum_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }

@@ -4,7 +4,8 @@
 //
 // in one pass over the keys with the running maximum and sum of the softmax (fp32); 2^x takes the place of e^x, log2(e) goes
 // into the scale.  A query that sees no key gives zeros.  Kept for the adjoint: log2 of each row's sum (+inf for a row
-// without keys, so that its probabilities come out as zero there).
+// without keys, so that its probabilities come out as zero there) and, of 16-bit results, what their rounding took: the adjoint's
+// D = dO . out is a difference's second member, and off by that rounding where few keys share the weight (see there).
 //
 // Two forms, attention_rows and attention_split below; what they are made of is in attention_parts.h.
 #include "ddl_common.h"
@@ -254,10 +255,21 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     Out::park(room, run.acc, total > 0.f ? 1.0f / total : 0.f, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     T* out = static_cast<T*>(a.out) + batch * a.out_at.batch + head * a.out_at.head;
-    Out::write(room, a.chunks, lane, [&](int col) -> T* {
-        const int row = first_row + wave * kRows + col;
-        return row < a.tokens ? out + row * a.out_at.token : nullptr;
-    });
+    const auto place = [&](T* base) {
+        return [=](int col) -> T* {
+            const int row = first_row + wave * kRows + col;
+            return row < a.tokens ? base + row * a.out_at.token : nullptr;
+        };
+    };
+    Out::write(room, a.chunks, lane, place(out));
+    if constexpr (LSE && sizeof(T) == 2) {
+        if (a.rest) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::template park<true>(room, run.acc, total > 0.f ? 1.0f / total : 0.f, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::write(room, a.chunks, lane, place(static_cast<T*>(a.rest) + batch * a.out_at.batch + head * a.out_at.head));
+        }
+    }
 }
 
 template <typename T, int DP>
@@ -379,7 +391,9 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         }
         if (whole) {
             const int tk = row / a.group, hd = kv_head * a.group + row - tk * a.group;
-            store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + tk * a.out_at.token + hd * a.out_at.head + d, sum);
+            const int64_t to = batch * a.out_at.batch + tk * a.out_at.token + hd * a.out_at.head + d;
+            store_piece<true>(static_cast<T*>(a.out) + to, sum);
+            if (LSE && sizeof(T) == 2 && a.rest) store_piece<true>(static_cast<T*>(a.rest) + to, lost<T>(sum));
         } else {
             *reinterpret_cast<float4*>(partial + row * (DP + kStats) + d) = sum;
         }
@@ -443,9 +457,12 @@ __global__ __launch_bounds__(kThreads) void attention_join(const AttnArgs a) {
     const float inv = total > 0.f ? 1.0f / total : 0.f;
     const int bk = at / rows, row = at - bk * rows, batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int token = row / a.group, head = kv_head * a.group + row - token * a.group;
-    if (there)
-        store_piece<true>(static_cast<T*>(a.out) + batch * a.out_at.batch + token * a.out_at.token + head * a.out_at.head + d,
-                          make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    if (there) {
+        const int64_t to = batch * a.out_at.batch + token * a.out_at.token + head * a.out_at.head + d;
+        const float4 mean = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        store_piece<true>(static_cast<T*>(a.out) + to, mean);
+        if (sizeof(T) == 2 && a.rest) store_piece<true>(static_cast<T*>(a.rest) + to, lost<T>(mean));
+    }
     if (lane == 0 && a.lse) a.lse[(static_cast<int64_t>(batch) * a.heads + head) * a.tokens + token] = exact > 0.f ? top + __builtin_amdgcn_logf(exact) : INFINITY;
 }
 
@@ -502,7 +519,7 @@ int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys, int
 
 int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
                   int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, const int32_t* lengths, int causal,
-                  float scale, void* out, const int64_t* out_strides, float* lse, float* workspace, int64_t workspace_elems, void* stream) {
+                  float scale, void* out, const int64_t* out_strides, void* out_rest, float* lse, float* workspace, int64_t workspace_elems, void* stream) {
     using namespace ddl;
     AttnArgs a{};
     bool nothing;
@@ -510,7 +527,9 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
                                       kv_heads, dim, lengths, causal, scale))
         return rc;
     if (nothing || tokens == 0) return 0;
-    a.out = out, a.out_at = place_of(out_strides), a.lse = lse;
+    if (out_rest && (dtype == DDL_DT_F32 || !lse)) return fail(DDL_E_ARG, "ddl_attention: only 16-bit results that an adjoint follows have a rest");
+    if (!aligned_to(out_rest, 16)) return fail(DDL_E_ALIGN, "ddl_attention: the rest is not 16-byte aligned");
+    a.out = out, a.out_at = place_of(out_strides), a.rest = out_rest, a.lse = lse;
     a.splits = splits_for(batch, tokens, keys, heads, kv_heads);
     const int64_t need = ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim);
     if (need && (!workspace || workspace_elems < need))

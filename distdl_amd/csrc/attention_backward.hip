@@ -6,6 +6,10 @@
 // scores and dO . v twice (seven products instead of five): attention_backward_rows, a wavefront for 32 queries that walks over
 // the keys, and attention_backward_keys, a wavefront for 32 keys that walks over the queries of all heads that share
 // them -- the gradient of a shared key head is summed there, in registers.
+//
+// 16-bit types: dS is rounded for the product (gradients are then off by 1.4 times what rounding the exact ones gives).  D comes from out and the rest
+// that the forward kept, or, where all keys are in one tile, from p and dP themselves; from the rounded out alone the gradients of a
+// query with four keys were off by 2.4 times as much, with 200 keys by 1.6.
 #include "ddl_common.h"
 
 #include "attention_parts.h"
@@ -50,7 +54,8 @@ __device__ inline void load_column(Frag* column, const T* row, bool there, int c
 
 // dq of 32 queries a wavefront, 128 a workgroup, tiles of keys and values through LDS as in attention_rows; and their D.
 // [4,4096,16,128] bf16, all keys: 755 us (1093 TFLOP/s for three products; 782 before its two kinds of work were woven), head size 64: 407.
-template <typename T, int DP>
+// ONE (16-bit types): all keys are in one tile, D from them.
+template <typename T, int DP, bool ONE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_backward_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
@@ -77,23 +82,41 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         const char* to = lds + (t & 1) * kTileBytes;
         k_copy.request(to, t * KEYS, end), v_copy.request(to + 2 * kTileBytes, t * KEYS, end);
     };
-    if (a.dq) request(0);
+    if (ONE || a.dq) request(0);
     Frag q_column[Tile::kSteps], g_column[Tile::kSteps];
     load_column<T, DP>(q_column, static_cast<const T*>(a.q) + batch * a.q_at.batch + my_row * a.q_at.token + head * a.q_at.head, mine, a.chunks, half);
     load_column<T, DP>(g_column, static_cast<const T*>(a.dout) + batch * a.dout_at.batch + my_row * a.dout_at.token + head * a.dout_at.head, mine, a.chunks, half);
     float delta = 0.f, lse = INFINITY;
-    {
-        Frag o_column[Tile::kSteps];
-        load_column<T, DP>(o_column, static_cast<const T*>(a.out) + batch * a.out_at.batch + my_row * a.out_at.token + head * a.out_at.head, mine, a.chunks, half);
+    const int64_t stat = static_cast<int64_t>(bh) * a.tokens + my_row;
+    if (mine) lse = a.lse[stat];
+    constexpr uint32_t kK = 0, kV = 2 * kTileBytes, kNext = 32 * Tile::kRowBytes;
+    if constexpr (ONE) {
+        wait_for_copies();
+        lds_barrier();
+#pragma unroll 1
+        for (int n = 0; 32 * n < wave_most; ++n) {
+            floatx16 s[2];
+            clear(s);
+            tile.straight(s[0], kK, n, q_column);
+            tile.straight(s[1], kV, n, g_column);
 #pragma unroll
-        for (int s = 0; s < Tile::kSteps; ++s) delta += chunk_dot(g_column[s], o_column[s], static_cast<const T*>(nullptr));
-        delta = add_halves(delta);
-        const int64_t at = static_cast<int64_t>(bh) * a.tokens + my_row;
-        if (mine) {
-            lse = a.lse[at];
-            if (half == 0) a.delta[at] = delta;
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.scale_log2, -lse));
+                if (32 * n + (r & 3) + 8 * (r >> 2) < seen - 4 * half) delta = __builtin_fmaf(p, s[1][r], delta);
+            }
+        }
+    } else {
+        const int64_t row = batch * a.out_at.batch + my_row * a.out_at.token + head * a.out_at.head;
+        for (const void* of : {static_cast<const void*>(a.out), static_cast<const void*>(a.rest)}) {
+            if (!of) continue;
+            Frag o_column[Tile::kSteps];
+            load_column<T, DP>(o_column, static_cast<const T*>(of) + row, mine, a.chunks, half);
+#pragma unroll
+            for (int s = 0; s < Tile::kSteps; ++s) delta += chunk_dot(g_column[s], o_column[s], static_cast<const T*>(nullptr));
         }
     }
+    delta = add_halves(delta);
+    if (mine && half == 0) a.delta[stat] = delta;
     if (!a.dq) return;      // D alone
     floatx16 acc[Tile::kBlocks];
     clear(acc);
@@ -101,9 +124,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         wait_for_copies();
         lds_barrier();
         request(t + 1);
-        constexpr uint32_t kK = 0, kV = 2 * kTileBytes, kNext = 32 * Tile::kRowBytes;
         bool done = t * KEYS >= wave_most;
-        if constexpr (sizeof(T) == 2 && NS == 2) {
+        if constexpr (sizeof(T) == 2 && NS == 2 && !ONE) {
             if (!done && (t + 1) * KEYS <= wave_least) {     // 64 keys that all see: the vector units are at 32 of them while the matrix cores are at others
                 done = true;
                 floatx16 p0, p1, d0, d1;
@@ -445,7 +467,7 @@ int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens, int64_t 
 }
 
 int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                           const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides, const float* lse, int dtype, int64_t batch,
+                           const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides, const void* out_rest, const float* lse, int dtype, int64_t batch,
                            int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, const int32_t* lengths, int causal, float scale,
                            void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides, float* workspace,
                            int64_t workspace_elems, void* stream) {
@@ -463,12 +485,14 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         if (!r.s) return fail(DDL_E_ARG, "ddl_attention_backward: no strides");
         if (!aligned_to(r.p, 16) || r.s[0] % per || r.s[1] % per || r.s[2] % per) return fail(DDL_E_ALIGN, "ddl_attention_backward: gradients are not 16-byte aligned");
     }
+    if (out_rest && dtype == DDL_DT_F32) return fail(DDL_E_ARG, "ddl_attention_backward: only 16-bit results have a rest");
+    if (!aligned_to(out_rest, 16)) return fail(DDL_E_ALIGN, "ddl_attention_backward: the rest is not 16-byte aligned");
     if (tokens && !lse) return fail(DDL_E_ARG, "ddl_attention_backward: no row sums");
     const int64_t need = ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim);
     if (need && (!workspace || workspace_elems < need))
         return fail(DDL_E_ARG, "ddl_attention_backward: workspace of %lld floats, %lld are needed", static_cast<long long>(workspace ? workspace_elems : 0), static_cast<long long>(need));
     if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention_backward: workspace is not 16-byte aligned");
-    a.dout = dout, a.dout_at = place_of(dout_strides), a.out = const_cast<void*>(out), a.out_at = place_of(out_strides), a.lse = const_cast<float*>(lse);
+    a.dout = dout, a.dout_at = place_of(dout_strides), a.out = const_cast<void*>(out), a.out_at = place_of(out_strides), a.rest = const_cast<void*>(out_rest), a.lse = const_cast<float*>(lse);
     a.dq = dq, a.dk = dk, a.dv = dv, a.dq_at = place_of(dq_strides), a.dk_at = place_of(dk_strides), a.dv_at = place_of(dv_strides);
     a.delta = workspace, a.partial = workspace + rounded4(batch * heads * tokens);
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -477,13 +501,20 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         constexpr int DP = decltype(dp)::value;
         constexpr int kRowsLds = backward_rows_lds<T, DP>(), kKeysLds = backward_keys_lds<T, DP>();
         if (a.tokens) {
-            if (const int rc = grant_lds<attention_backward_rows<T, DP>>(kRowsLds, "ddl_attention_backward")) return rc;
             a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
             const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
             if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
             a.folded = folds(a.causal, grid);
-            hipLaunchKernelGGL((attention_backward_rows<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kRowsLds, s, a);
-            if (const int rc = check_launch("ddl_attention_backward")) return rc;
+            const auto launch = [&](auto one) {
+                constexpr bool ONE = decltype(one)::value;
+                if (const int rc = grant_lds<attention_backward_rows<T, DP, ONE>>(kRowsLds, "ddl_attention_backward")) return rc;
+                hipLaunchKernelGGL((attention_backward_rows<T, DP, ONE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kRowsLds, s, a);
+                return check_launch("ddl_attention_backward");
+            };
+            int rc;
+            if constexpr (sizeof(T) == 2) rc = a.keys <= tile_rows<T>() ? launch(std::true_type{}) : launch(std::false_type{});
+            else rc = launch(std::false_type{});
+            if (rc) return rc;
         }
         if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
         if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kKeysLds, "ddl_attention_backward")) return rc;

@@ -377,6 +377,16 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// What rounding to T takes from a value.
+template <typename T>
+__device__ inline float lost(float v) {
+    T t;
+    store1(&t, v);
+    return v - load1(&t);
+}
+template <typename T>
+__device__ inline float4 lost(const float4& v) { return make_float4(lost<T>(v.x), lost<T>(v.y), lost<T>(v.z), lost<T>(v.w)); }
+
 // A wavefront's 32 columns of acc[d block][r] (d = 32 block + (r & 3) + 8 (r >> 2) + 4 half), times `factor`, as rows of DP elements
 // in its own room of LDS, kPitch bytes apart.
 template <typename T, int DP>
@@ -384,15 +394,18 @@ struct AttnOut {
     static constexpr int kPitch = DP * static_cast<int>(sizeof(T)) + 16;
     static constexpr int kRoom = 32 * kPitch;      // bytes for a wavefront
     static constexpr int kBlocks = DP / 32;
+    // REST: what the rounding to T takes from them instead.
+    template <bool REST = false>
     static __device__ void park(char* room, const floatx16 (&acc)[kBlocks], float factor, int lane) {
         char* row = room + (lane & 31) * kPitch;
         const int half = lane >> 5;
+        auto value = [&](float v) { return REST ? lost<T>(v * factor) : v * factor; };
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 T* at = reinterpret_cast<T*>(row) + 32 * d + 8 * q + 4 * half;
-                const float a = acc[d][4 * q] * factor, b = acc[d][4 * q + 1] * factor, c = acc[d][4 * q + 2] * factor, e = acc[d][4 * q + 3] * factor;
+                const float a = value(acc[d][4 * q]), b = value(acc[d][4 * q + 1]), c = value(acc[d][4 * q + 2]), e = value(acc[d][4 * q + 3]);
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(at) = make_float4(a, b, c, e);
                 } else if constexpr (std::is_same_v<T, bf16_t>) {
@@ -432,6 +445,7 @@ inline HeadsAt place_of(const int64_t* s) { return s ? HeadsAt{s[0], s[1], s[2]}
 struct AttnArgs {
     const void *q, *k, *v, *dout;
     void *out, *dq, *dk, *dv;
+    void* rest;                         // what out lost to its rounding (as out) or null
     HeadsAt q_at, k_at, v_at, out_at, dout_at, dq_at, dk_at, dv_at;
     float* lse;                         // [batch][heads][tokens], log2
     float* delta;                       // the same, sum of dout out

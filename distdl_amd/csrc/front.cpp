@@ -398,11 +398,12 @@ std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, 
     Tensor work;
     r.out = at::empty({batch, tokens, heads, dim}, r.q.options());
     if (want_lse) r.lse = floats(r.q, {batch, heads, tokens});
+    if (want_lse && r.q.element_size() == 2) r.rest = at::empty_like(r.out);
     const int64_t elems = ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim);
     if (elems) work = floats(r.q, {elems});
     check(ddl_attention(r.q.data_ptr(), Strides3(r.q), r.k.data_ptr(), Strides3(r.k), r.v.data_ptr(), Strides3(r.v), float_code(r.q), batch, tokens, keys, heads, kv_heads,
                         dim, length_pointer(lengths), causal, static_cast<float>(attention_scale(q_given, scale)), r.out.data_ptr(), Strides3(r.out),
-                        static_cast<float*>(pointer(r.lse)), static_cast<float*>(pointer(work)), elems, current_stream()),
+                        pointer(r.rest), static_cast<float*>(pointer(r.lse)), static_cast<float*>(pointer(work)), elems, current_stream()),
           "ddl_attention");
     r.padded_out = r.out;
     crop({&r.out}, own);
@@ -410,9 +411,12 @@ std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, 
 }
 
 std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout_given, const Tensor& q, const Tensor& k, const Tensor& v,
-                                                                                   const Tensor& out, const Tensor& lse, const MaybeTensor& lengths, bool causal,
+                                                                                   const Tensor& out, const MaybeTensor& rest, const Tensor& lse,
+                                                                                   const MaybeTensor& lengths, bool causal,
                                                                                    double scale, bool want_q, bool want_k, bool want_v) {
     if (!attention_operands(q, k, v, lengths, scale) || out.sizes() != q.sizes()) return std::nullopt;
+    if (rest && (!rest->is_cuda() || rest->device() != q.device() || rest->scalar_type() != q.scalar_type() || rest->sizes() != out.sizes() || rest->strides() != out.strides()))
+        return std::nullopt;
     const int64_t batch = q.size(0), tokens = q.size(1), keys = k.size(1), heads = q.size(2), kv_heads = k.size(2), dim = q.size(3);
     for (const Tensor& t : {q, k, v, out})
         if (t.numel() && !read_in_place(t, dim)) return std::nullopt;
@@ -429,7 +433,7 @@ std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backw
     if (elems) work = floats(q, {elems});
     auto at_rest = [](const Tensor& t, const Tensor& like) { return Strides3(t.defined() ? t : like); };
     check(ddl_attention_backward(dout.data_ptr(), Strides3(dout), q.data_ptr(), Strides3(q), k.data_ptr(), Strides3(k), v.data_ptr(), Strides3(v), out.data_ptr(),
-                                 Strides3(out), lse.data_ptr<float>(), float_code(q), batch, tokens, keys, heads, kv_heads, dim, length_pointer(lengths), causal,
+                                 Strides3(out), pointer(rest), lse.data_ptr<float>(), float_code(q), batch, tokens, keys, heads, kv_heads, dim, length_pointer(lengths), causal,
                                  static_cast<float>(scale), pointer(dq), at_rest(dq, q), pointer(dk), at_rest(dk, k), pointer(dv), at_rest(dv, v),
                                  static_cast<float*>(pointer(work)), elems, current_stream()),
           "ddl_attention_backward");

@@ -60,15 +60,15 @@ std::optional<Two> head_norm_rotary(const MaybeTensor& q, const MaybeTensor& k, 
 std::optional<Four> head_norm_rotary_backward(const MaybeTensor& dyq, const MaybeTensor& dyk, const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight,
                                               const MaybeTensor& k_weight, const Rotation& rotation, double eps, bool want_q_weight, bool want_k_weight);
 // Attention's result, each query's sum if that was asked for, and what the adjoint takes: the operands (copies with padded heads where the kernels
-// do not read them as they lie) and the result with heads as long as theirs.
+// do not read them as they lie), the result with heads as long as theirs and what its rounding took (16-bit types).
 struct Attended {
-    Tensor out, lse, q, k, v, padded_out;
+    Tensor out, lse, q, k, v, padded_out, rest;
 };
 std::optional<Attended> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, const std::optional<double>& scale,
                                   bool want_lse);
 double attention_scale(const Tensor& q, const std::optional<double>& scale);
 std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                                                                                   const Tensor& lse, const MaybeTensor& lengths, bool causal, double scale,
+                                                                                   const MaybeTensor& rest, const Tensor& lse, const MaybeTensor& lengths, bool causal, double scale,
                                                                                    bool want_q, bool want_k, bool want_v);
 
 // The boxes of one launch with everything but the base addresses: a call adds those

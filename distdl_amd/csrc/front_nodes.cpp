@@ -469,13 +469,13 @@ struct AttentionShard {
     void identify(Key& key) const { key(int64_t{causal})(c10::bit_cast<int64_t>(scale))(general); }
     variable_list run(const std::vector<Tensor>& kept, const Tensor& dy_given, const Asked& asked) const {
         const Tensor dy = dy_given.detach();
-        const MaybeTensor lengths = defined(kept[5]);
+        const MaybeTensor lengths = defined(kept[5]), rest = defined(kept[6]);
         const bool need_q = has(asked.now, 0), need_k = has(asked.now, 1), need_v = has(asked.now, 2);
         std::optional<Three> res;
         {
             at::NoGradGuard no_grad;
-            res = attention_backward(dy, kept[0], kept[1], kept[2], kept[3], kept[4], lengths, causal, scale, need_q, need_k, need_v);
-            if (!res) res = general->call<Three>(dy, kept[0], kept[1], kept[2], kept[3], kept[4], lengths, causal, scale, need_q, need_k, need_v);
+            res = attention_backward(dy, kept[0], kept[1], kept[2], kept[3], rest, kept[4], lengths, causal, scale, need_q, need_k, need_v);
+            if (!res) res = general->call<Three>(dy, kept[0], kept[1], kept[2], kept[3], rest, kept[4], lengths, causal, scale, need_q, need_k, need_v);
         }
         return final_gradients(listed(*res), kName);
     }
@@ -497,6 +497,7 @@ MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, c
     node->save(res->padded_out.is_same(res->out) ? res->out.detach() : res->padded_out);      // the result: the same memory and version, without this node
     node->save(res->lse);
     node->save(lengths ? *lengths : Tensor());
+    node->save(res->rest);
     torch::autograd::create_gradient_edge(res->out, node);
     return res->out;
 }

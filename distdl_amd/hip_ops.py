@@ -1295,7 +1295,7 @@ def _attention_operands(q, k, v, lengths, scale, name):
 
 def attention(q, k, v, lengths=None, causal=False, scale=None, want_lse=False):
     """Attention of ``q`` [batch, tokens, heads, head_dim] to ``k``, ``v`` [batch, keys, kv_heads, head_dim], see ``ddl_attention``: a new
-    tensor like ``q``, and with ``want_lse`` what the adjoint needs."""
+    tensor like ``q``, and with ``want_lse`` what the adjoint needs: ``(out, lse, rest)``, the rest None in float32."""
     head_dim = q.shape[-1] if q.dim() else 0
     q, k, v, lengths, scale, dim = _attention_operands(q, k, v, lengths, scale, "attention")
     batch, tokens, heads, _ = q.shape
@@ -1303,30 +1303,31 @@ def attention(q, k, v, lengths=None, causal=False, scale=None, want_lse=False):
     lib = _lib.load()
     if heads == 0:
         out = torch.empty(q.shape[:3] + (head_dim,), dtype=q.dtype, device=q.device)
-        return (out, torch.empty((batch, 0, tokens), dtype=torch.float32, device=q.device)) if want_lse else out
+        return (out, torch.empty((batch, 0, tokens), dtype=torch.float32, device=q.device), None) if want_lse else out
     with _on_device_of(q):
         out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
         lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if want_lse else None
+        rest = torch.empty_like(out) if want_lse and q.element_size() == 2 else None
         elems = lib.ddl_attention_workspace(batch, tokens, keys, heads, kv_heads, dim)
         work = torch.empty(elems, dtype=torch.float32, device=q.device) if elems else None
         rc = lib.ddl_attention(q.data_ptr(), _attention_strides(q), k.data_ptr(), _attention_strides(k), v.data_ptr(), _attention_strides(v),
                                _LN_DTYPES[q.dtype], batch, tokens, keys, heads, kv_heads, dim, _ptr(lengths), int(causal), scale, out.data_ptr(),
-                               _attention_strides(out), _ptr(lse), _ptr(work), elems, _stream())
+                               _attention_strides(out), _ptr(rest), _ptr(lse), _ptr(work), elems, _stream())
         _lib.check(rc, "ddl_attention")
         if dim != head_dim:
-            out = contiguous(out[..., :head_dim])
-    return (out, lse) if want_lse else out
+            out, rest = (None if t is None else contiguous(t[..., :head_dim]) for t in (out, rest))
+    return (out, lse, rest) if want_lse else out
 
 
-def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scale=None, want_q=True, want_k=True, want_v=True):
-    """Adjoint of ``attention``: ``(dq, dk, dv)``, None where not wanted."""
+def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scale=None, want_q=True, want_k=True, want_v=True, rest=None):
+    """Adjoint of ``attention``: ``(dq, dk, dv)``, None where not wanted.  ``rest``: what ``out`` lost to its rounding, if that was kept."""
     name = "attention_backward"
     head_dim = q.shape[-1]
     q, k, v, lengths, scale, dim = _attention_operands(q, k, v, lengths, scale, name)
     batch, tokens, heads, _ = q.shape
     keys, kv_heads = k.shape[1:3]
-    _require_gpu(dout, out, lse)
-    for t in (dout, out):
+    _require_gpu(dout, out, lse, rest)
+    for t in (dout, out) if rest is None else (dout, out, rest):
         if t.shape[:3] != q.shape[:3] or t.shape[3] != head_dim:
             raise ValueError(f"{name}: {tuple(t.shape)} does not fit queries {tuple(q.shape[:3]) + (head_dim,)}")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (batch, heads, tokens) or not lse.is_contiguous() or lse.device != q.device:
@@ -1337,12 +1338,16 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scal
                      for t, want in ((q, want_q), (k, want_k), (v, want_v)))
     with _on_device_of(q):
         dout, out = (_aligned_heads(_heads(t, name, q), dim) for t in (dout, out))
+        if rest is not None:
+            rest = _aligned_heads(_heads(rest, name, q), dim)
+            if rest.stride() != out.stride():      # both are read at the same places
+                rest, out = contiguous(rest), contiguous(out)
         grads = [torch.empty(t.shape, dtype=q.dtype, device=q.device) if want else None for t, want in ((q, want_q), (k, want_k), (v, want_v))]
         elems = lib.ddl_attention_backward_workspace(batch, tokens, keys, heads, kv_heads, dim)
         work = torch.empty(max(elems, 1), dtype=torch.float32, device=q.device)
         arguments = [a for t in (dout, q, k, v, out) for a in (t.data_ptr(), _attention_strides(t))]
         results = [a for t in grads for a in ((None, None) if t is None else (t.data_ptr(), _attention_strides(t)))]
-        rc = lib.ddl_attention_backward(*arguments, lse.data_ptr(), _LN_DTYPES[q.dtype], batch, tokens, keys, heads, kv_heads, dim, _ptr(lengths),
+        rc = lib.ddl_attention_backward(*arguments, _ptr(rest), lse.data_ptr(), _LN_DTYPES[q.dtype], batch, tokens, keys, heads, kv_heads, dim, _ptr(lengths),
                                         int(causal), scale, *results, work.data_ptr(), elems, _stream())
         _lib.check(rc, "ddl_attention_backward")
         if dim != head_dim:

@@ -13,29 +13,30 @@ from .module import Module
 
 
 class _AttentionShard(torch.autograd.Function):
-    """Attention and its adjoint; kept for it are the operands, the result and one sum for each query and head."""
+    """Attention and its adjoint; kept for it are the operands, the result with what its rounding took (16-bit types), and one sum for each
+    query and head."""
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, causal, scale):
-        out, lse = hip_ops.attention(q, k, v, lengths, causal, scale, want_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, lse, rest = hip_ops.attention(q, k, v, lengths, causal, scale, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, rest)
         ctx.how = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, lse, lengths, rest = ctx.saved_tensors
         if grad_output.dtype != q.dtype:
             grad_output = grad_output.detach().to(q.dtype)
-        return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, *ctx.how, *ctx.needs_input_grad[:3]) + (None, None, None)
+        return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, *ctx.how, *ctx.needs_input_grad[:3], rest) + (None, None, None)
 
 
-def _general_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v):
-    """The adjoint for what its native form does not take.  ``q``, ``k``, ``v`` and ``out`` may be copies whose heads are padded with zeros."""
+def _general_backward(grad_output, q, k, v, out, rest, lse, lengths, causal, scale, want_q, want_k, want_v):
+    """The adjoint for what its native form does not take.  ``q``, ``k``, ``v``, ``out`` and ``rest`` may be copies whose heads are padded with zeros."""
     own = grad_output.shape[-1]
-    q, k, v, out = (t[..., :own] for t in (q, k, v, out))
-    return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v)
+    q, k, v, out, rest = (None if t is None else t[..., :own] for t in (q, k, v, out, rest))
+    return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v, rest)
 
 
 def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None):

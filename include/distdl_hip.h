@@ -667,6 +667,8 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  *            head h uses key head h * kv_heads / heads
  *   lse      [batch, heads, tokens] floats or NULL: log2 of a query's sum of
  *            exp(scale q . k) (+inf without keys), for the adjoint
+ *   out_rest like out, or NULL: with an lse, what the rounding of a 16-bit out took,
+ *            for the adjoint
  *   workspace  device memory of ddl_attention_workspace(...) floats, 16-byte
  *            aligned (few queries: the keys are split over workgroups)
  * 0 < scale <= 1e38.  Values of keys that some query of a sequence sees are to be
@@ -682,13 +684,14 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
                   int dtype, int64_t batch, int64_t tokens, int64_t keys,
                   int64_t heads, int64_t kv_heads, int64_t head_dim,
                   const int32_t* lengths, int causal, float scale, void* out,
-                  const int64_t* out_strides, float* lse, float* workspace,
-                  int64_t workspace_elems, void* stream);
+                  const int64_t* out_strides, void* out_rest, float* lse,
+                  float* workspace, int64_t workspace_elems, void* stream);
 
 /* The adjoint of ddl_attention: with dS_ij = p_ij (dout_i . v_j - dout_i . out_i),
  *   dq_i = scale sum dS_ij k_j,  dk_j = scale sum dS_ij q_i,  dv_j = sum p_ij dout_i,
  * summed over all heads that share a key head; zeros for queries and keys that
- * nothing is summed for.  out and lse as ddl_attention returned them; dq, dk or
+ * nothing is summed for.  out, out_rest (NULL: not kept, gradients of queries
+ * with few keys are less exact) and lse as ddl_attention returned them; dq, dk or
  * dv may be NULL; `workspace`: device memory of
  * ddl_attention_backward_workspace(...) floats, 16-byte aligned.  Nothing is added
  * atomically: equal calls give equal bits.  Probabilities and dS are rounded to
@@ -701,7 +704,8 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides,
                            const void* q, const int64_t* q_strides, const void* k,
                            const int64_t* k_strides, const void* v,
                            const int64_t* v_strides, const void* out,
-                           const int64_t* out_strides, const float* lse, int dtype,
+                           const int64_t* out_strides, const void* out_rest,
+                           const float* lse, int dtype,
                            int64_t batch, int64_t tokens, int64_t keys,
                            int64_t heads, int64_t kv_heads, int64_t head_dim,
                            const int32_t* lengths, int causal, float scale,

@@ -11,8 +11,9 @@ the second product, fp32 keeps them) and e = 2^-24:
   sum of the probabilities as rounded: with p (1 + d), |d| <= u, for p, sum p (1 + d) v / sum p (1 + d) is sum p d (v - out) off to first
   order, at most u sum p |v - out| <= u (sum p |v| + |out|).  (With values of 0 and one of 1 that has little weight the sum is twice
   u sum p |v|, so the second term is needed.)  The adjoint's probabilities come from the unrounded total;
-* gradients: dv as out, with sums over queries of p |dy|; dS = p (dP - D), dP and D off by 130 e sum |dy v| each (D: from `out`, which
-  is off by its own tolerance: 2 u sum |dy out| + (u + 2 c) sum |dy| (p |v|) more), so dS is off by
+* gradients: dv as out, with sums over queries of p |dy|; dS = p (dP - D), dP and D off by 130 e sum |dy v| each (D: from `out` and
+  what its rounding took, rounded, so off by its tolerance without the result's own: (u + u^2) sum |dy out| + (u + 2 c) sum |dy| (p |v|) more, fp32
+  u sum |dy out| instead of the first), so dS is off by
   p ((u + 2 c) (|dP| + |D|) + 260 e sum |dy v| + D's), and dq, dk sum that times |k|, |q|; sums of n terms add n e of their magnitude.
 The sums of magnitudes are formed in 64 bits with absolute values.  float16 loses 2^-25 next to zero for every rounding (a probability,
 a result) on top.
@@ -57,7 +58,7 @@ def _bounds(q, k, v, lengths, causal, scale, u, tiny, dy=None, rounded=True):
             g = dy[b, :, h]
             dp, dd = g @ vb.T, (g * o).sum(-1)[:, None]
             mag, mago, magp = np.abs(g) @ np.abs(vb).T, (np.abs(g) * np.abs(o)).sum(-1)[:, None], (np.abs(g) * (p @ np.abs(vb))).sum(-1)[:, None]
-            off = p * ((up + 2 * c) * (np.abs(dp) + np.abs(dd)) + 260 * e * mag + (u + up) * mago + (up + 2 * c) * magp) + tiny * see
+            off = p * ((up + 2 * c) * (np.abs(dp) + np.abs(dd)) + 260 * e * mag + (up + u * u if u > e else u) * mago + tiny * np.abs(g).sum(-1)[:, None] + (up + 2 * c) * magp) + tiny * see
             ds = p * (dp - dd)
             e_sum = (tokens + keys) * e
             dq[b, :, h] = u * np.abs(scale * ds @ kb) + scale * (off + e_sum * np.abs(ds)) @ np.abs(kb) + tiny
@@ -84,7 +85,7 @@ def _inputs(dt, batch, tokens, keys, heads, kv_heads, dim, seed=0):
     return q, k, v, dy
 
 
-def _check(dt, q, k, v, lengths=None, causal=False, scale=None, dy=None):
+def _check(dt, q, k, v, lengths=None, causal=False, scale=None, dy=None, rounded=None):
     from distdl_amd import nn
     u, tiny = torch.finfo(dt).eps / 2, 2.0 ** -25 if dt == torch.float16 else 0.0
     if dy is not None:
@@ -96,7 +97,7 @@ def _check(dt, q, k, v, lengths=None, causal=False, scale=None, dy=None):
     sc = q.shape[-1] ** -0.5 if scale is None else scale
     qn, kn, vn = _f64(q), _f64(k), _f64(v)
     want = o_heads.attention(qn, kn, vn, n, causal, sc, None if dy is None else _f64(dy))
-    tol = _bounds(qn, kn, vn, n, causal, sc, u, tiny, None if dy is None else _f64(dy), dt != torch.float32)
+    tol = _bounds(qn, kn, vn, n, causal, sc, u, tiny, None if dy is None else _f64(dy), dt != torch.float32 if rounded is None else rounded)
     _within("out", out, want[0], tol[0])
     if dy is not None:
         grads = torch.autograd.grad(out, [q, k, v], dy)
@@ -234,6 +235,15 @@ def test_key_heads_without_heads():
     out = nn.attention_shard(q, k, k)
     assert out.shape == q.shape
     assert not torch.autograd.grad(out.sum(), [k])[0].any()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("keys,tokens", [(1, 5), (50, 5), (200, 5), (200, 3000)])
+def test_gradients_of_a_single_key(dt, keys, tokens):
+    """A probability of one is not rounded, and dS, the difference of two equal sums, is zero but for errors of 32 bits: the bounds without the
+    roundings to the element type, all keys in one tile or not."""
+    q, k, v, dy = _inputs(dt, 2, tokens, keys, 8, 2, 64, seed=15)
+    _check(dt, q, k, v, torch.tensor([1, 0], dtype=torch.int32, device="cuda"), dy=dy, rounded=False)
 
 
 @pytest.mark.parametrize("dt", TYPES)

@@ -111,7 +111,7 @@ def test_rotation_of_the_oracle_keeps_lengths_and_turns_back():
 def _attention(lib, **change):
     st = _i64(64, 64, 64)
     a = dict(q=16, qs=st, k=16, ks=st, v=16, vs=st, dtype=_lib.DDL_DT_BF16, batch=1, tokens=1, keys=1, heads=2, kv=1, dim=64, lengths=None, causal=0,
-             scale=0.125, out=16, outs=st, lse=None, work=None, elems=0, stream=None)
+             scale=0.125, out=16, outs=st, rest=None, lse=None, work=None, elems=0, stream=None)
     assert set(change) <= set(a)
     a.update(change)
     return lib.ddl_attention(*a.values())
@@ -122,7 +122,8 @@ ATTENTION_REFUSALS = [
     (dict(kv=0), -4, "cannot share"), (dict(heads=3, kv=2), -4, "cannot share"), (dict(scale=0.0), -1, "positive"), (dict(scale=-1.0), -1, "positive"),
     (dict(scale=float("nan")), -1, "positive"), (dict(scale=float("inf")), -1, "positive"), (dict(scale=2e38), -1, "positive"), (dict(heads=0), -4, "without heads"), (dict(q=None), -1, "null"), (dict(v=None), -1, "null"),
     (dict(outs=None), -1, "null"), (dict(k=8), -3, "aligned"), (dict(ks=_i64(64, 60, 64)), -3, "multiples"), (dict(ks=_i64(64, 1 << 22, 64)), -5, "2^22"),
-    (dict(vs=_i64(64, -64, 64)), -5, "2^22"), (dict(tokens=1 << 30), -5, "2^30"), (dict(keys=1 << 30), -5, "2^30"),
+    (dict(vs=_i64(64, -64, 64)), -5, "2^22"), (dict(rest=16), -1, "rest"), (dict(rest=16, lse=16, dtype=_lib.DDL_DT_F32), -1, "rest"), (dict(rest=8, lse=16), -3, "rest"),
+    (dict(tokens=1 << 30), -5, "2^30"), (dict(keys=1 << 30), -5, "2^30"),
 ]
 
 
@@ -149,10 +150,12 @@ def test_attention_asks_for_its_workspaces():
     need = lib.ddl_attention_backward_workspace(2, 5, 7, 4, 2, 64)
     assert need >= 2 * 5 * 4
     st = _i64(64, 64, 64)
-    call = [16, st] * 5 + [16, _lib.DDL_DT_BF16, 2, 5, 7, 4, 2, 64, None, 0, 0.125] + [16, st] * 3
+    call = [16, st] * 5 + [None, 16, _lib.DDL_DT_BF16, 2, 5, 7, 4, 2, 64, None, 0, 0.125] + [16, st] * 3
     assert lib.ddl_attention_backward(*call, 16, need - 1, None) == -1 and "workspace" in lib.ddl_last_error().decode()
-    assert lib.ddl_attention_backward(*call[:10], None, *call[11:], 16, need, None) == -1 and "row sums" in lib.ddl_last_error().decode()
-    assert lib.ddl_attention_backward(*call[:22], None, *call[23:], 16, need, None) == -1 and "no strides" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:11], None, *call[12:], 16, need, None) == -1 and "row sums" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:23], None, *call[24:], 16, need, None) == -1 and "no strides" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:10], 8, *call[11:], 16, need, None) == -3 and "rest" in lib.ddl_last_error().decode()
+    assert lib.ddl_attention_backward(*call[:10], 16, 16, _lib.DDL_DT_F32, *call[13:], 16, need, None) == -1 and "rest" in lib.ddl_last_error().decode()
 
 
 def test_attention_layers_and_functions_refuse():
