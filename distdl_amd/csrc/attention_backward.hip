@@ -53,7 +53,9 @@ __device__ inline void load_column(Frag* column, const T* row, bool there, int c
 }
 
 // dq of 32 queries a wavefront, 128 a workgroup, tiles of keys and values through LDS as in attention_rows; and their D.
-// [4,4096,16,128] bf16, all keys: 755 us (1093 TFLOP/s for three products; 782 before its two kinds of work were woven), head size 64: 407.
+// [4,4096,16,128] bf16, all keys: 717 us (1150 TFLOP/s for three products), head size 64: 407, causal [4,2048,8,128] 71.  Bound by the matrix
+// cores and the vector work that does not fit next to them.
+// Where there are few blocks of queries, `splits` workgroups share the keys of one and leave sums in fp32.
 // ONE (16-bit types): all keys are in one tile, D from them.
 template <typename T, int DP, bool ONE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_backward_rows(const AttnArgs a) {
@@ -62,6 +64,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     constexpr int KEYS = tile_rows<T>(), NS = KEYS / 32, kTileBytes = KEYS * Tile::kRowBytes;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    const int split = blockIdx.y;
     int bh, block;
     block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, bh, block);
     const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
@@ -76,13 +79,14 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     const T* k = static_cast<const T*>(a.k) + batch * a.k_at.batch + kv_head * a.k_at.head;
     const T* v = static_cast<const T*>(a.v) + batch * a.v_at.batch + kv_head * a.v_at.head;
     Tile tile(lds, lane);
-    const int tiles = (end + KEYS - 1) / KEYS;
+    const int tiles = (end + KEYS - 1) / KEYS, share = scalar(tiles / a.splits), more = tiles - share * a.splits;
+    const int t0 = share * split + min(split, more), t1 = t0 + share + (split < more ? 1 : 0), limit = min(end, t1 * KEYS);
     const AttnCopy<T, DP, KEYS, kWaves, (DP > 96)> k_copy(k, a.k_at.token, a.chunks, wave, lane), v_copy(v, a.v_at.token, a.chunks, wave, lane);
-    auto request = [&](int t) {
-        const char* to = lds + (t & 1) * kTileBytes;
-        k_copy.request(to, t * KEYS, end), v_copy.request(to + 2 * kTileBytes, t * KEYS, end);
+    auto request = [&](int t, int set) {
+        const char* to = lds + set;
+        k_copy.request(to, t * KEYS, limit), v_copy.request(to + 2 * kTileBytes, t * KEYS, limit);
     };
-    if (ONE || a.dq) request(0);
+    if (ONE || a.dq) request(t0, 0);
     Frag q_column[Tile::kSteps], g_column[Tile::kSteps];
     load_column<T, DP>(q_column, static_cast<const T*>(a.q) + batch * a.q_at.batch + my_row * a.q_at.token + head * a.q_at.head, mine, a.chunks, half);
     load_column<T, DP>(g_column, static_cast<const T*>(a.dout) + batch * a.dout_at.batch + my_row * a.dout_at.token + head * a.dout_at.head, mine, a.chunks, half);
@@ -116,18 +120,21 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         }
     }
     delta = add_halves(delta);
-    if (mine && half == 0) a.delta[stat] = delta;
+    if (mine && half == 0 && split == 0) a.delta[stat] = delta;
     if (!a.dq) return;      // D alone
     floatx16 acc[Tile::kBlocks];
     clear(acc);
-    for (int t = 0; t < tiles; ++t) {
+    int set = 0;      // of tiles: the first or the second
+    for (int t = t0; t < t1; ++t) {
         wait_for_copies();
         lds_barrier();
-        request(t + 1);
-        bool done = t * KEYS >= wave_most;
+        // Behind the first product where there is other work as well: in front of it the kernel spills with DP = 128, and what it reads back waits for
+        // these copies (dq of [4,4096,16,128] bf16 785 us instead of 717, of [4,2048,8,128] causal 82 instead of 71).
+        auto ask = [&] { request(t + 1, kTileBytes - set); };
+        bool done = t * KEYS >= wave_most, asked = false;
         if constexpr (sizeof(T) == 2 && NS == 2 && !ONE) {
             if (!done && (t + 1) * KEYS <= wave_least) {     // 64 keys that all see: the vector units are at 32 of them while the matrix cores are at others
-                done = true;
+                done = asked = true;
                 floatx16 p0, p1, d0, d1;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p0[r] = p1[r] = d0[r] = d1[r] = 0.f;
@@ -139,6 +146,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
                 };
                 auto nothing = [](int) {};
                 tile.template straight_woven<0>(p0, kK, q_column, nothing);
+                ask();
                 tile.template straight_woven<16>(d0, kV, g_column, exponential(p0));
                 tile.template straight_woven<16>(p1, kK + kNext, q_column, difference(d0, p0));
                 const typename Tile::Packed first = Tile::pack(d0);
@@ -147,6 +155,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
                 tile.template transposed_woven<0>(acc, kK + kNext, Tile::pack(d1), nothing);
             }
         }
+        if (!asked) ask();
         if (!done) {
             const bool masked = (t + 1) * KEYS > wave_least;
             const int rest = seen - t * KEYS - 4 * half;
@@ -165,16 +174,44 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
                 tile.transposed(acc, kK, n, Tile::pack(s[0]));
             }
         }
-        tile.shift(t & 1 ? -kTileBytes : kTileBytes);
+        tile.shift(kTileBytes - 2 * set), set = kTileBytes - set;
     }
     wait_for_copies();
     lds_barrier();
+    if (a.splits > 1) {
+        typedef AttnOut<float, DP> Out;
+        char* room = lds + wave * Out::kRoom;
+        Out::park(room, acc, a.scale, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int dim = a.chunks * Tile::kPerChunk;
+        float* to = a.partial + (static_cast<int64_t>(split) * a.batch * a.heads + bh) * a.tokens * dim;
+        Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_row + col < a.tokens ? to + static_cast<int64_t>(wave_row + col) * dim : nullptr; });
+        return;
+    }
     typedef AttnOut<T, DP> Out;
     char* room = lds + wave * Out::kRoom;
     Out::park(room, acc, a.scale, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     T* dq = static_cast<T*>(a.dq) + batch * a.dq_at.batch + head * a.dq_at.head;
     Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_row + col < a.tokens ? dq + (wave_row + col) * a.dq_at.token : nullptr; });
+}
+
+// dq from the splits' sums, in their order: four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_backward_rows_join(const AttnArgs a) {
+    const int quads = a.chunks * AttnElem<T>::kPerChunk / 4;
+    const int64_t all = static_cast<int64_t>(a.batch) * a.heads * a.tokens * quads, at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (at >= all) return;
+    const float4* p = reinterpret_cast<const float4*>(a.partial) + at;
+    float4 sum = p[0];
+    for (int s = 1; s < a.splits; ++s) {
+        const float4 more = p[all * s];
+        sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+    }
+    const int64_t row = at / quads;
+    const int d = 4 * static_cast<int>(at - row * quads), bh = static_cast<int>(row / a.tokens), token = static_cast<int>(row - static_cast<int64_t>(bh) * a.tokens);
+    const int batch = bh / a.heads, head = bh - batch * a.heads;
+    store_piece<true>(static_cast<T*>(a.dq) + batch * a.dq_at.batch + token * a.dq_at.token + head * a.dq_at.head + d, sum);
 }
 
 template <typename T, int DP>
@@ -320,11 +357,12 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     };
     // 64 queries that see all of the wavefront's keys: while the vector units are at the first 32, the matrix cores form the scores of the
     // others, and while they are at those, the sums of the first.
-    auto pair_step = [&](const float* rows, auto fk, auto fv) {
+    auto pair_step = [&](const float* rows, auto&& ask, auto fk, auto fv) {
         floatx16 p0, p1, d0, d1;
         zero(p0), zero(p1), zero(d0), zero(d1);
         OfRows lse0(rows);
         tile.template straight_woven<0>(p0, kQ, k_column, nothing);
+        ask();
         if constexpr (fk) {
             tile.template straight_woven<16>(d0, kG, v_column, exponential(p0, lse0));
             const typename Tile::Packed b0 = Tile::pack(p0);
@@ -350,18 +388,21 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
         for (int it = it0; it < it1; ++it) {
             wait_for_copies();
             lds_barrier();
-            // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
-            request(it + 1, next), store_rows(it + 1);
             const int first = (first_tile + now.tile) * ROWS, set = set_of(it);
-            now = next, next = after(next);
-            load_rows(it + 2, next);
+            // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
+            auto ask = [&] {
+                request(it + 1, next), store_rows(it + 1);
+                now = next, next = after(next);
+                load_rows(it + 2, next);
+            };
             const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 4 * half;
             bool done = false;
             if constexpr (sizeof(T) == 2 && NS == 2 && !(ROLES && fk)) {      // (the two columns and dk leave no registers for 64 at a time)
                 done = first >= wave_all;
-                if (done) pair_step(rows, fk, fv);
+                if (done) pair_step(rows, ask, fk, fv);
             }
             if (!done) {
+                ask();
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
                     if (first + 32 * (n + 1) > wave_need) block_step(n, first, rows, first + 32 * n < wave_all, fk, fv);
@@ -428,7 +469,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_join(const AttnAr
 
 template <typename T, int DP>
 constexpr int backward_rows_lds() {
-    constexpr int tiles = 4 * tile_rows<T>() * AttnTile<T, DP>::kRowBytes, out = kWaves * AttnOut<T, DP>::kRoom;
+    constexpr int tiles = 4 * tile_rows<T>() * AttnTile<T, DP>::kRowBytes, out = kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
 }
 template <typename T, int DP>
@@ -452,6 +493,18 @@ int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64
 template <typename T>
 constexpr int least_of_split() { return sizeof(T) == 2 ? 8 : 2; }
 
+// Workgroups that share the keys of a block of queries: as many as the chip has CUs in all, with at least `least` keys.  (dq of fp32 [1,64,8,64],
+// 4096 keys: 40 us, most of it the call, instead of 403; fp32 [1,448,16,64], 1500 keys: 56 instead of 153; [1,2048,8,128] bf16 57 instead of 61.)
+int row_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t least) {
+    if (batch < 1 || tokens < 1 || keys < 1 || heads < 1) return 1;
+    int dev;
+    int64_t splits = compute_units(dev) / (batch * heads * ((tokens + kRows * kWaves - 1) / (kRows * kWaves)));
+    if (splits > keys / least) splits = keys / least;
+    return static_cast<int>(splits < 1 ? 1 : splits);
+}
+template <typename T>
+constexpr int least_keys() { return sizeof(T) == 2 ? 256 : 64; }
+
 int64_t rounded4(int64_t n) { return (n + 3) / 4 * 4; }
 
 }  // namespace
@@ -463,7 +516,9 @@ int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens, int64_t 
     using namespace ddl;
     if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || dim < 1 || keys < 0) return 0;
     const int64_t splits = key_splits(batch, tokens, keys, heads, kv_heads, true, least_of_split<float>());      // the most that a call takes
-    return rounded4(batch * heads * tokens) + (splits > 1 ? splits * 2 * batch * kv_heads * keys * dim : 0);
+    const int64_t shares = row_splits(batch, tokens, keys, heads, least_keys<float>());
+    const int64_t of_keys = splits > 1 ? splits * 2 * batch * kv_heads * keys * dim : 0, of_rows = shares > 1 ? shares * batch * heads * tokens * dim : 0;
+    return rounded4(batch * heads * tokens) + (of_keys > of_rows ? of_keys : of_rows);      // (the kernels run one after the other)
 }
 
 int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -502,19 +557,25 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         constexpr int kRowsLds = backward_rows_lds<T, DP>(), kKeysLds = backward_keys_lds<T, DP>();
         if (a.tokens) {
             a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+            a.splits = a.dq ? row_splits(batch, tokens, keys, heads, least_keys<T>()) : 1;
             const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
             if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
             a.folded = folds(a.causal, grid);
             const auto launch = [&](auto one) {
                 constexpr bool ONE = decltype(one)::value;
                 if (const int rc = grant_lds<attention_backward_rows<T, DP, ONE>>(kRowsLds, "ddl_attention_backward")) return rc;
-                hipLaunchKernelGGL((attention_backward_rows<T, DP, ONE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kRowsLds, s, a);
+                hipLaunchKernelGGL((attention_backward_rows<T, DP, ONE>), dim3(static_cast<uint32_t>(grid), a.splits), dim3(kThreads), kRowsLds, s, a);
                 return check_launch("ddl_attention_backward");
             };
             int rc;
             if constexpr (sizeof(T) == 2) rc = a.keys <= tile_rows<T>() ? launch(std::true_type{}) : launch(std::false_type{});
             else rc = launch(std::false_type{});
             if (rc) return rc;
+            if (a.splits > 1) {
+                const int64_t threads = static_cast<int64_t>(a.batch) * a.heads * a.tokens * (dim / 4);
+                hipLaunchKernelGGL((attention_backward_rows_join<T>), dim3(static_cast<uint32_t>((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+                if (const int joined = check_launch("ddl_attention_backward")) return joined;
+            }
         }
         if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
         if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kKeysLds, "ddl_attention_backward")) return rc;
