@@ -397,7 +397,7 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
             };
             const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 4 * half;
             bool done = false;
-            if constexpr (sizeof(T) == 2 && NS == 2 && !(ROLES && fk)) {      // (the two columns and dk leave no registers for 64 at a time)
+            if constexpr (sizeof(T) == 2 && NS == 2 && !(fk && DP > 96)) {      // (the two columns and dk leave no registers for 64 at a time)
                 done = first >= wave_all;
                 if (done) pair_step(rows, ask, fk, fv);
             }
