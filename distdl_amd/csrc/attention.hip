@@ -99,8 +99,8 @@ constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // front of its last block, is then enough for two buffers of each.  What follows it is copied to where
 // everybody has just finished reading: keys two tiles ahead, values NS - 1 blocks ahead.
 //
-// [4,4096,16,128] bf16, all keys: 624 us (881 TFLOP/s; 754 with the parts one behind the other and tiles through registers); head size
-// 64: 303 us, causal: 273 us (1000), fp32 [2,2048,8,64] 159 us (108).  Bound by issue: the exponentials and the softmax's other
+// [4,4096,16,128] bf16, all keys: 624 us (881 TFLOP/s; 729 us with the parts one behind the other and tiles through registers), in runs of
+// 20 calls 536; head size 64: 303 us, causal: 273 us (1000), fp32 [2,2048,8,64] 159 us (108).  Bound by issue: the exponentials and the softmax's other
 // vector work next to the matrix instructions, of which each pipe is busy about half of the time.
 template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_rows(const AttnArgs a) {
