@@ -214,32 +214,69 @@ __global__ __launch_bounds__(kThreads) void attention_backward_rows_join(const A
     store_piece<true>(static_cast<T*>(a.dq) + batch * a.dq_at.batch + token * a.dq_at.token + head * a.dq_at.head + d, sum);
 }
 
+constexpr int kPairRows = 64;
 template <typename T, int DP>
 constexpr int query_tile() { return sizeof(T) == 2 || AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32; }
 
+// Which queries a wavefront's 32 keys are seen by, and which of them, ROWS of one head at a time, are this workgroup's share.
+template <int ROWS>
+struct QueriesOfKeys {
+    int wave_key, my_key;
+    int need;                      // first query that sees this lane's key
+    int wave_need, wave_all;       // first one that sees any of the wavefront's, and from where on they see all
+    int first_tile, head_tiles;    // of a head, for the workgroup
+    int it0, it1;                  // its share of all heads' tiles
+    __device__ QueriesOfKeys(const AttnArgs& a, int first_key, int wave, int lane, int length, int split) {
+        auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        wave_key = first_key + wave * kRows, my_key = wave_key + (lane & 31);
+        const int shift = a.causal ? a.keys - a.tokens : 0x3FFFFFFF;      // query i sees key j from i = j - shift on
+        need = my_key < length ? max(my_key - shift, 0) : 0x7FFFFFFF;
+        const int block_need = scalar(first_key < length ? max(first_key - shift, 0) : a.tokens);
+        wave_need = scalar(wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF);
+        wave_all = scalar(wave_key + kRows <= length ? max(wave_key + kRows - 1 - shift, 0) : 0x7FFFFFFF);
+        first_tile = min(block_need, a.tokens) / ROWS, head_tiles = block_need < a.tokens ? (a.tokens + ROWS - 1) / ROWS - first_tile : 0;
+        const int64_t all = static_cast<int64_t>(head_tiles) * a.group;
+        it0 = static_cast<int>(all * split / a.splits), it1 = static_cast<int>(all * (split + 1) / a.splits);
+    }
+    struct At {                    // an iteration's head of the group and tile
+        int head, tile;
+    };
+    __device__ At start() const {
+        At at{0, 0};
+        if (it0 < it1) at.head = it0 / head_tiles, at.tile = it0 - at.head * head_tiles;
+        return at;
+    }
+    __device__ At after(At at) const {
+        if (++at.tile == head_tiles) at.tile = 0, ++at.head;
+        return at;
+    }
+};
+
+// Row values (sums or D) of the rows that this half of the lanes holds, four at a time, the next four on their way.
+struct OfRows {
+    const float* at;
+    floatx4v now, next;
+    __device__ explicit OfRows(const float* rows) : at(rows), next(*reinterpret_cast<const floatx4v*>(rows)) {}
+    __device__ float operator()(int r) {
+        if (r % 4 == 0) {
+            now = next;
+            if (r < 12) next = *reinterpret_cast<const floatx4v*>(at + 2 * (r + 4));
+        }
+        return now[r % 4];
+    }
+};
+
 // dk and dv of 32 keys a wavefront, 128 a workgroup; 32 or 64 queries of one head at a time through LDS, with their sums and D.  Where
 // there are few blocks of keys, `splits` workgroups share the queries of one and leave sums in fp32.
-//
-// 16-bit rows of more than 128 bytes: keys and values, both sums and both products of a step are more than the 256 registers with which
-// two wavefronts fit on a SIMD, and one alone leaves the matrix cores idle while it forms probabilities.  There a second set of four
-// wavefronts takes half of the work: the first four keep dk, the others dv, and both form the probabilities, five
-// products instead of four.  [4,4096,16,128] bf16: 1409 us (976 TFLOP/s for the five), both sums in one wavefront 2460.  Head size 64, one
-// role: 545 us, before its two kinds of work were woven 703.
-//
-// 64 queries at a time where LDS has room for two workgroups' (32: 1916 us with two roles then, 64: 1641).
+// [4,4096,16,64] bf16: 545 us, before its two kinds of work were woven 703.
 template <typename T, int DP>
-constexpr bool two_roles() { return sizeof(T) == 2 && DP > 64; }
-
-template <typename T, int DP>
-__global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!two_roles<T, DP>() && DP * sizeof(T) > 128 ? 1 : 2)) void attention_backward_keys(const AttnArgs a) {
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attention_backward_keys(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
     typedef typename Tile::Frag Frag;
-    constexpr bool ROLES = two_roles<T, DP>();
-    constexpr int WAVES = ROLES ? 2 * kWaves : kWaves, ROWS = query_tile<T, DP>(), NS = ROWS / 32;
+    constexpr int ROWS = query_tile<T, DP>(), NS = ROWS / 32;
     constexpr int kTileBytes = ROWS * Tile::kRowBytes, kSetBytes = 2 * kTileBytes + 2 * ROWS * 4;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
-    const bool for_k = !ROLES || wave < kWaves, for_v = !ROLES || wave >= kWaves;
     const int pairs = a.batch * a.kv_heads;
     int bk, unit;
     block_of(blockIdx.x, pairs, a.blocks * a.splits, false, bk, unit);
@@ -247,76 +284,44 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
     const int block = unit / a.splits, split = unit - block * a.splits;
     const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
-    const int first_key = block * kRows * kWaves, wave_key = first_key + wave % kWaves * kRows, my_key = wave_key + (lane & 31);
-    // Query i sees key j from i = j - shift on.
-    const int shift = a.causal ? a.keys - a.tokens : 0x3FFFFFFF;
-    const int need = my_key < length ? max(my_key - shift, 0) : 0x7FFFFFFF;      // first query that sees this lane's key
-    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int block_need = scalar(first_key < length ? max(first_key - shift, 0) : a.tokens);
-    const int wave_need = scalar(wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF);
-    const int wave_all = scalar(wave_key + kRows <= length ? max(wave_key + kRows - 1 - shift, 0) : 0x7FFFFFFF);   // from here on queries see all of the wavefront's keys
-    const int first_tile = min(block_need, a.tokens) / ROWS, head_tiles = block_need < a.tokens ? (a.tokens + ROWS - 1) / ROWS - first_tile : 0;
-    const int64_t all = static_cast<int64_t>(head_tiles) * a.group;
-    const int it0 = static_cast<int>(all * split / a.splits), it1 = static_cast<int>(all * (split + 1) / a.splits);
+    const QueriesOfKeys<ROWS> see(a, block * kRows * kWaves, wave, lane, length, split);
+    typedef typename QueriesOfKeys<ROWS>::At At;
+    const int it0 = see.it0, it1 = see.it1, wave_key = see.wave_key, my_key = see.my_key;
     const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
     const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
     const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
     Tile tile(lds, lane);
-    AttnCopy<T, DP, ROWS, WAVES> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
-    // Where an iteration's queries are: the head of the group and its first query.
-    struct At {
-        int head, tile;
-    };
-    auto after = [&](At at) {
-        if (++at.tile == head_tiles) at.tile = 0, ++at.head;
-        return at;
-    };
+    AttnCopy<T, DP, ROWS, kWaves> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
     auto set_of = [&](int it) { return ((it - it0) & 1) * kSetBytes; };
     auto request = [&](int it, At at) {
         if (it >= it1) return;
         char* to = lds + set_of(it);
         q_copy.base = reinterpret_cast<const char*>(q0 + at.head * a.q_at.head), g_copy.base = reinterpret_cast<const char*>(g0 + at.head * a.dout_at.head);
-        const int first = (first_tile + at.tile) * ROWS;
+        const int first = (see.first_tile + at.tile) * ROWS;
         q_copy.request(to, first, a.tokens), g_copy.request(to + kTileBytes, first, a.tokens);
     };
     float row_next = 0.f;       // of the queries on their way: threads 0 .. ROWS - 1 their sums, the next as many their D
     auto load_rows = [&](int it, At at) {
         if (it >= it1 || tid >= 2 * ROWS) return;
-        const int row = (first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
+        const int row = (see.first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
         const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
         row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
     };
     auto store_rows = [&](int it) {
         if (it < it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + set_of(it) + 2 * kTileBytes)[tid] = row_next;
     };
-    At next{0, 0};
-    if (it0 < it1) next.head = it0 / head_tiles, next.tile = it0 - next.head * head_tiles;
-    At now = next;
+    At next = see.start(), now = next;
     request(it0, next);
     load_rows(it0, next), store_rows(it0);
-    next = after(next);
+    next = see.after(next);
     load_rows(it0 + 1, next);
     Frag k_column[Tile::kSteps], v_column[Tile::kSteps];
     const bool mine = my_key < length;
     load_column<T, DP>(k_column, static_cast<const T*>(a.k) + batch * a.k_at.batch + my_key * a.k_at.token + kv_head * a.k_at.head, mine, a.chunks, half);
-    if (for_k) load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
-    floatx16 sums[ROLES ? 1 : 2][Tile::kBlocks];      // two roles: one sum a wavefront
-    floatx16(&dk)[Tile::kBlocks] = sums[0], (&dv)[Tile::kBlocks] = sums[ROLES ? 0 : 1];
+    load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
+    floatx16 dk[Tile::kBlocks], dv[Tile::kBlocks];
     clear(dk), clear(dv);
     auto nothing = [](int) {};
-    // Row values (sums or D) of the rows that this half of the lanes holds, four at a time, the next four on their way.
-    struct OfRows {
-        const float* at;
-        floatx4v now, next;
-        __device__ explicit OfRows(const float* rows) : at(rows), next(*reinterpret_cast<const floatx4v*>(rows)) {}
-        __device__ float operator()(int r) {
-            if (r % 4 == 0) {
-                now = next;
-                if (r < 12) next = *reinterpret_cast<const floatx4v*>(at + 2 * (r + 4));
-            }
-            return now[r % 4];
-        }
-    };
     auto exponential = [&](floatx16& p, OfRows& lse) {
         return [&](int r) { p[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, -lse(r)))); };
     };
@@ -329,11 +334,11 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
         for (int r = 0; r < 16; ++r) v[r] = 0.f;
     };
     // 32 queries, some of which (`masked`) may not see some of the wavefront's keys.
-    auto block_step = [&](int n, int first, const float* rows, bool masked, auto fk, auto fv) {
+    auto block_step = [&](int n, int first, const float* rows, bool masked) {
         floatx16 p, d;
         zero(p), zero(d);
         tile.straight(p, kQ, n, k_column);
-        if constexpr (fk) tile.straight(d, kG, n, v_column);
+        tile.straight(d, kG, n, v_column);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const floatx4v lse = *reinterpret_cast<const floatx4v*>(rows + 32 * n + 8 * g);
@@ -342,85 +347,68 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
         }
         if (masked) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = first + 32 * n + 4 * half + (r & 3) + 8 * (r >> 2) >= need ? p[r] : 0.f;
+            for (int r = 0; r < 16; ++r) p[r] = first + 32 * n + 4 * half + (r & 3) + 8 * (r >> 2) >= see.need ? p[r] : 0.f;
         }
-        if constexpr (fv) tile.transposed(dv, kG, n, Tile::pack(p));
-        if constexpr (fk) {
+        tile.transposed(dv, kG, n, Tile::pack(p));
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const floatx4v delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 32 * n + 8 * g);
+        for (int g = 0; g < 4; ++g) {
+            const floatx4v delta = *reinterpret_cast<const floatx4v*>(rows + ROWS + 32 * n + 8 * g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[4 * g + i] = p[4 * g + i] * (d[4 * g + i] - delta[i]);
-            }
-            tile.transposed(dk, kQ, n, Tile::pack(d));
+            for (int i = 0; i < 4; ++i) d[4 * g + i] = p[4 * g + i] * (d[4 * g + i] - delta[i]);
         }
+        tile.transposed(dk, kQ, n, Tile::pack(d));
     };
     // 64 queries that see all of the wavefront's keys: while the vector units are at the first 32, the matrix cores form the scores of the
     // others, and while they are at those, the sums of the first.
-    auto pair_step = [&](const float* rows, auto&& ask, auto fk, auto fv) {
+    auto pair_step = [&](const float* rows, auto&& ask) {
         floatx16 p0, p1, d0, d1;
         zero(p0), zero(p1), zero(d0), zero(d1);
         OfRows lse0(rows);
         tile.template straight_woven<0>(p0, kQ, k_column, nothing);
         ask();
-        if constexpr (fk) {
-            tile.template straight_woven<16>(d0, kG, v_column, exponential(p0, lse0));
-            const typename Tile::Packed b0 = Tile::pack(p0);
-            OfRows delta0(rows + ROWS);
-            tile.template straight_woven<16>(p1, kQ + kNext, k_column, difference(d0, p0, delta0));
-            const typename Tile::Packed a0 = Tile::pack(d0);
-            OfRows lse1(rows + 32);
-            tile.template straight_woven<16>(d1, kG + kNext, v_column, exponential(p1, lse1));
-            const typename Tile::Packed b1 = Tile::pack(p1);
-            OfRows delta1(rows + ROWS + 32);
-            if constexpr (fv) tile.template transposed_woven<0>(dv, kG, b0, nothing);
-            tile.template transposed_woven<16>(dk, kQ, a0, difference(d1, p1, delta1));
-            if constexpr (fv) tile.template transposed_woven<0>(dv, kG + kNext, b1, nothing);
-            tile.template transposed_woven<0>(dk, kQ + kNext, Tile::pack(d1), nothing);
-        } else {
-            tile.template straight_woven<16>(p1, kQ + kNext, k_column, exponential(p0, lse0));
-            OfRows lse1(rows + 32);
-            tile.template transposed_woven<16>(dv, kG, Tile::pack(p0), exponential(p1, lse1));
-            tile.template transposed_woven<0>(dv, kG + kNext, Tile::pack(p1), nothing);
-        }
+        tile.template straight_woven<16>(d0, kG, v_column, exponential(p0, lse0));
+        const typename Tile::Packed b0 = Tile::pack(p0);
+        OfRows delta0(rows + ROWS);
+        tile.template straight_woven<16>(p1, kQ + kNext, k_column, difference(d0, p0, delta0));
+        const typename Tile::Packed a0 = Tile::pack(d0);
+        OfRows lse1(rows + 32);
+        tile.template straight_woven<16>(d1, kG + kNext, v_column, exponential(p1, lse1));
+        const typename Tile::Packed b1 = Tile::pack(p1);
+        OfRows delta1(rows + ROWS + 32);
+        tile.template transposed_woven<0>(dv, kG, b0, nothing);
+        tile.template transposed_woven<16>(dk, kQ, a0, difference(d1, p1, delta1));
+        tile.template transposed_woven<0>(dv, kG + kNext, b1, nothing);
+        tile.template transposed_woven<0>(dk, kQ + kNext, Tile::pack(d1), nothing);
     };
-    auto walk = [&](auto fk, auto fv) {
-        for (int it = it0; it < it1; ++it) {
-            wait_for_copies();
-            lds_barrier();
-            const int first = (first_tile + now.tile) * ROWS, set = set_of(it);
-            // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
-            auto ask = [&] {
-                request(it + 1, next), store_rows(it + 1);
-                now = next, next = after(next);
-                load_rows(it + 2, next);
-            };
-            const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 4 * half;
-            bool done = false;
-            if constexpr (sizeof(T) == 2 && NS == 2 && !(fk && DP > 96)) {      // (the two columns and dk leave no registers for 64 at a time)
-                done = first >= wave_all;
-                if (done) pair_step(rows, ask, fk, fv);
-            }
-            if (!done) {
-                ask();
+    for (int it = it0; it < it1; ++it) {
+        wait_for_copies();
+        lds_barrier();
+        const int first = (see.first_tile + now.tile) * ROWS, set = set_of(it);
+        // `next` is the iteration after this one: its tiles are asked for, its rows' sums stored; those of the one after it loaded
+        auto ask = [&] {
+            request(it + 1, next), store_rows(it + 1);
+            now = next, next = see.after(next);
+            load_rows(it + 2, next);
+        };
+        const float* rows = reinterpret_cast<const float*>(lds + set + 2 * kTileBytes) + 4 * half;
+        bool done = false;
+        if constexpr (sizeof(T) == 2 && NS == 2) {
+            done = first >= see.wave_all;
+            if (done) pair_step(rows, ask);
+        }
+        if (!done) {
+            ask();
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
-                    if (first + 32 * (n + 1) > wave_need) block_step(n, first, rows, first + 32 * n < wave_all, fk, fv);
-            }
-            tile.shift(set ? -kSetBytes : kSetBytes);
+            for (int n = 0; n < NS; ++n)
+                if (first + 32 * (n + 1) > see.wave_need) block_step(n, first, rows, first + 32 * n < see.wave_all);
         }
-    };
-    const std::true_type yes{};
-    const std::false_type no{};
-    if constexpr (!ROLES) walk(yes, yes);
-    else if (for_k) walk(yes, no);
-    else walk(no, yes);
+        tile.shift(set ? -kSetBytes : kSetBytes);
+    }
     wait_for_copies();
     lds_barrier();
     const int dim = a.chunks * Tile::kPerChunk;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        if (!(which ? for_v : for_k)) continue;
         if (a.splits == 1) {
             typedef AttnOut<T, DP> Out;
             char* room = lds + wave * Out::kRoom;
@@ -435,6 +423,160 @@ __global__ __launch_bounds__((two_roles<T, DP>() ? 2 * kThreads : kThreads), (!t
         } else {
             typedef AttnOut<float, DP> Out;
             char* room = lds + wave * Out::kRoom;
+            float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
+            if (which) Out::park(room, dv, 1.f, lane);
+            else Out::park(room, dk, a.scale, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_key + col < a.keys ? to + static_cast<int64_t>(wave_key + col) * dim : nullptr; });
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// The same for 16-bit heads of more than 64 elements.  Keys and values, both sums and both products of a step are more than the 256 registers with which
+// two wavefronts fit on a SIMD, and one alone leaves the matrix cores idle while it forms probabilities.  So two sets of four wavefronts share
+// the work: the first form the probabilities and dS of 32 queries and leave them in LDS, rounded as the products take them and for the lanes that
+// take them, and the second add them to both sums a step later: two products each, and while one wavefront of a SIMD is at its exponentials, the
+// other has matrix instructions.  Three sets of tiles: of the queries whose turn it is, those before and those on their way.
+template <typename T, int DP>
+__global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(const AttnArgs a) {
+    typedef AttnTile<T, DP> Tile;
+    typedef typename Tile::Frag Frag;
+    constexpr int WAVES = 2 * kWaves, ROWS = kPairRows, kTileBytes = ROWS * Tile::kRowBytes, kSetBytes = 2 * kTileBytes, kSets = 3;
+    constexpr int kRowsAt = kSets * kSetBytes, kHandedAt = kRowsAt + kSets * 2 * ROWS * 4;
+    constexpr uint32_t kQ = 0, kG = kTileBytes, kBlock = 32 * Tile::kRowBytes;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
+    const int pairs = a.batch * a.kv_heads;
+    int bk, unit;
+    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, bk, unit);
+    unit = a.blocks * a.splits - 1 - unit;      // the first keys, which most queries see in the causal form, first
+    const int block = unit / a.splits, split = unit - block * a.splits;
+    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
+    const int length = sequence_keys(a, batch);
+    const QueriesOfKeys<ROWS> see(a, block * kRows * kWaves, wave % kWaves, lane, length, split);
+    const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
+    const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
+    const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
+    Tile tile(lds, lane);
+    AttnCopy<T, DP, ROWS, WAVES> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
+    auto request = [&](int it, const typename QueriesOfKeys<ROWS>::At& at, int set) {
+        if (it >= see.it1) return;
+        char* to = lds + set * kSetBytes;
+        q_copy.base = reinterpret_cast<const char*>(q0 + at.head * a.q_at.head), g_copy.base = reinterpret_cast<const char*>(g0 + at.head * a.dout_at.head);
+        const int first = (see.first_tile + at.tile) * ROWS;
+        q_copy.request(to, first, a.tokens), g_copy.request(to + kTileBytes, first, a.tokens);
+    };
+    float row_next = 0.f;       // of the queries on their way: threads 0 .. ROWS - 1 their sums, the next as many their D
+    auto load_rows = [&](int it, const typename QueriesOfKeys<ROWS>::At& at) {
+        if (it >= see.it1 || tid >= 2 * ROWS) return;
+        const int row = (see.first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
+        const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
+        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
+    };
+    auto store_rows = [&](int it, int set) {
+        if (it < see.it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + kRowsAt + set * 2 * ROWS * 4)[tid] = row_next;
+    };
+    typename QueriesOfKeys<ROWS>::At next = see.start(), now = next;
+    request(see.it0, next, 0);
+    load_rows(see.it0, next), store_rows(see.it0, 0);
+    next = see.after(next);
+    load_rows(see.it0 + 1, next);
+    // What wavefronts w and w + 4 hand on: 32 queries of either half of a tile have a place.
+    auto handed = [&](int n, int which) { return lds + kHandedAt + ((n * kWaves + wave % kWaves) * 4 + which) * 16 * kWave + 16 * lane; };
+    auto seen = [&](int first) { return first + 32 > see.wave_need; };      // any of these 32 queries, by any of the wavefront's keys?
+    // All wavefronts, tile by tile: own(first, n) for the halves of this one.
+    int set = 0;
+    auto advance = [&](int by) { tile.shift(set + by >= kSets ? (by - kSets) * kSetBytes : by * kSetBytes); };
+    auto walk = [&](auto&& one, auto&& other) {
+        for (int it = see.it0; it < see.it1; ++it) {
+            wait_for_copies();
+            lds_barrier();
+            const int after = set == kSets - 1 ? 0 : set + 1, first = (see.first_tile + now.tile) * ROWS;
+            request(it + 1, next, after), store_rows(it + 1, after);
+            now = next, next = see.after(next);
+            load_rows(it + 2, next);
+            one(first);
+            lds_barrier();
+            other(first);
+            set = after;
+        }
+        lds_barrier();
+    };
+    auto nothing = [](int) {};
+    if (wave < kWaves) {
+        Frag k_column[Tile::kSteps], v_column[Tile::kSteps];
+        const bool mine = see.my_key < length;
+        load_column<T, DP>(k_column, static_cast<const T*>(a.k) + batch * a.k_at.batch + see.my_key * a.k_at.token + kv_head * a.k_at.head, mine, a.chunks, half);
+        load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + see.my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
+        auto form = [&](int n, int first) {
+            if (!seen(first)) return;
+            const float* rows = reinterpret_cast<const float*>(lds + kRowsAt + set * 2 * ROWS * 4) + 32 * n + 4 * half;
+            floatx16 p, d;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = d[r] = 0.f;
+            tile.template straight_woven<0>(p, kQ + n * kBlock, k_column, nothing);
+            OfRows lse(rows), delta(rows + ROWS);
+            tile.template straight_woven<16>(d, kG + n * kBlock, v_column, [&](int r) { p[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, -lse(r)))); });
+            if (first < see.wave_all) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = first + 4 * half + (r & 3) + 8 * (r >> 2) >= see.need ? p[r] : 0.f;
+            }
+            const typename Tile::Packed b = Tile::pack(p);
+            *reinterpret_cast<shortx8*>(handed(n, 0)) = b.lo, *reinterpret_cast<shortx8*>(handed(n, 1)) = b.hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) d[r] = p[r] * (d[r] - delta(r));
+            const typename Tile::Packed s = Tile::pack(d);
+            *reinterpret_cast<shortx8*>(handed(n, 2)) = s.lo, *reinterpret_cast<shortx8*>(handed(n, 3)) = s.hi;
+        };
+        walk([&](int first) { form(0, first); },
+             [&](int first) {
+                 form(1, first + 32);
+                 advance(1);
+             });
+        lds_barrier();      // (the others' last step)
+        return;
+    }
+    floatx16 dk[Tile::kBlocks], dv[Tile::kBlocks];
+    clear(dk), clear(dv);
+    auto add = [&](int n, int first) {
+        if (!seen(first)) return;
+        typename Tile::Packed p, d;
+        p.lo = *reinterpret_cast<const shortx8*>(handed(n, 0)), p.hi = *reinterpret_cast<const shortx8*>(handed(n, 1));
+        d.lo = *reinterpret_cast<const shortx8*>(handed(n, 2)), d.hi = *reinterpret_cast<const shortx8*>(handed(n, 3));
+        tile.template transposed_woven<0>(dv, kG + n * kBlock, p, nothing);
+        tile.template transposed_woven<0>(dk, kQ + n * kBlock, d, nothing);
+    };
+    int before = -1;      // first query of the tile before, whose second half is still to be added
+    walk(
+        [&](int first) {
+            if (before >= 0) {
+                add(1, before + 32);
+                // (the set before this one, which is `set` by now)
+                tile.shift(set == 0 ? -(kSets - 1) * kSetBytes : kSetBytes);
+            }
+            before = first;
+        },
+        [&](int first) { add(0, first); });
+    if (before >= 0) add(1, before + 32);
+    lds_barrier();
+    const int dim = a.chunks * Tile::kPerChunk, wave_key = see.wave_key;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (a.splits == 1) {
+            typedef AttnOut<T, DP> Out;
+            char* room = lds + (wave - kWaves) * Out::kRoom;
+            const HeadsAt& at = which ? a.dv_at : a.dk_at;
+            T* to = static_cast<T*>(which ? a.dv : a.dk);
+            if (!to) continue;
+            to += batch * at.batch + kv_head * at.head;
+            if (which) Out::park(room, dv, 1.f, lane);
+            else Out::park(room, dk, a.scale, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_key + col < a.keys ? to + (wave_key + col) * at.token : nullptr; });
+        } else {
+            typedef AttnOut<float, DP> Out;
+            char* room = lds + (wave - kWaves) * Out::kRoom;
             float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
             if (which) Out::park(room, dv, 1.f, lane);
             else Out::park(room, dk, a.scale, lane);
@@ -474,7 +616,15 @@ constexpr int backward_rows_lds() {
 }
 template <typename T, int DP>
 constexpr int backward_keys_lds() {
-    constexpr int tiles = 2 * query_tile<T, DP>() * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4), out = (two_roles<T, DP>() ? 2 : 1) * kWaves * AttnOut<float, DP>::kRoom;
+    constexpr int tiles = 2 * query_tile<T, DP>() * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4), out = kWaves * AttnOut<float, DP>::kRoom;
+    return tiles > out ? tiles : out;
+}
+
+template <typename T, int DP>
+constexpr bool in_pairs() { return sizeof(T) == 2 && DP > 64; }
+template <typename T, int DP>
+constexpr int backward_pairs_lds() {
+    constexpr int tiles = 3 * kPairRows * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4) + 2 * kWaves * 4 * 16 * kWave, out = kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
 }
 
@@ -554,7 +704,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
     return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr int DP = decltype(dp)::value;
-        constexpr int kRowsLds = backward_rows_lds<T, DP>(), kKeysLds = backward_keys_lds<T, DP>();
+        constexpr int kRowsLds = backward_rows_lds<T, DP>();
         if (a.tokens) {
             a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
             a.splits = a.dq ? row_splits(batch, tokens, keys, heads, least_keys<T>()) : 1;
@@ -578,12 +728,19 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
             }
         }
         if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
-        if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kKeysLds, "ddl_attention_backward")) return rc;
         a.splits = key_splits(batch, tokens, keys, heads, kv_heads, a.causal, least_of_split<T>());
         a.blocks = (a.keys + kRows * kWaves - 1) / (kRows * kWaves);
         const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads, grid = pairs * a.blocks * a.splits;
         if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
-        hipLaunchKernelGGL((attention_backward_keys<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(two_roles<T, DP>() ? 2 * kThreads : kThreads), kKeysLds, s, a);
+        if constexpr (in_pairs<T, DP>()) {
+            constexpr int kLds = backward_pairs_lds<T, DP>();
+            if (const int rc = grant_lds<attention_backward_pairs<T, DP>>(kLds, "ddl_attention_backward")) return rc;
+            hipLaunchKernelGGL((attention_backward_pairs<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(2 * kThreads), kLds, s, a);
+        } else {
+            constexpr int kLds = backward_keys_lds<T, DP>();
+            if (const int rc = grant_lds<attention_backward_keys<T, DP>>(kLds, "ddl_attention_backward")) return rc;
+            hipLaunchKernelGGL((attention_backward_keys<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), kLds, s, a);
+        }
         if (const int rc = check_launch("ddl_attention_backward")) return rc;
         if (a.splits == 1) return 0;
         const int64_t threads = 2 * pairs * a.keys * (dim / 4);
