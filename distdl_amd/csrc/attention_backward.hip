@@ -454,13 +454,14 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
     const int block = unit / a.splits, split = unit - block * a.splits;
     const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
+    typedef typename QueriesOfKeys<ROWS>::At At;
     const QueriesOfKeys<ROWS> see(a, block * kRows * kWaves, wave % kWaves, lane, length, split);
     const T* q0 = static_cast<const T*>(a.q) + batch * a.q_at.batch + static_cast<int64_t>(kv_head) * a.group * a.q_at.head;
     const T* g0 = static_cast<const T*>(a.dout) + batch * a.dout_at.batch + static_cast<int64_t>(kv_head) * a.group * a.dout_at.head;
     const int64_t row0 = (static_cast<int64_t>(batch) * a.heads + static_cast<int64_t>(kv_head) * a.group) * a.tokens;
     Tile tile(lds, lane);
     AttnCopy<T, DP, ROWS, WAVES> q_copy(q0, a.q_at.token, a.chunks, wave, lane), g_copy(g0, a.dout_at.token, a.chunks, wave, lane);
-    auto request = [&](int it, const typename QueriesOfKeys<ROWS>::At& at, int set) {
+    auto request = [&](int it, const At& at, int set) {
         if (it >= see.it1) return;
         char* to = lds + set * kSetBytes;
         q_copy.base = reinterpret_cast<const char*>(q0 + at.head * a.q_at.head), g_copy.base = reinterpret_cast<const char*>(g0 + at.head * a.dout_at.head);
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
         q_copy.request(to, first, a.tokens), g_copy.request(to + kTileBytes, first, a.tokens);
     };
     float row_next = 0.f;       // of the queries on their way: threads 0 .. ROWS - 1 their sums, the next as many their D
-    auto load_rows = [&](int it, const typename QueriesOfKeys<ROWS>::At& at) {
+    auto load_rows = [&](int it, const At& at) {
         if (it >= see.it1 || tid >= 2 * ROWS) return;
         const int row = (see.first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
         const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
@@ -477,31 +478,34 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
     auto store_rows = [&](int it, int set) {
         if (it < see.it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + kRowsAt + set * 2 * ROWS * 4)[tid] = row_next;
     };
-    typename QueriesOfKeys<ROWS>::At next = see.start(), now = next;
-    request(see.it0, next, 0);
-    load_rows(see.it0, next), store_rows(see.it0, 0);
-    next = see.after(next);
+    At now = see.start(), next = see.after(now);
+    request(see.it0, now, 0);
+    load_rows(see.it0, now), store_rows(see.it0, 0);
     load_rows(see.it0 + 1, next);
     // What wavefronts w and w + 4 hand on: 32 queries of either half of a tile have a place.
     auto handed = [&](int n, int which) { return lds + kHandedAt + ((n * kWaves + wave % kWaves) * 4 + which) * 16 * kWave + 16 * lane; };
     auto seen = [&](int first) { return first + 32 > see.wave_need; };      // any of these 32 queries, by any of the wavefront's keys?
-    // All wavefronts, tile by tile: own(first, n) for the halves of this one.
+    auto first_of = [&](const At& at) { return (see.first_tile + at.tile) * ROWS; };
+    // All wavefronts, tile by tile: what one set does between the barriers.  A tile is asked for as soon as nobody is at the one before the last, and has
+    // come when half of the last is done.
     int set = 0;
-    auto advance = [&](int by) { tile.shift(set + by >= kSets ? (by - kSets) * kSetBytes : by * kSetBytes); };
-    auto walk = [&](auto&& one, auto&& other) {
+    auto walk = [&](auto&& start, auto&& one, auto&& other) {
+        wait_for_copies();
+        lds_barrier();
+        request(see.it0 + 1, next, 1);
+        if (see.it0 < see.it1) start();
         for (int it = see.it0; it < see.it1; ++it) {
+            const At third = see.after(next);
+            const int after = set == kSets - 1 ? 0 : set + 1;
+            store_rows(it + 1, after), load_rows(it + 2, third);
+            one(first_of(now));
             wait_for_copies();
             lds_barrier();
-            const int after = set == kSets - 1 ? 0 : set + 1, first = (see.first_tile + now.tile) * ROWS;
-            request(it + 1, next, after), store_rows(it + 1, after);
-            now = next, next = see.after(next);
-            load_rows(it + 2, next);
-            one(first);
+            request(it + 2, third, after == kSets - 1 ? 0 : after + 1);
+            other(first_of(now), it + 1 < see.it1);
+            now = next, next = third, set = after;
             lds_barrier();
-            other(first);
-            set = after;
         }
-        lds_barrier();
     };
     auto nothing = [](int) {};
     if (wave < kWaves) {
@@ -509,13 +513,24 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
         const bool mine = see.my_key < length;
         load_column<T, DP>(k_column, static_cast<const T*>(a.k) + batch * a.k_at.batch + see.my_key * a.k_at.token + kv_head * a.k_at.head, mine, a.chunks, half);
         load_column<T, DP>(v_column, static_cast<const T*>(a.v) + batch * a.v_at.batch + see.my_key * a.v_at.token + kv_head * a.v_at.head, mine, a.chunks, half);
-        auto form = [&](int n, int first) {
-            if (!seen(first)) return;
-            const float* rows = reinterpret_cast<const float*>(lds + kRowsAt + set * 2 * ROWS * 4) + 32 * n + 4 * half;
-            floatx16 p, d;
+        // The scores run a step ahead, so that every product has vector work next to it: dO . v the exponentials, the next scores dS.
+        floatx16 p, ahead;
+        auto zero = [](floatx16& v) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = d[r] = 0.f;
-            tile.template straight_woven<0>(p, kQ + n * kBlock, k_column, nothing);
+            for (int r = 0; r < 16; ++r) v[r] = 0.f;
+        };
+        // Queries first .. + 31, half n of this tile; then the scores at `scores` of the next tile or half, unless nobody needs them.
+        auto form = [&](int n, int first, bool more, auto&& move, uint32_t scores) {
+            const float* rows = reinterpret_cast<const float*>(lds + kRowsAt + set * 2 * ROWS * 4) + 32 * n + 4 * half;
+            if (!seen(first)) {
+                move();
+                zero(ahead);
+                if (more) tile.template straight_woven<0>(ahead, scores, k_column, nothing);
+                p = ahead;
+                return;
+            }
+            floatx16 d;
+            zero(d), zero(ahead);
             OfRows lse(rows), delta(rows + ROWS);
             tile.template straight_woven<16>(d, kG + n * kBlock, v_column, [&](int r) { p[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, -lse(r)))); });
             if (first < see.wave_all) {
@@ -524,16 +539,27 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
             }
             const typename Tile::Packed b = Tile::pack(p);
             *reinterpret_cast<shortx8*>(handed(n, 0)) = b.lo, *reinterpret_cast<shortx8*>(handed(n, 1)) = b.hi;
+            move();
+            auto difference = [&](int r) { d[r] = pinned(p[r] * (d[r] - delta(r))); };
+            if (more) {
+                tile.template straight_woven<16>(ahead, scores, k_column, difference);
+            } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) d[r] = p[r] * (d[r] - delta(r));
+                for (int r = 0; r < 16; ++r) difference(r);
+            }
             const typename Tile::Packed s = Tile::pack(d);
             *reinterpret_cast<shortx8*>(handed(n, 2)) = s.lo, *reinterpret_cast<shortx8*>(handed(n, 3)) = s.hi;
+            p = ahead;
         };
-        walk([&](int first) { form(0, first); },
-             [&](int first) {
-                 form(1, first + 32);
-                 advance(1);
-             });
+        walk(
+            [&] {
+                zero(p);
+                tile.template straight_woven<0>(p, kQ, k_column, nothing);
+            },
+            [&](int first) { form(0, first, true, [] {}, kQ + kBlock); },
+            [&](int first, bool more) {
+                form(1, first + 32, more, [&] { tile.shift(set == kSets - 1 ? -(kSets - 1) * kSetBytes : kSetBytes); }, kQ);
+            });
         lds_barrier();      // (the others' last step)
         return;
     }
@@ -548,16 +574,15 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
         tile.template transposed_woven<0>(dk, kQ + n * kBlock, d, nothing);
     };
     int before = -1;      // first query of the tile before, whose second half is still to be added
-    walk(
-        [&](int first) {
-            if (before >= 0) {
-                add(1, before + 32);
-                // (the set before this one, which is `set` by now)
-                tile.shift(set == 0 ? -(kSets - 1) * kSetBytes : kSetBytes);
-            }
-            before = first;
-        },
-        [&](int first) { add(0, first); });
+    walk([] {},
+         [&](int first) {
+             if (before >= 0) {
+                 add(1, before + 32);
+                 tile.shift(set == 0 ? -(kSets - 1) * kSetBytes : kSetBytes);      // from the set before this one
+             }
+             before = first;
+         },
+         [&](int first, bool) { add(0, first); });
     if (before >= 0) add(1, before + 32);
     lds_barrier();
     const int dim = a.chunks * Tile::kPerChunk, wave_key = see.wave_key;
