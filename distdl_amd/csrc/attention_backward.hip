@@ -5,7 +5,7 @@
 // Two kernels, so that every sum has one owner and one order and nothing is added atomically, at the price of forming the
 // scores and dO . v twice (seven products instead of five): attention_backward_rows, a wavefront for 32 queries that walks over
 // the keys, and attention_backward_keys, a wavefront for 32 keys that walks over the queries of all heads that share
-// them -- the gradient of a shared key head is summed there, in registers.
+// them -- the gradient of a shared key head is summed there, in registers (attention_backward_pairs: the same by two wavefronts).
 //
 // 16-bit types: dS is rounded for the product (gradients are then off by 1.4 times what rounding the exact ones gives).  D comes from out and the rest
 // that the forward kept, or, where all keys are in one tile, from p and dP themselves; from the rounded out alone the gradients of a
@@ -436,8 +436,12 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
 // The same for 16-bit heads of more than 64 elements.  Keys and values, both sums and both products of a step are more than the 256 registers with which
 // two wavefronts fit on a SIMD, and one alone leaves the matrix cores idle while it forms probabilities.  So two sets of four wavefronts share
 // the work: the first form the probabilities and dS of 32 queries and leave them in LDS, rounded as the products take them and for the lanes that
-// take them, and the second add them to both sums a step later: two products each, and while one wavefront of a SIMD is at its exponentials, the
-// other has matrix instructions.  Three sets of tiles: of the queries whose turn it is, those before and those on their way.
+// take them, and the second add them to both sums a step later, two products each.  Three sets of tiles: of the queries whose turn it is, those
+// before and those on their way.
+//
+// dk and dv of [4,4096,16,128] bf16: 1177 us (934 TFLOP/s), causal 588.  Both sums in one wavefront took 2460; dk in one set and dv in the other, both
+// forming the probabilities, 1409; the first set without the scores of the step ahead 1317.  Bound by the first set's steps and their barriers:
+// matrix cores and LDS are each busy for less than half of the time.
 template <typename T, int DP>
 __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
@@ -655,7 +659,7 @@ constexpr int backward_pairs_lds() {
 
 // Workgroups that share the queries of a block of keys: as many as the chip has CUs in all, twice that where the blocks' lengths differ (causal), and
 // with at least `least` times 32 queries.  (dk and dv of [2,448,16,64] bf16, 1500 keys, in one part 22 us, in two 43: the sums' way through memory;
-// [2,2048,8,128] in one part each 84 us, in two 120; [4,2048,8,128] causal, one key head, eight parts each 113 us, four 154, sixteen 140.
+// [2,2048,8,128] in one part each 78 us, in two 110; [4,2048,8,128] causal, one key head, eight parts each 102 us, four 129, twelve 120.
 // fp32 [3,333,8,40], 77 keys, at least 64 queries each: 16 us, 256: 43.)
 int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, bool causal, int least) {
     if (batch < 1 || tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1) return 1;

@@ -11,7 +11,7 @@
 // of its own column, so a column's maximum and sum need one exchange between the lanes' halves, and the second product
 // takes them back as they lie: which row a reduction index stands for is free as long as both operands agree, so the tile is
 // read for the rows that each lane happens to hold (16-bit: ds_read_b64_tr_b16, four rows of one column; fp32: a word a row).
-// Nothing of P goes through LDS.
+// Nothing of P goes through LDS (but from one wavefront to another in attention_backward_pairs).
 //
 // A tile's rows are DP elements of ROWB bytes, a power of two, in chunks of 16 bytes; chunk c of row r lies at c ^ swizzle(r), a
 // permutation of r's low four bits that gives 16 rows of one chunk different banks (straight reads), and the four rows
