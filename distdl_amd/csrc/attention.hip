@@ -109,9 +109,11 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     constexpr int KEYS = keys_of_tile<T>(), NS = KEYS / 32, kTileBytes = KEYS * Tile::kRowBytes;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
-    int bh, block;
-    block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, bh, block);     // the last rows, which see most keys in the causal form, first
-    const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
+    int u, block, batch, head;
+    bool late;
+    block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, u, block, late);     // the last rows, which see most keys in the causal form, first
+    head_of(a, u, a.heads, a.group, late, batch, head);
+    const int bh = batch * a.heads + head, kv_head = head / a.group;
     const int length = sequence_keys(a, batch);
     const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
     const int seen = keys_seen(a, my_row, length);
@@ -547,7 +549,7 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
                 a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
                 const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
                 if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
-                a.folded = folds(a.causal, grid);
+                a.folded = folds(a, grid);
                 hipLaunchKernelGGL((attention_rows<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (rows_lds<T, DP>()), s, a);
                 return check_launch("ddl_attention");
             }

@@ -65,9 +65,11 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
     const int split = blockIdx.y;
-    int bh, block;
-    block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, bh, block);
-    const int batch = bh / a.heads, head = bh - batch * a.heads, kv_head = head / a.group;
+    int u, block, batch, head;
+    bool late;
+    block_of(blockIdx.x, a.batch * a.heads, a.blocks, a.folded, u, block, late);
+    head_of(a, u, a.heads, a.group, late, batch, head);
+    const int bh = batch * a.heads + head, kv_head = head / a.group;
     const int length = sequence_keys(a, batch);
     const int first_row = block * kRows * kWaves, wave_row = first_row + wave * kRows, my_row = wave_row + (lane & 31);
     const bool mine = my_row < a.tokens;
@@ -278,11 +280,13 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
     const int pairs = a.batch * a.kv_heads;
-    int bk, unit;
-    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, bk, unit);
+    int u, unit, batch, kv_head;
+    bool late;
+    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, u, unit, late);
+    head_of(a, u, a.kv_heads, 1, false, batch, kv_head);
+    const int bk = batch * a.kv_heads + kv_head;
     unit = a.blocks * a.splits - 1 - unit;      // the first keys, which most queries see in the causal form, first
     const int block = unit / a.splits, split = unit - block * a.splits;
-    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
     const QueriesOfKeys<ROWS> see(a, block * kRows * kWaves, wave, lane, length, split);
     typedef typename QueriesOfKeys<ROWS>::At At;
@@ -452,11 +456,13 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = lane >> 5;
     const int pairs = a.batch * a.kv_heads;
-    int bk, unit;
-    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, bk, unit);
+    int u, unit, batch, kv_head;
+    bool late;
+    block_of(blockIdx.x, pairs, a.blocks * a.splits, false, u, unit, late);
+    head_of(a, u, a.kv_heads, 1, false, batch, kv_head);
+    const int bk = batch * a.kv_heads + kv_head;
     unit = a.blocks * a.splits - 1 - unit;      // the first keys, which most queries see in the causal form, first
     const int block = unit / a.splits, split = unit - block * a.splits;
-    const int batch = bk / a.kv_heads, kv_head = bk - batch * a.kv_heads;
     const int length = sequence_keys(a, batch);
     typedef typename QueriesOfKeys<ROWS>::At At;
     const QueriesOfKeys<ROWS> see(a, block * kRows * kWaves, wave % kWaves, lane, length, split);
@@ -739,7 +745,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
             a.splits = a.dq ? row_splits(batch, tokens, keys, heads, least_keys<T>()) : 1;
             const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
             if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
-            a.folded = folds(a.causal, grid);
+            a.folded = folds(a, grid);
             const auto launch = [&](auto one) {
                 constexpr bool ONE = decltype(one)::value;
                 if (const int rc = grant_lds<attention_backward_rows<T, DP, ONE>>(kRowsLds, "ddl_attention_backward")) return rc;

@@ -477,7 +477,7 @@ __device__ inline int sequence_keys(const AttnArgs& a, int batch) {
 // Workgroup `id` of `blocks` x `heads`: neighbouring numbers go to different XCDs, each of which takes its own share of the heads,
 // so that what they have in common stays in its L2.  Blocks come in descending order, the longest first where a row sees the keys before it;
 // `folded`: the second half of them in ascending order.
-__device__ inline void block_of(int id, int heads, int blocks, bool folded, int& head, int& block) {
+__device__ inline void block_of(int id, int heads, int blocks, bool folded, int& head, int& block, bool& late) {
     if (heads % 8 == 0) {
         const int share = heads / 8, slot = id >> 3;
         head = (id & 7) * share + slot % share, block = slot / share;
@@ -485,7 +485,34 @@ __device__ inline void block_of(int id, int heads, int blocks, bool folded, int&
         head = id % heads, block = id / heads;
     }
     const int down = blocks / 2;
-    block = folded && block >= down ? block - down : blocks - 1 - block;
+    late = folded && block >= down;
+    block = late ? block - down : blocks - 1 - block;
+}
+
+// The sequence with `rank` longer ones before it; up to 64 sequences, in every wavefront for itself.
+__device__ inline int sequence_of_rank(const AttnArgs& a, int rank) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int n = lane < a.batch ? a.lengths[lane] : 0;
+    int before = 0;
+    for (int j = 0; j < a.batch; ++j) {
+        const int m = __builtin_amdgcn_readlane(n, j);
+        before += m > n || (m == n && j < lane) ? 1 : 0;
+    }
+    return __ffsll(static_cast<unsigned long long>(__ballot(lane < a.batch && before == rank))) - 1;
+}
+
+// Sequence and head of number `u` of a workgroup's, `group` heads of which share a key head.  Sequences of equal lengths one after the other, for the
+// L2s; of different lengths, every XCD takes heads of all of them, the longest first, and the workgroups that come `late` to a CU the other way round
+// (bf16 [8,448,16,64] to 500 .. 1500 keys: forward 37 us instead of 42, dq 45 instead of 51; [32,448,16,64] 94 instead of 106, 117 instead of 129;
+// dk and dv of [4,1000,12,128] 80 instead of 112; causal [8,2048,8,128], two key heads, 85 and 85).
+__device__ inline void head_of(const AttnArgs& a, int u, int heads, int group, bool late, int& batch, int& head) {
+    if (!a.lengths || a.batch == 1) {
+        batch = u / heads, head = u - batch * heads;
+        return;
+    }
+    const int key_head = u / (group * a.batch), in = u - key_head * group * a.batch, at = in / group;
+    head = key_head * group + in - at * group;
+    batch = a.batch <= kWave ? sequence_of_rank(a, late ? a.batch - 1 - at : at) : at;
 }
 
 // More LDS than a kernel gets unasked: set once for each kernel and device.
@@ -501,11 +528,12 @@ int grant_lds(int bytes, const char* what) {
     return 0;
 }
 
-// Where all workgroups of a causal launch are resident at once, two on a CU, the second one on a CU is one of the short half that goes with
-// the long one there (8192 queries, 8 heads of 128, fp16: 178 us instead of 186; [4,2048,8,128] 51 instead of 54); with more of them than that, longest first is what levels them.
-inline bool folds(int causal, int64_t grid) {
+// Where all workgroups of a launch whose lengths differ (causal, or sequences' own) are resident at once, two on a CU, the second one on a CU is one
+// of the short half that goes with the long one there (causal, 8192 queries, 8 heads of 128, fp16: 178 us instead of 186; [4,2048,8,128] 51 instead
+// of 54); with more of them than that, longest first is what levels them.
+inline bool folds(const AttnArgs& a, int64_t grid) {
     int dev;
-    return causal && grid <= 2 * static_cast<int64_t>(compute_units(dev));
+    return (a.causal || a.lengths) && grid <= 2 * static_cast<int64_t>(compute_units(dev));
 }
 
 struct HeadsOperand {

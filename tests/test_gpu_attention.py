@@ -450,3 +450,24 @@ def test_layers_over_batch_and_heads_of_four_workers():
             assert torch.equal(mine, all_.chunk(2, 0)[index[0]].chunk(2, 2)[index[2]])
     for got, want in zip(parts[0][4], whole[4]):
         assert (got - want).abs().max() <= 2.0 ** -17 * batch * tokens * heads * want.abs().max()
+
+
+@pytest.mark.parametrize("batch", [3, 64, 65, 130])
+def test_sequences_of_many_lengths(batch):
+    """Equal ones, none and all among them, more than a wavefront has lanes: every sequence as it comes out alone."""
+    from distdl_amd import nn
+    g = torch.Generator().manual_seed(16)
+    q, k, v, dy = _inputs(torch.bfloat16, batch, 260, 100, 4, 2, 32, seed=16)
+    lengths = torch.randint(-3, 104, (batch,), generator=g, dtype=torch.int32)
+    lengths[0], lengths[1], lengths[2] = 100, 0, 100
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = nn.attention_shard(*leaves, lengths.cuda())
+    whole = [out.detach()] + list(torch.autograd.grad(out, leaves, dy))
+    u = torch.finfo(torch.bfloat16).eps / 2
+    for b in {0, 1, 2, batch // 2, batch - 1}:
+        n = int(lengths[b].clip(0, 100))
+        one = [t.detach()[b:b + 1] for t in (q, k, v, dy)]
+        want = o_heads.attention(*(_f64(t) for t in one[:3]), [n], False, None, _f64(one[3]))
+        tol = _bounds(*(_f64(t) for t in one[:3]), [n], False, 32 ** -0.5, u, 0.0, _f64(one[3]))
+        for name, got, exact, t, more in zip(("out", "dq", "dk", "dv"), whole, (want[0],) + want[2:], tol, (0, u, u, u)):
+            _within(name, got[b:b + 1], exact, t, more)
