@@ -14,10 +14,12 @@ from .module import Module
 
 class _AttentionShard(torch.autograd.Function):
     """Attention and its adjoint; kept for it are the operands, the result with what its rounding took (16-bit types), and one sum for each
-    query and head."""
+    query and head (nothing where no adjoint follows: ``keep``)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, lengths, causal, scale):
+    def forward(ctx, q, k, v, lengths, causal, scale, keep=True):
+        if not keep:
+            return hip_ops.attention(q, k, v, lengths, causal, scale)
         out, lse, rest = hip_ops.attention(q, k, v, lengths, causal, scale, want_lse=True)
         ctx.save_for_backward(q, k, v, out, lse, lengths, rest)
         ctx.how = (causal, scale)
@@ -29,7 +31,7 @@ class _AttentionShard(torch.autograd.Function):
         q, k, v, out, lse, lengths, rest = ctx.saved_tensors
         if grad_output.dtype != q.dtype:
             grad_output = grad_output.detach().to(q.dtype)
-        return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, *ctx.how, *ctx.needs_input_grad[:3], rest) + (None, None, None)
+        return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, *ctx.how, *ctx.needs_input_grad[:3], rest) + (None,) * 4
 
 
 def _general_backward(grad_output, q, k, v, out, rest, lse, lengths, causal, scale, want_q, want_k, want_v):
@@ -50,9 +52,9 @@ def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None):
     out = _lib.front().attention_shard(q, k, v, lengths, causal, scale, _lib.callback(_general_backward))
     if out is not None:
         return out
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _AttentionShard.apply(q, k, v, lengths, bool(causal), scale)
-    return hip_ops.attention(q, k, v, lengths, causal, scale)
+    # (through the function without gradients as well: a tangent is then refused, and a trace holds the call)
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _AttentionShard.apply(q, k, v, lengths, bool(causal), scale, keep)
 
 
 class DistributedAttention(Module):

@@ -60,7 +60,7 @@ class _RotaryShard(torch.autograd.Function):
     def forward(ctx, q, k, frequencies, positions, interleaved, amplitude):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(frequencies, positions)
-        ctx.how, ctx.dtype = (interleaved, amplitude), (q if q is not None else k).dtype
+        ctx.how, ctx.dtype = (interleaved, amplitude), None if q is None and k is None else (q if q is not None else k).dtype
         return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude)
 
     @staticmethod
@@ -116,10 +116,9 @@ def _row(weight):
     return None if weight is None else weight.detach().reshape(-1)
 
 
-def _records(frequencies, *tensors):
+def _refuse_gradient_of(frequencies):
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise ValueError("rotary frequencies have no gradient: detach them")
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplitude=1.0):
@@ -131,9 +130,9 @@ def rotary_shard(q, k, frequencies, positions=None, *, interleaved=False, amplit
     res = _lib.front().rotary_shard(q, k, frequencies, positions, interleaved, amplitude, _lib.callback(_general_rotary_backward))
     if res is not None:
         return res
-    if _records(frequencies, q, k):
-        return _RotaryShard.apply(q, k, frequencies, positions, bool(interleaved), float(amplitude))
-    return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude)
+    _refuse_gradient_of(frequencies)
+    # (without gradients as well: a tangent is then refused, and a trace holds the call)
+    return _RotaryShard.apply(q, k, frequencies, positions, bool(interleaved), float(amplitude))
 
 
 def head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions=None, *, eps=1e-6, interleaved=False, amplitude=1.0):
@@ -143,9 +142,8 @@ def head_norm_rotary_shard(q, k, q_weight, k_weight, frequencies, positions=None
                                               _lib.callback(_general_head_norm_backward))
     if res is not None:
         return res
-    if _records(frequencies, q, k, q_weight, k_weight):
-        return _HeadNormRotaryShard.apply(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(interleaved), float(amplitude))
-    return hip_ops.head_rotary(q, k, frequencies, positions, interleaved, amplitude, norm=True, q_weight=_row(q_weight), k_weight=_row(k_weight), eps=eps)
+    _refuse_gradient_of(frequencies)
+    return _HeadNormRotaryShard.apply(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(interleaved), float(amplitude))
 
 
 class DistributedRotary(Module):
