@@ -500,7 +500,7 @@ bool takes_split(const AttnArgs& a, bool wide) {
 // least 512 keys 16, with 128 13.4 (but one sequence of 65536 keys 22.7 instead of 18.9: the join); two workgroups for each CU:
 // [8,1,32,128] to 2048 keys 43 us instead of 39.
 int splits_for(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads) {
-    if (tokens < 1 || keys <= 512 || heads < 1 || kv_heads < 1 || batch < 1) return 1;
+    if (keys <= 512) return 1;
     int dev;
     const int64_t units = split_units(batch, tokens, heads, kv_heads), most = (keys + 255) / 256;
     const int64_t splits = (compute_units(dev) + units - 1) / units;
@@ -514,7 +514,7 @@ extern "C" {
 
 int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
     using namespace ddl;
-    if (dim < 1 || dim > 128) return 0;
+    if (!has_work(batch, tokens, keys, heads, kv_heads, dim)) return 0;
     const int splits = splits_for(batch, tokens, keys, heads, kv_heads);
     return splits > 1 ? static_cast<int64_t>(splits) * batch * tokens * heads * (padded_dim(dim) + kStats) : 0;
 }

@@ -699,7 +699,7 @@ extern "C" {
 
 int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
     using namespace ddl;
-    if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || dim < 1 || keys < 0) return 0;
+    if (!has_work(batch, tokens, keys, heads, kv_heads, dim)) return 0;
     const int64_t splits = key_splits(batch, tokens, keys, heads, kv_heads, true, least_of_split<float>());      // the most that a call takes
     const int64_t shares = row_splits(batch, tokens, keys, heads, least_keys<float>());
     const int64_t of_keys = splits > 1 ? splits * 2 * batch * kv_heads * keys * dim : 0, of_rows = shares > 1 ? shares * batch * heads * tokens * dim : 0;

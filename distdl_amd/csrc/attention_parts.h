@@ -536,6 +536,18 @@ inline bool folds(const AttnArgs& a, int64_t grid) {
     return (a.causal || a.lengths) && grid <= 2 * static_cast<int64_t>(compute_units(dev));
 }
 
+// Extents that the kernels' numbers hold, and heads that share key heads evenly: what the entry points refuse before they divide by any of them.
+inline bool counts_fit(int64_t batch, int64_t tokens, int64_t keys, int64_t heads) {
+    constexpr int64_t kMost = 0x3FFFFFFF;
+    return heads <= kMost && keys <= kMost && (heads == 0 || (tokens <= kMost / heads && batch <= kMost / heads));
+}
+inline bool heads_fit(int64_t heads, int64_t kv_heads) { return heads == 0 || (kv_heads > 0 && heads % kv_heads == 0); }
+
+// Is there any work of these extents that a workspace could be for?
+inline bool has_work(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    return batch > 0 && tokens > 0 && keys >= 0 && heads > 0 && dim > 0 && dim <= 128 && heads_fit(heads, kv_heads) && counts_fit(batch, tokens, keys, heads);
+}
+
 struct HeadsOperand {
     const void* p;
     const int64_t* strides;
@@ -551,10 +563,9 @@ inline int fill_attention(AttnArgs& a, bool& nothing, const char* what, std::ini
     const int per = dtype == DDL_DT_F32 ? 4 : 8;
     if (dim % per) return fail(DDL_E_ALIGN, "%s: heads of %lld elements are no multiple of 16 bytes", what, static_cast<long long>(dim));
     if (!(scale > 0.f && scale <= 1.0e38f)) return fail(DDL_E_ARG, "%s: scale %g is not positive", what, static_cast<double>(scale));
-    if (heads && (kv_heads == 0 || heads % kv_heads))
+    if (!heads_fit(heads, kv_heads))
         return fail(DDL_E_SHAPE, "%s: %lld heads cannot share %lld key heads", what, static_cast<long long>(heads), static_cast<long long>(kv_heads));
-    if ((heads && (tokens > 0x3FFFFFFF / heads || batch > 0x3FFFFFFF / heads)) || keys > 0x3FFFFFFF || heads > 0x3FFFFFFF)
-        return fail(DDL_E_UNSUPP, "%s: 2^30 rows or keys", what);
+    if (!counts_fit(batch, tokens, keys, heads)) return fail(DDL_E_UNSUPP, "%s: 2^30 rows or keys", what);
     if (heads == 0 && kv_heads) return fail(DDL_E_SHAPE, "%s: key heads without heads", what);
     nothing = batch == 0 || heads == 0 || (tokens == 0 && keys == 0);
     if (nothing) return 0;

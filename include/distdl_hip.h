@@ -670,7 +670,8 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  *   out_rest like out, or NULL: with an lse, what the rounding of a 16-bit out took,
  *            for the adjoint
  *   workspace  device memory of ddl_attention_workspace(...) floats, 16-byte
- *            aligned (few queries: the keys are split over workgroups)
+ *            aligned (few queries: the keys are split over workgroups); 0 for
+ *            extents that ddl_attention refuses
  * 0 < scale <= 1e38.  Values of keys that some query of a sequence sees are to be
  * finite (a zero probability times an infinite one is not a number).  16-byte
  * aligned tensors with strides and head_dim that are multiples
