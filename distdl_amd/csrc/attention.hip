@@ -538,6 +538,7 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
         return fail(DDL_E_ARG, "ddl_attention: workspace of %lld floats, %lld are needed", static_cast<long long>(workspace ? workspace_elems : 0), static_cast<long long>(need));
     if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention: workspace is not 16-byte aligned");
     a.partial = workspace;
+    if (lse && !adjoint_launches(a, dtype, dim)) return fail(DDL_E_UNSUPP, "ddl_attention: 2^32 threads in its adjoint");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_attention_kernel(dtype, dim, [&](auto* e, auto dp) -> int {
         typedef std::remove_pointer_t<decltype(e)> T;
@@ -545,19 +546,19 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
         const auto launch = [&](auto with_lse) {
             constexpr bool LSE = decltype(with_lse)::value;
             if (!takes_split(a, sizeof(T) == 2 && DP > 64)) {
-                if (const int rc = grant_lds<attention_rows<T, DP, LSE>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
-                a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+                a.blocks = static_cast<int>(blocks_of(a.tokens));
                 const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
-                if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
+                if (!launches(grid, kThreads)) return fail(DDL_E_UNSUPP, "ddl_attention: 2^32 threads");
+                if (const int rc = grant_lds<attention_rows<T, DP, LSE>>(rows_lds<T, DP>(), "ddl_attention")) return rc;
                 a.folded = folds(a, grid);
                 hipLaunchKernelGGL((attention_rows<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (rows_lds<T, DP>()), s, a);
                 return check_launch("ddl_attention");
             }
-            if (const int rc = grant_lds<attention_split<T, DP, LSE>>(split_lds<T, DP>(), "ddl_attention")) return rc;
             const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
             a.blocks = static_cast<int>((rows + kRows - 1) / kRows);
             const int64_t grid = static_cast<int64_t>(a.batch) * a.kv_heads * a.splits * a.blocks;
-            if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention: 2^31 workgroups");
+            if (!launches(grid, kThreads)) return fail(DDL_E_UNSUPP, "ddl_attention: 2^32 threads");
+            if (const int rc = grant_lds<attention_split<T, DP, LSE>>(split_lds<T, DP>(), "ddl_attention")) return rc;
             hipLaunchKernelGGL((attention_split<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
             return check_launch("ddl_attention");
         };

@@ -656,8 +656,6 @@ constexpr int backward_keys_lds() {
 }
 
 template <typename T, int DP>
-constexpr bool in_pairs() { return sizeof(T) == 2 && DP > 64; }
-template <typename T, int DP>
 constexpr int backward_pairs_lds() {
     constexpr int tiles = 3 * kPairRows * (2 * AttnTile<T, DP>::kRowBytes + 2 * 4) + 2 * kWaves * 4 * 16 * kWave, out = kWaves * AttnOut<float, DP>::kRoom;
     return tiles > out ? tiles : out;
@@ -670,7 +668,7 @@ constexpr int backward_pairs_lds() {
 int key_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t kv_heads, bool causal, int least) {
     if (batch < 1 || tokens < 1 || keys < 1 || heads < 1 || kv_heads < 1) return 1;
     int dev;
-    const int64_t units = batch * kv_heads * ((keys + kRows * kWaves - 1) / (kRows * kWaves)), tiles = heads / kv_heads * ((tokens + 31) / 32);
+    const int64_t units = batch * kv_heads * blocks_of(keys), tiles = heads / kv_heads * ((tokens + 31) / 32);
     int64_t splits = (causal ? 2 : 1) * static_cast<int64_t>(compute_units(dev)) / units;
     if (splits > tiles / least) splits = tiles / least;
     return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
@@ -683,7 +681,7 @@ constexpr int least_of_split() { return sizeof(T) == 2 ? 8 : 2; }
 int row_splits(int64_t batch, int64_t tokens, int64_t keys, int64_t heads, int64_t least) {
     if (batch < 1 || tokens < 1 || keys < 1 || heads < 1) return 1;
     int dev;
-    int64_t splits = compute_units(dev) / (batch * heads * ((tokens + kRows * kWaves - 1) / (kRows * kWaves)));
+    int64_t splits = compute_units(dev) / (batch * heads * blocks_of(tokens));
     if (splits > keys / least) splits = keys / least;
     return static_cast<int>(splits < 1 ? 1 : splits);
 }
@@ -732,6 +730,7 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
     if (need && (!workspace || workspace_elems < need))
         return fail(DDL_E_ARG, "ddl_attention_backward: workspace of %lld floats, %lld are needed", static_cast<long long>(workspace ? workspace_elems : 0), static_cast<long long>(need));
     if (need && !aligned_to(workspace, 16)) return fail(DDL_E_ALIGN, "ddl_attention_backward: workspace is not 16-byte aligned");
+    if (!adjoint_launches(a, dtype, dim)) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^32 threads");
     a.dout = dout, a.dout_at = place_of(dout_strides), a.out = const_cast<void*>(out), a.out_at = place_of(out_strides), a.rest = const_cast<void*>(out_rest), a.lse = const_cast<float*>(lse);
     a.dq = dq, a.dk = dk, a.dv = dv, a.dq_at = place_of(dq_strides), a.dk_at = place_of(dk_strides), a.dv_at = place_of(dv_strides);
     a.delta = workspace, a.partial = workspace + rounded4(batch * heads * tokens);
@@ -741,10 +740,9 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         constexpr int DP = decltype(dp)::value;
         constexpr int kRowsLds = backward_rows_lds<T, DP>();
         if (a.tokens) {
-            a.blocks = (a.tokens + kRows * kWaves - 1) / (kRows * kWaves);
+            a.blocks = static_cast<int>(blocks_of(a.tokens));
             a.splits = a.dq ? row_splits(batch, tokens, keys, heads, least_keys<T>()) : 1;
             const int64_t grid = static_cast<int64_t>(a.blocks) * a.batch * a.heads;
-            if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
             a.folded = folds(a, grid);
             const auto launch = [&](auto one) {
                 constexpr bool ONE = decltype(one)::value;
@@ -764,10 +762,9 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides, const 
         }
         if (a.keys == 0 || (!a.dk && !a.dv)) return 0;
         a.splits = key_splits(batch, tokens, keys, heads, kv_heads, a.causal, least_of_split<T>());
-        a.blocks = (a.keys + kRows * kWaves - 1) / (kRows * kWaves);
+        a.blocks = static_cast<int>(blocks_of(a.keys));
         const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads, grid = pairs * a.blocks * a.splits;
-        if (grid > 0x7FFFFFFF) return fail(DDL_E_UNSUPP, "ddl_attention_backward: 2^31 workgroups");
-        if constexpr (in_pairs<T, DP>()) {
+        if constexpr (in_pairs(sizeof(T), DP)) {
             constexpr int kLds = backward_pairs_lds<T, DP>();
             if (const int rc = grant_lds<attention_backward_pairs<T, DP>>(kLds, "ddl_attention_backward")) return rc;
             hipLaunchKernelGGL((attention_backward_pairs<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(2 * kThreads), kLds, s, a);

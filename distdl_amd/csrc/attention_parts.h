@@ -548,6 +548,19 @@ inline bool has_work(int64_t batch, int64_t tokens, int64_t keys, int64_t heads,
     return batch > 0 && tokens > 0 && keys >= 0 && heads > 0 && dim > 0 && dim <= 128 && heads_fit(heads, kv_heads) && counts_fit(batch, tokens, keys, heads);
 }
 
+// A launch has fewer than 2^32 threads.
+constexpr bool launches(int64_t workgroups, int threads) { return workgroups <= 0xFFFFFFFFll / threads; }
+inline int64_t blocks_of(int64_t rows) { return (rows + kRows * kWaves - 1) / (kRows * kWaves); }
+
+// The adjoint's kernel of keys and values takes two sets of wavefronts for 16-bit rows of more than 64 elements.
+constexpr bool in_pairs(int element_bytes, int64_t dim) { return element_bytes == 2 && dim > 64; }
+
+// Can the adjoint be launched?  (Only few workgroups are multiplied by splits.)
+inline bool adjoint_launches(const AttnArgs& a, int dtype, int64_t dim) {
+    return launches(blocks_of(a.tokens) * a.batch * a.heads, kThreads) &&
+           launches(blocks_of(a.keys) * a.batch * a.kv_heads, in_pairs(dtype == DDL_DT_F32 ? 4 : 2, dim) ? 2 * kThreads : kThreads);
+}
+
 struct HeadsOperand {
     const void* p;
     const int64_t* strides;

@@ -676,8 +676,10 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  * finite (a zero probability times an infinite one is not a number).  16-byte
  * aligned tensors with strides and head_dim that are multiples
  * of 16 bytes (DDL_E_ALIGN; zeros behind a head's elements change nothing),
- * head_dim <= 128 (DDL_E_UNSUPP).  Probabilities are rounded to the element
- * type for the product with the values. */
+ * head_dim <= 128, launches of fewer than 2^32 threads, 256 of them for 128
+ * queries of a head, and with an lse the adjoint's as well, 256 (16-bit heads of
+ * more than 64 elements: 512) for 128 keys of a key head (DDL_E_UNSUPP).
+ * Probabilities are rounded to the element type for the product with the values. */
 int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys,
                                 int64_t heads, int64_t kv_heads, int64_t head_dim);
 int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
