@@ -560,17 +560,17 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k, const 
             if (!launches(grid, kThreads)) return fail(DDL_E_UNSUPP, "ddl_attention: 2^32 threads");
             if (const int rc = grant_lds<attention_split<T, DP, LSE>>(split_lds<T, DP>(), "ddl_attention")) return rc;
             hipLaunchKernelGGL((attention_split<T, DP, LSE>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), (split_lds<T, DP>()), s, a);
+            if (const int rc = check_launch("ddl_attention")) return rc;
+            if (a.splits == 1) return 0;
+            const int64_t all = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
+            constexpr int kGroups = kThreads / join_lanes<DP>();
+            if (a.splits <= kSplitsInFlight)
+                hipLaunchKernelGGL((attention_join<T, DP, 1>), dim3(static_cast<uint32_t>((all + kGroups - 1) / kGroups)), dim3(kThreads), 0, s, a);
+            else
+                hipLaunchKernelGGL((attention_join<T, DP, kGroups>), dim3(static_cast<uint32_t>(all)), dim3(kThreads), 0, s, a);
             return check_launch("ddl_attention");
         };
-        if (const int rc = lse ? launch(std::true_type{}) : launch(std::false_type{})) return rc;
-        if (a.splits <= 1) return 0;
-        const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
-        constexpr int kGroups = kThreads / join_lanes<DP>();
-        if (a.splits <= kSplitsInFlight)
-            hipLaunchKernelGGL((attention_join<T, DP, 1>), dim3(static_cast<uint32_t>((rows + kGroups - 1) / kGroups)), dim3(kThreads), 0, s, a);
-        else
-            hipLaunchKernelGGL((attention_join<T, DP, kGroups>), dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, s, a);
-        return check_launch("ddl_attention");
+        return lse ? launch(std::true_type{}) : launch(std::false_type{});
     });
 }
 
