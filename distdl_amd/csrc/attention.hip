@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kStats = 4;               // behind the sums of a row over a split's keys: its maximum, its two totals, nothing
 constexpr float kSlack = 8.f;           // the running maximum is moved when it lags by more than this (in powers of two)
+constexpr float kHuge = 1048576.f;      // a maximum from which on its rounding shows (by 2^-4)
 
 // The softmax of a wavefront's columns as far as it has come.
 //
@@ -29,23 +30,28 @@ template <int BLOCKS, bool EXACT>
 struct Running {
     floatx16 acc[BLOCKS];
     float top = -INFINITY, total = 0.f, exact = 0.f;      // of this lane's column; the totals of this lane's half of the rows
+    float mul, base = 0.f;                                // a probability is 2^(mul score - base)
+    float lag = kSlack;                                 // from where on the maximum follows
 
-    __device__ Running() {
+    __device__ explicit Running(float scale) : mul(scale) {
 #pragma unroll
         for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     }
     // The maximum follows the scores of 32 keys, which this looks at: only where it lags by a factor of 2^8, since the sums have room for that
-    // and most blocks then leave them alone, and to a whole power of two, so that what has been summed (and `before`, what waits to
+    // and most blocks leave them alone, and to a whole power of two, so that what has been summed (and `before`, what waits to
     // be) moves without a rounding.
+    //
+    // Once a maximum is huge the rounding of score times scale shows, and the difference to it is formed from the rounded products, whose largest is the
+    // maximum itself: here, for every block from then on.
     template <typename Tile>
-    __device__ void follow(const floatx16& s, float scale, const Tile&, typename Tile::Packed* before) {
+    __device__ void follow(floatx16& s, float scale, const Tile&, typename Tile::Packed* before) {
         float m = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int r = 2; r < 16; ++r) m = fmaxf(m, s[r]);
         m = max_halves(m) * scale;
-        if (__any(m > top + kSlack)) {
+        if (__any(m > top + lag)) {
             const float moved = fmaxf(top, ceilf(m)), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
             top = moved;
             total *= factor;
@@ -55,15 +61,21 @@ struct Running {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= factor;
             if (before) Tile::scale_packed(*before, factor);
+            base = top == -INFINITY ? 0.f : top;
+            if (__any(fabsf(base) > kHuge)) lag = -INFINITY, mul = 1.f;
+            if (lag < 0.f) {
+                const float from = base;
+                base = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = pinned(s[r] * scale) - from;
+            }
         }
     }
-    __device__ float from() const { return top == -INFINITY ? 0.f : top; }
     // Scores to probabilities relative to the maximum, packed and added to the total.
     template <typename Tile>
-    __device__ typename Tile::Packed take(floatx16& s, float scale, const Tile&) {
-        const float base = from();
+    __device__ typename Tile::Packed take(floatx16& s, const Tile&) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], mul, -base));
         const typename Tile::Packed p = Tile::pack(s);
         total = Tile::add_packed(total, p);
         add_exact(s);
@@ -144,7 +156,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     }
     wait_for_copies();
     lds_barrier();
-    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run;
+    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
     floatx16 scores;
     typename Tile::Packed before;
     auto score = [&](floatx16& to, int s) {
@@ -159,7 +171,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         floatx16 next;
         if constexpr (ahead) score(next, s + 1);
         if constexpr (behind) values(s - 1);
-        before = run.take(scores, a.scale_log2, tile);
+        before = run.take(scores, tile);
         if constexpr (ahead) scores = next;
     };
     // The same in full, 16-bit types: after every matrix instruction (32 cycles) an LDS read for the one after the next two and a share of the
@@ -170,7 +182,6 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         if constexpr (sizeof(T) == 2) {
             constexpr int kPhase = decltype(phase)::value, kSlots = 2 * Tile::kSteps;
             const uint32_t kb = k_block((kPhase + 1) % kPhases), vb = v_block((kPhase + kPhases - 1) % kPhases);
-            const float base = run.from();
             floatx16 next;
 #pragma unroll
             for (int r = 0; r < 16; ++r) next[r] = 0.f;
@@ -181,7 +192,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             };
             auto share = [&](int slot) {
 #pragma unroll
-                for (int r = 16 * slot / kSlots; r < 16 * (slot + 1) / kSlots; ++r) scores[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], a.scale_log2, -base)));
+                for (int r = 16 * slot / kSlots; r < 16 * (slot + 1) / kSlots; ++r) scores[r] = pinned(__builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], run.mul, -run.base)));
             };
             read(0), read(1);
             __builtin_amdgcn_sched_barrier(0);
@@ -204,7 +215,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             floatx16 next;
             score(next, s + 1);
             values(s - 1);
-            before = run.take(scores, a.scale_log2, tile);
+            before = run.take(scores, tile);
             scores = next;
         }
     };
@@ -323,7 +334,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
         column[s] = f;
     }
-    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run;
+    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
     for (; t < t1; t += kWaves) {
         const int after = t + kWaves;
         wait_for_copies();
@@ -348,7 +359,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         for (int i = 0; i < Tile::kSteps; ++i) mfma_chunk(s, kf[i], column[i], static_cast<const T*>(nullptr));
         if ((t + 1) * KEYS > least) mask_scores(s, seen - t * KEYS - 4 * half);
         run.follow(s, a.scale_log2, tile, nullptr);
-        const typename Tile::Packed p = run.take(s, a.scale_log2, tile);
+        const typename Tile::Packed p = run.take(s, tile);
         if constexpr (kEarly) {
 #pragma unroll
             for (int i = 0; i < 2 * Tile::kBlocks; ++i) mfma_chunk(run.acc[i % Tile::kBlocks], vf[i], i / Tile::kBlocks ? p.hi : p.lo, static_cast<const T*>(nullptr));
