@@ -18,7 +18,15 @@ namespace ddl {
 namespace {
 
 constexpr int kStats = 4;               // behind the sums of a row over a split's keys: its maximum, its two totals, nothing
-constexpr float kSlack = 8.f;           // the running maximum is moved when it lags by more than this (in powers of two)
+// In powers of two: what a probability may come to before the running maximum is moved, and what the largest one then comes to.
+//
+// fp16 has full steps only down to 2^-14, and next to a key of large weight many small ones would lose theirs (of 299 keys with 2^-23 of the largest
+// one's weight each, whose values are the result, a fifth): what its range has above one is used, up to 2^15.  The room between the two is what keeps
+// most blocks from moving anything ([4,4096,16,64], all keys: 310 us with eight of them or six, 316 with four, 319 with three).
+template <typename T>
+constexpr float kMost = std::is_same_v<T, __half> ? 15.f : 8.f;
+template <typename T>
+constexpr float kLargest = std::is_same_v<T, __half> ? 9.f : 0.f;
 constexpr float kHuge = 1048576.f;      // a maximum from which on its rounding shows (by 2^-4)
 
 // The softmax of a wavefront's columns as far as it has come.
@@ -26,12 +34,12 @@ constexpr float kHuge = 1048576.f;      // a maximum from which on its rounding 
 // Two totals: of the probabilities as they are rounded for the product, which is what the result is divided by (the weights of a mean add
 // up to one then, and a single large one is exact), and, EXACT, of the unrounded ones, from which the adjoint forms them anew:
 // divided by the other one they would all be off by its rounding, up to half a step where one key has most of the weight.
-template <int BLOCKS, bool EXACT>
+template <typename T, int BLOCKS, bool EXACT>
 struct Running {
     floatx16 acc[BLOCKS];
     float top = -INFINITY, total = 0.f, exact = 0.f;      // of this lane's column; the totals of this lane's half of the rows
     float mul, base = 0.f;                                // a probability is 2^(mul score - base)
-    float lag = kSlack;                                 // from where on the maximum follows
+    float lag = kMost<T>;                                 // from where on the maximum follows
 
     __device__ explicit Running(float scale) : mul(scale) {
 #pragma unroll
@@ -39,7 +47,7 @@ struct Running {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     }
-    // The maximum follows the scores of 32 keys, which this looks at: only where it lags by a factor of 2^8, since the sums have room for that
+    // The maximum follows the scores of 32 keys, which this looks at: only where a probability would get too large, since the sums have room until then
     // and most blocks leave them alone, and to a whole power of two, so that what has been summed (and `before`, what waits to
     // be) moves without a rounding.
     //
@@ -52,7 +60,7 @@ struct Running {
         for (int r = 2; r < 16; ++r) m = fmaxf(m, s[r]);
         m = max_halves(m) * scale;
         if (__any(m > top + lag)) {
-            const float moved = fmaxf(top, ceilf(m)), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
+            const float moved = fmaxf(top, ceilf(m) - kLargest<T>), factor = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - moved);
             top = moved;
             total *= factor;
             if (EXACT) exact *= factor;
@@ -67,7 +75,10 @@ struct Running {
                 const float from = base;
                 base = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = pinned(s[r] * scale) - from;
+                for (int r = 0; r < 16; ++r) {
+                    const float d = pinned(s[r] * scale) - from;
+                    s[r] = d > kMost<T> ? kMost<T> : d;      // (`moved` is a multiple of 16 and more there)
+                }
             }
         }
     }
@@ -156,7 +167,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     }
     wait_for_copies();
     lds_barrier();
-    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
+    Running<T, Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
     floatx16 scores;
     typename Tile::Packed before;
     auto score = [&](floatx16& to, int s) {
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attent
         if (my_row < rows && 2 * s + half < a.chunks) f = *reinterpret_cast<const Frag*>(q + token * a.q_at.token + head * a.q_at.head + (2 * s + half) * Tile::kPerChunk);
         column[s] = f;
     }
-    Running<Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
+    Running<T, Tile::kBlocks, LSE && sizeof(T) == 2> run(a.scale_log2);
     for (; t < t1; t += kWaves) {
         const int after = t + kWaves;
         wait_for_copies();

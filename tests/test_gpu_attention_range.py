@@ -1,9 +1,41 @@
-"""Attention with scores that leave no digits for a difference."""
+"""Attention where a type's range ends: in float16 with probabilities and gradients of which float16 itself would keep little (many keys, one of which has
+most of the weight, and gradients far below or above one), and with scores that leave no digits for a difference.
+
+Tolerances: half a step of the type, u = 2^-11 of the value, for the rounding of a result, of a probability and of its gradient; what lies below the
+type's normal numbers costs a result 2^-25 as well, but no sum before it.  Scores are sums of one product here, so a probability is off by c = 2^-18 beside
+its rounding: of an exponential and a logarithm in 32 bits, 2^-21 each with arguments below 2^5 (2^-24 of them, times 2^5 ln 2), and of totals whose
+terms are equal but for one of them (sums of integers up to 2^24, exact; n 2^-24 <= 2^-11 of the rest next to a large one: c = 2^-10 there).
+"""
 
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+U, TINY, C = 2.0 ** -11, 2.0 ** -25, 2.0 ** -18
+
+
+@pytest.mark.parametrize("keys", [300, 8192])
+@pytest.mark.parametrize("batch,tokens,heads", [(1, 1, 1), (2, 5, 4), (96, 130, 8)])
+@pytest.mark.parametrize("below", [14.25, 18.25, 21.25, 23.25])
+@pytest.mark.parametrize("dim", [32, 128])
+def test_keys_far_below_one_of_large_weight(keys, batch, tokens, heads, below, dim):
+    """One key with value 0 has 2^below times the weight of every other, whose values are about one: the result is theirs alone.
+
+    Their probability is rounded by u of itself, the sum of the rounded ones by as much, and so is the result.  (The scores are 0.5 and below + 0.5
+    in powers of two: none of the probabilities is a whole one.)"""
+    from distdl_amd import nn
+    q = torch.zeros(batch, tokens, heads, dim, dtype=torch.float16, device="cuda")
+    k, v = (torch.zeros(batch, keys, 1, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    q[..., 0], k[:, keys // 3, :, 0] = 1.0, below
+    q[..., 1], k[..., 1] = 0.5, 1.0
+    v.copy_(torch.rand(v.shape, generator=torch.Generator().manual_seed(keys)) + 0.5)
+    v[:, keys // 3] = 0.0
+    out = nn.attention_shard(q, k, v, scale=0.6931471805599453).double()
+    weight = 2.0 ** -below
+    want = (weight * v.double().sum(1, keepdim=True) / (1 + (keys - 1) * weight)).expand(out.shape)
+    tol = 3 * U * want + 2 * 2.0 ** -10 * want + TINY
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / want).max()
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
