@@ -698,7 +698,8 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
  * dv may be NULL; `workspace`: device memory of
  * ddl_attention_backward_workspace(...) floats, 16-byte aligned.  Nothing is added
  * atomically: equal calls give equal bits.  Probabilities and dS are rounded to
- * the element type for their products: in fp16, dS beyond 65504 is infinite.
+ * the element type for their products (in fp16 dS times a power of two of each
+ * query's or key's own, so that small and large gradients keep their digits).
  * Limits as ddl_attention's. */
 int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens,
                                          int64_t keys, int64_t heads,

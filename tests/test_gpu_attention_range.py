@@ -38,6 +38,80 @@ def test_keys_far_below_one_of_large_weight(keys, batch, tokens, heads, below, d
     assert ((out - want).abs() <= tol).all(), ((out - want).abs() / want).max()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("tokens,keys,heads", [(5, 60, 2), (1, 700, 4), (130, 700, 2), (70, 8192, 2), (700, 3001, 1)])
+@pytest.mark.parametrize("gradient,value", [(2.0 ** -14, 1.0), (2.0 ** -8, 2.0 ** -6), (2.0 ** -8, 1.0), (1.0, 1.0), (2.0 ** 14, 2.0 ** 14)])
+def test_gradients_far_from_one(gradient, value, tokens, keys, heads, dim):
+    """Half of the keys have a value, scores are zero: dS = +- g value / 2 keys for each of them, from 2^-32 to 2^21, and dq and dk are sums of equal signs.
+
+    dS is rounded by u; its p is off by c, and D, the mean of the values times g, by 2^-20 of dP - D (the mean is rounded twice in 32 bits, the rest that is kept
+    of it by u^2 of the value); the sums of n terms by n 2^-24; results by u."""
+    from distdl_amd import nn
+    g = torch.Generator().manual_seed(keys + tokens)
+    q, dy = (torch.zeros(1, tokens, heads, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    k, v = (torch.zeros(1, keys, 1, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    with_value = (torch.randperm(keys, generator=g) < keys // 2).cuda()
+    q[..., 0] = 1.0
+    k[:, with_value, :, 1], v[:, with_value, :, 2] = 1.0, value
+    dy[..., 2] = gradient * (1 + torch.rand(1, tokens, heads, generator=g).cuda())
+    scale = 4 / (gradient * value)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(nn.attention_shard(*leaves, scale=scale), leaves, dy)
+    size, share = dy[..., 2].double() * value, (keys // 2) / keys
+    want_q = scale * size * share * (1 - share)
+    want_k = torch.where(with_value, 1 - share, -share) * scale * size.sum() / keys
+    off = 2 * U + C + 2.0 ** -20
+    assert ((dq[..., 1].double() - want_q).abs() <= (off + keys * 2.0 ** -24) * want_q).all(), (dq[..., 1].double() / want_q - 1).abs().max()
+    assert ((dk[0, :, 0, 0].double() - want_k).abs() <= (off + tokens * heads * 2.0 ** -24) * want_k.abs() + TINY).all(), (dk[0, :, 0, 0].double() / want_k - 1).abs().max()
+    dq[..., 1], dk[..., 0] = 0, 0
+    assert not dq.any() and not dk.any()
+
+
+@pytest.mark.parametrize("dim", [40, 64, 128])
+@pytest.mark.parametrize("batch,tokens,keys,heads,causal", [(2, 9, 60, 2, False), (1, 150, 900, 2, False), (1, 300, 300, 4, True), (3, 200, 70, 2, True)])
+@pytest.mark.parametrize("rise", [-20, 0, 20])
+def test_gradients_that_rise_and_fall_along_keys_and_queries(rise, batch, tokens, keys, heads, causal, dim):
+    """Values that change by 2^rise along the keys and gradients that do along the queries: bounds of the general test without what float16 loses next to zero,
+    but for 2^-34 of the largest dS of a query or key and for 2^-25 of what is kept of the result's rounding, and of a gradient."""
+    from distdl_amd import nn
+    from oracle import heads as o_heads
+    from test_gpu_attention import _bounds
+    g = torch.Generator().manual_seed(tokens + keys)
+
+    def normal(n, h, rises, scale=1.0):
+        t = torch.randn(batch, n, h, dim, generator=g) * scale
+        return (t * 2.0 ** (rises * (torch.arange(n) / n - 0.5))[:, None, None] if rises else t).half().cuda()
+
+    q, k, v, dy = normal(tokens, heads, 0), normal(keys, 1, 0), normal(keys, 1, rise), normal(tokens, heads, rise, 2.0 ** -4)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    scale = dim ** -0.5
+    grads = torch.autograd.grad(nn.attention_shard(*leaves, causal=causal), leaves, dy)
+    qn, kn, vn, dyn = (t.detach().double().cpu().numpy() for t in (q, k, v, dy))
+    want = o_heads.attention(qn, kn, vn, None, causal, scale, dyn)[2:]
+    tol = _bounds(qn, kn, vn, None, causal, scale, U, 0.0, dyn)[1:]
+    p, ds, lost = _parts(qn, kn, vn, dyn, causal, scale)
+    more_q = torch.einsum("bhij,bjd->bihd", lost + 2.0 ** -34 * ds.abs().amax(-1, keepdim=True), torch.from_numpy(abs(kn[:, :, 0])))
+    more_k = torch.einsum("bhij,bihd->bjd", lost + 2.0 ** -34 * ds.abs().amax((1, 2), keepdim=True), torch.from_numpy(abs(qn)))[:, :, None]
+    for name, got, exact, bound, more in (("dq", grads[0], want[0], tol[0], more_q), ("dk", grads[1], want[1], tol[1], more_k)):
+        got, exact = got.double().cpu(), torch.from_numpy(exact)
+        bound = torch.from_numpy(bound) + scale * more + U * exact.abs() + TINY
+        # (a gradient itself may leave the type: from 65520 on it rounds to infinity, and may do so as far below as it may be off)
+        beyond = torch.where(exact.abs() + bound >= 65520, got == exact.sign() * torch.inf, False)
+        near = (got - exact).abs() <= bound
+        assert (near | beyond).all(), f"{name}: {((got - exact).abs() / bound)[~beyond].max():.3g} of the tolerance"
+        assert beyond.sum() < 0.05 * beyond.numel()
+
+
+def _parts(q, k, v, dy, causal, scale):
+    """In 64 bits, [batch, heads, tokens, keys]: probabilities, their gradients dS, and what 2^-25 of every element of the result makes of dS."""
+    q, k, v, dy = (torch.from_numpy(t) for t in (q, k, v, dy))
+    s = scale * torch.einsum("bihd,bjd->bhij", q, k[:, :, 0])
+    hidden = torch.arange(k.shape[1]) > torch.arange(q.shape[1])[:, None] + k.shape[1] - q.shape[1] if causal else torch.zeros(q.shape[1], k.shape[1], dtype=torch.bool)
+    p = s.masked_fill(hidden, -torch.inf).softmax(-1).nan_to_num(0.0)
+    dp = torch.einsum("bihd,bjd->bhij", dy, v[:, :, 0])
+    return p, p * (dp - (p * dp).sum(-1, keepdim=True)), p * TINY * dy.abs().sum(-1).transpose(1, 2)[..., None]
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("batch,tokens,heads,keys", [(1, 1, 1, 40), (1, 70, 2, 1000), (160, 130, 1, 100)])
 @pytest.mark.parametrize("power", [18, 24, 26, 27, 28, 32, 36, 60])
