@@ -282,6 +282,12 @@ constexpr int kHandedBytes = 2 * kWaves * 4 * 16 * kWave;      // probabilities 
 template <typename T, int DP>
 constexpr int query_tile() { return sizeof(T) == 2 || AttnTile<T, DP>::kRowBytes <= 128 ? 64 : 32; }
 
+// Probabilities of many keys are small, and fp16 has full steps down to 2^-14 only: they are formed as 2^kUp times as much, from sums that are less by kUp,
+// and so are the sums of dv and, next to Fitted's factor, dk.  (A probability is at most one; the rest of the range is for large scores, whose sums are
+// off by their rounding.)
+template <typename T>
+constexpr int kUp = Fitted<T>::kNeeded ? 10 : 0;
+
 // Which queries a wavefront's 32 keys are seen by, and which of them, ROWS of one head at a time, are this workgroup's share.
 template <int ROWS>
 struct QueriesOfKeys {
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
         if (it >= it1 || tid >= 2 * ROWS) return;
         const int row = (see.first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
         const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
-        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
+        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] - kUp<T> : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
     };
     auto store_rows = [&](int it) {
         if (it < it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + set_of(it) + 2 * kTileBytes)[tid] = row_next;
@@ -478,6 +484,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
     wait_for_copies();
     lds_barrier();
     const int dim = a.chunks * Tile::kPerChunk;
+    constexpr float kDown = 1.f / (1 << kUp<T>);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         if (a.splits == 1) {
@@ -487,16 +494,16 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
             T* to = static_cast<T*>(which ? a.dv : a.dk);
             if (!to) continue;
             to += batch * at.batch + kv_head * at.head;
-            if (which) Out::park(room, dv, 1.f, lane);
-            else Out::park(room, dk, a.scale, lane);
+            if (which) Out::park(room, dv, kDown, lane);
+            else Out::park(room, dk, a.scale * kDown, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_key + col < a.keys ? to + (wave_key + col) * at.token : nullptr; });
         } else {
             typedef AttnOut<float, DP> Out;
             char* room = lds + wave * Out::kRoom;
             float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
-            if (which) Out::park(room, dv, 1.f, lane);
-            else Out::park(room, dk, a.scale, lane);
+            if (which) Out::park(room, dv, kDown, lane);
+            else Out::park(room, dk, a.scale * kDown, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_key + col < a.keys ? to + static_cast<int64_t>(wave_key + col) * dim : nullptr; });
         }
@@ -550,7 +557,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
         if (it >= see.it1 || tid >= 2 * ROWS) return;
         const int row = (see.first_tile + at.tile) * ROWS + (tid & (ROWS - 1));
         const int64_t place = row0 + static_cast<int64_t>(at.head) * a.tokens + row;
-        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
+        row_next = tid < ROWS ? (row < a.tokens ? a.lse[place] - kUp<T> : INFINITY) : (row < a.tokens ? a.delta[place] : 0.f);
     };
     auto store_rows = [&](int it, int set) {
         if (it < see.it1 && tid < 2 * ROWS) reinterpret_cast<float*>(lds + kRowsAt + set * 2 * ROWS * 4)[tid] = row_next;
@@ -669,6 +676,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
     fitted.undo(dk);
     lds_barrier();
     const int dim = a.chunks * Tile::kPerChunk, wave_key = see.wave_key;
+    constexpr float kDown = 1.f / (1 << kUp<T>);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         if (a.splits == 1) {
@@ -678,16 +686,16 @@ __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(cons
             T* to = static_cast<T*>(which ? a.dv : a.dk);
             if (!to) continue;
             to += batch * at.batch + kv_head * at.head;
-            if (which) Out::park(room, dv, 1.f, lane);
-            else Out::park(room, dk, a.scale, lane);
+            if (which) Out::park(room, dv, kDown, lane);
+            else Out::park(room, dk, a.scale * kDown, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, a.chunks, lane, [&](int col) -> T* { return wave_key + col < a.keys ? to + (wave_key + col) * at.token : nullptr; });
         } else {
             typedef AttnOut<float, DP> Out;
             char* room = lds + (wave - kWaves) * Out::kRoom;
             float* to = a.partial + ((static_cast<int64_t>(split) * 2 + which) * pairs + bk) * a.keys * dim;
-            if (which) Out::park(room, dv, 1.f, lane);
-            else Out::park(room, dk, a.scale, lane);
+            if (which) Out::park(room, dv, kDown, lane);
+            else Out::park(room, dk, a.scale * kDown, lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             Out::write(room, dim / 4, lane, [&](int col) -> float* { return wave_key + col < a.keys ? to + static_cast<int64_t>(wave_key + col) * dim : nullptr; });
         }

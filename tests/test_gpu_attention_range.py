@@ -112,6 +112,24 @@ def _parts(q, k, v, dy, causal, scale):
     return p, p * (dp - (p * dp).sum(-1, keepdim=True)), p * TINY * dy.abs().sum(-1).transpose(1, 2)[..., None]
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("tokens,keys", [(3, 1000001), (130, 330011)])
+def test_gradients_of_values_of_very_many_keys(tokens, keys, dim):
+    """Scores of zero: every probability is 1 / keys, rounded by u, and off by 2^-18 of it (the logarithm's argument and the exponential's, below 2^5, by 2^-19 and
+    2^-20 together; the total is a sum of ones, exact).  So dv = sum dy / keys is off by u and 2^-18 of the magnitudes, the sum's
+    tokens 2^-24 of them, and u and 2^-25 for the result."""
+    from distdl_amd import nn
+    g = torch.Generator().manual_seed(keys)
+    q, dy = (torch.randn(1, tokens, 1, dim, generator=g).half().cuda() for _ in range(2))
+    dy = dy * 256
+    k, v = (torch.zeros(1, keys, 1, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    v.requires_grad_()
+    dv, = torch.autograd.grad(nn.attention_shard(q, k, v), [v], dy)
+    want, size = dy.double().sum(1, keepdim=True) / keys, dy.double().abs().sum(1, keepdim=True) / keys
+    tol = (U + C + tokens * 2.0 ** -24) * size + U * want.abs() + TINY
+    assert ((dv.double() - want).abs() <= tol).all(), ((dv.double() - want).abs() / tol).max()
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("batch,tokens,heads,keys", [(1, 1, 1, 40), (1, 70, 2, 1000), (160, 130, 1, 100)])
 @pytest.mark.parametrize("power", [18, 24, 26, 27, 28, 32, 36, 60])
