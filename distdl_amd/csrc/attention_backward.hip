@@ -299,7 +299,7 @@ struct QueriesOfKeys {
     __device__ QueriesOfKeys(const AttnArgs& a, int first_key, int wave, int lane, int length, int split) {
         auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
         wave_key = first_key + wave * kRows, my_key = wave_key + (lane & 31);
-        const int shift = a.causal ? a.keys - a.tokens : 0x3FFFFFFF;      // query i sees key j from i = j - shift on
+        const int shift = a.causal ? causal_shift(a, length) : 0x3FFFFFFF;      // query i sees key j from i = j - shift on
         need = my_key < length ? max(my_key - shift, 0) : 0x7FFFFFFF;
         const int block_need = scalar(first_key < length ? max(first_key - shift, 0) : a.tokens);
         wave_need = scalar(wave_key < length ? max(wave_key - shift, 0) : 0x7FFFFFFF);

@@ -452,7 +452,7 @@ struct AttnArgs {
     const int32_t* lengths;             // [batch] or null
     int tokens, keys, heads, kv_heads, group, batch;
     int chunks;                         // of 16 bytes of a head
-    int causal;
+    int causal;                         // 0, 1 or kOwnEnds
     float scale, scale_log2;
     int blocks;                         // of rows (or keys) of a head
     int folded;                         // order of the blocks, see block_of
@@ -460,11 +460,15 @@ struct AttnArgs {
     float* partial;                     // sums of the splits
 };
 
+// Of the causal form: the last query sees all keys, up to the tensor's end or the sequence's own.
+constexpr int kOwnEnds = 2;
+__device__ inline int causal_shift(const AttnArgs& a, int length) { return (a.causal == kOwnEnds ? length : a.keys) - a.tokens; }
+
 // Keys that the query at `token` sees of a sequence of `length`.
 __device__ inline int keys_seen(const AttnArgs& a, int token, int length) {
     if (token >= a.tokens) return 0;
     if (!a.causal) return length;
-    const int own = token + 1 + a.keys - a.tokens;
+    const int own = token + 1 + causal_shift(a, length);
     return min(length, max(own, 0));
 }
 
@@ -602,7 +606,7 @@ inline int fill_attention(AttnArgs& a, bool& nothing, const char* what, std::ini
     }
     a.lengths = lengths;
     a.tokens = static_cast<int>(tokens), a.keys = static_cast<int>(keys), a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
-    a.group = static_cast<int>(heads / kv_heads), a.batch = static_cast<int>(batch), a.chunks = static_cast<int>(dim / per), a.causal = causal != 0;
+    a.group = static_cast<int>(heads / kv_heads), a.batch = static_cast<int>(batch), a.chunks = static_cast<int>(dim / per), a.causal = causal == kOwnEnds ? kOwnEnds : causal != 0;
     a.scale = scale, a.scale_log2 = scale * kLog2e;
     return 0;
 }

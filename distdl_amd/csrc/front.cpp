@@ -387,7 +387,7 @@ const int32_t* length_pointer(const MaybeTensor& t) { return static_cast<const i
 
 double attention_scale(const Tensor& q, const std::optional<double>& scale) { return scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))); }
 
-std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, const Tensor& v_given, const MaybeTensor& lengths, bool causal,
+std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, const Tensor& v_given, const MaybeTensor& lengths, int causal,
                                   const std::optional<double>& scale, bool want_lse) {
     if (!attention_operands(q_given, k_given, v_given, lengths, scale)) return std::nullopt;
     const int64_t per = 16 / q_given.element_size(), own = q_given.size(3), dim = (own + per - 1) / per * per;
@@ -412,7 +412,7 @@ std::optional<Attended> attention(const Tensor& q_given, const Tensor& k_given, 
 
 std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout_given, const Tensor& q, const Tensor& k, const Tensor& v,
                                                                                    const Tensor& out, const MaybeTensor& rest, const Tensor& lse,
-                                                                                   const MaybeTensor& lengths, bool causal,
+                                                                                   const MaybeTensor& lengths, int causal,
                                                                                    double scale, bool want_q, bool want_k, bool want_v) {
     if (!attention_operands(q, k, v, lengths, scale) || out.sizes() != q.sizes()) return std::nullopt;
     if (rest && (!rest->is_cuda() || rest->device() != q.device() || rest->scalar_type() != q.scalar_type() || rest->sizes() != out.sizes() || rest->strides() != out.strides()))

@@ -64,11 +64,11 @@ std::optional<Four> head_norm_rotary_backward(const MaybeTensor& dyq, const Mayb
 struct Attended {
     Tensor out, lse, q, k, v, padded_out, rest;
 };
-std::optional<Attended> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, const std::optional<double>& scale,
+std::optional<Attended> attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, int causal, const std::optional<double>& scale,
                                   bool want_lse);
 double attention_scale(const Tensor& q, const std::optional<double>& scale);
 std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                                                                                   const MaybeTensor& rest, const Tensor& lse, const MaybeTensor& lengths, bool causal, double scale,
+                                                                                   const MaybeTensor& rest, const Tensor& lse, const MaybeTensor& lengths, int causal, double scale,
                                                                                    bool want_q, bool want_k, bool want_v);
 
 // The boxes of one launch with everything but the base addresses: a call adds those

@@ -463,7 +463,7 @@ std::optional<Two> head_norm_rotary_shard(const MaybeTensor& q, const MaybeTenso
 
 struct AttentionShard {
     static constexpr const char* kName = "AttentionShardBackward";
-    bool causal = false;
+    int causal = 0;
     double scale = 1.0;
     Shared general;
     void identify(Key& key) const { key(int64_t{causal})(c10::bit_cast<int64_t>(scale))(general); }
@@ -481,7 +481,7 @@ struct AttentionShard {
     }
 };
 
-MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, bool causal, std::optional<double> scale, const Shared& general) {
+MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, int causal, std::optional<double> scale, const Shared& general) {
     if (!unobserved() || !ordinary(q) || !ordinary(k) || !ordinary(v) || !ordinary(lengths)) return std::nullopt;
     const bool graph = at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v));
     std::optional<Attended> res;

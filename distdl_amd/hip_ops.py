@@ -1267,6 +1267,9 @@ def _attention_strides(t):
     return _lib.i64_array([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])])
 
 
+CAUSAL_OWN_ENDS = 2      # of ``causal``: the last query sees all keys of its sequence
+
+
 def _attention_operands(q, k, v, lengths, scale, name):
     """Checked operands: ``(q, k, v, lengths, scale, dim)``, heads padded to ``dim``, a multiple of 16 bytes."""
     _require_gpu(q, k, v, lengths)
@@ -1294,8 +1297,8 @@ def _attention_operands(q, k, v, lengths, scale, name):
 
 
 def attention(q, k, v, lengths=None, causal=False, scale=None, want_lse=False):
-    """Attention of ``q`` [batch, tokens, heads, head_dim] to ``k``, ``v`` [batch, keys, kv_heads, head_dim], see ``ddl_attention``: a new
-    tensor like ``q``, and with ``want_lse`` what the adjoint needs: ``(out, lse, rest)``, the rest None in float32."""
+    """Attention of ``q`` [batch, tokens, heads, head_dim] to ``k``, ``v`` [batch, keys, kv_heads, head_dim], see ``ddl_attention`` (``causal``: False,
+    True or ``CAUSAL_OWN_ENDS``): a new tensor like ``q``, and with ``want_lse`` what the adjoint needs: ``(out, lse, rest)``, the rest None in float32."""
     head_dim = q.shape[-1] if q.dim() else 0
     q, k, v, lengths, scale, dim = _attention_operands(q, k, v, lengths, scale, "attention")
     batch, tokens, heads, _ = q.shape

@@ -41,20 +41,29 @@ def _general_backward(grad_output, q, k, v, out, rest, lse, lengths, causal, sca
     return hip_ops.attention_backward(grad_output, q, k, v, out, lse, lengths, causal, scale, want_q, want_k, want_v, rest)
 
 
-def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None):
+def _causal_form(causal, own_ends):
+    if own_ends and not causal:
+        raise ValueError("own_ends says where the causal form ends: it needs causal=True")
+    return hip_ops.CAUSAL_OWN_ENDS if own_ends else int(bool(causal))
+
+
+def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None, own_ends=False):
     """``softmax(scale q k^T) v`` for each head.
 
     q: [batch, tokens, heads, head_dim]; k, v: [batch, keys, kv_heads, head_dim], ``heads`` a multiple of ``kv_heads`` (head h
     uses key head ``h * kv_heads // heads``), head_dim up to 128.  ``lengths``: int32 [batch], the keys that each sequence has
     (None: all); what lies behind them is not read and gets zero gradients.  ``causal``: query i sees keys up to
-    ``i + keys - tokens``, so the last query sees all.  A query that sees no key gives zeros.  ``scale`` defaults to
-    ``head_dim ** -0.5`` and has to be positive."""
+    ``i + keys - tokens``, so the last query sees all that the tensor has room for: the form for padded sequences that attend to themselves.
+    With ``own_ends`` it is ``i + lengths[b] - tokens``: the queries are the last tokens of each sequence, as where several new ones
+    meet a cache whose sequences have different lengths (without it the shorter sequences' first tokens would see those behind them).
+    A query that sees no key gives zeros.  ``scale`` defaults to ``head_dim ** -0.5`` and has to be positive."""
+    causal = _causal_form(causal, own_ends)
     out = _lib.front().attention_shard(q, k, v, lengths, causal, scale, _lib.callback(_general_backward))
     if out is not None:
         return out
     # (through the function without gradients as well: a tangent is then refused, and a trace holds the call)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    return _AttentionShard.apply(q, k, v, lengths, bool(causal), scale, keep)
+    return _AttentionShard.apply(q, k, v, lengths, causal, scale, keep)
 
 
 class DistributedAttention(Module):
@@ -65,11 +74,11 @@ class DistributedAttention(Module):
     ----------
     P_x :
         Partition of queries, keys and values.
-    causal, scale :
+    causal, scale, own_ends :
         See ``attention_shard``.
     """
 
-    def __init__(self, P_x, causal=False, scale=None):
+    def __init__(self, P_x, causal=False, scale=None, own_ends=False):
         super().__init__()
         self.P_x = P_x
         if not self.P_x.active:
@@ -78,12 +87,13 @@ class DistributedAttention(Module):
             raise ValueError(f"attention needs whole sequences and heads, [batch, 1, heads, 1], got a partition of shape {list(P_x.shape)}")
         if scale is not None and not scale > 0:
             raise ValueError(f"scale {scale} is not positive")
-        self.causal, self.scale = bool(causal), scale
+        _causal_form(causal, own_ends)
+        self.causal, self.scale, self.own_ends = bool(causal), scale, bool(own_ends)
 
     def extra_repr(self) -> str:
-        return f'causal={self.causal}, scale={self.scale}' if self.P_x.active else ''
+        return f'causal={self.causal}, scale={self.scale}, own_ends={self.own_ends}' if self.P_x.active else ''
 
     def forward(self, q, k, v, lengths=None):
         if not self.P_x.active:
             return q
-        return attention_shard(q, k, v, lengths, causal=self.causal, scale=self.scale)
+        return attention_shard(q, k, v, lengths, causal=self.causal, scale=self.scale, own_ends=self.own_ends)

@@ -660,7 +660,11 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  *   out[i] = sum over j of p_ij v_j,   p_ij = exp(scale q_i . k_j) / sum over j
  * over the keys j < lengths[batch] (device, int32, values outside 0 .. keys
  * count as those; NULL: all), and with causal != 0 over those with
- * j <= i + keys - tokens of them.  A query without keys gives zeros.  Keys and
+ * j <= i + keys - tokens of them, or, causal = DDL_CAUSAL_OWN_ENDS,
+ * j <= i + lengths[batch] - tokens: the queries are the last ones of every
+ * sequence, as next to a cache of sequences of different lengths (padded
+ * sequences that attend to themselves, tokens = keys, want the former).
+ * A query without keys gives zeros.  Keys and
  * values from a sequence's length on are not read.
  *   q, out   [batch, tokens, heads, head_dim]
  *   k, v     [batch, keys, kv_heads, head_dim], heads a multiple of kv_heads:
@@ -680,6 +684,7 @@ int ddl_head_norm_rotary_backward(const void* dyq, const int64_t* dyq_strides,
  * queries of a head, and with an lse the adjoint's as well, 256 (16-bit heads of
  * more than 64 elements: 512) for 128 keys of a key head (DDL_E_UNSUPP).
  * Probabilities are rounded to the element type for the product with the values. */
+#define DDL_CAUSAL_OWN_ENDS 2
 int64_t ddl_attention_workspace(int64_t batch, int64_t tokens, int64_t keys,
                                 int64_t heads, int64_t kv_heads, int64_t head_dim);
 int ddl_attention(const void* q, const int64_t* q_strides, const void* k,

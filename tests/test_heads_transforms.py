@@ -85,3 +85,13 @@ def test_neither_queries_nor_keys_is_refused():
     for call in (lambda: nn.rotary_shard(None, None, freq), lambda: nn.head_norm_rotary_shard(None, None, None, None, freq)):
         with pytest.raises(ValueError, match="neither"):
             call()
+
+
+def test_own_ends_belong_to_the_causal_form():
+    from distdl_amd.backends.stub_hip import SimWorld
+    q = torch.zeros(1, 2, 2, 8)
+    P = SimWorld(1).partition(0).create_partition_inclusive([0]).create_cartesian_topology_partition([1, 1, 1, 1])
+    for call in (lambda: nn.attention_shard(q, q, q, own_ends=True), lambda: nn.DistributedAttention(P, own_ends=True)):
+        with pytest.raises(ValueError, match="own_ends"):
+            call()
+    assert "own_ends=True" in repr(nn.DistributedAttention(P, causal=True, own_ends=True))
