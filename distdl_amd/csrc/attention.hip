@@ -122,9 +122,10 @@ constexpr int keys_of_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // front of its last block, is then enough for two buffers of each.  What follows it is copied to where
 // everybody has just finished reading: keys two tiles ahead, values NS - 1 blocks ahead.
 //
-// [4,4096,16,128] bf16, all keys: 624 us (881 TFLOP/s; 729 us with the parts one behind the other and tiles through registers), in runs of
-// 20 calls 536; head size 64: 303 us, causal: 273 us (1000), fp32 [2,2048,8,64] 159 us (108).  Bound by issue: the exponentials and the softmax's other
-// vector work next to the matrix instructions, of which each pipe is busy about half of the time.
+// [4,4096,16,128] bf16, all keys, in runs of 20 calls: 551 us (997 TFLOP/s); the first launches of a process, whose clock has yet to rise, take up to 624,
+// where the parts one behind the other and tiles through registers took 729.  Head size 64: 310 us; causal, with sums kept: 292; fp16 551 and 325; fp32 [2,2048,8,64]
+// 160 us (108 TFLOP/s).  Bound by issue: the exponentials and the softmax's other vector work next to the matrix instructions, of which each pipe is busy
+// about half of the time (matrix 55 %, vector 46 %).
 template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_rows(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
@@ -306,8 +307,8 @@ constexpr int rows_lds() {
 // Few queries, many keys: the queries of all heads that share a key head (row = token x group + head in the group) in one
 // wavefront, the keys dealt to `splits` workgroups and there, 32 at a time, to the four wavefronts, each with tiles of its own
 // and no barrier; the four are joined through LDS, the workgroups by attention_join (or, with one split, at once).  Bound by memory where
-// there are enough tiles ([64,1,32,128] bf16, 8 key heads of 2048: 76 us, 4.7 TB/s), by the latency of a few tiles and the join's
-// launch where there are not ([1,1,8,128], 65536 keys of one head: 18.9 us).
+// there are enough tiles ([64,1,32,128] bf16, 8 key heads of 2048: 104 us, 5.2 TB/s), by the latency of a few tiles and the join's
+// launch where there are not ([1,1,8,128], 65536 keys of one head: 17.8 us).
 // (Rows of more than 256 bytes fill the registers of a SIMD with one wavefront: 128 of them for the tiles on their way.)
 template <typename T, int DP, bool LSE>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void attention_split(const AttnArgs a) {

@@ -43,7 +43,8 @@ __device__ inline float chunk_dot(const shortx8& a, const shortx8& b, const T*) 
 // dS in fp16, which has steps down to 2^-24 and values up to 2^16: gradients of 10^-5 would be lost over some thousand keys, and those of 10^5 infinite.  So a
 // column's dS are multiplied by a power of two, `up`, with which the largest so far is below 2^15, and its sum is with it; the factor only
 // falls, where a larger dS comes, and then to where that one is below 2^10.  The other types have the range of 32 bits and need none.
-// ([4,4096,16,64] fp16 forward and adjoint 1525 us instead of 1417 without, head size 128: 2680 and 2580.)
+// ([4,4096,16,64] fp16 forward and adjoint 1500 us instead of 1382 without, head size 128: 2690 and 2490; with the largest found while the matrix cores are
+// busy, before the look, 1540 and 2720.)
 template <typename T>
 struct Fitted {
     static constexpr bool kNeeded = false;
@@ -109,8 +110,8 @@ __device__ inline void load_column(Frag* column, const T* row, bool there, int c
 }
 
 // dq of 32 queries a wavefront, 128 a workgroup, tiles of keys and values through LDS as in attention_rows; and their D.
-// [4,4096,16,128] bf16, all keys: 717 us (1150 TFLOP/s for three products), head size 64: 407, causal [4,2048,8,128] 71.  Bound by the matrix
-// cores and the vector work that does not fit next to them.
+// [4,4096,16,128] bf16, all keys: 717 us (1150 TFLOP/s for three products), head size 64: 414, causal [4,2048,8,128] 72; fp16 800 and 477.  Bound by the matrix
+// cores (62 % busy) and the vector work that does not fit next to them.
 // Where there are few blocks of queries, `splits` workgroups share the keys of one and leave sums in fp32.
 // ONE (16-bit types): all keys are in one tile, D from them.
 template <typename T, int DP, bool ONE>
@@ -338,7 +339,7 @@ struct OfRows {
 
 // dk and dv of 32 keys a wavefront, 128 a workgroup; 32 or 64 queries of one head at a time through LDS, with their sums and D.  Where
 // there are few blocks of keys, `splits` workgroups share the queries of one and leave sums in fp32.
-// [4,4096,16,64] bf16: 545 us, before its two kinds of work were woven 703.
+// [4,4096,16,64] bf16: 565 us (before its two kinds of work were woven 703), fp16 655.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attention_backward_keys(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;
@@ -517,9 +518,9 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void attent
 // take them, and the second add them to both sums a step later, two products each.  Three sets of tiles: of the queries whose turn it is, those
 // before and those on their way.
 //
-// dk and dv of [4,4096,16,128] bf16: 1177 us (934 TFLOP/s), causal 588.  Both sums in one wavefront took 2460; dk in one set and dv in the other, both
+// dk and dv of [4,4096,16,128] bf16: 1154 us (953 TFLOP/s), causal 590 to 630, fp16 1330.  Both sums in one wavefront took 2460; dk in one set and dv in the other, both
 // forming the probabilities, 1409; the first set without the scores of the step ahead 1317.  Bound by the first set's steps and their barriers:
-// matrix cores and LDS are each busy for less than half of the time.
+// matrix cores (46 %) and LDS (38 %) are each busy for less than half of the time.
 template <typename T, int DP>
 __global__ __launch_bounds__(2 * kThreads, 2) void attention_backward_pairs(const AttnArgs a) {
     typedef AttnTile<T, DP> Tile;

@@ -68,8 +68,9 @@ __device__ inline void mfma_chunk(floatx16& acc, const shortx8& a, const shortx8
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), acc, 0, 0, 0);
 }
 
-// Eight values rounded to the 16-bit type (half a step each: 2^-9 of a probability in bf16, 2^-12 in fp16; sums of
-// many of them average it out).
+// Eight values rounded to the 16-bit type, by at most half a step each: 2^-8 of a probability or dS in bf16, 2^-11 in fp16.  The matrix instructions of
+// 16-bit types take no others, those of fp32 have a sixteenth of their rate, and keys and values carry the same rounding already; results are off by
+// 1.3 to 1.5 times what rounding the exact ones gives (where they are rounded, sums of many average it out).
 __device__ inline shortx8 pack8(const floatx16& v, int first, const bf16_t*) {
     uint32_t w[4];
 #pragma unroll
@@ -533,8 +534,8 @@ int grant_lds(int bytes, const char* what) {
 }
 
 // Where all workgroups of a launch whose lengths differ (causal, or sequences' own) are resident at once, two on a CU, the second one on a CU is one
-// of the short half that goes with the long one there (causal, 8192 queries, 8 heads of 128, fp16: 178 us instead of 186; [4,2048,8,128] 51 instead
-// of 54); with more of them than that, longest first is what levels them.
+// of the short half that goes with the long one there (single launches, both in one run: causal, 8192 queries, 8 heads of 128, fp16 178 us instead of
+// 186; [4,2048,8,128] 51 instead of 54); with more of them than that, longest first is what levels them.
 inline bool folds(const AttnArgs& a, int64_t grid) {
     int dev;
     return (a.causal || a.lengths) && grid <= 2 * static_cast<int64_t>(compute_units(dev));

@@ -56,7 +56,12 @@ def attention_shard(q, k, v, lengths=None, *, causal=False, scale=None, own_ends
     ``i + keys - tokens``, so the last query sees all that the tensor has room for: the form for padded sequences that attend to themselves.
     With ``own_ends`` it is ``i + lengths[b] - tokens``: the queries are the last tokens of each sequence, as where several new ones
     meet a cache whose sequences have different lengths (without it the shorter sequences' first tokens would see those behind them).
-    A query that sees no key gives zeros.  ``scale`` defaults to ``head_dim ** -0.5`` and has to be positive."""
+    A query that sees no key gives zeros.  ``scale`` defaults to ``head_dim ** -0.5`` and has to be positive.
+
+    Values of keys that a sequence has are to be finite, for gradients all operands, also where a query does not see a key (zero times infinity is no number).  16-bit types
+    round probabilities, and dS in the adjoint, to theirs for the products.  Where gradients are recorded, 16-bit types keep a tensor as large as the
+    result beside it, what its rounding took, which the adjoint needs for small differences.  Heads that are no multiple of 16 bytes, and operands that
+    do not lie at multiples of 16 bytes, are copied at every call, a cache as well."""
     causal = _causal_form(causal, own_ends)
     out = _lib.front().attention_shard(q, k, v, lengths, causal, scale, _lib.callback(_general_backward))
     if out is not None:
@@ -73,7 +78,7 @@ class DistributedAttention(Module):
     Parameters
     ----------
     P_x :
-        Partition of queries, keys and values.
+        Partition of queries, keys and values.  ``lengths`` of ``forward`` are those of the worker's own sequences.
     causal, scale, own_ends :
         See ``attention_shard``.
     """

@@ -705,9 +705,10 @@ int ddl_attention(const void* q, const int64_t* q_strides, const void* k,
  * atomically: equal calls give equal bits.  Probabilities and dS are rounded to
  * the element type for their products (in fp16 dS times a power of two of each
  * query's or key's own, so that small and large gradients keep their digits).
+ * All operands are to be finite, but for keys and values from a sequence's length on.
  * Scores, scale q . k in powers of two, are to stay below 2^20: the adjoint forms
  * probabilities from lse, whose rounding is in them from there on (ddl_attention
- * itself takes any finite ones).
+ * itself takes all that are finite).
  * Limits as ddl_attention's. */
 int64_t ddl_attention_backward_workspace(int64_t batch, int64_t tokens,
                                          int64_t keys, int64_t heads,
