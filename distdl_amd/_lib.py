@@ -156,6 +156,23 @@ SIGNATURES = {
     "ddl_attention_backward_workspace": (c_int64, [c_int64] * 6),
     "ddl_attention_backward": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p, c_void_p, c_int] + [c_int64] * 6 + [c_void_p, c_int, c_float] +
                                [c_void_p, POINTER(c_int64)] * 3 + [c_void_p, c_int64, c_void_p]),
+    "ddl_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_int, c_int64, c_void_p]),
+    "ddl_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "ddl_rms_norm_backward_workspace": (c_int64, [c_int64, c_int64]),
+    "ddl_rms_norm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
+                                      c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
+    "ddl_expert_plan_workspace": (c_int64, [c_int64, c_int64]),
+    "ddl_expert_plan": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "ddl_expert_sort": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ddl_expert_combine": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ddl_expert_combine_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_void_p, c_void_p]),
+    "ddl_expert_linear": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "ddl_expert_linear_8bit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int,
+                                       c_void_p]),
+    "ddl_expert_linear_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                           c_void_p, c_void_p]),
     "ddl_colsum_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -1,0 +1,117 @@
+// The experts' products: what their kernels share.  Rows lie expert by expert, expert e's from offsets[e] to offsets[e + 1] (device
+// memory: the host knows their number in all, and launches as many workgroups as any distribution of them can need).
+#ifndef DDL_EXPERT_PARTS_H
+#define DDL_EXPERT_PARTS_H
+#include "gemm_tiles.h"
+
+namespace ddl {
+
+// y[rows, n] = a[rows, k] . w[expert]^T by tiles of rows of one expert (w: n rows of k elements; read along n if `transposed`, when
+// it is k rows of n), or w's gradient by tiles of every expert's matrix.
+struct ExpertArgs {
+    const void *a, *w;
+    void* y;
+    const int32_t* offsets;
+    const float *a_scales, *w_scales;     // e4m3
+    int experts, rows, out_dtype;
+    int64_t n, k, lda, ldw, w_stride, ldy;
+    int tiles_m, tiles_n;                 // tiles_m: of an expert's matrix (gradients of the weights)
+};
+
+// Kernels of expert_linear16.hip: tiles of 64 or 128 rows and columns at any address (edge 64, 128), or large ones, of 128 x 256 (low) or 256 x 256.
+enum class ExpertTile { kAny64, kAny128, kLow, kLarge };
+int run_expert_rows16(const char* who, ExpertTile tile, bool f16, bool transposed, ExpertArgs g, int dev, hipStream_t s);
+int run_expert_weights16(const char* who, ExpertTile tile, bool f16, ExpertArgs g, int dev, hipStream_t s);
+// Of expert_linear32.hip.
+int run_expert_rows32(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
+int run_expert_weights32(const char* who, ExpertArgs g, hipStream_t s);
+int run_expert_tiles8(const char* who, ExpertArgs g, int dev, hipStream_t s);
+
+#ifdef __HIPCC__
+namespace {
+
+// First and last row of expert e, whatever the offsets hold; of e = experts: the rows behind the last expert's.
+__device__ inline void rows_of_expert(const ExpertArgs& g, int e, int& lo, int& hi) {
+    lo = min(max(g.offsets[e], 0), g.rows);
+    hi = e == g.experts ? g.rows : min(max(g.offsets[e + 1], lo), g.rows);
+}
+
+struct ExpertTask {
+    int expert;        // g.experts: rows that belong to none, which get zeros; -1: nothing to do
+    int row, rows;     // first row of the tile, and rows from it to the expert's last
+    int tn;
+};
+
+// Tile number `id` of those of `edge` rows: every XCD has a contiguous part of their sequence, which goes expert by expert and inside
+// one in bands of eight tiles of rows, so that the workgroups resident on an XCD share their operands in its L2.  The same in all
+// lanes of a wavefront, each of which looks at one expert of 64.
+__device__ inline ExpertTask find_tile(const ExpertArgs& g, int edge, int id) {
+    const int lane = threadIdx.x & 63;
+    ExpertTask task{-1, 0, 0, 0};
+    auto tiles_of = [&](int e, int& lo, int& n) {
+        int hi = 0;
+        lo = 0, n = 0;
+        if (e <= g.experts) rows_of_expert(g, e, lo, hi), n = hi - lo;
+        return (n + edge - 1) / edge;
+    };
+    int total = 0, lo, n;
+    for (int e0 = 0; e0 <= g.experts; e0 += 64) {
+        int t = tiles_of(e0 + lane, lo, n);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) t += __shfl_xor(t, d);
+        total += __builtin_amdgcn_readfirstlane(t);
+    }
+    const int all = total * g.tiles_n, per = all / kXcds, main = per * kXcds;
+    if (id >= all) return task;
+    if (id < main) id = (id % kXcds) * per + id / kXcds;
+    int before = 0;   // tiles of rows of the experts in front
+    for (int e0 = 0; e0 <= g.experts; e0 += 64) {
+        const int t = tiles_of(e0 + lane, lo, n);
+        int run = t;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(run, d);
+            if (lane >= d) run += v;
+        }
+        const int first = (before + run - t) * g.tiles_n, count = t * g.tiles_n;
+        const uint64_t here = __ballot(id >= first && id < first + count);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            const int rest = id - __builtin_amdgcn_readlane(first, l), tiles_m = __builtin_amdgcn_readlane(t, l);
+            constexpr int kBand = 8;
+            const int band = rest / (kBand * g.tiles_n), band_h = min(kBand, tiles_m - band * kBand), in_band = rest - band * kBand * g.tiles_n;
+            const int skip = (band * kBand + in_band % band_h) * edge;
+            task.expert = e0 + l;
+            task.row = __builtin_amdgcn_readlane(lo, l) + skip, task.rows = __builtin_amdgcn_readlane(n, l) - skip, task.tn = in_band / band_h;
+            break;
+        }
+        before += __builtin_amdgcn_readlane(run, 63);
+    }
+    return task;
+}
+
+// Tile `id` of the experts' matrices: expert, tile row and column, each XCD with a contiguous part of them.
+__device__ inline void find_matrix_tile(const ExpertArgs& g, int id, int& expert, int& tm, int& tn) {
+    const int each = g.tiles_m * g.tiles_n, all = each * g.experts, per = all / kXcds, main = per * kXcds;
+    if (id < main) id = (id % kXcds) * per + id / kXcds;
+    expert = id / each;
+    const int rest = id - expert * each;
+    constexpr int kBand = 8;
+    const int band = rest / (kBand * g.tiles_n), band_h = min(kBand, g.tiles_m - band * kBand), in_band = rest - band * kBand * g.tiles_n;
+    tm = band * kBand + in_band % band_h, tn = in_band / band_h;
+}
+
+// Zeros in rows [row, row + rows) and columns [col, col + cols) of y, by all threads of the workgroup.
+template <typename E>
+__device__ inline void zero_block(E* y, int64_t ldy, int64_t row, int rows, int64_t col, int cols) {
+    for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
+        const int r = i / cols;
+        y[(row + r) * ldy + col + (i - r * cols)] = E{};
+    }
+}
+
+}  // namespace
+#endif
+
+}  // namespace ddl
+#endif  // DDL_EXPERT_PARTS_H

@@ -1356,3 +1356,295 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, causal=False, scal
         if dim != head_dim:
             grads = [None if t is None else contiguous(t[..., :head_dim]) for t in grads]
     return tuple(grads)
+
+
+# ------------------------------------------------- experts' feed-forward --
+
+def _flat_rows(t, name, like=None):
+    """``t`` [..., cols] as [rows, cols] with unit stride of the last; a copy where it has another."""
+    if t.dim() < 1 or t.dtype not in _LN_DTYPES:
+        raise ValueError(f"{name}: need float32, bfloat16 or float16 rows, got {tuple(t.shape)} {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape != like.shape):
+        raise ValueError(f"{name}: operands differ in shape, type or device ({tuple(t.shape)} {t.dtype} on {t.device}, "
+                         f"{tuple(like.shape)} {like.dtype} on {like.device})")
+    cols = t.shape[-1]
+    if cols < 1:
+        raise ValueError(f"{name}: rows without columns")
+    rows = t.numel() // cols
+    if t.dim() == 2 and (cols == 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols):
+        return t
+    _require_gpu(t)
+    with _on_device_of(t):
+        return contiguous(t).view(rows, cols)
+
+
+def _pitch(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _row_weight(weight, like, name):
+    if weight is None:
+        return None
+    if weight.dtype != like.dtype or weight.device != like.device or weight.numel() != like.shape[-1] or not weight.is_contiguous():
+        raise ValueError(f"{name}: the weight must be contiguous, of the rows' type and device, with {like.shape[-1]} elements, "
+                         f"got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
+    return weight
+
+
+def _check_eps(eps, name):
+    eps = float(eps)
+    if not eps >= 0:
+        raise ValueError(f"{name}: eps {eps} is negative")
+    return eps
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6, eight_bit=False, own_squares=False, part_squares=None, total_cols=None):
+    """Rows divided by their root mean square, times ``weight``, see ``ddl_rms_norm``: ``(y, h, codes, scales)`` in the shape of x, None where not
+    made; h is x where there is no residual.  ``own_squares``: this worker's sums for each row instead, ``(sums, h)``; ``part_squares`` [P, rows]: all workers'."""
+    name = "rms_norm"
+    eps = _check_eps(eps, name)
+    _require_gpu(x, weight, residual, part_squares)
+    x2 = _flat_rows(x, name)
+    r2 = None if residual is None else _flat_rows(residual, name, x)
+    w = _row_weight(weight, x, name)
+    rows, cols = x2.shape
+    nparts = 0
+    if part_squares is not None:
+        if part_squares.dtype != torch.float32 or part_squares.dim() != 2 or part_squares.shape[1] != rows or not part_squares.is_contiguous() or \
+           part_squares.device != x.device:
+            raise ValueError(f"{name}: part_squares must be contiguous float32 [workers, {rows}] on {x.device}")
+        nparts = part_squares.shape[0]
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = codes = scales = sums = None
+    if own_squares:
+        sums = torch.empty(rows, dtype=torch.float32, device=x.device)
+    elif eight_bit:
+        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    else:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on_device_of(x):
+        rc = _lib.load().ddl_rms_norm(x2.data_ptr(), _ptr(r2), _ptr(w), _LN_DTYPES[x.dtype], rows, cols, _pitch(x2), 0 if r2 is None else _pitch(r2), eps,
+                                      None if r2 is None else h.data_ptr(), _ptr(y), _ptr(codes), _ptr(scales), _ptr(sums), _ptr(part_squares), nparts,
+                                      cols if total_cols is None else int(total_cols), _stream())
+    _lib.check(rc, "ddl_rms_norm")
+    return (sums, h) if own_squares else (y, h, codes, scales)
+
+
+def quantize_rows(x):
+    """``(codes, scales)``: rows in e4m3 with a float32 scale each, see ``ddl_quantize_rows``."""
+    _require_gpu(x)
+    x2 = _flat_rows(x, "quantize_rows")
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with _on_device_of(x):
+        rc = _lib.load().ddl_quantize_rows(x2.data_ptr(), _LN_DTYPES[x.dtype], x2.shape[0], x2.shape[1], _pitch(x2), codes.data_ptr(), scales.data_ptr(), _stream())
+    _lib.check(rc, "ddl_quantize_rows")
+    return codes, scales
+
+
+def rms_norm_backward(dy, h, weight=None, dh=None, eps=1e-6, want_input=True, want_weight=True, own_sums=False, part_squares=None, part_sums=None, total_cols=None):
+    """Adjoint of ``rms_norm``: ``(dx, dweight)``, None where not wanted; with ``own_sums`` this worker's sums for each row instead."""
+    name = "rms_norm_backward"
+    eps = _check_eps(eps, name)
+    _require_gpu(dy, h, weight, dh, part_squares, part_sums)
+    h2, dy2 = _flat_rows(h, name), _flat_rows(dy, name, h)
+    dh2 = None if dh is None else _flat_rows(dh, name, h)
+    w = _row_weight(weight, h, name)
+    rows, cols = h2.shape
+    nparts = 0
+    if part_sums is not None:
+        for t in (part_squares, part_sums):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != part_sums.shape or t.shape[1] != rows or not t.is_contiguous():
+                raise ValueError(f"{name}: part_squares and part_sums must be contiguous float32 [workers, {rows}]")
+        nparts = part_sums.shape[0]
+    lib = _lib.load()
+    dx = dw = work = sums = None
+    elems = 0
+    if own_sums:
+        sums = torch.empty(rows, dtype=torch.float32, device=h.device)
+    else:
+        if want_input:
+            dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        if want_weight and w is not None:
+            dw = torch.empty(cols, dtype=h.dtype, device=h.device)
+            elems = lib.ddl_rms_norm_backward_workspace(rows, cols)
+            work = torch.empty(elems, dtype=torch.float32, device=h.device)
+    with _on_device_of(h):
+        rc = lib.ddl_rms_norm_backward(dy2.data_ptr(), h2.data_ptr(), _ptr(dh2), _ptr(w), _LN_DTYPES[h.dtype], rows, cols, _pitch(dy2), _pitch(h2),
+                                       0 if dh2 is None else _pitch(dh2), eps, _ptr(dx), _ptr(dw), _ptr(work), elems, _ptr(sums), _ptr(part_squares),
+                                       _ptr(part_sums), nparts, cols if total_cols is None else int(total_cols), _stream())
+    _lib.check(rc, "ddl_rms_norm_backward")
+    return sums if own_sums else (dx, dw)
+
+
+def expert_plan(ids, low, high):
+    """``(place, offsets)`` of the choices ``ids`` [tokens, chosen] among the experts [low, high), see ``ddl_expert_plan``."""
+    _require_gpu(ids)
+    if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"expert_plan: need int32 or int64 [tokens, chosen], got {tuple(ids.shape)} {ids.dtype}")
+    tokens, chosen = ids.shape
+    lib = _lib.load()
+    with _on_device_of(ids):
+        if chosen > 1 and ids.stride(1) != 1:
+            ids = contiguous(ids)
+        place = torch.empty((tokens, chosen), dtype=torch.int32, device=ids.device)
+        offsets = torch.empty(max(0, high - low) + 1, dtype=torch.int32, device=ids.device)
+        elems = lib.ddl_expert_plan_workspace(tokens * chosen, high - low)
+        work = torch.empty(elems, dtype=torch.int32, device=ids.device) if elems else None
+        rc = lib.ddl_expert_plan(ids.data_ptr(), ids.element_size(), tokens, chosen, ids.stride(0) if tokens > 1 else chosen, low, high, place.data_ptr(),
+                                 offsets.data_ptr(), _ptr(work), elems, _stream())
+    _lib.check(rc, "ddl_expert_plan")
+    return place, offsets
+
+
+def _check_place(place, offsets, like, name):
+    if place.dtype != torch.int32 or place.dim() != 2 or not place.is_contiguous() or place.device != like.device or offsets.dtype != torch.int32 or \
+       offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous() or offsets.device != like.device:
+        raise ValueError(f"{name}: the plan must be contiguous int32 on {like.device}, got {place.dtype} on {place.device}, {offsets.dtype} on {offsets.device}")
+
+
+def _held(offsets):
+    return offsets.data_ptr() + 4 * (offsets.numel() - 1)
+
+
+def _rows_of(t, count, name, what):
+    """``t`` as [count, cols] with unit stride of the last; a copy where it has another."""
+    if t.dim() != 2 or t.shape[0] != count or t.shape[1] < 1:
+        raise ValueError(f"{name}: need [{count}, cols] {what}, got {tuple(t.shape)}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (count > 1 and t.stride(0) < t.shape[1]):
+        with _on_device_of(t):
+            t = contiguous(t)
+    return t
+
+
+def expert_sort(x, place, offsets, scales=None):
+    """Rows ``x`` [tokens, cols] (elements of 1, 2 or 4 bytes) in the order of their experts: ``(rows [tokens * chosen, cols], their scales)``, see ``ddl_expert_sort``."""
+    name = "expert_sort"
+    _require_gpu(x, place, offsets, scales)
+    _check_place(place, offsets, x, name)
+    tokens, chosen = place.shape
+    if x.element_size() not in (1, 2, 4) or x.is_complex():
+        raise ValueError(f"{name}: elements of 1, 2 or 4 bytes are moved, got {x.dtype}")
+    x = _rows_of(x, tokens, name, "rows, one for each token")
+    if scales is not None and (scales.dtype != torch.float32 or scales.numel() != tokens or not scales.is_contiguous() or scales.device != x.device):
+        raise ValueError(f"{name}: scales must be contiguous float32, one for each of {tokens} tokens on {x.device}")
+    out = torch.empty((tokens * chosen, x.shape[1]), dtype=x.dtype, device=x.device)
+    out_scales = None if scales is None else torch.empty(tokens * chosen, dtype=torch.float32, device=x.device)
+    with _on_device_of(x):
+        rc = _lib.load().ddl_expert_sort(x.data_ptr(), x.element_size(), tokens, chosen, x.shape[1], _pitch(x), place.data_ptr(), _held(offsets), out.data_ptr(),
+                                         _ptr(scales), _ptr(out_scales), _stream())
+    _lib.check(rc, "ddl_expert_sort")
+    return out, out_scales
+
+
+def _slot_weights(weights, place, name):
+    if weights.dtype != torch.float32 or weights.shape != place.shape or weights.device != place.device:
+        raise ValueError(f"{name}: weights must be float32 {tuple(place.shape)} on {place.device}, got {tuple(weights.shape)} {weights.dtype} on {weights.device}")
+    if not weights.is_contiguous():
+        with _on_device_of(weights):
+            weights = contiguous(weights)
+    return weights
+
+
+def expert_combine(y, place, offsets, weights=None):
+    """Each token's rows of ``y`` [tokens * chosen, cols], times ``weights`` [tokens, chosen] (None: ones), added up, see ``ddl_expert_combine``."""
+    name = "expert_combine"
+    _require_gpu(y, place, offsets, weights)
+    _check_place(place, offsets, y, name)
+    tokens, chosen = place.shape
+    if y.dtype not in _LN_DTYPES:
+        raise ValueError(f"{name}: need float32, bfloat16 or float16 rows, got {y.dtype}")
+    y = _rows_of(y, tokens * chosen, name, "rows, one for each choice")
+    weights = None if weights is None else _slot_weights(weights, place, name)
+    out = torch.empty((tokens, y.shape[1]), dtype=y.dtype, device=y.device)
+    with _on_device_of(y):
+        rc = _lib.load().ddl_expert_combine(y.data_ptr(), _LN_DTYPES[y.dtype], tokens, chosen, y.shape[1], _pitch(y), place.data_ptr(), _held(offsets), _ptr(weights),
+                                            out.data_ptr(), _stream())
+    _lib.check(rc, "ddl_expert_combine")
+    return out
+
+
+def expert_combine_backward(dout, y, place, offsets, weights, want_rows=True, want_weights=True):
+    """Adjoint of ``expert_combine``: ``(dy, dweights)``, None where not wanted."""
+    name = "expert_combine_backward"
+    _require_gpu(dout, y, place, offsets, weights)
+    _check_place(place, offsets, dout, name)
+    tokens, chosen = place.shape
+    dout = _rows_of(dout, tokens, name, "gradients, one row for each token")
+    weights = _slot_weights(weights, place, name)
+    if want_weights:
+        if y.dtype != dout.dtype or y.shape[1:] != dout.shape[1:]:
+            raise ValueError(f"{name}: gradients {tuple(dout.shape)} {dout.dtype} of rows {tuple(y.shape)} {y.dtype}")
+        y = _rows_of(y, tokens * chosen, name, "rows, one for each choice")
+    if dout.dtype not in _LN_DTYPES:
+        raise ValueError(f"{name}: need float32, bfloat16 or float16 rows, got {dout.dtype}")
+    dy = torch.empty((tokens * chosen, dout.shape[1]), dtype=dout.dtype, device=dout.device) if want_rows else None
+    dweights = torch.empty((tokens, chosen), dtype=torch.float32, device=dout.device) if want_weights else None
+    with _on_device_of(dout):
+        rc = _lib.load().ddl_expert_combine_backward(dout.data_ptr(), y.data_ptr() if want_weights else None, _LN_DTYPES[dout.dtype], tokens, chosen, dout.shape[1],
+                                                     _pitch(dout), _pitch(y) if want_weights else 0, place.data_ptr(), _held(offsets), weights.data_ptr(), _ptr(dy),
+                                                     _ptr(dweights), _stream())
+    _lib.check(rc, "ddl_expert_combine_backward")
+    return dy, dweights
+
+
+def _expert_operands(x, weight, offsets, name):
+    _require_gpu(x, weight, offsets)
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"{name}: rows {tuple(x.shape)} {x.dtype} on {x.device} and weights {tuple(weight.shape)} {weight.dtype} on {weight.device} do not fit "
+                         "[rows, in] and [experts, out, in]")
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (weight.shape[0] + 1,) or offsets.device != x.device:
+        raise ValueError(f"{name}: offsets must be int32 [{weight.shape[0] + 1}] on {x.device}, got {tuple(offsets.shape)} {offsets.dtype} on {offsets.device}")
+    with _on_device_of(x):
+        return _rows_of(x, x.shape[0], name, "rows"), contiguous(weight), contiguous(offsets)
+
+
+def expert_linear(x, weight, offsets, x_scales=None, weight_scales=None, dtype=None):
+    """Rows ``x`` [rows, in] by the weights [experts, out, in] of their experts, see ``ddl_expert_linear``; e4m3 rows and weights with their scales,
+    see ``ddl_expert_linear_8bit``, in ``dtype`` (default bfloat16)."""
+    name = "expert_linear"
+    x, weight, offsets = _expert_operands(x, weight, offsets, name)
+    (experts, n, k), rows = weight.shape, x.shape[0]
+    lib = _lib.load()
+    if x.dtype == torch.float8_e4m3fn:
+        dtype = torch.bfloat16 if dtype is None else dtype
+        if dtype not in _LN_DTYPES:
+            raise ValueError(f"{name}: results are float32, bfloat16 or float16, not {dtype}")
+        for scales, shape, what in ((x_scales, (rows,), "x_scales"), (weight_scales, (experts, n), "weight_scales")):
+            if scales is None or scales.dtype != torch.float32 or tuple(scales.shape) != shape or scales.device != x.device:
+                raise ValueError(f"{name}: {what} must be float32 {shape} on {x.device}")
+        y = torch.empty((rows, n), dtype=dtype, device=x.device)
+        with _on_device_of(x):
+            x_scales, weight_scales = contiguous(x_scales), contiguous(weight_scales)
+            rc = lib.ddl_expert_linear_8bit(x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), offsets.data_ptr(), experts, rows, n, k,
+                                            _pitch(x), y.data_ptr(), _LN_DTYPES[dtype], _stream())
+        _lib.check(rc, "ddl_expert_linear_8bit")
+        return y
+    if x.dtype not in _LN_DTYPES:
+        raise ValueError(f"{name}: need float32, bfloat16, float16 or e4m3 rows, got {x.dtype}")
+    if x_scales is not None or weight_scales is not None or dtype not in (None, x.dtype):
+        raise ValueError(f"{name}: scales and another type of the result are for e4m3 rows, these are {x.dtype}")
+    y = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+    with _on_device_of(x):
+        rc = lib.ddl_expert_linear(x.data_ptr(), weight.data_ptr(), _LN_DTYPES[x.dtype], offsets.data_ptr(), experts, rows, n, k, _pitch(x), y.data_ptr(), _stream())
+    _lib.check(rc, "ddl_expert_linear")
+    return y
+
+
+def expert_linear_backward(dy, x, weight, offsets, want_input=True, want_weight=True):
+    """Adjoint of ``expert_linear``: ``(dx, dweight)``, None where not wanted."""
+    name = "expert_linear_backward"
+    x, weight, offsets = _expert_operands(x, weight, offsets, name)
+    (experts, n, k), rows = weight.shape, x.shape[0]
+    _require_gpu(dy)
+    if dy.dtype != x.dtype or tuple(dy.shape) != (rows, n):
+        raise ValueError(f"{name}: gradients {tuple(dy.shape)} {dy.dtype} of results {(rows, n)} {x.dtype}")
+    dy = _rows_of(dy, rows, name, "gradients")
+    dx = torch.empty((rows, k), dtype=x.dtype, device=x.device) if want_input else None
+    dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if want_weight else None
+    with _on_device_of(x):
+        rc = _lib.load().ddl_expert_linear_backward(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _LN_DTYPES[x.dtype], offsets.data_ptr(), experts, rows, n, k,
+                                                    _pitch(dy), _pitch(x), _ptr(dx), _ptr(dw), _stream())
+    _lib.check(rc, "ddl_expert_linear_backward")
+    return dx, dw

@@ -13,6 +13,12 @@ from .conv_feature import DistributedFeatureConv1d  # noqa: F401
 from .conv_feature import DistributedFeatureConv2d  # noqa: F401
 from .conv_feature import DistributedFeatureConv3d  # noqa: F401
 from .embedding import DistributedEmbedding  # noqa: F401
+from .experts import DistributedExpertLinear  # noqa: F401
+from .experts import ExpertPlan  # noqa: F401
+from .experts import expert_combine  # noqa: F401
+from .experts import expert_linear_shard  # noqa: F401
+from .experts import expert_plan  # noqa: F401
+from .experts import expert_sort  # noqa: F401
 from .halo_exchange import HaloExchange  # noqa: F401
 from .layernorm import DistributedLayerNorm  # noqa: F401
 from .linear import DistributedLinear  # noqa: F401
@@ -21,6 +27,9 @@ from .linear_rs import DistributedLinearReduceScatter  # noqa: F401
 from .reduce_scatter import ReduceScatter  # noqa: F401
 from .module import Module  # noqa: F401
 from .repartition import Repartition  # noqa: F401
+from .rms_norm import DistributedRMSNorm  # noqa: F401
+from .rms_norm import quantize_rows  # noqa: F401
+from .rms_norm import rms_norm_shard  # noqa: F401
 from .rotary import DistributedHeadNormRotary  # noqa: F401
 from .rotary import DistributedRotary  # noqa: F401
 from .rotary import head_norm_rotary_shard  # noqa: F401
@@ -35,4 +44,6 @@ __all__ = [
     "HaloExchange", "DistributedLayerNorm", "DistributedLinear", "DistributedLinearAllGather", "DistributedLinearReduceScatter", "Module", "ReduceScatter",
     "Repartition", "SumReduce", "DistributedTranspose", "DistributedRotary", "DistributedHeadNormRotary", "rotary_frequencies",
     "rotary_shard", "head_norm_rotary_shard", "DistributedAttention", "attention_shard",
+    "DistributedRMSNorm", "rms_norm_shard", "quantize_rows", "ExpertPlan", "expert_plan", "expert_sort", "expert_combine",
+    "DistributedExpertLinear", "expert_linear_shard",
 ]

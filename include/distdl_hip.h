@@ -727,6 +727,127 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides,
                            const int64_t* dv_strides, float* workspace,
                            int64_t workspace_elems, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Experts' feed-forward block: norm in front of it, tokens to their experts and
+ * back, the experts' products (no counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* Root-mean-square norm of the rows of x [rows, cols], pitch ld_x:
+ *   y = h / sqrt(mean of h^2 + eps) * weight,  h = x, or x + residual.
+ *   residual  like x with pitch ld_residual, or NULL; then `sum` [rows, cols] gets h,
+ *             rounded to the type, which is also what is normalised
+ *   weight    cols elements of the type, or NULL
+ *   y         [rows, cols]; or, instead of it,
+ *   codes     [rows, cols] e4m3 (OCP) and scales [rows]: code = e4m3(y / scale),
+ *             scale = max(max |y| / 448, 2^-126).  A row with an infinity or not a
+ *             number in it stands for no numbers.
+ * Columns spread over workers: with own_squares [rows] the launch leaves this
+ * worker's sums of h^2 there (and `sum`) and nothing else; with part_squares
+ * [nparts, rows], those of all workers, rows are normalised as if they had
+ * total_cols columns.  Device memory at the alignment of an element; the results
+ * are contiguous and none of them overlaps an operand.  fp32, bf16 or fp16; 1 to 16384 columns here (DDL_E_UNSUPP
+ * above); the sum of a row's squares is to be a 32-bit float. */
+int ddl_rms_norm(const void* x, const void* residual, const void* weight,
+                 int dtype, int64_t rows, int64_t cols, int64_t ld_x,
+                 int64_t ld_residual, float eps, void* sum, void* y, void* codes,
+                 float* scales, float* own_squares, const float* part_squares,
+                 int nparts, int64_t total_cols, void* stream);
+
+/* The rows themselves in 8 bits: codes and scales as above. */
+int ddl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols,
+                      int64_t ld_x, void* codes, float* scales, void* stream);
+
+/* The adjoint of ddl_rms_norm: g = dy weight, xhat = h / sqrt(mean of h^2 + eps),
+ *   dx = (g - xhat mean(g xhat)) / sqrt(mean of h^2 + eps) + dh (NULL: nothing),
+ *   dweight = sum over rows of dy xhat;
+ * dx is the gradient of x and of the residual.  dx or dweight may be NULL;
+ * `workspace` for dweight: ddl_rms_norm_backward_workspace(rows, cols) floats.
+ * Columns spread over workers: with own_sums [rows] the launch leaves this worker's
+ * sums of g h and nothing else; with part_squares and part_sums [nparts, rows] it
+ * takes all workers'.  Sums have one order: equal calls give equal bits. */
+int64_t ddl_rms_norm_backward_workspace(int64_t rows, int64_t cols);
+int ddl_rms_norm_backward(const void* dy, const void* h, const void* dh,
+                          const void* weight, int dtype, int64_t rows,
+                          int64_t cols, int64_t ld_dy, int64_t ld_h,
+                          int64_t ld_dh, float eps, void* dx, void* dweight,
+                          float* workspace, int64_t workspace_elems,
+                          float* own_sums, const float* part_squares,
+                          const float* part_sums, int nparts, int64_t total_cols,
+                          void* stream);
+
+/* The order of tokens' choices by experts.  ids [tokens, chosen] (int32 or int64 by
+ * id_bytes, rows ld_ids elements apart) holds the experts that each token was sent
+ * to; slot s = token * chosen + j.  Choices outside [low, high) are not held here.
+ *   place [tokens * chosen]   the row of slot s when the held slots lie expert by
+ *                             expert, in the order of the slots within one; slots
+ *                             that are not held come behind all that are
+ *   offsets [high - low + 1]  expert e's rows are offsets[e - low] to offsets[e - low + 1]
+ * `workspace`: ddl_expert_plan_workspace(...) int32.  Up to 2047 experts are held here, fewer than
+ * 2^31 slots (DDL_E_UNSUPP). */
+int64_t ddl_expert_plan_workspace(int64_t slots, int64_t held_experts);
+int ddl_expert_plan(const void* ids, int id_bytes, int64_t tokens,
+                    int64_t chosen, int64_t ld_ids, int64_t low, int64_t high,
+                    int32_t* place, int32_t* offsets, int32_t* workspace,
+                    int64_t workspace_elems, void* stream);
+
+/* Rows to their experts: out[place[t * chosen + j]] = x[t], zeros for slots whose
+ * place is *held or above (held: the last of the plan's offsets, device).  Elements of 1, 2
+ * or 4 bytes are moved as they are; scales (NULL, or a float for each token) go
+ * to out_scales along with them. */
+int ddl_expert_sort(const void* x, int elem_bytes, int64_t tokens, int64_t chosen,
+                    int64_t cols, int64_t ld_x, const int32_t* place,
+                    const int32_t* held, void* out, const float* scales,
+                    float* out_scales, void* stream);
+
+/* Rows back: out[t] = sum over j of weights[t * chosen + j] y[place[t * chosen + j]]
+ * over the slots that are held (weights NULL: ones, which is the adjoint of the
+ * sort), in the order of j in 32 bits. */
+int ddl_expert_combine(const void* y, int dtype, int64_t tokens, int64_t chosen,
+                       int64_t cols, int64_t ld_y, const int32_t* place,
+                       const int32_t* held, const float* weights, void* out,
+                       void* stream);
+
+/* The adjoint of ddl_expert_combine: dy[place[s]] = weights[s] dout[t] (zeros for
+ * slots that are not held) and dweights[s] = dout[t] . y[place[s]] (zero).  dy or
+ * dweights may be NULL, y if dweights is. */
+int ddl_expert_combine_backward(const void* dout, const void* y, int dtype,
+                                int64_t tokens, int64_t chosen, int64_t cols,
+                                int64_t ld_dout, int64_t ld_y, const int32_t* place,
+                                const int32_t* held, const float* weights,
+                                void* dy, float* dweights, void* stream);
+
+/* The experts' products: y[i] = w[e] x[i] for rows i of expert e, offsets[e] <= i <
+ * offsets[e + 1] (device, int32 [experts + 1], not decreasing; values outside 0 .. rows
+ * count as those), zeros for rows from offsets[experts] on.
+ *   x [rows, k], pitch ld_x;  w [experts, n, k], contiguous;  y [rows, n], contiguous
+ * fp32, bf16 or fp16, summed in 32 bits.  Rows in front of offsets[0] are left as they are.  16-bit
+ * matrices have at least 8 rows and columns; pitches up to 2^22 elements; matrices
+ * of fewer than 2^29 elements (DDL_E_UNSUPP). */
+int ddl_expert_linear(const void* x, const void* w, int dtype,
+                      const int32_t* offsets, int64_t experts, int64_t rows,
+                      int64_t n, int64_t k, int64_t ld_x, void* y, void* stream);
+
+/* The same of e4m3 (OCP) rows and weights:
+ *   y[i, j] = x_scales[i] w_scales[e, j] sum over k of w[e, j, k] x[i, k],
+ * in fp32, bf16 or fp16.  The matrix cores add e4m3 products in eights (k = 8 i to
+ * 8 i + 7), whose members they cut off at 2^-13 of the largest one's power of two, and
+ * the eights' sums in 32 bits.  k and ld_x are multiples of 16, x and w 16-byte aligned
+ * (DDL_E_ALIGN). */
+int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w,
+                           const float* w_scales, const int32_t* offsets,
+                           int64_t experts, int64_t rows, int64_t n, int64_t k,
+                           int64_t ld_x, void* y, int out_dtype, void* stream);
+
+/* The adjoint of ddl_expert_linear: dx[i] = w[e]^T dy[i] (zeros for rows without an expert) and
+ * dw[e] = sum over its rows of dy[i] x[i]^T (zeros without rows).  dx or dw may be NULL.
+ * Gradients of fp32 weights take rows x pitch of fewer than 2^29 elements (DDL_E_UNSUPP).
+ * Nothing is added atomically: equal calls give equal bits. */
+int ddl_expert_linear_backward(const void* dy, const void* x, const void* w,
+                               int dtype, const int32_t* offsets,
+                               int64_t experts, int64_t rows, int64_t n, int64_t k,
+                               int64_t ld_dy, int64_t ld_x, void* dx, void* dw,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif
