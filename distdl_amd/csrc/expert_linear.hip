@@ -1,5 +1,5 @@
 // The products of rows with the weights of the expert that each was sent to, and their adjoint: the entry points and the
-// kernel for few rows.  (expert_linear16.hip, expert_linear32.hip: tiles.)
+// kernel for few rows.  (expert_linear8.hip, expert_linear16.hip, expert_linear32.hip: tiles.)
 //
 // expert_stream (bf16, fp16 and e4m3; few rows for each expert): bound by reading the weights once.  A workgroup has 32 rows of one
 // expert's weights; its wavefronts take the 128-byte lines of those in turn, 16 rows at a time straight from memory into registers
@@ -234,7 +234,12 @@ int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w, 
     ExpertArgs g{};
     g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.a_scales = x_scales, g.w_scales = w_scales, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows);
     g.out_dtype = out_dtype, g.n = n, g.k = k, g.lda = pitch, g.ldw = k, g.w_stride = n * k, g.ldy = n;
-    return launch_stream<kE4m3>(who, g, static_cast<hipStream_t>(stream));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t each = rows / (experts ? experts : 1);
+    if (each <= kStreamRows) return launch_stream<kE4m3>(who, g, s);
+    int dev = 0;
+    const int cus = compute_units(dev);
+    return run_expert_rows8(who, tile_for(true, (rows + 255) / 256 * ((n + 255) / 256), each, cus) != ExpertTile::kLarge, g, dev, s);
 }
 
 int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int dtype, const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k,

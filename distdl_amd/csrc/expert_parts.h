@@ -25,7 +25,8 @@ int run_expert_weights16(const char* who, ExpertTile tile, bool f16, ExpertArgs 
 // Of expert_linear32.hip.
 int run_expert_rows32(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32(const char* who, ExpertArgs g, hipStream_t s);
-int run_expert_tiles8(const char* who, ExpertArgs g, int dev, hipStream_t s);
+// Of expert_linear8.hip: tiles of 128 (low) or 256 rows by 256 columns.
+int run_expert_rows8(const char* who, bool low, const ExpertArgs& g, int dev, hipStream_t s);
 
 #ifdef __HIPCC__
 namespace {

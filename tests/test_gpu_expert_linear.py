@@ -38,6 +38,8 @@ IN_EIGHTS = 7 * 2.0 ** -13
 CASES = [
     ([1], 0, 8, 8), ([0], 3, 16, 24), ([0, 0, 5], 0, 64, 40), ([3, 0, 2, 1], 4, 128, 96), ([16, 1, 0, 33, 7], 0, 264, 72), ([40, 9], 2, 1000, 100), ([1, 2, 3], 0, 72, 520),
     ([200, 0, 57, 130], 11, 320, 264), ([300, 513], 0, 136, 264), ([700, 0, 900], 5, 512, 768), ([2100, 1500], 0, 256, 512), ([5] * 70, 1, 64, 32),
+    # what fills the chip with large tiles: results, gradients of the rows, of the weights
+    ([3001, 0, 1200], 7, 72, 8000), ([3001, 0, 1200], 7, 8000, 72), ([9, 0, 130, 2, 64, 1, 70, 200], 3, 2056, 2040),
     # rows that are no multiple of 16 bytes
     ([5, 0, 9], 2, 9, 11), ([100, 37], 3, 77, 65), ([260, 300], 0, 513, 331), ([1, 1], 0, 1001, 15)]
 
@@ -65,7 +67,7 @@ def test_products_and_adjoint(counts, spare, k, n, dtype):
 
 
 E4M3 = [([1], 0, 16, 1), ([0], 2, 16, 8), ([3, 0, 2, 1], 4, 128, 96), ([16, 1, 0, 33, 7], 0, 272, 72), ([40, 9], 2, 1008, 100), ([200, 0, 57, 130], 11, 320, 264), ([700, 0, 900], 5, 512, 768),
-        ([2100, 1500], 0, 256, 513), ([5] * 70, 1, 64, 32), ([300, 300], 7, 144, 520)]
+        ([2100, 1500], 0, 256, 513), ([5] * 70, 1, 64, 32), ([300, 300], 7, 144, 520), ([33, 100], 0, 16, 8), ([90], 0, 2048, 300), ([3001, 0, 1200], 7, 400, 8000), ([4200], 0, 1296, 7900)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES)
