@@ -71,6 +71,22 @@ std::optional<std::tuple<MaybeTensor, MaybeTensor, MaybeTensor>> attention_backw
                                                                                    const MaybeTensor& rest, const Tensor& lse, const MaybeTensor& lengths, int causal, double scale,
                                                                                    bool want_q, bool want_k, bool want_v);
 
+// Experts' feed-forward operators (front_experts.cpp).  y: rows, or their codes with scales; h: x + residual, where there is one.
+struct Normed {
+    Tensor y, h, scales;
+};
+std::optional<Normed> rms_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps, bool eight_bit);
+std::optional<std::tuple<Tensor, Tensor>> quantize_rows(const Tensor& x);
+std::optional<Two> rms_norm_backward(const Tensor& dy, const Tensor& h, const MaybeTensor& weight, const MaybeTensor& dh, double eps, bool want_input, bool want_weight);
+std::optional<std::tuple<Tensor, Tensor>> expert_plan(const Tensor& ids, int64_t low, int64_t high);
+std::optional<Two> expert_sort(const Tensor& x, const Tensor& place, const Tensor& offsets, const MaybeTensor& scales);
+MaybeTensor expert_combine(const Tensor& y, const Tensor& place, const Tensor& offsets, const MaybeTensor& weights);
+std::optional<Two> expert_combine_backward(const Tensor& dout, const Tensor& y, const Tensor& place, const Tensor& offsets, const Tensor& weights, bool want_rows,
+                                           bool want_weights);
+MaybeTensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets);
+MaybeTensor expert_linear_8bit(const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& x_scales, const Tensor& w_scales, at::ScalarType dtype);
+std::optional<Two> expert_linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& offsets, bool want_input, bool want_weight);
+
 // The boxes of one launch with everything but the base addresses: a call adds those
 // of the slots.  Calls only read the object.
 class Boxes {

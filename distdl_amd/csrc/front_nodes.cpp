@@ -502,6 +502,185 @@ MaybeTensor attention_shard(const Tensor& q, const Tensor& k, const Tensor& v, c
     return res->out;
 }
 
+// --------------------------------------------------------------- experts --
+
+struct RmsNormShard {
+    static constexpr const char* kName = "RmsNormShardBackward";
+    static constexpr int kResults = 2;
+    double eps = 0.0;
+    bool added = false;     // a residual was: the sum is the second result
+    Shared general;
+    void identify(Key& key) const { key(c10::bit_cast<int64_t>(eps))(int64_t{added})(general); }
+    variable_list run(const std::vector<Tensor>& kept, const variable_list& grads, const Asked& asked) const {
+        const bool need_x = has(asked.now, 0), need_w = has(asked.now, 1), need_r = has(asked.now, 2);
+        const MaybeTensor weight = defined(kept[1]), dy = arrived(grads[0], true), dh = added ? arrived(grads[1], need_x || need_r) : std::nullopt;
+        Two res(dh, std::nullopt);
+        {
+            at::NoGradGuard no_grad;
+            if (!dy) {       // only the sum was used
+                if (need_w && weight) std::get<1>(res) = at::zeros_like(*weight);
+            } else if (std::optional<Two> made = rms_norm_backward(*dy, kept[0], weight, dh, eps, need_x || need_r, need_w)) {
+                res = *made;
+            } else {
+                res = general->call<Two>(*dy, kept[0], weight, dh, eps, need_x || need_r, need_w);
+            }
+        }
+        const MaybeTensor none, dx = std::get<0>(res);
+        return final_gradients(gradients({need_x ? dx : none, std::get<1>(res), need_r ? dx : none}), kName);
+    }
+};
+
+std::optional<Two> rms_norm_shard(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps, const Shared& general) {
+    if (!unobserved() || !ordinary(x) || !ordinary(weight) || !ordinary(residual)) return std::nullopt;
+    std::optional<Normed> res;
+    {
+        at::NoGradGuard no_grad;
+        res = rms_norm(x, weight, residual, eps, false);
+    }
+    if (!res) return std::nullopt;
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(residual))) {
+        auto node = make_node(RmsNormShard{eps, residual.has_value(), general}, {x, weight, residual});
+        node->save(residual ? res->h.detach() : x);      // the sum: the same memory and version, without this node
+        node->save(weight ? *weight : Tensor());
+        torch::autograd::create_gradient_edge(res->y, node);
+        if (residual) torch::autograd::create_gradient_edge(res->h, node);
+    }
+    return Two(res->y, defined(res->h));
+}
+
+// Rows in 8 bits: codes, scales and the sum; where no gradient could be recorded.
+std::optional<Three> rms_norm_eight(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps) {
+    if (!unobserved() || !ordinary(x) || !ordinary(weight) || !ordinary(residual)) return std::nullopt;
+    at::NoGradGuard no_grad;
+    const std::optional<Normed> res = rms_norm(x, weight, residual, eps, true);
+    if (!res) return std::nullopt;
+    return Three(res->y, res->scales, defined(res->h));
+}
+
+std::optional<std::tuple<Tensor, Tensor>> rows_eight(const Tensor& x) {
+    if (!unobserved() || !ordinary(x)) return std::nullopt;
+    at::NoGradGuard no_grad;
+    return quantize_rows(x);
+}
+
+std::optional<std::tuple<Tensor, Tensor>> plan_experts(const Tensor& ids, int64_t low, int64_t high) {
+    if (!unobserved() || !ordinary(ids)) return std::nullopt;
+    return expert_plan(ids, low, high);
+}
+
+std::optional<Two> sort_eight(const Tensor& x, const Tensor& place, const Tensor& offsets, const Tensor& scales) {
+    if (!unobserved() || !ordinary(x) || !ordinary(place) || !ordinary(offsets) || !ordinary(scales)) return std::nullopt;
+    at::NoGradGuard no_grad;
+    return expert_sort(x, place, offsets, scales);
+}
+
+struct ExpertSort {
+    static constexpr const char* kName = "ExpertSortBackward";
+    Shared general;
+    void identify(Key& key) const { key(general); }
+    variable_list run(const std::vector<Tensor>& kept, const Tensor& dy_given, const Asked&) const {
+        const Tensor dy = dy_given.detach();
+        MaybeTensor dx;
+        {
+            at::NoGradGuard no_grad;
+            dx = expert_combine(dy, kept[0], kept[1], std::nullopt);
+            if (!dx) dx = general->call<Tensor>(dy, kept[0], kept[1]);
+        }
+        return final_gradients({*dx}, kName);
+    }
+};
+
+MaybeTensor expert_sort_shard(const Tensor& x, const Tensor& place, const Tensor& offsets, const Shared& general) {
+    if (!unobserved() || !ordinary(x) || !ordinary(place) || !ordinary(offsets) || !float_code(x)) return std::nullopt;
+    std::optional<Two> res;
+    {
+        at::NoGradGuard no_grad;
+        res = expert_sort(x, place, offsets, std::nullopt);
+    }
+    if (!res) return std::nullopt;
+    Tensor out = *std::get<0>(*res);
+    if (at::GradMode::is_enabled() && wanted(x)) {
+        auto node = make_node(ExpertSort{general}, {x});
+        node->save(place);
+        node->save(offsets);
+        torch::autograd::create_gradient_edge(out, node);
+    }
+    return out;
+}
+
+struct ExpertCombine {
+    static constexpr const char* kName = "ExpertCombineBackward";
+    Shared general;
+    void identify(Key& key) const { key(general); }
+    variable_list run(const std::vector<Tensor>& kept, const Tensor& dout_given, const Asked& asked) const {
+        const Tensor dout = dout_given.detach();
+        const MaybeTensor weights = defined(kept[1]);
+        const bool need_y = has(asked.now, 0), need_w = has(asked.now, 1);
+        std::optional<Two> res;
+        {
+            at::NoGradGuard no_grad;
+            if (weights) res = expert_combine_backward(dout, kept[0], kept[2], kept[3], *weights, need_y, need_w);
+            else if (const auto sorted = expert_sort(dout, kept[2], kept[3], std::nullopt)) res = Two(std::get<0>(*sorted), std::nullopt);
+            if (!res) res = general->call<Two>(dout, kept[0], weights, kept[2], kept[3], need_y, need_w);
+        }
+        return final_gradients(gradients({std::get<0>(*res), std::get<1>(*res)}), kName);
+    }
+};
+
+MaybeTensor expert_combine_shard(const Tensor& y, const MaybeTensor& weights, const Tensor& place, const Tensor& offsets, const Shared& general) {
+    if (!unobserved() || !ordinary(y) || !ordinary(weights) || !ordinary(place) || !ordinary(offsets)) return std::nullopt;
+    MaybeTensor out;
+    {
+        at::NoGradGuard no_grad;
+        out = expert_combine(y, place, offsets, weights);
+    }
+    if (!out || !at::GradMode::is_enabled() || !(wanted(y) || wanted(weights))) return out;
+    auto node = make_node(ExpertCombine{general}, {y, weights});
+    node->save(y);
+    node->save(weights ? *weights : Tensor());
+    node->save(place);
+    node->save(offsets);
+    torch::autograd::create_gradient_edge(*out, node);
+    return out;
+}
+
+struct ExpertLinear {
+    static constexpr const char* kName = "ExpertLinearBackward";
+    Shared general;
+    void identify(Key& key) const { key(general); }
+    variable_list run(const std::vector<Tensor>& kept, const Tensor& dy_given, const Asked& asked) const {
+        const Tensor dy = dy_given.detach();
+        const bool need_x = has(asked.now, 0), need_w = has(asked.now, 1);
+        std::optional<Two> res;
+        {
+            at::NoGradGuard no_grad;
+            res = expert_linear_backward(dy, kept[0], kept[1], kept[2], need_x, need_w);
+            if (!res) res = general->call<Two>(dy, kept[0], kept[1], kept[2], need_x, need_w);
+        }
+        return final_gradients(gradients({std::get<0>(*res), std::get<1>(*res)}), kName);
+    }
+};
+
+MaybeTensor expert_linear_shard(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Shared& general) {
+    if (!unobserved() || !ordinary(x) || !ordinary(weight) || !ordinary(offsets)) return std::nullopt;
+    MaybeTensor y;
+    {
+        at::NoGradGuard no_grad;
+        y = expert_linear(x, weight, offsets);
+    }
+    if (!y || !at::GradMode::is_enabled() || !(wanted(x) || wanted(weight))) return y;
+    auto node = make_node(ExpertLinear{general}, {x, weight});
+    for (const Tensor& t : {x, weight, offsets}) node->save(t);
+    torch::autograd::create_gradient_edge(*y, node);
+    return y;
+}
+
+MaybeTensor expert_linear_eight(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& x_scales, const Tensor& w_scales, at::ScalarType dtype) {
+    if (!unobserved() || !ordinary(x) || !ordinary(weight) || !ordinary(offsets) || !ordinary(x_scales) || !ordinary(w_scales)) return std::nullopt;
+    at::NoGradGuard no_grad;
+    return expert_linear_8bit(x, weight, offsets, x_scales, w_scales, dtype);
+}
+
 // ----------------------------------------------------------------- moves --
 
 // Pooled communication buffers that have been reallocated since this extension was loaded.
@@ -630,6 +809,15 @@ void define_nodes(py::module_& m) {
     m.def("rotary_shard", &rotary_shard, unlocked());
     m.def("head_norm_rotary_shard", &head_norm_rotary_shard, unlocked());
     m.def("attention_shard", &attention_shard, unlocked());
+    m.def("rms_norm_shard", &rms_norm_shard, unlocked());
+    m.def("rms_norm_eight", &rms_norm_eight, unlocked());
+    m.def("quantize_rows", &rows_eight, unlocked());
+    m.def("expert_plan", &plan_experts, unlocked());
+    m.def("expert_sort_shard", &expert_sort_shard, unlocked());
+    m.def("expert_sort_eight", &sort_eight, unlocked());
+    m.def("expert_combine_shard", &expert_combine_shard, unlocked());
+    m.def("expert_linear_shard", &expert_linear_shard, unlocked());
+    m.def("expert_linear_eight", &expert_linear_eight, unlocked());
     m.def("move", &move, unlocked());
     m.def("alias", &alias, unlocked());
     m.def("attachable", &attachable);

@@ -9,6 +9,7 @@ import numbers
 
 import torch
 
+from .. import _lib
 from .. import hip_ops
 from ..utilities.slicing import compute_subshape
 from ..utilities.slicing import compute_start_index
@@ -42,7 +43,38 @@ def expert_plan(experts, num_experts, *, window=None):
     low, high = _window(window, int(num_experts))
     if experts.dim() != 2 or experts.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"expert_plan: need int32 or int64 [tokens, chosen], got {tuple(experts.shape)} {experts.dtype}")
-    return ExpertPlan(*hip_ops.expert_plan(experts.detach(), low, high), (low, high))
+    res = _lib.front().expert_plan(experts, low, high)
+    if res is None:
+        res = _ExpertPlan.apply(experts, low, high)
+    return ExpertPlan(*res, (low, high))
+
+
+class _ExpertPlan(torch.autograd.Function):
+    """For a trace to hold the call, as the other functions without a gradient here."""
+
+    @staticmethod
+    def forward(ctx, ids, low, high):
+        res = hip_ops.expert_plan(ids, low, high)
+        ctx.mark_non_differentiable(*res)
+        return res
+
+
+class _ExpertSortEight(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, place, offsets, scales):
+        res = hip_ops.expert_sort(x, place, offsets, scales)
+        ctx.mark_non_differentiable(*res)
+        return res
+
+
+class _ExpertLinearEight(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, offsets, x_scales, weight_scales, dtype):
+        y = hip_ops.expert_linear(x, weight, offsets, x_scales, weight_scales, dtype)
+        ctx.mark_non_differentiable(y)
+        return y
 
 
 class _ExpertSort(torch.autograd.Function):
@@ -73,9 +105,18 @@ class _ExpertCombine(torch.autograd.Function):
         y, weights, place, offsets = ctx.saved_tensors
         need_y, need_w = ctx.needs_input_grad[:2]
         grad = grad if grad.dtype == y.dtype else grad.to(y.dtype)
-        if weights is None:
-            return hip_ops.expert_sort(grad, place, offsets)[0] if need_y else None, None, None, None
-        return hip_ops.expert_combine_backward(grad, y, place, offsets, weights, need_y, need_w) + (None, None)
+        return _general_combine_backward(grad, y, weights, place, offsets, need_y, need_w) + (None, None)
+
+
+def _general_sort_backward(grad, place, offsets):
+    """The adjoint for what its native form does not take; so the others."""
+    return hip_ops.expert_combine(grad, place, offsets)
+
+
+def _general_combine_backward(grad, y, weights, place, offsets, want_rows, want_weights):
+    if weights is None:
+        return hip_ops.expert_sort(grad, place, offsets)[0] if want_rows else None, None
+    return hip_ops.expert_combine_backward(grad, y, place, offsets, weights, want_rows, want_weights)
 
 
 def expert_sort(x, plan, scales=None):
@@ -86,16 +127,19 @@ def expert_sort(x, plan, scales=None):
     if scales is not None:
         if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
             raise ValueError("rows with scales have no gradient: call this under torch.no_grad(), or detach the operands")
-        return hip_ops.expert_sort(x.detach(), plan.place, plan.offsets, scales.detach())
+        res = _lib.front().expert_sort_eight(x, plan.place, plan.offsets, scales)
+        return res if res is not None else _ExpertSortEight.apply(x, plan.place, plan.offsets, scales)
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"expert_sort: float32, bfloat16 and float16 rows, others with their scales, got {x.dtype}")
-    return _ExpertSort.apply(x, plan.place, plan.offsets)
+    res = _lib.front().expert_sort_shard(x, plan.place, plan.offsets, _lib.callback(_general_sort_backward))
+    return res if res is not None else _ExpertSort.apply(x, plan.place, plan.offsets)
 
 
 def expert_combine(y, plan, weights=None):
     """What came of each token's choices, ``y`` [tokens * chosen, cols] in the experts' order, times ``weights`` (float32 [tokens, chosen]; None: ones), added up: [tokens, cols].
     Choices that the plan left out add nothing; what lies behind the last expert's rows is not read."""
-    return _ExpertCombine.apply(y, weights, plan.place, plan.offsets)
+    res = _lib.front().expert_combine_shard(y, weights, plan.place, plan.offsets, _lib.callback(_general_combine_backward))
+    return res if res is not None else _ExpertCombine.apply(y, weights, plan.place, plan.offsets)
 
 
 class _ExpertLinear(torch.autograd.Function):
@@ -113,6 +157,10 @@ class _ExpertLinear(torch.autograd.Function):
         return hip_ops.expert_linear_backward(grad, x, weight, offsets, *ctx.needs_input_grad[:2]) + (None,)
 
 
+def _general_linear_backward(grad, x, weight, offsets, want_input, want_weight):
+    return hip_ops.expert_linear_backward(grad, x, weight, offsets, want_input, want_weight)
+
+
 def expert_linear_shard(x, weight, offsets, *, x_scales=None, weight_scales=None, dtype=None):
     """Rows of ``x`` [rows, in], sorted by expert, times their experts' weights [experts, out, in]: [rows, out].
 
@@ -122,10 +170,14 @@ def expert_linear_shard(x, weight, offsets, *, x_scales=None, weight_scales=None
     if x.dtype == torch.float8_e4m3fn:
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scales, weight_scales)):
             raise ValueError("products of rows in 8 bits have no gradient: call this under torch.no_grad(), or detach the scales")
-        return hip_ops.expert_linear(x, weight, offsets, x_scales, weight_scales, dtype)
+        res = None
+        if x_scales is not None and weight_scales is not None:
+            res = _lib.front().expert_linear_eight(x, weight, offsets, x_scales, weight_scales, torch.bfloat16 if dtype is None else dtype)
+        return res if res is not None else _ExpertLinearEight.apply(x, weight, offsets, x_scales, weight_scales, dtype)
     if x_scales is not None or weight_scales is not None or dtype not in (None, x.dtype):
         raise ValueError(f"expert_linear_shard: scales and another type of the result are for e4m3 rows, these are {x.dtype}")
-    return _ExpertLinear.apply(x, weight, offsets)
+    res = _lib.front().expert_linear_shard(x, weight, offsets, _lib.callback(_general_linear_backward))
+    return res if res is not None else _ExpertLinear.apply(x, weight, offsets)
 
 
 class DistributedExpertLinear(Module):

@@ -9,6 +9,7 @@ import numbers
 import numpy as np
 import torch
 
+from .. import _lib
 from .. import hip_ops
 from ..utilities.slicing import compute_subshape
 from ..utilities.slicing import range_index
@@ -71,6 +72,32 @@ class _RmsNormShard(torch.autograd.Function):
         return dx if need_x else None, dw, dx if need_r else None, None, None, None
 
 
+def _general_backward(dy, h, weight, dh, eps, want_input, want_weight):
+    """The adjoint for what its native form does not take."""
+    dx, dw = hip_ops.rms_norm_backward(dy, h, None if weight is None else weight.detach().reshape(-1), dh, eps, want_input, want_weight)
+    return dx, None if dw is None else dw.view(weight.shape)
+
+
+class _RmsNormEight(torch.autograd.Function):
+    """Rows in 8 bits, for a trace to hold the call and a tangent to be refused."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        _, h, codes, scales = hip_ops.rms_norm(x, None if weight is None else weight.detach().reshape(-1), residual, eps, eight_bit=True)
+        res = (codes, scales) if residual is None else (codes, scales, h)
+        ctx.mark_non_differentiable(*res)
+        return res
+
+
+class _QuantizeRows(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x):
+        res = hip_ops.quantize_rows(x)
+        ctx.mark_non_differentiable(*res)
+        return res
+
+
 def rms_norm_shard(x, weight=None, residual=None, *, eps=1e-6, eight_bit=False):
     """Rows (the last dimension) of ``x`` divided by ``sqrt(mean of their squares + eps)`` and multiplied by ``weight`` (its elements, of x's type, or None).
 
@@ -79,12 +106,16 @@ def rms_norm_shard(x, weight=None, residual=None, *, eps=1e-6, eight_bit=False):
     max(max |y| / 448, 2^-126)``: ``(codes, scales)`` or ``(codes, scales, h)``.  These have no gradient, so they are refused where one would be recorded.  Up to
     16384 columns.  The sum of a row's squares has to be a float32."""
     if not eight_bit:
+        res = _lib.front().rms_norm_shard(x, weight, residual, eps, _lib.callback(_general_backward))
+        if res is not None:
+            return res[0] if residual is None else res
         return _RmsNormShard.apply(x, weight, residual, float(eps), None, None)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise ValueError("rows in 8 bits have no gradient: call this under torch.no_grad(), or detach the operands")
-    _, h, codes, scales = hip_ops.rms_norm(x.detach(), None if weight is None else weight.detach().reshape(-1), None if residual is None else residual.detach(),
-                                           float(eps), eight_bit=True)
-    return (codes, scales) if residual is None else (codes, scales, h)
+    res = _lib.front().rms_norm_eight(x, weight, residual, eps)
+    if res is not None:
+        return res[:2] if residual is None else res
+    return _RmsNormEight.apply(x, weight, residual, float(eps))
 
 
 def quantize_rows(x):
@@ -92,7 +123,8 @@ def quantize_rows(x):
     A row with an infinity in it stands for no numbers.  No gradient."""
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("rows in 8 bits have no gradient: call this under torch.no_grad(), or detach the operand")
-    return hip_ops.quantize_rows(x.detach())
+    res = _lib.front().quantize_rows(x)
+    return res if res is not None else _QuantizeRows.apply(x)
 
 
 class DistributedRMSNorm(Module):
