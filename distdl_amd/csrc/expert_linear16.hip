@@ -51,7 +51,7 @@ template <ExpertTile TILE, bool F16>
 __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void expert_weights16(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int e, tm, tn, lo, hi;
-    find_matrix_tile(g, blockIdx.x, e, tm, tn);
+    if (!find_matrix_tile(g, blockIdx.x, e, tm, tn)) return;
     rows_of_expert(g, e, lo, hi);
     lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
     const int64_t m0 = static_cast<int64_t>(tm) * Shape<TILE>::bm, n0 = static_cast<int64_t>(tn) * Shape<TILE>::bn;
@@ -93,7 +93,7 @@ template <ExpertTile TILE, bool F16>
 int launch_weights(const char* who, ExpertArgs g, int dev, hipStream_t s) {
     static std::atomic<bool> reserved[kMaxDevices];
     g.tiles_m = static_cast<int>((g.n + Shape<TILE>::bm - 1) / Shape<TILE>::bm), g.tiles_n = static_cast<int>((g.k + Shape<TILE>::bn - 1) / Shape<TILE>::bn);
-    return launch<TILE>(who, expert_weights16<TILE, F16>, reserved, g, static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.experts, dev, s);
+    return launch<TILE>(who, expert_weights16<TILE, F16>, reserved, g, matrix_blocks(g), dev, s);
 }
 
 template <typename Fn>

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void expert_rows32(const ExpertArgs g) {
 __global__ __launch_bounds__(256) void expert_weights32(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int e, tm, tn, lo, hi;
-    find_matrix_tile(g, blockIdx.x, e, tm, tn);
+    if (!find_matrix_tile(g, blockIdx.x, e, tm, tn)) return;
     rows_of_expert(g, e, lo, hi);
     lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
     const int64_t m0 = static_cast<int64_t>(tm) * kEdge32, n0 = static_cast<int64_t>(tn) * kEdge32;
@@ -63,7 +63,7 @@ int run_expert_rows32(const char* who, bool transposed, ExpertArgs g, hipStream_
 
 int run_expert_weights32(const char* who, ExpertArgs g, hipStream_t s) {
     g.tiles_m = static_cast<int>((g.n + kEdge32 - 1) / kEdge32), g.tiles_n = static_cast<int>((g.k + kEdge32 - 1) / kEdge32);
-    return launch32(who, expert_weights32, g, static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.experts, s);
+    return launch32(who, expert_weights32, g, matrix_blocks(g), s);
 }
 
 }  // namespace ddl

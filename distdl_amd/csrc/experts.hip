@@ -3,8 +3,9 @@
 //
 // The plan is a counting sort by expert that keeps the slots' order within one, so that results do not depend on which wavefront
 // came first.  A wavefront walks over its part of the slots 64 at a time; the lanes with the same expert find each other by
-// one ballot for each bit of the number.  Up to kSlots slots it is one launch of one workgroup; more are counted by one launch and
-// placed by a second, whose workgroups add up the counts of those in front of them.
+// one ballot for each bit of the number.  Up to kAlone slots it is one launch of one workgroup; more are counted by one launch and
+// placed by a second, whose workgroups add up the counts of those in front of them: bound by latency, so a workgroup has 512 slots while
+// that makes no more than kMostParts of them.
 //
 // Everything that moves rows goes by tokens, not by sorted rows: a token's row is read once, however many experts it goes to
 // (sort; adjoint of combine), and what comes back is added up in registers in the order of the choices (combine; adjoint of the sort).  Bound by
@@ -17,14 +18,15 @@ namespace {
 
 constexpr int kWave = 64;
 constexpr int kPlanThreads = 512, kPlanWaves = kPlanThreads / kWave;
-constexpr int kSlots = 4096;            // of a workgroup of the plan
+constexpr int kAlone = 2048;            // slots up to which one workgroup makes the plan
+constexpr int kMostParts = 128;         // workgroups otherwise
 constexpr int kMaxHeld = 2047;          // experts; one bucket more for what is not held
 
 struct PlanArgs {
     const void* ids;
     int id_bytes;
     int64_t ld_ids, low;
-    int slots, held, bits;              // bits: of bucket numbers 0 .. held
+    int slots, part, held, bits;        // part: slots of a workgroup; bits: of bucket numbers 0 .. held
     FastDiv chosen;
     int32_t *place, *offsets, *counts;  // counts: [workgroups, held + 1]
 };
@@ -56,7 +58,7 @@ __device__ inline void count_slots(const PlanArgs& a, int first, int last, int p
     const int buckets = a.held + 1, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     for (int i = threadIdx.x; i < kPlanWaves * buckets; i += kPlanThreads) lds[i] = 0;
     __syncthreads();
-    const int from = first + wave * per_wave, to = min(from + per_wave, last);
+    const int from = min(wave * per_wave, last - first) + first, to = min(last - from, per_wave) + from;
     int* const mine = lds + wave * buckets;   // of this wavefront alone: its own LDS accesses complete in order
     for (int s = from + lane; s - lane < to; s += kWave) {
         const bool on = s < to;
@@ -69,8 +71,8 @@ __device__ inline void count_slots(const PlanArgs& a, int first, int last, int p
 
 __global__ __launch_bounds__(kPlanThreads) void expert_count(const PlanArgs a) {
     extern __shared__ int lds[];
-    const int buckets = a.held + 1, first = static_cast<int>(blockIdx.x) * kSlots, last = min(first + kSlots, a.slots);
-    count_slots(a, first, last, kSlots / kPlanWaves, lds);
+    const int buckets = a.held + 1, first = static_cast<int>(blockIdx.x) * a.part, last = min(a.slots - first, a.part) + first;
+    count_slots(a, first, last, a.part / kPlanWaves, lds);
     for (int b = threadIdx.x; b < buckets; b += kPlanThreads) {
         int n = 0;
 #pragma unroll
@@ -85,8 +87,8 @@ __global__ __launch_bounds__(kPlanThreads) void expert_place(const PlanArgs a) {
     const int buckets = a.held + 1, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     int* const base = lds + kPlanWaves * buckets;
     int* const sums = base + buckets;
-    const int first = static_cast<int>(blockIdx.x) * kSlots, last = min(first + kSlots, a.slots);
-    const int per_wave = gridDim.x == 1 ? ((a.slots + kPlanThreads - 1) / kPlanThreads) * kWave : kSlots / kPlanWaves;
+    const int first = static_cast<int>(blockIdx.x) * a.part, last = min(a.slots - first, a.part) + first;
+    const int per_wave = a.part / kPlanWaves;
     count_slots(a, first, last, per_wave, lds);
     // Slots of the buckets in front of each one: a running sum over the buckets, kPlanThreads at a time.
     int carry = 0;
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(kPlanThreads) void expert_place(const PlanArgs a) {
         }
     }
     __syncthreads();
-    const int from = first + wave * per_wave, to = min(from + per_wave, last);
+    const int from = min(wave * per_wave, last - first) + first, to = min(last - from, per_wave) + from;
     int* const next = lds + wave * buckets;
     for (int s = from + lane; s - lane < to; s += kWave) {
         const bool on = s < to;
@@ -410,8 +412,8 @@ int lay_out(const char* who, RowArgs& a, int per, bool whole, int64_t& blocks) {
 int check_tokens(const char* who, int64_t tokens, int64_t chosen, int64_t cols) {
     if (tokens < 0 || chosen < 0 || cols < 1)
         return fail(DDL_E_ARG, "%s: %lld tokens of %lld choices, rows of %lld columns", who, static_cast<long long>(tokens), static_cast<long long>(chosen), static_cast<long long>(cols));
-    if (cols > 0x3FFFFFFF || chosen > 0x7FFFFFFF || (chosen && tokens > 0x7FFFFFFF / chosen) || tokens > 0x7FFFFFFF)
-        return fail(DDL_E_UNSUPP, "%s: 2^31 slots or 2^30 columns", who);
+    if (cols > 0x3FFFFFFF || chosen > 0x7FFFFFFF || (chosen && tokens > 0x40000000 / chosen) || tokens > 0x40000000)
+        return fail(DDL_E_UNSUPP, "%s: more than 2^30 slots or columns", who);
     return 0;
 }
 
@@ -433,6 +435,12 @@ int with_added(int dtype, int64_t cols, Fn&& fn) {
     return rc;
 }
 
+// Slots of a workgroup of the plan: a whole number of wavefronts for each of its own.
+int64_t part_of(int64_t slots) {
+    const int64_t least = (slots + kPlanThreads - 1) / kPlanThreads, rest = (least + kMostParts - 1) / kMostParts;
+    return kPlanThreads * (slots <= kAlone ? (least > 0 ? least : 1) : rest);
+}
+
 int check_dtype(const char* who, int dtype) {
     return dtype == DDL_DT_F32 || dtype == DDL_DT_BF16 || dtype == DDL_DT_F16 ? 0 : fail(DDL_E_ARG, "%s: dtype %d", who, dtype);
 }
@@ -443,8 +451,9 @@ int check_dtype(const char* who, int dtype) {
 extern "C" {
 
 int64_t ddl_expert_plan_workspace(int64_t slots, int64_t held_experts) {
-    if (slots <= ddl::kSlots || slots > 0x7FFFFFFF || held_experts < 0 || held_experts > ddl::kMaxHeld) return 0;
-    return (slots + ddl::kSlots - 1) / ddl::kSlots * (held_experts + 1);
+    if (slots <= ddl::kAlone || slots > 0x40000000 || held_experts < 0 || held_experts > ddl::kMaxHeld) return 0;
+    const int64_t part = ddl::part_of(slots);
+    return (slots + part - 1) / part * (held_experts + 1);
 }
 
 int ddl_expert_plan(const void* ids, int id_bytes, int64_t tokens, int64_t chosen, int64_t ld_ids, int64_t low, int64_t high, int32_t* place, int32_t* offsets,
@@ -463,7 +472,8 @@ int ddl_expert_plan(const void* ids, int id_bytes, int64_t tokens, int64_t chose
     a.chosen = make_fastdiv(static_cast<uint32_t>(chosen ? chosen : 1)), a.place = place, a.offsets = offsets, a.counts = workspace;
     while ((1 << a.bits) <= a.held) ++a.bits;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t blocks = slots ? static_cast<uint32_t>((slots + kSlots - 1) / kSlots) : 1;
+    a.part = static_cast<int>(part_of(slots));
+    const uint32_t blocks = slots ? static_cast<uint32_t>((slots + a.part - 1) / a.part) : 1;
     const int count_bytes = kPlanWaves * (a.held + 1) * 4, lds_bytes = count_bytes + (a.held + 1 + kPlanWaves) * 4;
     static_assert((kPlanWaves + 1) * (kMaxHeld + 1) * 4 + kPlanWaves * 4 <= 160 * 1024, "the counters do not fit");
     if (lds_bytes > 64 * 1024) {   // what a launch gets without asking

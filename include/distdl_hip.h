@@ -782,8 +782,8 @@ int ddl_rms_norm_backward(const void* dy, const void* h, const void* dh,
  *                             expert, in the order of the slots within one; slots
  *                             that are not held come behind all that are
  *   offsets [high - low + 1]  expert e's rows are offsets[e - low] to offsets[e - low + 1]
- * `workspace`: ddl_expert_plan_workspace(...) int32.  Up to 2047 experts are held here, fewer than
- * 2^31 slots (DDL_E_UNSUPP). */
+ * `workspace`: ddl_expert_plan_workspace(...) int32.  Up to 2047 experts are held here, up to 2^30
+ * slots (DDL_E_UNSUPP). */
 int64_t ddl_expert_plan_workspace(int64_t slots, int64_t held_experts);
 int ddl_expert_plan(const void* ids, int id_bytes, int64_t tokens,
                     int64_t chosen, int64_t ld_ids, int64_t low, int64_t high,

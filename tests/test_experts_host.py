@@ -52,8 +52,8 @@ PLAN = dict(ids=16, id_bytes=8, tokens=4, chosen=2, ld=2, low=0, high=8, place=1
 
 @pytest.mark.parametrize("change,code,what", [
     (dict(id_bytes=2), -1, "2 bytes"), (dict(tokens=-1), -1, "tokens"), (dict(high=-1), -1, "experts"), (dict(low=-1), -1, "experts"), (dict(high=2048), -5, "2047"),
-    (dict(tokens=1 << 30), -5, "2^31"), (dict(offsets=None), -1, "null"), (dict(ids=None), -1, "null"), (dict(place=None), -1, "null"), (dict(tokens=4000), -1, "workspace"),
-    (dict(tokens=4000, work=16, elems=17), -1, "18 are needed"),
+    (dict(tokens=1 << 30), -5, "2^30"), (dict(offsets=None), -1, "null"), (dict(ids=None), -1, "null"), (dict(place=None), -1, "null"), (dict(tokens=4000), -1, "workspace"),
+    (dict(tokens=4000, work=16, elems=143), -1, "144 are needed"),
 ])
 def test_plan_refuses(change, code, what):
     refused("ddl_expert_plan", PLAN, change, code, what)
@@ -66,7 +66,7 @@ COMBINE_BACKWARD = dict(dout=16, y=16, dtype=BF16, tokens=4, chosen=2, cols=64, 
 
 @pytest.mark.parametrize("name,defaults,change,code,what", [
     ("ddl_expert_sort", SORT, dict(bytes=8), -1, "8 bytes"), ("ddl_expert_sort", SORT, dict(cols=0), -1, "columns"), ("ddl_expert_sort", SORT, dict(ld=63), -1, "pitch"),
-    ("ddl_expert_sort", SORT, dict(place=None), -1, "null"), ("ddl_expert_sort", SORT, dict(scales=16), -1, "null"), ("ddl_expert_sort", SORT, dict(tokens=1 << 31), -5, "2^31"),
+    ("ddl_expert_sort", SORT, dict(place=None), -1, "null"), ("ddl_expert_sort", SORT, dict(scales=16), -1, "null"), ("ddl_expert_sort", SORT, dict(tokens=1 << 31), -5, "2^30"),
     ("ddl_expert_sort", SORT, dict(tokens=1 << 28, cols=1 << 20, ld=1 << 20), -5, "wavefronts"),
     ("ddl_expert_combine", COMBINE, dict(dtype=F64), -1, "dtype"), ("ddl_expert_combine", COMBINE, dict(ld=60), -1, "pitch"), ("ddl_expert_combine", COMBINE, dict(y=None), -1, "null"),
     ("ddl_expert_combine", COMBINE, dict(held=None), -1, "null"), ("ddl_expert_combine", COMBINE, dict(chosen=-1), -1, "choices"),
@@ -106,7 +106,7 @@ def test_nothing_is_no_launch():
     assert call("ddl_expert_linear_backward", LINEAR_BACKWARD, dict(rows=0, dw=None)) == 0
 
 
-@pytest.mark.parametrize("extents", [(-1, 8), (1 << 40, 8), (5000, -1), (5000, 2048), (4096, 8)])
+@pytest.mark.parametrize("extents", [(-1, 8), (1 << 40, 8), (5000, -1), (5000, 2048), (2048, 8)])
 def test_plans_without_a_workspace(extents):
     assert _lib.load().ddl_expert_plan_workspace(*extents) == 0
 
