@@ -215,6 +215,22 @@ ExpertTile best_for_weights(bool aligned, int64_t rows, int64_t experts, int64_t
     return best;
 }
 
+// fp32: is a product quicker on 128 x 128 tiles of the bf16 matrix cores than on 64 x 64 ones of the fp32 cores?  Each CU's tiles one after the other, a start and
+// some time for each 32 of the reduction; linear_f32_split.hip's own fit for the first.  ([1024, 8192] by 3584: 545 us on the latter, 468 on the former.)
+bool split_pays(double large, double small, int64_t depth, int cus) {
+    const double steps = ceil(depth / 32.0), fill = large < cus ? large / cus : 1;
+    const double split = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), plain = 5 + (small < cus ? 1 : small / cus) * (1.5 + steps * 0.58);
+    return split < plain;
+}
+int rows32(const char* who, bool transposed, const ExpertArgs& g, int cus, hipStream_t s) {
+    const double large = row_tiles(g.rows, g.experts, 128) * static_cast<double>((g.n + 127) / 128), small = row_tiles(g.rows, g.experts, 64) * static_cast<double>((g.n + 63) / 64);
+    return split_pays(large, small, g.k, cus) ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, transposed, g, s);
+}
+int weights32(const char* who, const ExpertArgs& g, int cus, hipStream_t s) {
+    const double large = static_cast<double>(g.experts) * ((g.n + 127) / 128) * ((g.k + 127) / 128), small = static_cast<double>(g.experts) * ((g.n + 63) / 64) * ((g.k + 63) / 64);
+    return split_pays(large, small, g.rows / g.experts, cus) ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, g, s);
+}
+
 // expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again.
 double stream_us(int64_t rows, int64_t experts, int64_t cols, int64_t depth) {
     const double each = static_cast<double>(rows) / experts, used = static_cast<double>(rows < experts ? rows : experts);
@@ -253,7 +269,7 @@ int ddl_expert_linear(const void* x, const void* w, int dtype, const int32_t* of
     g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype;
     g.n = n, g.k = k, g.lda = rows > 1 ? ld_x : k, g.ldw = k, g.w_stride = n * k, g.ldy = n;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == DDL_DT_F32) return run_expert_rows32(who, false, g, s);
+    if (dtype == DDL_DT_F32) return rows32(who, false, g, cus, s);
     const bool aligned = aligned_to(x, 16) && aligned_to(w, 16) && g.lda % 8 == 0 && k % 8 == 0;
     double us;
     const ExpertTile tile = best_for_rows(kCosts16, aligned, rows, experts, n, 2 * k, cus, &us);
@@ -313,7 +329,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
         d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
         int rc;
         if (dtype == DDL_DT_F32) {
-            rc = run_expert_rows32(who, true, d, s);
+            rc = rows32(who, true, d, cus, s);
         } else {
             const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;
             double us;
@@ -324,7 +340,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
     if (dw && experts) {
         ExpertArgs d = g;
         d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
-        if (dtype == DDL_DT_F32) return run_expert_weights32(who, d, s);
+        if (dtype == DDL_DT_F32) return weights32(who, d, cus, s);
         const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
         return run_expert_weights16(who, best_for_weights(aligned, rows, experts, n, k, cus), f16, d, dev, s);
     }

@@ -22,9 +22,12 @@ struct ExpertArgs {
 enum class ExpertTile { kAny64, kAny128, kLow, kLarge };
 int run_expert_rows16(const char* who, ExpertTile tile, bool f16, bool transposed, ExpertArgs g, int dev, hipStream_t s);
 int run_expert_weights16(const char* who, ExpertTile tile, bool f16, ExpertArgs g, int dev, hipStream_t s);
-// Of expert_linear32.hip.
+// Of expert_linear32.hip: tiles of 64 x 64.
 int run_expert_rows32(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32(const char* who, ExpertArgs g, hipStream_t s);
+// Of expert_linear32_split.hip: tiles of 128 x 128.
+int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
+int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
 // Of expert_linear8.hip: tiles of 128 (low) or 256 rows by 256 columns.
 int run_expert_rows8(const char* who, bool low, const ExpertArgs& g, int dev, hipStream_t s);
 

@@ -40,6 +40,8 @@ CASES = [
     ([200, 0, 57, 130], 11, 320, 264), ([300, 513], 0, 136, 264), ([700, 0, 900], 5, 512, 768), ([2100, 1500], 0, 256, 512), ([5] * 70, 1, 64, 32),
     # what fills the chip with large tiles: results, gradients of the rows, of the weights
     ([3001, 0, 1200], 7, 72, 8000), ([3001, 0, 1200], 7, 8000, 72), ([9, 0, 130, 2, 64, 1, 70, 200], 3, 2056, 2040),
+    # fp32 on the bf16 matrix cores' tiles
+    ([513, 0, 600, 490], 3, 1100, 1000), ([400, 0, 700], 0, 2050, 2049),
     # rows that are no multiple of 16 bytes
     ([5, 0, 9], 2, 9, 11), ([100, 37], 3, 77, 65), ([260, 300], 0, 513, 331), ([1, 1], 0, 1001, 15)]
 
