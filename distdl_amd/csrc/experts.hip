@@ -156,6 +156,7 @@ __global__ __launch_bounds__(kPlanThreads) void expert_place(const PlanArgs a) {
 
 // -------------------------------------------------------------- rows --
 
+// Whatever a plan's tensors hold, only rows 0 .. slots - 1 are touched: places from `held` on have no row in the sums, places outside the slots none at all.
 struct RowArgs {
     const void *in, *y;                 // by tokens; by places
     void *out, *dy;
@@ -163,6 +164,7 @@ struct RowArgs {
     float *out_scales, *dweights;
     const int32_t *place, *held;
     int64_t ld_in, ld_y, tokens;
+    uint32_t slots;
     int chosen, cols;                   // cols in elements of the kernel's type
     int vectors;                        // of a row
     int lanes_log2;                     // lanes of a row's group: 1 to 64
@@ -293,6 +295,7 @@ __global__ __launch_bounds__(kRowThreads) void sort_rows(const RowArgs a) {
     const float scale = a.scales && task.first == 0 ? a.scales[task.token] : 0.f;
     for (int j = 0; j < a.chosen; ++j) {
         const int to = a.place[task.token * a.chosen + j];
+        if (static_cast<uint32_t>(to) >= a.slots) continue;
         const bool here = to < held;
         T* const out = static_cast<T*>(a.out) + static_cast<int64_t>(to) * a.cols;
 #pragma unroll
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_rows(const RowArgs a) {
     for (int j = 0; j < a.chosen; ++j) {
         const int64_t slot = task.token * a.chosen + j;
         const int from = a.place[slot];
-        if (from >= held) continue;
+        if (from >= held || static_cast<uint32_t>(from) >= a.slots) continue;
         const float weight = a.weights ? a.weights[slot] : 1.f;
         const T* const y = static_cast<const T*>(a.y) + from * a.ld_y;
         Chunk<T, VEC> c[kAtOnce];
@@ -354,10 +357,10 @@ __global__ __launch_bounds__(kRowThreads) void combine_rows_backward(const RowAr
     for (int j = 0; j < a.chosen; ++j) {
         const int64_t slot = token * a.chosen + j;
         const int at_row = a.place[slot];
-        const bool here = at_row < held;
+        const bool row = static_cast<uint32_t>(at_row) < a.slots, here = row && at_row < held;
         const float weight = here ? a.weights[slot] : 0.f;
         const T* const y = static_cast<const T*>(a.y) + (a.dweights && here ? at_row * a.ld_y : 0);
-        T* const dy = static_cast<T*>(a.dy) + static_cast<int64_t>(at_row) * a.cols;
+        T* const dy = static_cast<T*>(a.dy) + (row ? static_cast<int64_t>(at_row) * a.cols : 0);
         float dot = 0.f;
         for (int c0 = task.first; task.on && c0 < a.vectors; c0 += kAtOnce * task.lanes) {
             Chunk<T, VEC> g[kAtOnce], v[kAtOnce];
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_rows_backward(const RowAr
 #pragma unroll
                     for (int i = 0; i < N; ++i) dot += i >= twice ? f[i] * e[i] : 0.f;
                 }
-                if (a.dy) {
+                if (a.dy && row) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) f[i] = here ? f[i] * weight : 0.f;
                     store_chunk<T, VEC>(dy + start_of<N>(at, a.cols), chunk_of<VEC>(f, static_cast<T*>(nullptr)));
@@ -498,7 +501,7 @@ int ddl_expert_sort(const void* x, int elem_bytes, int64_t tokens, int64_t chose
     if (tokens > 1 && ld_x < cols) return fail(DDL_E_ARG, "ddl_expert_sort: pitch below %lld columns", static_cast<long long>(cols));
     RowArgs a{};
     a.in = x, a.out = out, a.scales = scales, a.out_scales = out_scales, a.place = place, a.held = held, a.ld_in = ld_x, a.tokens = tokens;
-    a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
+    a.slots = static_cast<uint32_t>(tokens * chosen), a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
     return with_moved(elem_bytes, cols, [&](auto* e, auto vec) {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr bool VEC = decltype(vec)::value;
@@ -519,7 +522,7 @@ int ddl_expert_combine(const void* y, int dtype, int64_t tokens, int64_t chosen,
     if (tokens * chosen > 1 && ld_y < cols) return fail(DDL_E_ARG, "ddl_expert_combine: pitch below %lld columns", static_cast<long long>(cols));
     RowArgs a{};
     a.y = y, a.out = out, a.weights = weights, a.place = place, a.held = held, a.ld_y = ld_y, a.tokens = tokens;
-    a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
+    a.slots = static_cast<uint32_t>(tokens * chosen), a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
     return with_added(dtype, cols, [&](auto* e, auto vec) {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr bool VEC = decltype(vec)::value;
@@ -541,7 +544,7 @@ int ddl_expert_combine_backward(const void* dout, const void* y, int dtype, int6
         return fail(DDL_E_ARG, "ddl_expert_combine_backward: pitch below %lld columns", static_cast<long long>(cols));
     RowArgs a{};
     a.in = dout, a.y = y, a.dy = dy, a.weights = weights, a.dweights = dweights, a.place = place, a.held = held, a.ld_in = ld_dout, a.ld_y = ld_y;
-    a.tokens = tokens, a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
+    a.tokens = tokens, a.slots = static_cast<uint32_t>(tokens * chosen), a.chosen = static_cast<int>(chosen), a.cols = static_cast<int>(cols);
     return with_added(dtype, cols, [&](auto* e, auto vec) {
         typedef std::remove_pointer_t<decltype(e)> T;
         constexpr bool VEC = decltype(vec)::value;
