@@ -266,7 +266,7 @@ int ddl_expert_linear(const void* x, const void* w, int dtype, const int32_t* of
     int dev = 0;
     const int cus = compute_units(dev);
     ExpertArgs g{};
-    g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype;
+    g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
     g.n = n, g.k = k, g.lda = rows > 1 ? ld_x : k, g.ldw = k, g.w_stride = n * k, g.ldy = n;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == DDL_DT_F32) return rows32(who, false, g, cus, s);
@@ -297,7 +297,8 @@ int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w, 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     int dev = 0;
     double us;
-    const ExpertTile tile = best_for_rows(kCosts8, true, rows, experts, n, k, compute_units(dev), &us);
+    g.cus = compute_units(dev);
+    const ExpertTile tile = best_for_rows(kCosts8, true, rows, experts, n, k, g.cus, &us);
     if (!experts || stream_us(rows, experts, n, k) < us) return launch_stream<kE4m3>(who, g, s);
     return run_expert_rows8(who, tile != ExpertTile::kLarge, g, dev, s);
 }
@@ -323,7 +324,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f16 = dtype == DDL_DT_F16;
     ExpertArgs g{};
-    g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype;
+    g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
     if (dx && rows) {   // rows of n features by w read along its k columns
         ExpertArgs d = g;
         d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;

@@ -31,19 +31,20 @@ __device__ __forceinline__ void product_tile(const PartOf<uint16_t>& p, char* ld
 template <ExpertTile TILE, bool F16, bool WT>
 __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void expert_rows16(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const ExpertTask t = find_tile(g, Shape<TILE>::bm, blockIdx.x);
+    const ExpertTask t = find_tile<TILE == ExpertTile::kLarge>(g, Shape<TILE>::bm, blockIdx.x);
     if (t.expert < 0) return;
     const int64_t n0 = static_cast<int64_t>(t.tn) * Shape<TILE>::bn;
     uint16_t* const y = static_cast<uint16_t*>(g.y) + t.row * g.ldy + n0;
     if (t.expert == g.experts) {
-        zero_block(y, g.ldy, 0, min(t.rows, Shape<TILE>::bm), 0, static_cast<int>(min(g.n - n0, static_cast<int64_t>(Shape<TILE>::bn))));
+        zero_block(y, g.ldy, 0, min(t.rows, t.half ? Shape<TILE>::bm / 2 : Shape<TILE>::bm), 0, static_cast<int>(min(g.n - n0, static_cast<int64_t>(Shape<TILE>::bn))));
         return;
     }
     PartOf<uint16_t> p{};
     p.x = static_cast<const uint16_t*>(g.a) + t.row * g.lda;
     p.w = static_cast<const uint16_t*>(g.w) + t.expert * g.w_stride + (WT ? n0 : n0 * g.ldw);
     p.y = y, p.M = t.rows, p.N = g.n - n0, p.K = g.k, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.ldy, p.tiles_m = p.tiles_n = 1;
-    product_tile<TILE, F16, false, WT>(p, lds);
+    if (TILE == ExpertTile::kLarge && t.half) product_tile<ExpertTile::kLow, F16, false, WT>(p, lds);
+    else product_tile<TILE, F16, false, WT>(p, lds);
 }
 
 // a: dy [rows, n], w: x [rows, k]; y: dw, n x k for each expert.
@@ -86,7 +87,8 @@ int launch_rows(const char* who, ExpertArgs g, int dev, hipStream_t s) {
     g.tiles_n = static_cast<int>((g.n + Shape<TILE>::bn - 1) / Shape<TILE>::bn);
     // every expert, and the rows behind them, can end inside a tile
     const int64_t tiles_m = (g.rows + Shape<TILE>::bm - 1) / Shape<TILE>::bm + g.experts;
-    return launch<TILE>(who, expert_rows16<TILE, F16, WT>, reserved, g, tiles_m * g.tiles_n, dev, s);
+    const int64_t halves = TILE == ExpertTile::kLarge ? g.cus : 0;   // workgroups for those of the last round
+    return launch<TILE>(who, expert_rows16<TILE, F16, WT>, reserved, g, tiles_m * g.tiles_n + halves, dev, s);
 }
 
 template <ExpertTile TILE, bool F16>

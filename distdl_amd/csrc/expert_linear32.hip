@@ -11,7 +11,7 @@ constexpr int kEdge32 = 64, kStages32 = 4, kLds32 = kStages32 * 2 * kEdge32 * kR
 template <bool WT>
 __global__ __launch_bounds__(256) void expert_rows32(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const ExpertTask t = find_tile(g, kEdge32, blockIdx.x);
+    const ExpertTask t = find_tile<false>(g, kEdge32, blockIdx.x);
     if (t.expert < 0) return;
     const int64_t n0 = static_cast<int64_t>(t.tn) * kEdge32;
     float* const y = static_cast<float*>(g.y) + t.row * g.ldy + n0;

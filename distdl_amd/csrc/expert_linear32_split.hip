@@ -9,7 +9,7 @@ namespace {
 template <bool WT>
 __global__ __launch_bounds__(kBlock, 2) void expert_rows32_split(const ExpertArgs g) {
     __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
-    const ExpertTask t = find_tile(g, kTile, blockIdx.x);
+    const ExpertTask t = find_tile<false>(g, kTile, blockIdx.x);
     if (t.expert < 0) return;
     const int64_t n0 = static_cast<int64_t>(t.tn) * kTile;
     float* const y = static_cast<float*>(g.y) + t.row * g.ldy + n0;

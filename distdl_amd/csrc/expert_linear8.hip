@@ -262,7 +262,7 @@ template <int TM>
 __global__ __launch_bounds__(kThreads8, 2) void expert_rows8(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int BM = 32 * TM;
-    const ExpertTask t = find_tile(g, BM, blockIdx.x);
+    const ExpertTask t = find_tile<false>(g, BM, blockIdx.x);
     if (t.expert < 0) return;
     const int64_t n0 = static_cast<int64_t>(t.tn) * kColumns;
     const int cols = static_cast<int>(min(g.n - n0, static_cast<int64_t>(kColumns))), rows = min(t.rows, BM);
