@@ -173,7 +173,7 @@ const TileCost kCosts16[4] = {{ExpertTile::kAny64, 64, 64, 4, 1.3, 0.20, 0.72},
                               {ExpertTile::kAny128, 128, 128, 2, 3, 0.55, 0.65},
                               {ExpertTile::kLow, 128, 256, 1, 4, 0.47, 0.41},
                               {ExpertTile::kLarge, 256, 256, 1, 7, 0.95, 0.45}};
-const TileCost kCosts8[2] = {{ExpertTile::kLow, 128, 256, 1, 4, 0.60, 0.20}, {ExpertTile::kLarge, 256, 256, 1, 7, 0.95, 0.47}};
+const TileCost kCosts8[3] = {{ExpertTile::kAny64, 64, 64, 2, 3, 0.30, 0.22}, {ExpertTile::kLow, 128, 256, 1, 6, 0.58, 0.25}, {ExpertTile::kLarge, 256, 256, 1, 9, 0.98, 0.50}};
 
 double tiles_us(const TileCost& c, double tiles, double ktiles, int cus) {
     const double rounds = tiles / (static_cast<double>(c.side) * cus);
@@ -231,8 +231,9 @@ int weights32(const char* who, const ExpertArgs& g, int cus, hipStream_t s) {
     return split_pays(large, small, g.rows / g.experts, cus) ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, g, s);
 }
 
-// expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again.
+// expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again; not for more rows than it has in registers.
 double stream_us(int64_t rows, int64_t experts, int64_t cols, int64_t depth) {
+    if (rows > 64 * experts) return 1e30;
     const double each = static_cast<double>(rows) / experts, used = static_cast<double>(rows < experts ? rows : experts);
     return 2.5 + used * cols * depth / 5.5e6 * (1 + 0.05 * (each > 4 ? each - 4 : 0));
 }
@@ -300,7 +301,7 @@ int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w, 
     g.cus = compute_units(dev);
     const ExpertTile tile = best_for_rows(kCosts8, true, rows, experts, n, k, g.cus, &us);
     if (!experts || stream_us(rows, experts, n, k) < us) return launch_stream<kE4m3>(who, g, s);
-    return run_expert_rows8(who, tile != ExpertTile::kLarge, g, dev, s);
+    return run_expert_rows8(who, tile, g, dev, s);
 }
 
 int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int dtype, const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k,

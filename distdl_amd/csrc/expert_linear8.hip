@@ -6,7 +6,7 @@
 // pieces of x come two ahead of their products, four at a time for each of them, and those of w one k-tile ahead, during the last two pieces.
 // In front of those two is the k-tile's barrier: every wavefront has read what it needs of this tile, and the next one has landed.
 #include "expert_parts.h"
-#include "gemm16_elements.h"
+#include "gemm16_parts.h"
 #include <type_traits>
 
 namespace ddl {
@@ -29,6 +29,18 @@ struct Tile8 {
     int M, N, out_dtype;
     int64_t K, ldx, ldw, ldy;
 };
+
+// Four consecutive columns of a row.
+__device__ inline void store_floats(float* row, int n, int N, const float* v) {
+    if (n + 4 <= N) {
+        typedef floatx4 any __attribute__((aligned(4)));
+        *reinterpret_cast<any*>(row + n) = floatx4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < N) row[n + e] = v[e];
+    }
+}
 
 template <int TM>
 __device__ __forceinline__ void tile8(const Tile8& p, char* lds) {
@@ -204,15 +216,7 @@ __device__ __forceinline__ void tile8(const Tile8& p, char* lds) {
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[a][b][e] * xs[b] * ws[e];
-                if (m >= p.M) continue;
-                if (n + 4 <= p.N) {
-                    typedef floatx4 any __attribute__((aligned(4)));
-                    *reinterpret_cast<any*>(y + m * p.ldy + n) = floatx4{v[0], v[1], v[2], v[3]};
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < p.N) y[m * p.ldy + n + e] = v[e];
-                }
+                if (m < p.M) store_floats(y + m * p.ldy, n, p.N, v);
             }
         }
         return;
@@ -258,26 +262,125 @@ __device__ __forceinline__ void tile8(const Tile8& p, char* lds) {
     }
 }
 
-template <int TM>
-__global__ __launch_bounds__(kThreads8, 2) void expert_rows8(const ExpertArgs g) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 32 * TM;
-    const ExpertTask t = find_tile<false>(g, BM, blockIdx.x);
-    if (t.expert < 0) return;
-    const int64_t n0 = static_cast<int64_t>(t.tn) * kColumns;
-    const int cols = static_cast<int>(min(g.n - n0, static_cast<int64_t>(kColumns))), rows = min(t.rows, BM);
+// Tiles of 64 x 64 for products that do not fill the chip with larger ones: four wavefronts with 32 x 32 each, k-tiles through a ring of four, three of them
+// in flight, one barrier a k-tile.  Bound by a k-tile's latencies.  ([8 x 16, 8192] by 3584: 38 us, tiles of 128 x 256 47, wavefronts on parts of the
+// reduction 58; [16 x 128, 4096] by 512: 20, 28 and 41.)
+constexpr int kSmall = 64, kSmallThreads = 256, kSmallRing = 4, kSmallStage = 2 * kSmall * kRowBytes;
+
+__device__ __forceinline__ void small_tile8(const Tile8& p, char* lds) {
+    constexpr int J = kSmall / 8 / 4;   // request instructions of a wavefront for either operand
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, kg = lane >> 4;
+    const u32x4 buf_w = raw_buffer(p.w), buf_x = raw_buffer(p.x);
+    int off_w[J], off_x[J];
+    auto lane_offset = [&](int j, int rows, int64_t ld) -> int {
+        const int row = (J * wave + j) * 8 + (lane >> 3);
+        return static_cast<int>(static_cast<int64_t>(row < rows ? row : rows - 1) * ld) + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    };
+#pragma unroll
+    for (int j = 0; j < J; ++j) off_w[j] = lane_offset(j, p.N, p.ldw), off_x[j] = lane_offset(j, p.M, p.ldx);
+    const int ktiles = static_cast<int>((p.K + kRowBytes - 1) / kRowBytes), full_tiles = static_cast<int>(p.K / kRowBytes);
+    auto through = [&](const uint8_t* base, int off, int j, int t, char* to) {   // of the k-tile that K ends in, zeros behind its end
+        const int row = (J * wave + j) * 8 + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (static_cast<int64_t>(t) * kRowBytes + chunk * 16 < p.K) v = *reinterpret_cast<const uint4*>(base + off + static_cast<int64_t>(t) * kRowBytes);
+        *reinterpret_cast<uint4*>(to + (J * wave + j) * 1024 + lane * 16) = v;
+    };
+    auto request = [&](int t) {
+        char* const w = lds + t % kSmallRing * kSmallStage;
+        char* const x = w + kSmall * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (t < full_tiles) {
+                dma16(buf_w, off_w[j], t * kRowBytes, w + (J * wave + j) * 1024);
+                dma16(buf_x, off_x[j], t * kRowBytes, x + (J * wave + j) * 1024);
+            } else {
+                through(p.w, off_w[j], j, t, w);
+                through(p.x, off_x[j], j, t, x);
+            }
+        }
+    };
+    const int sw = (l16 >> 1) & 7, at0 = l16 * kRowBytes + (((2 * kg) ^ sw) << 4), at1 = l16 * kRowBytes + (((2 * kg + 1) ^ sw) << 4);
+    auto read = [&](const char* tile, int row) -> intx8 {
+        intx8 v;
+        const uint4 a = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at0), b = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return v;
+    };
+    const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+    floatx4 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < kSmallRing - 1; ++t)
+        if (t < ktiles) request(t);
+#pragma unroll 1
+    for (int t = 0; t < ktiles; ++t) {
+        // Tile t has landed (the two behind it may be in flight), and this wavefront has read tile t - 1.
+        if (t + kSmallRing - 2 < full_tiles) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(2 * J * (kSmallRing - 2)));
+        else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + kSmallRing - 1 < ktiles) request(t + kSmallRing - 1);
+        const char* const w = lds + t % kSmallRing * kSmallStage + wn * kRowBytes;
+        const char* const x = lds + t % kSmallRing * kSmallStage + (kSmall + wm) * kRowBytes;
+        const intx8 fw[2] = {read(w, 0), read(w, 16)}, fx[2] = {read(x, 0), read(x, 16)};
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[a], fx[b], acc[a][b], 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);   // scales of one
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int m = wm + b * 16 + l16;
+        if (m >= p.M) continue;
+        const float xs = p.x_scales[m];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const int n = wn + a * 16 + 4 * kg;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[a][b][e] * xs * p.w_scales[n + e < p.N ? n + e : p.N - 1];
+            if (p.out_dtype == DDL_DT_F32) store_floats(static_cast<float*>(p.y) + m * p.ldy, n, p.N, v);
+            else if (p.out_dtype == DDL_DT_F16) store_four<true>(static_cast<uint16_t*>(p.y), p.ldy, m, n, p.N, v);
+            else store_four<false>(static_cast<uint16_t*>(p.y), p.ldy, m, n, p.N, v);
+        }
+    }
+}
+
+// The tile of workgroup `id`, if it has one to compute (rows of no expert get their zeros here).
+template <int BM, int BN>
+__device__ inline bool tile_of(const ExpertArgs& g, int id, Tile8& p) {
+    const ExpertTask t = find_tile<false>(g, BM, id);
+    if (t.expert < 0) return false;
+    const int64_t n0 = static_cast<int64_t>(t.tn) * BN;
+    const int cols = static_cast<int>(min(g.n - n0, static_cast<int64_t>(BN))), rows = min(t.rows, BM);
     const int64_t at = t.row * g.ldy + n0;
     if (t.expert == g.experts) {
         if (g.out_dtype == DDL_DT_F32) zero_block(static_cast<float*>(g.y) + at, g.ldy, 0, rows, 0, cols);
         else zero_block(static_cast<uint16_t*>(g.y) + at, g.ldy, 0, rows, 0, cols);
-        return;
+        return false;
     }
-    Tile8 p;
     p.x = static_cast<const uint8_t*>(g.a) + t.row * g.lda, p.w = static_cast<const uint8_t*>(g.w) + t.expert * g.w_stride + n0 * g.ldw;
     p.x_scales = g.a_scales + t.row, p.w_scales = g.w_scales + t.expert * g.n + n0;
     p.y = g.out_dtype == DDL_DT_F32 ? static_cast<void*>(static_cast<float*>(g.y) + at) : static_cast<void*>(static_cast<uint16_t*>(g.y) + at);
     p.M = rows, p.N = cols, p.out_dtype = g.out_dtype, p.K = g.k, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.ldy;
-    tile8<TM>(p, lds);
+    return true;
+}
+
+template <int TM>
+__global__ __launch_bounds__(kThreads8, 2) void expert_rows8(const ExpertArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    Tile8 p;
+    if (tile_of<32 * TM, kColumns>(g, blockIdx.x, p)) tile8<TM>(p, lds);
+}
+
+__global__ __launch_bounds__(kSmallThreads, 2) void expert_rows8_small(const ExpertArgs g) {
+    __shared__ __attribute__((aligned(16))) char lds[kSmallRing * kSmallStage];
+    Tile8 p;
+    if (tile_of<kSmall, kSmall>(g, blockIdx.x, p)) small_tile8(p, lds);
 }
 
 template <int TM>
@@ -298,6 +401,14 @@ int launch8(const char* who, ExpertArgs g, int dev, hipStream_t s) {
 
 }  // namespace
 
-int run_expert_rows8(const char* who, bool low, const ExpertArgs& g, int dev, hipStream_t s) { return low ? launch8<4>(who, g, dev, s) : launch8<8>(who, g, dev, s); }
+int run_expert_rows8(const char* who, ExpertTile tile, ExpertArgs g, int dev, hipStream_t s) {
+    if (tile == ExpertTile::kLarge) return launch8<8>(who, g, dev, s);
+    if (tile == ExpertTile::kLow) return launch8<4>(who, g, dev, s);
+    g.tiles_n = static_cast<int>((g.n + kSmall - 1) / kSmall);
+    const int64_t blocks = ((g.rows + kSmall - 1) / kSmall + g.experts) * static_cast<int64_t>(g.tiles_n);
+    if (blocks * kSmallThreads > 0xFFFFFFFFll) return fail(DDL_E_UNSUPP, "%s: %lld tiles", who, static_cast<long long>(blocks));
+    hipLaunchKernelGGL(expert_rows8_small, dim3(static_cast<uint32_t>(blocks)), dim3(kSmallThreads), 0, s, g);
+    return check_launch(who);
+}
 
 }  // namespace ddl

@@ -28,8 +28,8 @@ int run_expert_weights32(const char* who, ExpertArgs g, hipStream_t s);
 // Of expert_linear32_split.hip: tiles of 128 x 128.
 int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
-// Of expert_linear8.hip: tiles of 128 (low) or 256 rows by 256 columns.
-int run_expert_rows8(const char* who, bool low, const ExpertArgs& g, int dev, hipStream_t s);
+// Of expert_linear8.hip: kAny64, kLow and kLarge (aligned operands, all of them).
+int run_expert_rows8(const char* who, ExpertTile tile, ExpertArgs g, int dev, hipStream_t s);
 
 #ifdef __HIPCC__
 namespace {
