@@ -80,9 +80,9 @@ __global__ __launch_bounds__(64 * kStreamWaves<KIND>) void expert_stream(const E
     int lo, hi;
     rows_of_expert(g, e, lo, hi);
     if (lo == hi) return;
-    if (e == g.experts) {
-        const int cols = static_cast<int>(min(g.n - n0, static_cast<int64_t>(kStreamCols)));
-        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(hi - lo) * cols; i += blockDim.x) store_out(g, lo + i / cols, n0 + i % cols, 0.f);
+    if (e == g.experts) {   // the rows of none lie side by side
+        const int64_t size = g.out_dtype == DDL_DT_F32 ? 4 : 2, thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+        zero_run(static_cast<char*>(g.y) + lo * g.ldy * size, (hi - lo) * g.ldy * size, thread, static_cast<int64_t>(gridDim.x) * blockDim.x);
         return;
     }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, part = lane >> 4;
@@ -215,20 +215,24 @@ ExpertTile best_for_weights(bool aligned, int64_t rows, int64_t experts, int64_t
     return best;
 }
 
-// fp32: is a product quicker on 128 x 128 tiles of the bf16 matrix cores than on 64 x 64 ones of the fp32 cores?  Each CU's tiles one after the other, a start and
-// some time for each 32 of the reduction; linear_f32_split.hip's own fit for the first.  ([1024, 8192] by 3584: 545 us on the latter, 468 on the former.)
-bool split_pays(double large, double small, int64_t depth, int cus) {
-    const double steps = ceil(depth / 32.0), fill = large < cus ? large / cus : 1;
-    const double split = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), plain = 5 + (small < cus ? 1 : small / cus) * (1.5 + steps * 0.58);
-    return split < plain;
+// fp32: the edge of the quickest tiles, 128 (bf16 matrix cores, linear_f32_split.hip's own fit), 64 or 32 (fp32 cores).  Each CU's tiles one after the other, a start and some
+// time for each 32 of the reduction, which four groups share in the smallest.  `tiles` gives their number for an edge.  ([1024, 8192] by 3584: 64 545 us, 128 468; four
+// rows to each of eight experts of [1024, 4096]: 64 71 us, 32 25.)
+template <typename Tiles>
+int best_edge32(Tiles&& tiles, int64_t depth, int cus) {
+    const double steps = ceil(depth / 32.0), large = tiles(128), fill = large < cus ? large / cus : 1;
+    auto turns = [&](double n) { return n < cus ? 1.0 : n / cus; };
+    const double us128 = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), us64 = 5 + turns(tiles(64)) * (1.5 + steps * 0.58),
+                 us32 = 5 + turns(tiles(32)) * (3 + ceil(steps / 4) * 0.54);
+    return us128 < us64 ? (us32 < us128 ? 32 : 128) : us32 < us64 ? 32 : 64;
 }
-int rows32(const char* who, bool transposed, const ExpertArgs& g, int cus, hipStream_t s) {
-    const double large = row_tiles(g.rows, g.experts, 128) * static_cast<double>((g.n + 127) / 128), small = row_tiles(g.rows, g.experts, 64) * static_cast<double>((g.n + 63) / 64);
-    return split_pays(large, small, g.k, cus) ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, transposed, g, s);
+int rows32(const char* who, bool transposed, const ExpertArgs& g, int dev, hipStream_t s) {
+    const int edge = best_edge32([&](int e) { return row_tiles(g.rows, g.experts, e) * static_cast<double>((g.n + e - 1) / e); }, g.k, g.cus);
+    return edge == 128 ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, edge == 32, transposed, g, dev, s);
 }
-int weights32(const char* who, const ExpertArgs& g, int cus, hipStream_t s) {
-    const double large = static_cast<double>(g.experts) * ((g.n + 127) / 128) * ((g.k + 127) / 128), small = static_cast<double>(g.experts) * ((g.n + 63) / 64) * ((g.k + 63) / 64);
-    return split_pays(large, small, g.rows / g.experts, cus) ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, g, s);
+int weights32(const char* who, const ExpertArgs& g, int dev, hipStream_t s) {
+    const int edge = best_edge32([&](int e) { return static_cast<double>(g.experts) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / g.experts, g.cus);
+    return edge == 128 ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, edge == 32, g, dev, s);
 }
 
 // expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again; not for more rows than it has in registers.
@@ -270,7 +274,7 @@ int ddl_expert_linear(const void* x, const void* w, int dtype, const int32_t* of
     g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
     g.n = n, g.k = k, g.lda = rows > 1 ? ld_x : k, g.ldw = k, g.w_stride = n * k, g.ldy = n;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == DDL_DT_F32) return rows32(who, false, g, cus, s);
+    if (dtype == DDL_DT_F32) return rows32(who, false, g, dev, s);
     const bool aligned = aligned_to(x, 16) && aligned_to(w, 16) && g.lda % 8 == 0 && k % 8 == 0;
     double us;
     const ExpertTile tile = best_for_rows(kCosts16, aligned, rows, experts, n, 2 * k, cus, &us);
@@ -331,7 +335,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
         d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
         int rc;
         if (dtype == DDL_DT_F32) {
-            rc = rows32(who, true, d, cus, s);
+            rc = rows32(who, true, d, dev, s);
         } else {
             const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;
             double us;
@@ -342,7 +346,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
     if (dw && experts) {
         ExpertArgs d = g;
         d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
-        if (dtype == DDL_DT_F32) return weights32(who, d, cus, s);
+        if (dtype == DDL_DT_F32) return weights32(who, d, dev, s);
         const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
         return run_expert_weights16(who, best_for_weights(aligned, rows, experts, n, k, cus), f16, d, dev, s);
     }

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void e
     const int64_t n0 = static_cast<int64_t>(t.tn) * Shape<TILE>::bn;
     uint16_t* const y = static_cast<uint16_t*>(g.y) + t.row * g.ldy + n0;
     if (t.expert == g.experts) {
-        zero_block(y, g.ldy, 0, min(t.rows, t.half ? Shape<TILE>::bm / 2 : Shape<TILE>::bm), 0, static_cast<int>(min(g.n - n0, static_cast<int64_t>(Shape<TILE>::bn))));
+        zero_block(y, g.ldy, min(t.rows, t.half ? Shape<TILE>::bm / 2 : Shape<TILE>::bm), static_cast<int>(min(g.n - n0, static_cast<int64_t>(Shape<TILE>::bn))));
         return;
     }
     PartOf<uint16_t> p{};
@@ -58,8 +58,7 @@ __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void e
     const int64_t m0 = static_cast<int64_t>(tm) * Shape<TILE>::bm, n0 = static_cast<int64_t>(tn) * Shape<TILE>::bn;
     uint16_t* const y = static_cast<uint16_t*>(g.y) + e * g.n * g.k + m0 * g.k + n0;
     if (lo == hi) {
-        zero_block(y, g.k, 0, static_cast<int>(min(g.n - m0, static_cast<int64_t>(Shape<TILE>::bm))), 0,
-                   static_cast<int>(min(g.k - n0, static_cast<int64_t>(Shape<TILE>::bn))));
+        zero_part(g, static_cast<uint16_t*>(g.y) + e * g.n * g.k, tm, tn);
         return;
     }
     PartOf<uint16_t> p{};

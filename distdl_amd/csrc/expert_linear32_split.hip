@@ -14,7 +14,7 @@ __global__ __launch_bounds__(kBlock, 2) void expert_rows32_split(const ExpertArg
     const int64_t n0 = static_cast<int64_t>(t.tn) * kTile;
     float* const y = static_cast<float*>(g.y) + t.row * g.ldy + n0;
     if (t.expert == g.experts) {
-        zero_block(y, g.ldy, 0, min(t.rows, kTile), 0, static_cast<int>(min(g.n - n0, static_cast<int64_t>(kTile))));
+        zero_block(y, g.ldy, min(t.rows, kTile), static_cast<int>(min(g.n - n0, static_cast<int64_t>(kTile))));
         return;
     }
     Part32 p{};
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(kBlock, 2) void expert_weights32_split(const Expert
     const int64_t m0 = static_cast<int64_t>(tm) * kTile, n0 = static_cast<int64_t>(tn) * kTile;
     float* const y = static_cast<float*>(g.y) + e * g.n * g.k + m0 * g.k + n0;
     if (lo == hi) {
-        zero_block(y, g.k, 0, static_cast<int>(min(g.n - m0, static_cast<int64_t>(kTile))), 0, static_cast<int>(min(g.k - n0, static_cast<int64_t>(kTile))));
+        zero_part(g, static_cast<float*>(g.y) + e * g.n * g.k, tm, tn);
         return;
     }
     Part32 p{};

@@ -359,8 +359,8 @@ __device__ inline bool tile_of(const ExpertArgs& g, int id, Tile8& p) {
     const int cols = static_cast<int>(min(g.n - n0, static_cast<int64_t>(BN))), rows = min(t.rows, BM);
     const int64_t at = t.row * g.ldy + n0;
     if (t.expert == g.experts) {
-        if (g.out_dtype == DDL_DT_F32) zero_block(static_cast<float*>(g.y) + at, g.ldy, 0, rows, 0, cols);
-        else zero_block(static_cast<uint16_t*>(g.y) + at, g.ldy, 0, rows, 0, cols);
+        if (g.out_dtype == DDL_DT_F32) zero_block(static_cast<float*>(g.y) + at, g.ldy, rows, cols);
+        else zero_block(static_cast<uint16_t*>(g.y) + at, g.ldy, rows, cols);
         return false;
     }
     p.x = static_cast<const uint8_t*>(g.a) + t.row * g.lda, p.w = static_cast<const uint8_t*>(g.w) + t.expert * g.w_stride + n0 * g.ldw;

@@ -131,7 +131,7 @@ MaybeTensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offset
 
 MaybeTensor expert_linear_8bit(const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& x_scales, const Tensor& w_scales, at::ScalarType dtype) {
     const int code = dtype == at::kFloat ? DDL_DT_F32 : dtype == at::kBFloat16 ? DDL_DT_BF16 : dtype == at::kHalf ? DDL_DT_F16 : 0;
-    if (!expert_operands(x, w, offsets) || x.scalar_type() != at::kFloat8_e4m3fn || !code || !floats_of(x_scales, {x.size(0)}) || !floats_of(w_scales, {w.size(0), w.size(1)}))
+    if (!expert_operands(x, w, offsets) || x.scalar_type() != at::kFloat8_e4m3fn || !code || !multiple(x.data_ptr(), 16) || !multiple(w.data_ptr(), 16) || !floats_of(x_scales, {x.size(0)}) || !floats_of(w_scales, {w.size(0), w.size(1)}))
         return std::nullopt;
     const int64_t rows = x.size(0), n = w.size(1), k = w.size(2);
     Tensor y = at::empty({rows, n}, x.options().dtype(dtype));

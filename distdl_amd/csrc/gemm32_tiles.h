@@ -14,8 +14,10 @@ typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
 constexpr int kDepth32 = kRowBytes / 4;   // floats of a k-tile
 typedef PartOf<float> Part32;
 
-// Workgroup `number` of the tiles_m x tiles_n x splits of a product.
-template <bool XT, bool WT, int NWM, int NWN, int KG, int STAGES>
+// Workgroup `number` of the tiles_m x tiles_n x splits of a product.  FOLD: the sum of every kFold rounds goes into another one, so that a long reduction is
+// not one chain of roundings.
+constexpr int kFold = 32;
+template <bool XT, bool WT, int NWM, int NWN, int KG, int STAGES, bool FOLD = false>
 __device__ __forceinline__ void small_product(const Part32& p, int number, int splits, float* __restrict__ partial, char* lds) {
     constexpr int NW = NWM * NWN, BM = 32 * NWM, BN = 32 * NWN;
     static_assert(NW * KG == 4, "four wavefronts per workgroup");
@@ -113,9 +115,13 @@ __device__ __forceinline__ void small_product(const Part32& p, int number, int s
         return v;
     };
 
-    floatx16 acc;
+    floatx16 acc, folded;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    for (int e = 0; e < 16; ++e) acc[e] = folded[e] = 0.f;
+    auto fold = [&]() {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) folded[e] += acc[e], acc[e] = 0.f;
+    };
     // Group i takes k-tiles t_begin + i, + KG, ...; all groups walk the same number of rounds, for the barriers.
     const int rounds = (t_end - t_begin + KG - 1) / KG;
     auto tile_at = [&](int r) { return t_begin + r * KG + group; };
@@ -164,6 +170,7 @@ __device__ __forceinline__ void small_product(const Part32& p, int number, int s
     const int plain = (t_end < full_tiles ? t_end : full_tiles) - t_begin - group;   // tiles of the range, counted from the group's first
 #pragma unroll 1
     for (; (r + STAGES) * KG < plain; ++r) {
+        if (FOLD && r % kFold == kFold - 1) fold();
         multiply(First{}, First{}, Second{});
         read_half(slot, Second{});
         multiply(First{}, Second{}, End{});
@@ -195,6 +202,10 @@ __device__ __forceinline__ void small_product(const Part32& p, int number, int s
         if (tile_at(r + STAGES) < t_end) request(tile_at(r + STAGES), slot);
         multiply(Second{}, Second{}, End{});
         slot = next;
+    }
+    if (FOLD) {
+        fold();
+        acc = folded;
     }
     // Lane holds row m = l32 and columns n = 8 g + 4 kh + {0..3} in acc[4 g + {0..3}].
     floatx4 quad[4];

@@ -1600,6 +1600,15 @@ def _expert_operands(x, weight, offsets, name):
         return _rows_of(x, x.shape[0], name, "rows"), contiguous(weight), contiguous(offsets)
 
 
+def _aligned_copy(t):
+    """A row-major copy, which lies at a multiple of 16 bytes."""
+    out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    if t.numel():
+        full = [slice(0, int(n)) for n in t.shape]
+        copy_box(t, full, out, full)
+    return out
+
+
 def expert_linear(x, weight, offsets, x_scales=None, weight_scales=None, dtype=None):
     """Rows ``x`` [rows, in] by the weights [experts, out, in] of their experts, see ``ddl_expert_linear``; e4m3 rows and weights with their scales,
     see ``ddl_expert_linear_8bit``, in ``dtype`` (default bfloat16)."""
@@ -1617,6 +1626,7 @@ def expert_linear(x, weight, offsets, x_scales=None, weight_scales=None, dtype=N
         y = torch.empty((rows, n), dtype=dtype, device=x.device)
         with _on_device_of(x):
             x_scales, weight_scales = contiguous(x_scales), contiguous(weight_scales)
+            x, weight = (_aligned_copy(t) if t.data_ptr() % 16 or _pitch(t) % 16 else t for t in (x, weight.view(-1, k)))
             rc = lib.ddl_expert_linear_8bit(x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), offsets.data_ptr(), experts, rows, n, k,
                                             _pitch(x), y.data_ptr(), _LN_DTYPES[dtype], _stream())
         _lib.check(rc, "ddl_expert_linear_8bit")

@@ -99,6 +99,18 @@ def test_strided_rows_and_one_gradient():
             near(torch.autograd.grad(nn.expert_linear_shard(x, b, offsets), [b], d)[0], want[2], terms[2], 30, dtype)
 
 
+def test_rows_in_8_bits_that_lie_anywhere():
+    """Rows and weights off 16 bytes and with pitches of their own are copied."""
+    g = torch.Generator().manual_seed(6)
+    offsets = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")
+    big, w = torch.randn(50, 100, generator=g).to(torch.float8_e4m3fn).cuda(), torch.randn(2 * 24 * 48 + 3, generator=g).to(torch.float8_e4m3fn).cuda()
+    xs, ws = torch.rand(100, generator=g).cuda()[::2], torch.rand(2, 24, generator=g).cuda()
+    for x, v in ((big[:, :48], w[:-3].view(2, 24, 48)), (big[:, 5:53], w[3:].view(2, 24, 48)), (big[:, 16:64], w[:-3].view(2, 24, 48))):
+        y = nn.expert_linear_shard(x, v, offsets, x_scales=xs, weight_scales=ws, dtype=torch.float32)
+        zx, zw = n64(x.float()) * n64(xs)[:, None], n64(v.float()) * n64(ws)[..., None]
+        near(y, o.product(zx, zw, [0, 20, 50]), o.product(np.abs(zx), np.abs(zw), [0, 20, 50]), 48, torch.float32, IN_EIGHTS)
+
+
 def test_offsets_that_hold_anything_stay_inside():
     """Whatever the offsets hold, rows of x, y and dw stay where they are; values outside 0 .. rows count as those."""
     x, w = torch.ones(40, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(3, 32, 64, dtype=torch.bfloat16, device="cuda")
