@@ -93,8 +93,9 @@ __device__ __forceinline__ void tile8(const Tile8& p, char* lds) {
         }
     };
 
-    // This lane's 32 bytes of its row of a piece: chunks 2 kg and 2 kg + 1, where the swizzle has them.
-    const int sw = (l16 >> 1) & 7, at0 = l16 * kRowBytes + (((2 * kg) ^ sw) << 4), at1 = l16 * kRowBytes + (((2 * kg + 1) ^ sw) << 4);
+    // This lane's 32 bytes of its row of a piece: chunks kg and 4 + kg, as the 16-bit tiles read them one after the other, where the swizzle has them (chunks
+    // 2 kg and 2 kg + 1 meet on their banks: half of the LDS cycles).
+    const int sw = (l16 >> 1) & 7, at0 = l16 * kRowBytes + ((kg ^ sw) << 4), at1 = l16 * kRowBytes + (((4 + kg) ^ sw) << 4);
     auto read = [&](const char* tile, int row) -> intx8 {
         intx8 v;
         const uint4 a = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at0), b = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at1);
@@ -299,7 +300,7 @@ __device__ __forceinline__ void small_tile8(const Tile8& p, char* lds) {
             }
         }
     };
-    const int sw = (l16 >> 1) & 7, at0 = l16 * kRowBytes + (((2 * kg) ^ sw) << 4), at1 = l16 * kRowBytes + (((2 * kg + 1) ^ sw) << 4);
+    const int sw = (l16 >> 1) & 7, at0 = l16 * kRowBytes + ((kg ^ sw) << 4), at1 = l16 * kRowBytes + (((4 + kg) ^ sw) << 4);
     auto read = [&](const char* tile, int row) -> intx8 {
         intx8 v;
         const uint4 a = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at0), b = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + at1);
