@@ -197,7 +197,9 @@ class DistributedRMSNorm(Module):
             weight = self.broadcast(weight)
         if weight is not None and weight.dtype != x.dtype:
             raise ValueError(f"DistributedRMSNorm's weight is {weight.dtype}, the input is {x.dtype}")
-        shape, flat = x.shape, x.shape[:x.dim() - dims] + (-1,)
+        shape, flat = x.shape, x.shape[:x.dim() - dims] + (int(np.prod(self.local_shape)),)
+        if residual is not None and residual.shape != shape:
+            raise ValueError(f"residual {tuple(residual.shape)} of an input {tuple(shape)}")
         if dims > 1:
             x, residual = x.reshape(flat), None if residual is None else residual.reshape(flat)
         if self.split:

@@ -223,3 +223,21 @@ def test_layer_over_four_workers(shape, dims):
         np.testing.assert_allclose(dx, want_dx[own], rtol=1e-5, atol=1e-5)
         if dw is not None and dw.size:
             np.testing.assert_allclose(dw.reshape(want_dw[own[3 - dims:]].shape), want_dw[own[3 - dims:]], rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_layer_without_rows(eight_bit):
+    """No row of several dimensions is no row, not an unknown number of columns; a residual of another shape is refused, also where its elements would be enough."""
+    from distdl_amd.backends.stub_hip import SimWorld
+
+    def body(P_world):
+        P = P_world.create_partition_inclusive([0]).create_cartesian_topology_partition([1, 1, 1])
+        layer = nn.DistributedRMSNorm(P, (4, 8))
+        x = torch.zeros(0, 4, 8, device="cuda")
+        with torch.no_grad():
+            res = layer(x, x.clone(), eight_bit=eight_bit)
+            with pytest.raises(ValueError, match="residual"):
+                layer(torch.zeros(3, 4, 8, device="cuda"), torch.zeros(3, 8, 4, device="cuda"), eight_bit=eight_bit)
+        return [tuple(t.shape) for t in res]
+
+    assert SimWorld(1).run(body)[0] == ([(0, 4, 8), (0,), (0, 4, 8)] if eight_bit else [(0, 4, 8)] * 2)
