@@ -216,23 +216,23 @@ ExpertTile best_for_weights(bool aligned, int64_t rows, int64_t experts, int64_t
 }
 
 // fp32: the edge of the quickest tiles, 128 (bf16 matrix cores, linear_f32_split.hip's own fit), 64 or 32 (fp32 cores).  Each CU's tiles one after the other, a start and some
-// time for each 32 of the reduction, which four groups share in the smallest.  `tiles` gives their number for an edge.  ([1024, 8192] by 3584: 64 545 us, 128 468; four
-// rows to each of eight experts of [1024, 4096]: 64 71 us, 32 25.)
+// time for each 32 of the reduction, which four groups share in the smallest.  `tiles` gives their number for an edge.  ([1024, 8192] by 3584: 64 545 us, 128 468; [64, 4096] by 1024 to
+// three experts: 64 71 us, 32 23.)
 template <typename Tiles>
 int best_edge32(Tiles&& tiles, int64_t depth, int cus) {
     const double steps = ceil(depth / 32.0), large = tiles(128), fill = large < cus ? large / cus : 1;
     auto turns = [&](double n) { return n < cus ? 1.0 : n / cus; };
-    const double us128 = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), us64 = 5 + turns(tiles(64)) * (1.5 + steps * 0.58),
-                 us32 = 5 + turns(tiles(32)) * (3 + ceil(steps / 4) * 0.54);
+    const double us128 = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), us64 = 5 + turns(tiles(64)) * (1 + steps * 0.57),
+                 us32 = 5 + turns(tiles(32)) * (1.5 + ceil(steps / 4) * 0.52);
     return us128 < us64 ? (us32 < us128 ? 32 : 128) : us32 < us64 ? 32 : 64;
 }
-int rows32(const char* who, bool transposed, const ExpertArgs& g, int dev, hipStream_t s) {
+int rows32(const char* who, bool transposed, const ExpertArgs& g, hipStream_t s) {
     const int edge = best_edge32([&](int e) { return row_tiles(g.rows, g.experts, e) * static_cast<double>((g.n + e - 1) / e); }, g.k, g.cus);
-    return edge == 128 ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, edge == 32, transposed, g, dev, s);
+    return edge == 128 ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, edge == 32, transposed, g, s);
 }
-int weights32(const char* who, const ExpertArgs& g, int dev, hipStream_t s) {
+int weights32(const char* who, const ExpertArgs& g, hipStream_t s) {
     const int edge = best_edge32([&](int e) { return static_cast<double>(g.experts) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / g.experts, g.cus);
-    return edge == 128 ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, edge == 32, g, dev, s);
+    return edge == 128 ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, edge == 32, g, s);
 }
 
 // expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again; not for more rows than it has in registers.
@@ -274,7 +274,7 @@ int ddl_expert_linear(const void* x, const void* w, int dtype, const int32_t* of
     g.a = x, g.w = w, g.y = y, g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
     g.n = n, g.k = k, g.lda = rows > 1 ? ld_x : k, g.ldw = k, g.w_stride = n * k, g.ldy = n;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == DDL_DT_F32) return rows32(who, false, g, dev, s);
+    if (dtype == DDL_DT_F32) return rows32(who, false, g, s);
     const bool aligned = aligned_to(x, 16) && aligned_to(w, 16) && g.lda % 8 == 0 && k % 8 == 0;
     double us;
     const ExpertTile tile = best_for_rows(kCosts16, aligned, rows, experts, n, 2 * k, cus, &us);
@@ -335,7 +335,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
         d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
         int rc;
         if (dtype == DDL_DT_F32) {
-            rc = rows32(who, true, d, dev, s);
+            rc = rows32(who, true, d, s);
         } else {
             const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;
             double us;
@@ -346,7 +346,7 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
     if (dw && experts) {
         ExpertArgs d = g;
         d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
-        if (dtype == DDL_DT_F32) return weights32(who, d, dev, s);
+        if (dtype == DDL_DT_F32) return weights32(who, d, s);
         const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
         return run_expert_weights16(who, best_for_weights(aligned, rows, experts, n, k, cus), f16, d, dev, s);
     }

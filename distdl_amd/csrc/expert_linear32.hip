@@ -7,7 +7,9 @@
 namespace ddl {
 namespace {
 
-constexpr int kStages32 = 4;
+// Two stages leave room for a second workgroup on a CU, which hides more than two stages more ([2048, 1024] by 1024 to eight experts 56 -> 53 us, weights' gradients of [512, 1024] by 4096
+// 105 -> 82; 32 x 32 tiles, sixteen rows to each of eight experts of [2048, 2048], 27 -> 23).
+constexpr int kStages32 = 2;
 constexpr int groups_of(int edge) { return edge == 64 ? 1 : 4; }
 constexpr int lds_of(int edge) { return groups_of(edge) * kStages32 * 2 * edge * kRowBytes; }
 
@@ -50,40 +52,34 @@ __global__ __launch_bounds__(256) void expert_weights32(const ExpertArgs g) {
 }
 
 template <int EDGE, typename Kernel>
-int launch32(const char* who, Kernel kernel, std::atomic<bool>* reserved, const ExpertArgs& g, int64_t blocks, int dev, hipStream_t s) {
+int launch32(const char* who, Kernel kernel, const ExpertArgs& g, int64_t blocks, hipStream_t s) {
     if (blocks * 256 > 0xFFFFFFFFll) return fail(DDL_E_UNSUPP, "%s: %lld tiles", who, static_cast<long long>(blocks));
-    if (lds_of(EDGE) > 65536 && !reserved[dev].load(std::memory_order_acquire)) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds_of(EDGE));
-        if (e != hipSuccess) return fail(static_cast<int>(e), "%s: cannot reserve %d bytes of LDS: %s", who, lds_of(EDGE), hipGetErrorString(e));
-        reserved[dev].store(true, std::memory_order_release);
-    }
+    static_assert(lds_of(EDGE) <= 64 * 1024, "what a launch gets without asking");
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), lds_of(EDGE), s, g);
     return check_launch(who);
 }
 
 template <int EDGE, bool WT>
-int launch_rows32(const char* who, ExpertArgs g, int dev, hipStream_t s) {
-    static std::atomic<bool> reserved[kMaxDevices];
+int launch_rows32(const char* who, ExpertArgs g, hipStream_t s) {
     g.tiles_n = static_cast<int>((g.n + EDGE - 1) / EDGE);
-    return launch32<EDGE>(who, expert_rows32<EDGE, WT>, reserved, g, ((g.rows + EDGE - 1) / EDGE + g.experts) * static_cast<int64_t>(g.tiles_n), dev, s);
+    return launch32<EDGE>(who, expert_rows32<EDGE, WT>, g, ((g.rows + EDGE - 1) / EDGE + g.experts) * static_cast<int64_t>(g.tiles_n), s);
 }
 
 template <int EDGE>
-int launch_weights32(const char* who, ExpertArgs g, int dev, hipStream_t s) {
-    static std::atomic<bool> reserved[kMaxDevices];
+int launch_weights32(const char* who, ExpertArgs g, hipStream_t s) {
     g.tiles_m = static_cast<int>((g.n + EDGE - 1) / EDGE), g.tiles_n = static_cast<int>((g.k + EDGE - 1) / EDGE);
-    return launch32<EDGE>(who, expert_weights32<EDGE>, reserved, g, matrix_blocks(g), dev, s);
+    return launch32<EDGE>(who, expert_weights32<EDGE>, g, matrix_blocks(g), s);
 }
 
 }  // namespace
 
-int run_expert_rows32(const char* who, bool small, bool transposed, const ExpertArgs& g, int dev, hipStream_t s) {
-    if (small) return transposed ? launch_rows32<32, true>(who, g, dev, s) : launch_rows32<32, false>(who, g, dev, s);
-    return transposed ? launch_rows32<64, true>(who, g, dev, s) : launch_rows32<64, false>(who, g, dev, s);
+int run_expert_rows32(const char* who, bool small, bool transposed, const ExpertArgs& g, hipStream_t s) {
+    if (small) return transposed ? launch_rows32<32, true>(who, g, s) : launch_rows32<32, false>(who, g, s);
+    return transposed ? launch_rows32<64, true>(who, g, s) : launch_rows32<64, false>(who, g, s);
 }
 
-int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, int dev, hipStream_t s) {
-    return small ? launch_weights32<32>(who, g, dev, s) : launch_weights32<64>(who, g, dev, s);
+int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, hipStream_t s) {
+    return small ? launch_weights32<32>(who, g, s) : launch_weights32<64>(who, g, s);
 }
 
 }  // namespace ddl

@@ -23,8 +23,8 @@ enum class ExpertTile { kAny64, kAny128, kLow, kLarge };
 int run_expert_rows16(const char* who, ExpertTile tile, bool f16, bool transposed, ExpertArgs g, int dev, hipStream_t s);
 int run_expert_weights16(const char* who, ExpertTile tile, bool f16, ExpertArgs g, int dev, hipStream_t s);
 // Of expert_linear32.hip: tiles of 32 x 32 (small) or 64 x 64.
-int run_expert_rows32(const char* who, bool small, bool transposed, const ExpertArgs& g, int dev, hipStream_t s);
-int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, int dev, hipStream_t s);
+int run_expert_rows32(const char* who, bool small, bool transposed, const ExpertArgs& g, hipStream_t s);
+int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, hipStream_t s);
 // Of expert_linear32_split.hip: tiles of 128 x 128.
 int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
