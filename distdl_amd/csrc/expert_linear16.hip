@@ -51,20 +51,18 @@ __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void e
 template <ExpertTile TILE, bool F16>
 __global__ __launch_bounds__(Shape<TILE>::threads, Shape<TILE>::per_simd) void expert_weights16(const ExpertArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    int e, tm, tn, lo, hi;
-    if (!find_matrix_tile(g, blockIdx.x, e, tm, tn)) return;
-    rows_of_expert(g, e, lo, hi);
-    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-    const int64_t m0 = static_cast<int64_t>(tm) * Shape<TILE>::bm, n0 = static_cast<int64_t>(tn) * Shape<TILE>::bn;
-    uint16_t* const y = static_cast<uint16_t*>(g.y) + e * g.n * g.k + m0 * g.k + n0;
-    if (lo == hi) {
-        zero_part(g, static_cast<uint16_t*>(g.y) + e * g.n * g.k, tm, tn);
+    MatrixTask t;
+    if (!find_matrix_tile(g, blockIdx.x, t)) return;
+    if (t.lo == t.hi) {
+        zero_part<uint16_t>(g, t);
         return;
     }
+    const int64_t m0 = static_cast<int64_t>(t.tm) * Shape<TILE>::bm, n0 = static_cast<int64_t>(t.tn) * Shape<TILE>::bn;
     PartOf<uint16_t> p{};
-    p.x = static_cast<const uint16_t*>(g.a) + lo * g.lda + m0;
-    p.w = static_cast<const uint16_t*>(g.w) + lo * g.ldw + n0;
-    p.y = y, p.M = g.n - m0, p.N = g.k - n0, p.K = hi - lo, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.k, p.tiles_m = p.tiles_n = 1;
+    p.x = static_cast<const uint16_t*>(g.a) + t.lo * g.lda + m0;
+    p.w = static_cast<const uint16_t*>(g.w) + t.lo * g.ldw + n0;
+    p.y = static_cast<uint16_t*>(g.y) + t.expert * g.n * g.k + m0 * g.k + n0;
+    p.M = g.n - m0, p.N = g.k - n0, p.K = t.hi - t.lo, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.k, p.tiles_m = p.tiles_n = 1;
     product_tile<TILE, F16, true, true>(p, lds);
 }
 

@@ -26,20 +26,18 @@ __global__ __launch_bounds__(kBlock, 2) void expert_rows32_split(const ExpertArg
 
 __global__ __launch_bounds__(kBlock, 2) void expert_weights32_split(const ExpertArgs g) {
     __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
-    int e, tm, tn, lo, hi;
-    if (!find_matrix_tile(g, blockIdx.x, e, tm, tn)) return;
-    rows_of_expert(g, e, lo, hi);
-    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-    const int64_t m0 = static_cast<int64_t>(tm) * kTile, n0 = static_cast<int64_t>(tn) * kTile;
-    float* const y = static_cast<float*>(g.y) + e * g.n * g.k + m0 * g.k + n0;
-    if (lo == hi) {
-        zero_part(g, static_cast<float*>(g.y) + e * g.n * g.k, tm, tn);
+    MatrixTask t;
+    if (!find_matrix_tile(g, blockIdx.x, t)) return;
+    if (t.lo == t.hi) {
+        zero_part<float>(g, t);
         return;
     }
+    const int64_t m0 = static_cast<int64_t>(t.tm) * kTile, n0 = static_cast<int64_t>(t.tn) * kTile;
     Part32 p{};
-    p.x = static_cast<const float*>(g.a) + lo * g.lda + m0;
-    p.w = static_cast<const float*>(g.w) + lo * g.ldw + n0;
-    p.y = y, p.M = g.n - m0, p.N = g.k - n0, p.K = hi - lo, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.k, p.tiles_m = p.tiles_n = 1;
+    p.x = static_cast<const float*>(g.a) + t.lo * g.lda + m0;
+    p.w = static_cast<const float*>(g.w) + t.lo * g.ldw + n0;
+    p.y = static_cast<float*>(g.y) + t.expert * g.n * g.k + m0 * g.k + n0;
+    p.M = g.n - m0, p.N = g.k - n0, p.K = t.hi - t.lo, p.ldx = g.lda, p.ldw = g.ldw, p.ldy = g.k, p.tiles_m = p.tiles_n = 1;
     split_product<true, true>(p, 0, 1, nullptr, lds);
 }
 
