@@ -148,3 +148,28 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+
+
+@pytest.mark.parametrize("tokens,chosen,experts,window,cols", [(1, 1, 1, None, 3), (37, 3, 5, (1, 4), 65), (300, 2, 8, None, 128)])
+def test_gradients_against_differences(tokens, chosen, experts, window, cols):
+    """The way there, a product and the way back are linear in every operand, so a difference of any width is the gradient times the step."""
+    g = torch.Generator().manual_seed(tokens)
+    plan = nn.expert_plan(torch.randint(0, experts, (tokens, chosen), generator=g).cuda(), experts, window=window)
+    held = len(plan.offsets) - 1
+    operands = [torch.randn(*s, generator=g).cuda() for s in ((tokens, cols), (held, 24, cols), (tokens, chosen))]
+    dout = torch.randn(tokens, 24, generator=g).cuda()
+
+    def run(x, w, weights):
+        return nn.expert_combine(nn.expert_linear_shard(nn.expert_sort(x, plan), w, plan.offsets), plan, weights)
+
+    leaves = [t.clone().requires_grad_() for t in operands]
+    grads = torch.autograd.grad(run(*leaves), leaves, dout)
+    for i, grad in enumerate(grads):
+        step = torch.randn(operands[i].shape, generator=g).cuda()
+        far = [t + step if j == i else t for j, t in enumerate(operands)]
+        moved = far[i].double() - operands[i].double()       # the step as the sum was rounded
+        change = ((run(*far).double() - run(*operands).double()) * dout.double()).sum()
+        # results: sums of cols and chosen terms, the weight and the rows rounded on the way; of the terms' sizes, at both ends; gradients as much again
+        sizes = (run(*[t.abs() for t in operands]).double() + run(*[t.abs() for t in far]).double())
+        bound = 4 * (cols + chosen + tokens * chosen + 8) * U * (sizes * dout.abs()).sum()
+        assert (change - (grad.double() * moved).sum()).abs() <= bound

@@ -282,3 +282,45 @@ def test_more_than_32_bits_of_elements(what):
         assert ((dx[-50:].double() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -4).all()
         want = y[100:].t().float() @ x[100:].float()
         assert ((dw[1].float() - want).abs() <= 2 ** -6 * want.abs() + 1e-3 * want.abs().max()).all()
+
+
+@pytest.mark.parametrize("counts,k,n", [([3, 5, 2], 64, 33), ([20, 60, 21], 272, 96), ([130, 200, 129], 1040, 1032), ([700, 300, 600], 2048, 4100), ([1400, 900, 1300], 528, 4096)])
+def test_experts_do_not_see_each_others_rows_in_8_bits(counts, k, n):
+    """As above, for codes and scales, by the kernel for few rows, the small and the large tiles."""
+    g = torch.Generator().manual_seed(k)
+    offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device="cuda")
+    x, w = (torch.randn(*s, generator=g).to(torch.float8_e4m3fn).cuda() for s in ((sum(counts), k), (3, n, k)))
+    xs, ws = torch.rand(sum(counts), generator=g).cuda(), torch.rand(3, n, generator=g).cuda()
+    clean = nn.expert_linear_shard(x, w, offsets, x_scales=xs, weight_scales=ws)
+    mid = slice(counts[0], counts[0] + counts[1])
+    x.view(torch.uint8)[mid], xs[mid], w.view(torch.uint8)[1], ws[1] = 0x7F, float("inf"), 0xFF, float("nan")
+    got = nn.expert_linear_shard(x, w, offsets, x_scales=xs, weight_scales=ws)
+    assert torch.equal(got[:mid.start], clean[:mid.start]) and torch.equal(got[mid.stop:], clean[mid.stop:]) and got[mid].isnan().all()
+
+
+def test_rows_in_8_bits_captured_with_other_choices_each_time():
+    """A prompt's rows and single tokens, from the norm to the products, replayed for choices that change which experts have rows."""
+    g = torch.Generator().manual_seed(8)
+    w8, ws = nn.quantize_rows(torch.randn(6, 264, 512, generator=g).to(torch.bfloat16).cuda())
+    for tokens in (3, 700):
+        x, r = (torch.randn(tokens, 512, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+        ids = torch.randint(0, 6, (tokens, 2), generator=g).cuda()
+
+        @torch.no_grad()
+        def step():
+            codes, scales, h = nn.rms_norm_shard(x, None, r, eight_bit=True)
+            plan = nn.expert_plan(ids, 6, window=(0, 6))
+            rows, row_scales = nn.expert_sort(codes, plan, scales)
+            return h, nn.expert_combine(nn.expert_linear_shard(rows, w8, plan.offsets, x_scales=row_scales, weight_scales=ws), plan)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for low, high in ((0, 6), (2, 3), (-1, 6), (-1, 0), (4, 6)):
+            ids.copy_(torch.randint(low, high, (tokens, 2), generator=g))
+            x.copy_(torch.randn(tokens, 512, generator=g))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, step()))
