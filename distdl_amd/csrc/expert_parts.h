@@ -16,6 +16,7 @@ struct ExpertArgs {
     int experts, rows, out_dtype, cus;
     int64_t n, k, lda, ldw, w_stride, ldy;
     int tiles_m, tiles_n;                 // tiles_m: of an expert's matrix (gradients of the weights)
+    int places, few;                      // of those with most rows, this many experts, and of them those with more rows than `few` (gradients of the weights)
 };
 
 // Kernels of expert_linear16.hip: tiles of 64 or 128 rows and columns at any address (edge 64, 128), or large ones, of 128 x 256 (low) or 256 x 256.
@@ -28,6 +29,8 @@ int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, hipSt
 // Of expert_linear32_split.hip: tiles of 128 x 128.
 int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
+// Of expert_outer.hip: gradients of the weights of all experts with at most g.few rows (matrices of at least 8 rows, and columns for 16 bytes).
+int run_expert_outer(const char* who, const ExpertArgs& g, hipStream_t s);
 // Of expert_linear8.hip: kAny64, kLow and kLarge (aligned operands, all of them).
 int run_expert_rows8(const char* who, ExpertTile tile, ExpertArgs g, int dev, hipStream_t s);
 
@@ -111,7 +114,7 @@ struct MatrixTask {
     int expert, lo, hi;   // its rows
     int number, tm, tn;   // of the tile, in the order of the workgroups
 };
-// Tile `id` of those of all experts' matrices; false: there is none of that number.  Experts with many rows come first, so that the last
+// Tile `id` of those of the experts' matrices; false: there is none of that number.  Experts with many rows come first, so that the last
 // tiles are short ones, and every XCD has an eighth of each expert's tiles side by side (of few tiles it takes them in turn): with an
 // expert for each XCD, the one with most rows kept its XCD busy for 600 us of [16384, 4096 -> 3584] to 8 experts of 0 to 3200 rows, here 428.
 __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask& task) {
@@ -123,7 +126,7 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
         const int xcd = id % kXcds, nth = id / kXcds, first = xcd * each / kXcds, share = (xcd + 1) * each / kXcds - first;
         place = nth / share, rest = first + nth % share;
     }
-    if (place >= g.experts) return false;
+    if (place >= g.places) return false;
     expert = place;
     if (g.experts <= 64) {   // a lane for each: how many have more rows, or as many and come before it; of those without rows, how many come before it
         const int lane = threadIdx.x & 63;
@@ -147,6 +150,7 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
     } else {
         rows_of_expert(g, expert, lo, hi);
     }
+    if (hi - lo <= g.few) return false;
     constexpr int kBand = 8;
     const int band = rest / (kBand * g.tiles_n), band_h = min(kBand, g.tiles_m - band * kBand), in_band = rest - band * kBand * g.tiles_n;
     const auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };   // so that the compiler knows it
@@ -156,7 +160,7 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
 // Workgroups that find_matrix_tile needs.
 inline int64_t matrix_blocks(const ExpertArgs& g) {
     const int64_t each = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    return each < 8 * kXcds ? each * g.experts : (each + kXcds - 1) / kXcds * kXcds * g.experts;
+    return each < 8 * kXcds ? each * g.places : (each + kXcds - 1) / kXcds * kXcds * g.places;
 }
 
 // Zeros in `bytes` from `to` on (any address), by the threads `first`, first + step, ...

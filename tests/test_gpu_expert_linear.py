@@ -68,6 +68,27 @@ def test_products_and_adjoint(counts, spare, k, n, dtype):
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+# few rows for most experts: all of them few, some with 33 and more, none at all; matrices that are no whole vectors or lines, and of the smallest sizes
+FEW = [([2, 1, 0, 4], 0, 256, 264), ([32, 0, 1], 0, 72, 130), ([33, 0, 1], 3, 72, 130), ([40, 1, 0, 2, 100, 0, 3, 1, 1, 70, 5, 5, 2, 33, 1], 9, 520, 96), ([0] * 69 + [20], 0, 64, 40),
+       ([0] * 40 + [500] + [0] * 23, 0, 136, 72), ([5, 9], 2, 9, 11), ([3, 2, 2], 1, 1001, 13), ([1] * 64, 0, 8, 8), ([0, 0, 0], 0, 2050, 9), ([7] * 30, 0, 1030, 258)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES)
+@pytest.mark.parametrize("counts,spare,k,n", FEW, ids=[f"{sum(c)}+{s}of{len(c)}-{k}x{n}" for c, s, k, n in FEW])
+def test_weights_gradients_of_few_rows(counts, spare, k, n, dtype):
+    g = torch.Generator().manual_seed(k * 7 + n)
+    rows, held = sum(counts) + spare, sum(counts)
+    x, dy = ((torch.randn(*s, generator=g)).to(dtype).cuda() for s in ((rows, k + 3), (rows, n + 5)))
+    x[held:], dy[held:] = float("nan"), float("inf")        # nobody's
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    w = torch.empty(len(counts), n, k, dtype=dtype, device="cuda")
+    for a, b in ((x[:, :k].contiguous(), dy[:, :n].contiguous()), (x[:, 3:], dy[:, 5:])):
+        dw = hip_ops.expert_linear_backward(b, a, w, torch.from_numpy(offsets).cuda(), False, True)[1]
+        za, zb = n64(a)[:held], n64(b)[:held]
+        want, terms = (np.stack([f(zb[lo:hi]).T @ f(za[lo:hi]) for lo, hi in zip(offsets[:-1], offsets[1:])]) for f in (lambda v: v, np.abs))
+        near(dw, want, terms, max(counts), dtype)
+
+
 E4M3 = [([1], 0, 16, 1), ([0], 2, 16, 8), ([3, 0, 2, 1], 4, 128, 96), ([16, 1, 0, 33, 7], 0, 272, 72), ([40, 9], 2, 1008, 100), ([200, 0, 57, 130], 11, 320, 264), ([700, 0, 900], 5, 512, 768),
         ([2100, 1500], 0, 256, 513), ([5] * 70, 1, 64, 32), ([300, 300], 7, 144, 520), ([33, 100], 0, 16, 8), ([90], 0, 2048, 300), ([3001, 0, 1200], 7, 400, 8000), ([4200], 0, 1296, 7900)]
 
