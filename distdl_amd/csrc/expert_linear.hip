@@ -1,7 +1,7 @@
 // The products of rows with the weights of the expert that each was sent to, and their adjoint: the entry points and the
 // kernel for few rows.  (expert_linear8.hip, expert_linear16.hip, expert_linear32.hip: tiles.)
 //
-// expert_stream (bf16, fp16 and e4m3; few rows for each expert): bound by reading the weights once.  A workgroup has 16 rows of one
+// expert_stream (few rows for each expert): bound by reading the weights once.  A workgroup has 16 rows of one
 // expert's weights; each of its wavefronts takes a part of the reduction, line after line of 128 bytes, straight from memory into
 // registers as a matrix instruction wants them (lane l has bytes 16 (l / 16) and 64 + 16 (l / 16) on of row l % 16: which element of a reduction a
 // lane holds is free if both operands agree), next to the same lines of up to 16 MB rows of the expert's.  The wavefronts' sums meet in
@@ -21,7 +21,7 @@ namespace {
 
 // ------------------------------------------------------------ few rows --
 
-enum Kind { kBf16, kF16, kE4m3 };
+enum Kind { kBf16, kF16, kE4m3, kF32 };
 
 constexpr int kStreamCols = 16;
 template <int KIND>
@@ -39,6 +39,13 @@ __device__ inline floatx4 multiply_line(const Line& w, const Line& x, floatx4 ac
         __builtin_memcpy(&a, &w, 32);
         __builtin_memcpy(&b, &x, 32);
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);   // scales of one
+    } else if constexpr (KIND == kF32) {
+        float a[8], b[8];
+        __builtin_memcpy(a, &w, 32);
+        __builtin_memcpy(b, &x, 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+        return acc;
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -73,7 +80,7 @@ __device__ inline void store_out(const ExpertArgs& g, int64_t row, int64_t n, fl
 template <int KIND, int MB>
 __global__ __launch_bounds__(64 * kStreamWaves<KIND>) void expert_stream(const ExpertArgs g) {
     constexpr int kWaves = kStreamWaves<KIND>, kAhead = 4;   // lines in flight together
-    constexpr int kBytes = KIND == kE4m3 ? 1 : 2;
+    constexpr int kBytes = KIND == kE4m3 ? 1 : KIND == kF32 ? 4 : 2;
     __shared__ floatx4 sums[kWaves][MB][64];
     const int e = blockIdx.y;
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kStreamCols;
@@ -219,19 +226,34 @@ ExpertTile best_for_weights(bool aligned, int64_t rows, int64_t experts, int64_t
 // time for each 32 of the reduction, which four groups share in the smallest.  `tiles` gives their number for an edge.  ([1024, 8192] by 3584: 64 545 us, 128 468; [64, 4096] by 1024 to
 // three experts: 64 71 us, 32 23.)
 template <typename Tiles>
-int best_edge32(Tiles&& tiles, int64_t depth, int cus) {
+int best_edge32(Tiles&& tiles, int64_t depth, int cus, double* us) {
     const double steps = ceil(depth / 32.0), large = tiles(128), fill = large < cus ? large / cus : 1;
     auto turns = [&](double n) { return n < cus ? 1.0 : n / cus; };
     const double us128 = 6 + ceil(large / cus) * (4.5 + steps * (1.57 + 0.15 * fill)), us64 = 5 + turns(tiles(64)) * (1 + steps * 0.57),
                  us32 = 5 + turns(tiles(32)) * (1.5 + ceil(steps / 4) * 0.52);
+    *us = fmin(us128, fmin(us64, us32));
     return us128 < us64 ? (us32 < us128 ? 32 : 128) : us32 < us64 ? 32 : 64;
 }
+// Experts that may have rows, at the most.
+double used_experts(int64_t rows, int64_t experts) { return static_cast<double>(rows < experts ? rows : experts); }
+
+// expert_stream for fp32: the weights at 5.5 TB/s, and for each row the 16 lines of rows that every strip of them reads again.  ([1, 8192] by 3584: tiles 39 us, here 21 (5.5 TB/s);
+// eight rows to each of eight experts of [1000, 260] 8.1 and 4.7, sixteen of [2048, 2048] 24 and 37.)
+bool streams32(const ExpertArgs& g, double tiles_us) {
+    if (!aligned_to(g.a, 16) || !aligned_to(g.w, 16) || g.lda % 4 || g.k % 4 || g.rows > 64ll * g.experts) return false;
+    const double bytes = used_experts(g.rows, g.experts) * g.n * g.k * 4, each = static_cast<double>(g.rows) / g.experts;
+    return 2.5 + bytes / 5.5e6 * (1 + 0.06 * each) < fmax(tiles_us, bytes / 5.1e6);
+}
 int rows32(const char* who, bool transposed, const ExpertArgs& g, hipStream_t s) {
-    const int edge = best_edge32([&](int e) { return row_tiles(g.rows, g.experts, e) * static_cast<double>((g.n + e - 1) / e); }, g.k, g.cus);
+    const double used = used_experts(g.rows, g.experts);
+    double us;
+    const int edge = best_edge32([&](int e) { return fmax(row_tiles(g.rows, g.experts, e), used) * static_cast<double>((g.n + e - 1) / e); }, g.k, g.cus, &us);
+    if (!transposed && streams32(g, us)) return launch_stream<kF32>(who, g, s);
     return edge == 128 ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, edge == 32, transposed, g, s);
 }
 int weights32(const char* who, const ExpertArgs& g, hipStream_t s) {
-    const int edge = best_edge32([&](int e) { return static_cast<double>(g.places) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / g.places, g.cus);
+    double us;
+    const int edge = best_edge32([&](int e) { return static_cast<double>(g.places) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / g.places, g.cus, &us);
     return edge == 128 ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, edge == 32, g, s);
 }
 

@@ -42,6 +42,8 @@ CASES = [
     ([3001, 0, 1200], 7, 72, 8000), ([3001, 0, 1200], 7, 8000, 72), ([9, 0, 130, 2, 64, 1, 70, 200], 3, 2056, 2040),
     # fp32 on the bf16 matrix cores' tiles
     ([513, 0, 600, 490], 3, 1100, 1000), ([400, 0, 700], 0, 2050, 2049),
+    # few rows of fp32 by wavefronts on parts of the reduction, up to four blocks of sixteen
+    ([30] * 8, 0, 260, 1000), ([8, 1, 0, 20] * 2, 5, 260, 1000), ([1], 0, 8192, 40), ([14, 15], 0, 36, 500),
     # rows that are no multiple of 16 bytes
     ([5, 0, 9], 2, 9, 11), ([100, 37], 3, 77, 65), ([260, 300], 0, 513, 331), ([1, 1], 0, 1001, 15)]
 
