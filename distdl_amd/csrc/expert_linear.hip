@@ -251,20 +251,24 @@ int rows32(const char* who, bool transposed, const ExpertArgs& g, hipStream_t s)
     if (!transposed && streams32(g, us)) return launch_stream<kF32>(who, g, s);
     return edge == 128 ? run_expert_rows32_split(who, transposed, g, s) : run_expert_rows32(who, edge == 32, transposed, g, s);
 }
+// Matrices that tiles are chosen for: of the experts that can have too many rows for expert_outer a few do, and then have many.  (All 3000 rows of [128 x 512, 1024] fp32 to one expert: 108 us,
+// with tiles for 46 experts of 65 rows 220.)
+int64_t likely_places(const ExpertArgs& g) { return g.few < 0 ? g.experts : (g.places + 3) / 4; }
 int weights32(const char* who, const ExpertArgs& g, hipStream_t s) {
+    const int64_t places = likely_places(g);
     double us;
-    const int edge = best_edge32([&](int e) { return static_cast<double>(g.places) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / g.places, g.cus, &us);
+    const int edge = best_edge32([&](int e) { return static_cast<double>(places) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / places, g.cus, &us);
     return edge == 128 ? run_expert_weights32_split(who, g, s) : run_expert_weights32(who, edge == 32, g, s);
 }
 
-// Gradients of the weights: experts with at most kFewRows rows go by expert_outer and the others, if there can be any, by tiles in a launch of their own.  So where most are
-// expected to be of the first kind (a row costs the 16-bit one more than tiles), where the second launch can find the others (find_matrix_tile puts up to 64 experts in order) and
-// costs less than what the first one saves, a quarter of a microsecond a megabyte.  ([64 x 1024, 1024] of twelve rows each: fp32 158 -> 58 us; of five to ten rows each, [32 x 1024, 2816] bf16
-// 73 -> 49, [64 x 512, 512] 22 -> 14; fp32 [16 x 3743, 4476] of 24 456 -> 353.  All 190 rows of [8 x 2048, 2048] to one expert: 35 -> 45.)
-constexpr int kFewRows = 32;
+// Gradients of the weights: experts with few rows go by expert_outer and the others, if there can be any, by tiles in a launch of their own.  Up to how many: where tiles take over if all
+// experts have as many (expert_outer's matrix instructions wait for two loads each).  So where most are expected to be of the first kind, and where the second launch costs less than what the first one
+// saves, a quarter of a microsecond a megabyte.  ([64 x 1024, 1024] of twelve rows each: fp32 158 -> 56 us, bf16 72 -> 23, of 48 145 -> 107 and 71 -> 30, of 256 317 -> 499 and 83 -> 62;
+// [8 x 2048, 2048] of 512 bf16 48 -> 52.)
+int few_rows(const ExpertArgs& g) { return g.out_dtype == DDL_DT_F32 ? 64 : 256; }
 bool mostly_few(const ExpertArgs& g) {
     const int64_t size = g.out_dtype == DDL_DT_F32 ? 4 : 2;
-    return g.rows <= (size == 4 ? 24 : 10) * static_cast<int64_t>(g.experts) && (g.rows <= kFewRows || (g.experts <= 64 && g.experts * g.n * g.k * size >= 12 << 20)) && g.n >= 8 && g.k * size >= 16;
+    return g.rows <= (size == 4 ? 40 : 160) * static_cast<int64_t>(g.experts) && (g.rows <= few_rows(g) || g.experts * g.n * g.k * size >= 12 << 20) && g.n >= 4 && g.k * size >= 16;
 }
 
 // expert_stream: the weights at 5.5 TB/s, and the rows that every strip of them reads again; not for more rows than it has in registers.
@@ -380,13 +384,13 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
         d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
         d.places = d.experts, d.few = -1;
         if (mostly_few(d)) {
-            d.few = kFewRows, d.places = d.rows / (kFewRows + 1);   // so many can have more
+            d.few = few_rows(d), d.places = d.rows / (d.few + 1);   // so many can have more
             if (int rc = run_expert_outer(who, d, s)) return rc;
             if (d.places == 0) return 0;
         }
         if (dtype == DDL_DT_F32) return weights32(who, d, s);
         const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
-        return run_expert_weights16(who, best_for_weights(aligned, rows, d.places, n, k, cus), f16, d, dev, s);
+        return run_expert_weights16(who, best_for_weights(aligned, rows, likely_places(d), n, k, cus), f16, d, dev, s);
     }
     return 0;
 }

@@ -1,17 +1,20 @@
-// The gradients of the experts' weights from few rows: dw[e] = sum over the expert's rows of dy_r x_r^T, an outer product for each.
+// The gradients of the experts' weights from few rows: dw[e] = sum over the expert's rows of dy_r x_r^T.
 //
-// Bound by writing dw once.  A wavefront has kSide rows of a matrix by 64 vectors of 16 bytes, kept as 32-bit sums in registers; for each row it reads its vectors of x and
-// (the same in all lanes) kSide elements of dy, and adds kSide products for each element of x.  No LDS, no barrier: what a tile of expert_linear16.hip or expert_linear32.hip waits
-// for at its start and end takes longer than writing it.  ([8 x 2048, 2048] of two rows each: fp32 57 -> 24 us (5.6 TB/s), bf16 29 -> 13; of eight 57 -> 27 and
-// 30 -> 19.)  An expert without rows gets its zeros the same way.  Operands of any address and pitch: the last vector of a row and the last rows of a matrix are moved
+// Bound by writing dw once.  A wavefront has a tile of 64 rows by 16 vectors of 16 bytes of a matrix, its sums in registers, and takes both operands from memory as they lie: a lane
+// reads, of some rows, four elements of dy and one vector of x.  Matrix instruction (i, j) takes element i of every lane's four and element j of its vector, so which row
+// and column of the tile it computes is spread over the lanes, and a lane ends up with whole vectors of dw.  (16-bit elements: eight rows' pairs are put into one register first.)
+// No LDS, no barrier: what a tile of expert_linear16.hip or expert_linear32.hip waits for at its start and end takes longer than writing it.  ([8 x 2048, 2048] bf16 of 2 to 32 rows each 29 us by
+// tiles, here 13 to 14 (5 TB/s), of 128 29 and 20; fp32 of 2 to 16 57 and 28, of 32 49 and 41.  With the products on the vector units, bf16 13 for two rows and 37 for 32.)
+// An expert without rows gets its zeros the same way.  Operands of any address and pitch: the last vector of a row and the last rows of a matrix are moved
 // back to end with it, what is written twice is the same.  Every XCD has an eighth of each expert's wavefronts side by side.
 #include "expert_parts.h"
+#include "gemm16_parts.h"
 #include "ln_elements.h"
 
 namespace ddl {
 namespace {
 
-constexpr int kSide = 8, kOuterThreads = 256, kOuterWaves = kOuterThreads / 64;
+constexpr int kOuterThreads = 256, kOuterWaves = kOuterThreads / 64, kDown = 4;   // kDown: elements of dy that a lane has of a row
 
 struct Outer {
     ExpertArgs g;
@@ -30,12 +33,6 @@ __device__ inline Vector<T, N> load_vector(const T* p) {
     };
     return reinterpret_cast<const Any*>(p)->v;
 }
-__device__ inline float element(const uint32_t* w, int i, const float*) { return __uint_as_float(w[i]); }
-__device__ inline float element(const uint32_t* w, int i, const bf16_t*) { return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16); }
-__device__ inline float element(const uint32_t* w, int i, const __half*) {
-    const __half2 two = __builtin_bit_cast(__half2, w[i / 2]);
-    return i % 2 ? __high2float(two) : __low2float(two);
-}
 __device__ inline u32x4 packed(const float* v, const float*) { return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
 __device__ inline u32x4 packed(const float* v, const bf16_t*) {
     return u32x4{f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
@@ -46,59 +43,88 @@ __device__ inline u32x4 packed(const float* v, const __half*) {
     for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, __floats2half2_rn(v[2 * i], v[2 * i + 1]));
     return o;
 }
+// Element c of eight rows, side by side.
+template <typename V>
+__device__ inline bf16x8 column(const V (&rows)[8], int c) {
+    u32x4 o;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) o[p] = __builtin_amdgcn_perm(rows[2 * p + 1].word[c / 2], rows[2 * p].word[c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(bf16x8, o);
+}
 
 // STREAM: past the caches.
 template <typename T, bool STREAM>
-__global__ __launch_bounds__(kOuterThreads) void expert_outer(const Outer a) {
-    constexpr int N = 16 / static_cast<int>(sizeof(T)), kAhead = 4;   // rows in flight together
+__global__ __launch_bounds__(kOuterThreads, 2) void expert_outer(const Outer a) {
+    constexpr bool k16 = sizeof(T) == 2;
+    constexpr int N = 16 / static_cast<int>(sizeof(T));               // elements of x that a lane has of a row
+    constexpr int kOwn = k16 ? 8 : 4, kRows = 4 * kOwn;               // rows of a lane, and of all four lanes with the same columns, at a time
     const ExpertArgs& g = a.g;
     const int xcd = blockIdx.x % kXcds, nth = blockIdx.x / kXcds, e = nth / a.share;
     const int block = (xcd + e) % kXcds * a.share + nth % a.share;   // few workgroups of an expert: another XCD's for the next one
-    const int lane = threadIdx.x & 63, wave = block * kOuterWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = wave / a.strips, vector = (wave - group * a.strips) * 64 + lane;
-    if (block >= a.blocks || group >= a.groups || vector * static_cast<int64_t>(N) >= g.k) return;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, part = lane >> 4, wave = block * kOuterWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = wave / a.strips;
+    if (block >= a.blocks || group >= a.groups) return;
     int lo, hi;
     rows_of_expert(g, e, lo, hi);
     if (hi - lo > g.few) return;
-    const int64_t k0 = min(vector * static_cast<int64_t>(N), g.k - N), n0 = min(group * static_cast<int64_t>(kSide), g.n - kSide);
-    const T* dy = static_cast<const T*>(g.a) + lo * g.lda + n0;
-    const T* x = static_cast<const T*>(g.w) + lo * g.ldw + k0;
-    float sum[kSide][N];
+    const int64_t k0 = static_cast<int64_t>(wave - group * a.strips) * (16 * N) + l16 * N, n0 = static_cast<int64_t>(group) * (16 * kDown);   // k0: of this lane
+    const int64_t at_k = min(k0, g.k - N), at_n = min(n0 + l16 * kDown, g.n - kDown);
+    floatx4 sum[kDown][N];
 #pragma unroll
-    for (int i = 0; i < kSide; ++i)
+    for (int i = 0; i < kDown; ++i)
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[i][j] = 0.f;
-    for (int left = hi - lo; left > 0; left -= kAhead, dy += kAhead * g.lda, x += kAhead * g.ldw) {
-        Vector<T, N> vx[kAhead];
-        Vector<T, kSide> vd[kAhead];
+        for (int j = 0; j < N; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int r0 = lo; r0 < hi; r0 += kRows) {
+        Vector<T, N> x[kOwn];
+        Vector<T, kDown> dy[kOwn];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int row = u < left ? u : 0;
-            vx[u] = load_vector<T, N>(x + row * g.ldw), vd[u] = load_vector<T, kSide>(dy + row * g.lda);
+        for (int u = 0; u < kOwn; ++u) {
+            const int64_t row = min(r0 + (k16 ? part * kOwn + u : u * 4 + part), hi - 1);
+            x[u] = load_vector<T, N>(static_cast<const T*>(g.w) + row * g.ldw + at_k);
+            dy[u] = load_vector<T, kDown>(static_cast<const T*>(g.a) + row * g.lda + at_n);
         }
-        asm volatile("" ::: "memory");   // else the compiler moves each row's loads behind the sums of the one before it
+        if (r0 + kRows > hi) {   // zeros for rows behind the expert's
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (u >= left) break;
-            uint32_t same[kSide * sizeof(T) / 4];
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(kSide * sizeof(T) / 4); ++i) same[i] = __builtin_amdgcn_readfirstlane(vd[u].word[i]);
-#pragma unroll
-            for (int i = 0; i < kSide; ++i) {
-                const float d = element(same, i, static_cast<const T*>(nullptr));
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum[i][j] += d * element(vx[u].word, j, static_cast<const T*>(nullptr));
+            for (int u = 0; u < kOwn; ++u) {
+                if (r0 + (k16 ? part * kOwn + u : u * 4 + part) >= hi) x[u] = {}, dy[u] = {};
             }
         }
-    }
-    T* const y = static_cast<T*>(g.y) + (e * g.n + n0) * g.k + k0;
+        if constexpr (k16) {
+            bf16x8 down[kDown];
 #pragma unroll
-    for (int i = 0; i < kSide; ++i) {
-        typedef u32x4 any __attribute__((aligned(2)));
-        any* const to = reinterpret_cast<any*>(y + i * g.k);
-        const u32x4 v = packed(sum[i], static_cast<const T*>(nullptr));
-        if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-        else *to = v;
+            for (int i = 0; i < kDown; ++i) down[i] = column(dy, i);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const bf16x8 across = column(x, j);
+#pragma unroll
+                for (int i = 0; i < kDown; ++i) sum[i][j] = mfma<std::is_same_v<T, __half>>(down[i], across, sum[i][j]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kOwn; ++u)
+#pragma unroll
+                for (int i = 0; i < kDown; ++i)
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(dy[u].word[i]), __uint_as_float(x[u].word[j]), sum[i][j], 0, 0, 0);
+        }
+    }
+    // Element q of sum[i][j]: what lane 4 part + q has as element i of dy, and this one as element j of x.
+    T* const y = static_cast<T*>(g.y) + e * g.n * g.k + at_k;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t n = n0 + (4 * part + q) * kDown, from = min(n, g.n - kDown);
+        if (n >= g.n || k0 >= g.k) continue;
+#pragma unroll
+        for (int i = 0; i < kDown; ++i) {
+            float v[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = sum[i][j][q];
+            typedef u32x4 any __attribute__((aligned(2)));
+            any* const to = reinterpret_cast<any*>(y + (from + i) * g.k);
+            if constexpr (STREAM) __builtin_nontemporal_store(packed(v, static_cast<const T*>(nullptr)), to);
+            else *to = packed(v, static_cast<const T*>(nullptr));
+        }
     }
 }
 
@@ -107,13 +133,13 @@ __global__ __launch_bounds__(kOuterThreads) void expert_outer(const Outer a) {
 int run_expert_outer(const char* who, const ExpertArgs& g, hipStream_t s) {
     const int elements = g.out_dtype == DDL_DT_F32 ? 4 : 8;
     Outer a{g};
-    a.strips = static_cast<int>((g.k + 64 * elements - 1) / (64 * elements)), a.groups = static_cast<int>((g.n + kSide - 1) / kSide);
+    a.strips = static_cast<int>((g.k + 16 * elements - 1) / (16 * elements)), a.groups = static_cast<int>((g.n + 16 * kDown - 1) / (16 * kDown));
     a.blocks = (a.strips * a.groups + kOuterWaves - 1) / kOuterWaves, a.share = (a.blocks + kXcds - 1) / kXcds;
     const int64_t blocks = static_cast<int64_t>(a.share) * kXcds * g.experts;
     if (blocks * kOuterThreads > 0xFFFFFFFFll) return fail(DDL_E_UNSUPP, "%s: %lld workgroups", who, static_cast<long long>(blocks));
-    // Rows of whole lines need no cache to put them together, and more rows of x and dy stay in the caches: [8 x 3584, 8192] bf16 of four rows each 85 -> 75 us, [16 x 3743, 4476] of
-    // 24 256 -> 220, of one 90 -> 128.
-    const bool stream = (g.k * (16 / elements) % 128 == 0 && aligned_to(g.y, 128)) || g.rows >= 8 * g.experts;
+    // Rows of whole lines need no cache to put them together, and more rows of x and dy stay there: [8 x 3584, 8192] bf16 of 64 rows each 121 -> 81 us; of no whole lines [16 x 3743, 4476]
+    // of one row 99 -> 186, of 24 118 -> 194, of 100 as much, of 256 335 -> 251.
+    const bool stream = (g.k * (16 / elements) % 128 == 0 && aligned_to(g.y, 128)) || g.rows >= 100ll * g.experts;
     const dim3 grid(static_cast<uint32_t>(blocks)), threads(kOuterThreads);
     auto launch = [&](auto* element) {
         typedef std::remove_pointer_t<decltype(element)> T;

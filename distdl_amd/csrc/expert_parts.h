@@ -16,7 +16,7 @@ struct ExpertArgs {
     int experts, rows, out_dtype, cus;
     int64_t n, k, lda, ldw, w_stride, ldy;
     int tiles_m, tiles_n;                 // tiles_m: of an expert's matrix (gradients of the weights)
-    int places, few;                      // of those with most rows, this many experts, and of them those with more rows than `few` (gradients of the weights)
+    int few, places;                      // gradients of the weights: of experts with more rows than this (-1: all), which are as many or less
 };
 
 // Kernels of expert_linear16.hip: tiles of 64 or 128 rows and columns at any address (edge 64, 128), or large ones, of 128 x 256 (low) or 256 x 256.
@@ -29,7 +29,7 @@ int run_expert_weights32(const char* who, bool small, const ExpertArgs& g, hipSt
 // Of expert_linear32_split.hip: tiles of 128 x 128.
 int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipStream_t s);
 int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
-// Of expert_outer.hip: gradients of the weights of all experts with at most g.few rows (matrices of at least 8 rows, and columns for 16 bytes).
+// Of expert_outer.hip: gradients of the weights of all experts with at most g.few rows (matrices of at least 4 rows, and columns for 16 bytes).
 int run_expert_outer(const char* who, const ExpertArgs& g, hipStream_t s);
 // Of expert_linear8.hip: kAny64, kLow and kLarge (aligned operands, all of them).
 int run_expert_rows8(const char* who, ExpertTile tile, ExpertArgs g, int dev, hipStream_t s);
@@ -128,8 +128,23 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
     }
     if (place >= g.places) return false;
     expert = place;
-    if (g.experts <= 64) {   // a lane for each: how many have more rows, or as many and come before it; of those without rows, how many come before it
-        const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63;
+    if (g.few >= 0) {   // in their order
+        int before = 0;   // of them in front
+        for (int e0 = 0;; e0 += 64) {
+            if (e0 >= g.experts) return false;
+            int from = 0, to = 0;
+            if (e0 + lane < g.experts) rows_of_expert(g, e0 + lane, from, to);
+            const uint64_t long_ones = __ballot(to - from > g.few);
+            const uint64_t here = long_ones & __ballot(before + __popcll(long_ones & ((1ull << lane) - 1)) == place);
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                expert = e0 + l, lo = __builtin_amdgcn_readlane(from, l), hi = __builtin_amdgcn_readlane(to, l);
+                break;
+            }
+            before += __popcll(long_ones);
+        }
+    } else if (g.experts <= 64) {   // a lane for each: how many have more rows, or as many and come before it; of those without rows, how many come before it
         int from = 0, to = 0;
         if (lane < g.experts) rows_of_expert(g, lane, from, to);
         const int rows = to - from;
@@ -150,7 +165,6 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
     } else {
         rows_of_expert(g, expert, lo, hi);
     }
-    if (hi - lo <= g.few) return false;
     constexpr int kBand = 8;
     const int band = rest / (kBand * g.tiles_n), band_h = min(kBand, g.tiles_m - band * kBand), in_band = rest - band * kBand * g.tiles_n;
     const auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };   // so that the compiler knows it

@@ -70,9 +70,11 @@ def test_products_and_adjoint(counts, spare, k, n, dtype):
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
-# few rows for most experts: all of them few, some with 33 and more, none at all; matrices that are no whole vectors or lines, and of the smallest sizes
-FEW = [([2, 1, 0, 4], 0, 256, 264), ([32, 0, 1], 0, 72, 130), ([33, 0, 1], 3, 72, 130), ([40, 1, 0, 2, 100, 0, 3, 1, 1, 70, 5, 5, 2, 33, 1], 9, 520, 96), ([0] * 69 + [20], 0, 64, 40),
-       ([0] * 40 + [500] + [0] * 23, 0, 136, 72), ([5, 9], 2, 9, 11), ([3, 2, 2], 1, 1001, 13), ([1] * 64, 0, 8, 8), ([0, 0, 0], 0, 2050, 9), ([7] * 30, 0, 1030, 258)]
+# few rows for most experts, or for all; from 65 (fp32) or 257 rows on the others' own launch, with more experts than a wavefront has lanes; no rows at all; matrices that are no whole
+# vectors or lines, and of the smallest sizes
+FEW = [([2, 1, 0, 4], 0, 256, 264), ([32, 0, 1], 0, 72, 130), ([33, 0, 1], 3, 72, 130), ([40, 1, 0, 2, 100, 0, 3, 1, 1, 70, 5, 5, 2, 33, 1], 9, 520, 1096), ([0] * 69 + [20], 0, 64, 40),
+       ([0] * 40 + [500] + [0] * 23, 0, 520, 522), ([5, 9], 2, 9, 11), ([3, 2, 2], 1, 1001, 13), ([1] * 64, 0, 8, 8), ([0, 0, 0], 0, 2050, 9), ([7] * 30, 0, 1030, 258),
+       ([64, 65, 256, 257, 31, 0], 5, 1288, 1000), ([3] * 30 + [300, 0, 257, 256] + [1] * 36 + [64, 0, 65, 400], 1, 520, 264), ([150, 90], 0, 77, 65)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES)
