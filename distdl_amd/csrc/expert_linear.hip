@@ -278,6 +278,11 @@ double stream_us(int64_t rows, int64_t experts, int64_t cols, int64_t depth) {
     return 2.5 + used * cols * depth / 5.5e6 * (1 + 0.05 * (each > 4 ? each - 4 : 0));
 }
 
+// Gradients of rows: expert_across, which reads the weights again for every 16 rows, where no expert is expected to have more, and little is lost if one has them all.
+bool few_for_all(const ExpertArgs& g) {
+    return (g.rows <= 16 || (g.rows <= 8 * static_cast<int64_t>(g.experts) && g.rows <= 256)) && g.n * (g.out_dtype == DDL_DT_F32 ? 4 : 2) >= 16;
+}
+
 int check_product(const char* who, int64_t experts, int64_t rows, int64_t n, int64_t k, int64_t least) {
     if (experts < 0 || rows < 0 || n < 1 || k < 1)
         return fail(DDL_E_ARG, "%s: %lld experts, %lld rows, %lld x %lld features", who, static_cast<long long>(experts), static_cast<long long>(rows), static_cast<long long>(n),
@@ -370,7 +375,9 @@ int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int
         ExpertArgs d = g;
         d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
         int rc;
-        if (dtype == DDL_DT_F32) {
+        if (few_for_all(d)) {
+            rc = run_expert_across(who, d, s);
+        } else if (dtype == DDL_DT_F32) {
             rc = rows32(who, true, d, s);
         } else {
             const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;

@@ -8,8 +8,7 @@
 // An expert without rows gets its zeros the same way.  Operands of any address and pitch: the last vector of a row and the last rows of a matrix are moved
 // back to end with it, what is written twice is the same.  Every XCD has an eighth of each expert's wavefronts side by side.
 #include "expert_parts.h"
-#include "gemm16_parts.h"
-#include "ln_elements.h"
+#include "expert_vectors.h"
 
 namespace ddl {
 namespace {
@@ -20,37 +19,6 @@ struct Outer {
     ExpertArgs g;
     int strips, groups, blocks, share;   // of an expert's matrix: wavefronts across and down, workgroups, of those an XCD's
 };
-
-// N elements as they lie.
-template <typename T, int N>
-struct Vector {
-    uint32_t word[N * sizeof(T) / 4];
-};
-template <typename T, int N>
-__device__ inline Vector<T, N> load_vector(const T* p) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Any {
-        Vector<T, N> v;
-    };
-    return reinterpret_cast<const Any*>(p)->v;
-}
-__device__ inline u32x4 packed(const float* v, const float*) { return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
-__device__ inline u32x4 packed(const float* v, const bf16_t*) {
-    return u32x4{f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
-}
-__device__ inline u32x4 packed(const float* v, const __half*) {
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, __floats2half2_rn(v[2 * i], v[2 * i + 1]));
-    return o;
-}
-// Element c of eight rows, side by side.
-template <typename V>
-__device__ inline bf16x8 column(const V (&rows)[8], int c) {
-    u32x4 o;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) o[p] = __builtin_amdgcn_perm(rows[2 * p + 1].word[c / 2], rows[2 * p].word[c / 2], c % 2 ? 0x07060302u : 0x05040100u);
-    return __builtin_bit_cast(bf16x8, o);
-}
 
 // STREAM: past the caches.
 template <typename T, bool STREAM>
@@ -120,10 +88,7 @@ __global__ __launch_bounds__(kOuterThreads, 2) void expert_outer(const Outer a) 
             float v[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = sum[i][j][q];
-            typedef u32x4 any __attribute__((aligned(2)));
-            any* const to = reinterpret_cast<any*>(y + (from + i) * g.k);
-            if constexpr (STREAM) __builtin_nontemporal_store(packed(v, static_cast<const T*>(nullptr)), to);
-            else *to = packed(v, static_cast<const T*>(nullptr));
+            store_vector<N, STREAM>(y + (from + i) * g.k, v);
         }
     }
 }

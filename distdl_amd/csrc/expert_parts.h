@@ -31,6 +31,8 @@ int run_expert_rows32_split(const char* who, bool transposed, ExpertArgs g, hipS
 int run_expert_weights32_split(const char* who, ExpertArgs g, hipStream_t s);
 // Of expert_outer.hip: gradients of the weights of all experts with at most g.few rows (matrices of at least 4 rows, and columns for 16 bytes).
 int run_expert_outer(const char* who, const ExpertArgs& g, hipStream_t s);
+// Of expert_across.hip: gradients of few rows (matrices with columns for 16 bytes).
+int run_expert_across(const char* who, const ExpertArgs& g, hipStream_t s);
 // Of expert_linear8.hip: kAny64, kLow and kLarge (aligned operands, all of them).
 int run_expert_rows8(const char* who, ExpertTile tile, ExpertArgs g, int dev, hipStream_t s);
 

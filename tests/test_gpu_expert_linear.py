@@ -44,6 +44,8 @@ CASES = [
     ([513, 0, 600, 490], 3, 1100, 1000), ([400, 0, 700], 0, 2050, 2049),
     # few rows of fp32 by wavefronts on parts of the reduction, up to four blocks of sixteen
     ([30] * 8, 0, 260, 1000), ([8, 1, 0, 20] * 2, 5, 260, 1000), ([1], 0, 8192, 40), ([14, 15], 0, 36, 500),
+    # few rows for most: their gradients by wavefronts on parts of the reduction, sixteen at a time
+    ([40, 1, 0, 2, 5, 1, 1], 3, 264, 72), ([33, 1, 0, 2, 1, 1, 1], 0, 77, 65), ([2] * 70, 1, 136, 1000), ([16], 0, 4100, 520), ([3] * 64, 0, 600, 40),
     # rows that are no multiple of 16 bytes
     ([5, 0, 9], 2, 9, 11), ([100, 37], 3, 77, 65), ([260, 300], 0, 513, 331), ([1, 1], 0, 1001, 15)]
 
