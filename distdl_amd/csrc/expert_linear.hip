@@ -1,5 +1,5 @@
 // The products of rows with the weights of the expert that each was sent to, and their adjoint: the entry points and the
-// kernel for few rows.  (expert_linear8.hip, expert_linear16.hip, expert_linear32.hip: tiles.)
+// kernel for few rows.  (expert_linear8.hip, expert_linear16.hip, expert_linear32.hip, expert_linear32_split.hip: tiles; expert_across.hip, expert_outer.hip: gradients of few rows.)
 //
 // expert_stream (few rows for each expert): bound by reading the weights once.  A workgroup has 16 rows of one
 // expert's weights; each of its wavefronts takes a part of the reduction, line after line of 128 bytes, straight from memory into

@@ -196,7 +196,7 @@ __device__ inline void zero_block(E* y, int64_t ldy, int rows, int cols) {
 }
 
 // Zeros in this workgroup's part of an expert's matrix, where all of its tiles' are: parts that lie side by side in the order of the workgroups, in whole lines
-// (a training step of two rows with [26 x 4384, 2296] fp32, of which one expert has them: 320 us tile by tile, 194 in the tiles' order, here 176: 6.0 TB/s).
+// (25 of [26 x 4384, 2296] fp32: 320 us tile by tile, 194 in the tiles' order, here 176: 6.0 TB/s).
 template <typename E>
 __device__ inline void zero_part(const ExpertArgs& g, const MatrixTask& t) {
     const int64_t bytes = g.n * g.k * static_cast<int64_t>(sizeof(E)), each = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
