@@ -1,12 +1,12 @@
 // Root-mean-square norm of rows, with the addition of a residual in front and an 8-bit output behind it in the same pass:
 //   h = x + residual (rounded to its type: the stream that goes on),  y = h / sqrt(mean of h^2 + eps) * weight,
-// or, in 8 bits, scale = max(max |y| / 448, 2^-126) and code = e4m3(y / scale) for each row; and the adjoint,
+// or, in 8 bits, scale = max(max |y| / 448, 2^-126) and code = e4m3(y / scale) for each row (the quotient rounded once); and the adjoint,
 //   g = dy weight,  xhat = h rstd,  dx = rstd (g - xhat mean(g xhat)) + dh,  dweight = sum over rows of dy xhat.
 //
 // Bound by HBM: every operand is read and every result written once.  A row is held in the registers of a group of 64 to 1024
 // threads, eight elements a thread and piece, so the sums, the largest value and the results need no second reading; the adjoint
 // forms rstd again from h, which it reads for the gradient anyway, instead of keeping it.  A group walks over some rows, the next one asked for
-// while one is summed ([8192, 8192] bf16 on operands that stay: norm with a residual 92 -> 80 us, in 8 bits 105 -> 91, adjoint 132 -> 107; groups of 256 or
+// while one is summed ([8192, 8192] bf16 on operands that stay: norm with a residual 92 -> 80 us, adjoint 132 -> 107; groups of 256 or
 // 512 threads with more pieces were no faster, the adjoint 119 to 180).  Rows at any address and of any
 // length: the last piece of a row is moved back until it ends with the row, and what it then holds twice does not count in the
 // sums.  Sums, rstd, scales and the weight's partial sums are 32-bit floats; results are rounded once.
@@ -178,6 +178,16 @@ __device__ inline float over_parts(const float* sums, int nparts, int64_t rows, 
     return t;
 }
 
+// v / scale as one rounding gives it, from the rounded reciprocal: the first product is off by less than 1.5 steps, the first correction leaves less than one, and the
+// second, of an exact remainder, the rounded quotient.  Both factors are lifted where remainders of quotients that are no code of zero would be subnormal numbers.  A remainder of
+// zero leaves a zero its sign.  ([8192, 8192] bf16 in 8 bits 40 us, by divisions 48; by the reciprocal alone 35, but next to a border some codes were their neighbours.  With norm and residual 95, 99
+// and 91.)
+__device__ inline float quotient(float v, float scale, float inverse) {
+    float q = v * inverse;
+    q = fmaf(-fmaf(q, scale, -v), inverse, q);
+    return fmaf(-fmaf(q, scale, -v), inverse, q);
+}
+
 template <int THREADS>
 constexpr int kBlockOf = THREADS < 256 ? 256 : THREADS;
 
@@ -272,7 +282,8 @@ __global__ __launch_bounds__(kBlockOf<THREADS>) void rms_rows(const RmsArgs a) {
                 }
             }
             over_group<THREADS, 1, true>(top, lds, turn);
-            const float scale = fmaxf(top[0] * (1.f / kE4m3Max), kSmallestScale), inverse = 1.f / scale;
+            const float scale = fmaxf(top[0] * (1.f / kE4m3Max), kSmallestScale);   // the rounded reciprocal's product
+            const float lift = scale < 0x1p-60f ? 0x1p64f : 1.f, lifted = scale * lift, inverse = 1.f / lifted;
             if (t == 0) a.scales[row] = scale;
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
@@ -280,7 +291,7 @@ __global__ __launch_bounds__(kBlockOf<THREADS>) void rms_rows(const RmsArgs a) {
                 result(p, y);
 #pragma unroll
                 for (int e = 0; e < kPiece; ++e) {
-                    const float v = y[e] * inverse;   // up to 448 and a rounding; not a number stays none
+                    const float v = quotient(y[e] * lift, lifted, inverse);   // up to 448 and a rounding; not a number stays none
                     y[e] = v != v ? v : fminf(fmaxf(v, -kE4m3Max), kE4m3Max);
                 }
                 int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);

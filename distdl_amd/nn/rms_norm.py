@@ -119,8 +119,8 @@ def rms_norm_shard(x, weight=None, residual=None, *, eps=1e-6, eight_bit=False):
 
 
 def quantize_rows(x):
-    """``(codes, scales)``: rows (the last dimension) of ``x`` in 8 bits, ``code = e4m3(x / scale)``, ``scale = max(max |x| / 448, 2^-126)`` for each row.
-    A row with an infinity in it stands for no numbers.  No gradient."""
+    """``(codes, scales)``: rows (the last dimension) of ``x`` in 8 bits, ``code = e4m3(x / scale)``, ``scale = max(max |x| / 448, 2^-126)`` for each row (by
+    the rounded 1 / 448; the code is that of the rounded quotient).  A row with an infinity in it stands for no numbers.  No gradient."""
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("rows in 8 bits have no gradient: call this under torch.no_grad(), or detach the operand")
     res = _lib.front().quantize_rows(x)

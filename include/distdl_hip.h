@@ -739,8 +739,9 @@ int ddl_attention_backward(const void* dout, const int64_t* dout_strides,
  *   weight    cols elements of the type, or NULL
  *   y         [rows, cols]; or, instead of it,
  *   codes     [rows, cols] e4m3 (OCP) and scales [rows]: code = e4m3(y / scale),
- *             scale = max(max |y| / 448, 2^-126).  A row with an infinity or not a
- *             number in it stands for no numbers.
+ *             scale = max(max |y| / 448, 2^-126).  The scale is the rounded product
+ *             with the rounded 1 / 448, the quotient is rounded once.  A row with an
+ *             infinity or not a number in it stands for no numbers.
  * Columns spread over workers: with own_squares [rows] the launch leaves this
  * worker's sums of h^2 there (and `sum`) and nothing else; with part_squares
  * [nparts, rows], those of all workers, rows are normalised as if they had
