@@ -81,7 +81,7 @@ std::optional<Two> rms_norm_backward(const Tensor& dy, const Tensor& h, const Ma
 std::optional<std::tuple<Tensor, Tensor>> expert_plan(const Tensor& ids, int64_t low, int64_t high);
 std::optional<Two> expert_sort(const Tensor& x, const Tensor& place, const Tensor& offsets, const MaybeTensor& scales);
 MaybeTensor expert_combine(const Tensor& y, const Tensor& place, const Tensor& offsets, const MaybeTensor& weights);
-std::optional<Two> expert_combine_backward(const Tensor& dout, const Tensor& y, const Tensor& place, const Tensor& offsets, const Tensor& weights, bool want_rows,
+std::optional<Two> expert_combine_backward(const Tensor& dout, const MaybeTensor& y, const Tensor& place, const Tensor& offsets, const Tensor& weights, bool want_rows,
                                            bool want_weights);
 MaybeTensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets);
 MaybeTensor expert_linear_8bit(const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& x_scales, const Tensor& w_scales, at::ScalarType dtype);

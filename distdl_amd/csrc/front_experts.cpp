@@ -105,16 +105,16 @@ MaybeTensor expert_combine(const Tensor& y, const Tensor& place, const Tensor& o
     return out;
 }
 
-std::optional<Two> expert_combine_backward(const Tensor& dout, const Tensor& y, const Tensor& place, const Tensor& offsets, const Tensor& weights, bool want_rows,
+std::optional<Two> expert_combine_backward(const Tensor& dout, const MaybeTensor& y, const Tensor& place, const Tensor& offsets, const Tensor& weights, bool want_rows,
                                            bool want_weights) {
-    if (!plan_tensors(place, offsets) || !rows_of(dout, place.size(0)) || !float_code(dout) || !floats_of(weights, place.sizes()) || !rows_of(y, place.numel()) ||
-        y.size(1) != dout.size(1) || y.scalar_type() != dout.scalar_type())
+    if (!plan_tensors(place, offsets) || !rows_of(dout, place.size(0)) || !float_code(dout) || !floats_of(weights, place.sizes()) ||
+        (want_weights && (!y || !rows_of(*y, place.numel()) || y->size(1) != dout.size(1) || y->scalar_type() != dout.scalar_type())))
         return std::nullopt;
     const int64_t cols = dout.size(1);
     Tensor dy, dweights;
     if (want_rows) dy = at::empty({place.numel(), cols}, dout.options());
     if (want_weights) dweights = floats(dout, place.sizes());
-    check(ddl_expert_combine_backward(dout.data_ptr(), y.data_ptr(), float_code(dout), place.size(0), place.size(1), cols, cols, cols, place.data_ptr<int32_t>(),
+    check(ddl_expert_combine_backward(dout.data_ptr(), want_weights ? pointer(y) : nullptr, float_code(dout), place.size(0), place.size(1), cols, cols, cols, place.data_ptr<int32_t>(),
                                       held_of(offsets), weights.data_ptr<float>(), pointer(dy), static_cast<float*>(pointer(dweights)), current_stream()),
           "ddl_expert_combine_backward");
     return Two(want_rows ? MaybeTensor(dy) : std::nullopt, want_weights ? MaybeTensor(dweights) : std::nullopt);

@@ -619,9 +619,9 @@ struct ExpertCombine {
         std::optional<Two> res;
         {
             at::NoGradGuard no_grad;
-            if (weights) res = expert_combine_backward(dout, kept[0], kept[2], kept[3], *weights, need_y, need_w);
+            if (weights) res = expert_combine_backward(dout, defined(kept[0]), kept[2], kept[3], *weights, need_y, need_w);
             else if (const auto sorted = expert_sort(dout, kept[2], kept[3], std::nullopt)) res = Two(std::get<0>(*sorted), std::nullopt);
-            if (!res) res = general->call<Two>(dout, kept[0], weights, kept[2], kept[3], need_y, need_w);
+            if (!res) res = general->call<Two>(dout, defined(kept[0]), weights, kept[2], kept[3], need_y, need_w);
         }
         return final_gradients(gradients({std::get<0>(*res), std::get<1>(*res)}), kName);
     }
@@ -636,7 +636,7 @@ MaybeTensor expert_combine_shard(const Tensor& y, const MaybeTensor& weights, co
     }
     if (!out || !at::GradMode::is_enabled() || !(wanted(y) || wanted(weights))) return out;
     auto node = make_node(ExpertCombine{general}, {y, weights});
-    node->save(y);
+    node->save(wanted(weights) ? y : Tensor());     // for the weights' gradient alone
     node->save(weights ? *weights : Tensor());
     node->save(place);
     node->save(offsets);

@@ -1566,7 +1566,7 @@ def expert_combine(y, place, offsets, weights=None):
 
 
 def expert_combine_backward(dout, y, place, offsets, weights, want_rows=True, want_weights=True):
-    """Adjoint of ``expert_combine``: ``(dy, dweights)``, None where not wanted."""
+    """Adjoint of ``expert_combine``: ``(dy, dweights)``, None where not wanted; ``y`` is for the weights' alone."""
     name = "expert_combine_backward"
     _require_gpu(dout, y, place, offsets, weights)
     _check_place(place, offsets, dout, name)
@@ -1574,6 +1574,8 @@ def expert_combine_backward(dout, y, place, offsets, weights, want_rows=True, wa
     dout = _rows_of(dout, tokens, name, "gradients, one row for each token")
     weights = _slot_weights(weights, place, name)
     if want_weights:
+        if y is None:
+            raise ValueError(f"{name}: the weights' gradients need the rows")
         if y.dtype != dout.dtype or y.shape[1:] != dout.shape[1:]:
             raise ValueError(f"{name}: gradients {tuple(dout.shape)} {dout.dtype} of rows {tuple(y.shape)} {y.dtype}")
         y = _rows_of(y, tokens * chosen, name, "rows, one for each choice")

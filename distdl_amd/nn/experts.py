@@ -96,7 +96,8 @@ class _ExpertCombine(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, y, weights, place, offsets):
-        ctx.save_for_backward(y, weights, place, offsets)
+        ctx.save_for_backward(y if weights is not None and ctx.needs_input_grad[1] else None, weights, place, offsets)
+        ctx.dtype = y.dtype
         return hip_ops.expert_combine(y, place, offsets, weights)
 
     @staticmethod
@@ -104,7 +105,7 @@ class _ExpertCombine(torch.autograd.Function):
     def backward(ctx, grad):
         y, weights, place, offsets = ctx.saved_tensors
         need_y, need_w = ctx.needs_input_grad[:2]
-        grad = grad if grad.dtype == y.dtype else grad.to(y.dtype)
+        grad = grad if grad.dtype == ctx.dtype else grad.to(ctx.dtype)
         return _general_combine_backward(grad, y, weights, place, offsets, need_y, need_w) + (None, None)
 
 
