@@ -178,6 +178,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     };
     auto values = [&](int s) { tile.transposed(run.acc, v_block(s), 0, before); };
     auto step = [&](int s, auto ahead, auto behind) {
+        if constexpr (sizeof(T) == 2) wait_states<12>(scores);
         if (32 * (s + 1) > wave_least) mask_scores(scores, seen - 32 * s - 4 * half);
         run.follow(scores, a.scale_log2, tile, behind ? &before : nullptr);
         floatx16 next;

@@ -203,6 +203,7 @@ __device__ __forceinline__ void small_product(const Part32& p, int number, int s
         multiply(Second{}, Second{}, End{});
         slot = next;
     }
+    wait_states_acc<18>(acc);
     if (FOLD) {
         fold();
         acc = folded;

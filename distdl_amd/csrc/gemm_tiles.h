@@ -47,6 +47,21 @@ __device__ inline void dma16(u32x4 buffer, int voffset, int soffset, const char*
 // and all LDS reads have returned.
 constexpr int wait_vm_lgkm0(int n) { return 0x0070 | (n & 15) | ((n >> 4) << 14); }
 
+// N wait states (instructions' slots) between matrix instructions and what reads their results from here on.  Hardware does not wait there; the compiler fills the slots
+// that a way through the program lacks, but where a longer and a shorter way from the same matrix instruction meet it may look at the longer one alone.  To be put where
+// ways meet behind matrix instructions whose results are read next: a reader needs 18 for 32 x 32 x 2 of fp32 and 12 for 32 x 32 x 16 of 16 bits.  (With 12 of those 18 the last
+// products of fp32 tiles were missing in some elements.)  The results go through the instruction, so that no copy of them comes before it: in accumulation registers, or in ordinary ones.
+template <int N, typename V>
+__device__ inline void wait_states_acc(V& results) {
+    static_assert(N > 16 && N <= 32, "two instructions");
+    asm volatile("s_nop 15\n\ts_nop %1" : "+a"(results) : "n"(N - 17));
+}
+template <int N, typename V>
+__device__ inline void wait_states(V& results) {
+    static_assert(N >= 1 && N <= 16, "one instruction");
+    asm volatile("s_nop %1" : "+v"(results) : "n"(N - 1));
+}
+
 // The columns of the output that one kind of tile covers: operands and result
 // already offset to the first of those columns.
 template <typename E>
