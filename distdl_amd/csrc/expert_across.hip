@@ -21,13 +21,13 @@ __global__ __launch_bounds__(64 * kAcrossWaves) void expert_across(const ExpertA
     const int e = blockIdx.y;
     int lo, hi;
     rows_of_expert(g, e, lo, hi);
-    if (lo == hi) return;
     T* const y = static_cast<T*>(g.y);
-    if (e == g.experts) {   // the rows of none lie side by side
-        const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-        zero_run(reinterpret_cast<char*>(y + lo * g.ldy), (hi - lo) * g.ldy * static_cast<int64_t>(sizeof(T)), thread, static_cast<int64_t>(gridDim.x) * blockDim.x);
+    if (e == g.experts) {   // rows of none: those behind the last expert's, and those in front of the first one's
+        zero_rows(g, lo, hi - lo, blockIdx.x, gridDim.x);
+        zero_rows(g, 0, min(max(g.offsets[0], 0), lo), blockIdx.x, gridDim.x);
         return;
     }
+    if (lo == hi) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, part = lane >> 4;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (16 * C);
     const T* const w = static_cast<const T*>(g.w) + e * g.w_stride + min(c0 + l16 * C, g.n - C);

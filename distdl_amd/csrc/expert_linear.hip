@@ -86,12 +86,12 @@ __global__ __launch_bounds__(64 * kStreamWaves<KIND>) void expert_stream(const E
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kStreamCols;
     int lo, hi;
     rows_of_expert(g, e, lo, hi);
-    if (lo == hi) return;
-    if (e == g.experts) {   // the rows of none lie side by side
-        const int64_t size = g.out_dtype == DDL_DT_F32 ? 4 : 2, thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-        zero_run(static_cast<char*>(g.y) + lo * g.ldy * size, (hi - lo) * g.ldy * size, thread, static_cast<int64_t>(gridDim.x) * blockDim.x);
+    if (e == g.experts) {   // rows of none: those behind the last expert's, and those in front of the first one's
+        zero_rows(g, lo, hi - lo, blockIdx.x, gridDim.x);
+        zero_rows(g, 0, min(max(g.offsets[0], 0), lo), blockIdx.x, gridDim.x);
         return;
     }
+    if (lo == hi) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, part = lane >> 4;
     const int64_t bytes = g.k * kBytes;
     const int lines = static_cast<int>(bytes / 128), end = static_cast<int>(bytes % 128) - part * 16;

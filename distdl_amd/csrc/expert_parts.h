@@ -45,6 +45,22 @@ __device__ inline void rows_of_expert(const ExpertArgs& g, int e, int& lo, int& 
     hi = e == g.experts ? g.rows : min(max(g.offsets[e + 1], lo), g.rows);
 }
 
+// Zeros in `bytes` from `to` on (any address), by the threads `first`, first + step, ...
+__device__ inline void zero_run(char* to, int64_t bytes, int64_t first, int64_t step) {
+    typedef u32x4 any __attribute__((aligned(1)));
+    if (bytes < 16) {
+        for (int64_t i = first; i < bytes; i += step) to[i] = 0;
+        return;
+    }
+    for (int64_t i = first * 16; i < bytes; i += step * 16) *reinterpret_cast<any*>(to + (i + 16 <= bytes ? i : bytes - 16)) = u32x4{0, 0, 0, 0};
+}
+
+// Zeros in rows from `row` on (they lie side by side), by `blocks` workgroups of which this one is number `block`.
+__device__ inline void zero_rows(const ExpertArgs& g, int row, int rows, int64_t block, int64_t blocks) {
+    const int64_t size = g.out_dtype == DDL_DT_F32 ? 4 : 2;
+    zero_run(static_cast<char*>(g.y) + row * g.ldy * size, rows * g.ldy * size, block * blockDim.x + threadIdx.x, blocks * blockDim.x);
+}
+
 struct ExpertTask {
     int expert;        // g.experts: rows that belong to none, which get zeros; -1: nothing to do
     int row, rows;     // first row of the tile, and rows from it to the expert's last
@@ -54,7 +70,7 @@ struct ExpertTask {
 
 // Tile number `id` of those of `edge` rows: every XCD has a contiguous part of their sequence, which goes expert by expert and inside
 // one in bands of eight tiles of rows, so that the workgroups resident on an XCD share their operands in its L2.  The same in all
-// lanes of a wavefront, each of which looks at one expert of 64.
+// lanes of a wavefront, each of which looks at one expert of 64.  Rows in front of the first expert's get their zeros here, from all workgroups.
 // HALVES: where the last round of one workgroup a CU would leave half of them idle or more, its tiles go in halves.  ([8192, 4096] by 4096 to 8 experts, bf16:
 // 262 -> 243 us, rows' gradients 260 -> 241; e4m3 tiles of half the rows take too much of a whole one's time to gain.)
 template <bool HALVES>
@@ -70,6 +86,11 @@ __device__ inline ExpertTask find_tile(const ExpertArgs& g, int edge, int id) {
     int total = 0, lo, n;
     for (int e0 = 0; e0 <= g.experts; e0 += 64) {
         int t = tiles_of(e0 + lane, lo, n);
+        const int front = e0 == 0 ? __builtin_amdgcn_readfirstlane(lo) : 0;
+        if (front > 0) {
+            zero_rows(g, 0, front, blockIdx.x, gridDim.x);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // a tile counts its own requests, and finds none of these
+        }
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) t += __shfl_xor(t, d);
         total += __builtin_amdgcn_readfirstlane(t);
@@ -177,16 +198,6 @@ __device__ inline bool find_matrix_tile(const ExpertArgs& g, int id, MatrixTask&
 inline int64_t matrix_blocks(const ExpertArgs& g) {
     const int64_t each = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
     return each < 8 * kXcds ? each * g.places : (each + kXcds - 1) / kXcds * kXcds * g.places;
-}
-
-// Zeros in `bytes` from `to` on (any address), by the threads `first`, first + step, ...
-__device__ inline void zero_run(char* to, int64_t bytes, int64_t first, int64_t step) {
-    typedef u32x4 any __attribute__((aligned(1)));
-    if (bytes < 16) {
-        for (int64_t i = first; i < bytes; i += step) to[i] = 0;
-        return;
-    }
-    for (int64_t i = first * 16; i < bytes; i += step * 16) *reinterpret_cast<any*>(to + (i + 16 <= bytes ? i : bytes - 16)) = u32x4{0, 0, 0, 0};
 }
 
 // Zeros in `rows` rows of `cols` elements from y on, by all threads of the workgroup: 32 of them for a row.

@@ -165,7 +165,8 @@ def _general_linear_backward(grad, x, weight, offsets, want_input, want_weight):
 def expert_linear_shard(x, weight, offsets, *, x_scales=None, weight_scales=None, dtype=None):
     """Rows of ``x`` [rows, in], sorted by expert, times their experts' weights [experts, out, in]: [rows, out].
 
-    ``offsets``: int32 [experts + 1] on the device, as ``ExpertPlan.offsets``, the first one 0; rows behind the last expert's become zeros, and take zero gradients.
+    ``offsets``: int32 [experts + 1] on the device, as ``ExpertPlan.offsets``, or a part of those for a part of the experts; rows in front of the first expert's and
+    behind the last one's become zeros, and take zero gradients.
     e4m3 rows (torch.float8_e4m3fn) come with ``x_scales`` [rows] and ``weight_scales`` [experts, out], both float32, and the result is in
     ``dtype`` (default bfloat16); they have no gradient, and their products are added as the matrix cores do, in eights whose members are cut off at 2^-13 of the largest.  16-bit matrices have at least 8 rows and columns, those of e4m3 a multiple of 16 columns."""
     if x.dtype == torch.float8_e4m3fn:

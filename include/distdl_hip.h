@@ -819,9 +819,10 @@ int ddl_expert_combine_backward(const void* dout, const void* y, int dtype,
 
 /* The experts' products: y[i] = w[e] x[i] for rows i of expert e, offsets[e] <= i <
  * offsets[e + 1] (device, int32 [experts + 1], not decreasing; values outside 0 .. rows
- * count as those), zeros for rows from offsets[experts] on.
+ * count as those), zeros for rows of no expert: those from offsets[experts] on, and
+ * those in front of offsets[0].
  *   x [rows, k], pitch ld_x;  w [experts, n, k], contiguous;  y [rows, n], contiguous
- * fp32, bf16 or fp16, summed in 32 bits.  Rows in front of offsets[0] are left as they are.  16-bit
+ * fp32, bf16 or fp16, summed in 32 bits.  16-bit
  * matrices have at least 8 rows and columns; pitches up to 2^22 elements; matrices
  * of fewer than 2^29 elements (DDL_E_UNSUPP). */
 int ddl_expert_linear(const void* x, const void* w, int dtype,
