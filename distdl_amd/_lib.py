@@ -173,6 +173,8 @@ SIGNATURES = {
                                        c_void_p]),
     "ddl_expert_linear_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                            c_void_p, c_void_p]),
+    "ddl_expert_linear_backward_long": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                                c_void_p, c_void_p]),
     "ddl_colsum_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

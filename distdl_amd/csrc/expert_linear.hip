@@ -254,7 +254,8 @@ int rows32(const char* who, bool transposed, const ExpertArgs& g, hipStream_t s)
 // Matrices that tiles are chosen for: of the experts that can have too many rows for expert_outer a few do, and then have many.  (All 3000 rows of [128 x 512, 1024] fp32 to one expert: 108 us,
 // with tiles for 46 experts of 65 rows 220.)
 int64_t likely_places(const ExpertArgs& g) { return g.few < 0 ? g.experts : (g.places + 3) / 4; }
-int weights32(const char* who, const ExpertArgs& g, hipStream_t s) {
+int weights32(const char* who, const ExpertArgs& g, bool within, hipStream_t s) {
+    if (!within) return run_expert_weights32_split(who, g, s);   // whose offsets have 64 bits
     const int64_t places = likely_places(g);
     double us;
     const int edge = best_edge32([&](int e) { return static_cast<double>(places) * ((g.n + e - 1) / e) * ((g.k + e - 1) / e); }, g.rows / places, g.cus, &us);
@@ -291,6 +292,58 @@ int check_product(const char* who, int64_t experts, int64_t rows, int64_t n, int
     if (rows > 0x3FFFFFFF || experts > 65534 || n > 0x3FFFFF || k > 0x3FFFFF || (n + 64) * (k + 64) > kMostSpan / 2)
         return fail(DDL_E_UNSUPP, "%s: %lld experts of %lld x %lld features and %lld rows", who, static_cast<long long>(experts), static_cast<long long>(n), static_cast<long long>(k),
                     static_cast<long long>(rows));
+    return 0;
+}
+
+// limited: fp32 weights' gradients of rows beyond 32-bit byte offsets are refused.
+int product_backward(const char* who, bool limited, const void* dy, const void* x, const void* w, int dtype, const int32_t* offsets, int64_t experts, int64_t rows, int64_t n,
+                     int64_t k, int64_t ld_dy, int64_t ld_x, void* dx, void* dw, void* stream) {
+    if (dtype != DDL_DT_F32 && dtype != DDL_DT_BF16 && dtype != DDL_DT_F16) return fail(DDL_E_ARG, "%s: dtype %d", who, dtype);
+    if (int rc = check_product(who, experts, rows, n, k, dtype == DDL_DT_F32 ? 1 : 8)) return rc;
+    if ((dx && rows) || (dw && experts)) {
+        if (!offsets || (rows && !dy) || (dx && experts && !w) || (dw && rows && !x)) return fail(DDL_E_ARG, "%s: null pointer", who);
+    }
+    if (rows > 1 && (ld_dy < n || (dw && ld_x < k))) return fail(DDL_E_ARG, "%s: pitch below %lld or %lld features", who, static_cast<long long>(n), static_cast<long long>(k));
+    if (ld_dy > 0x3FFFFF || (dw && ld_x > 0x3FFFFF)) return fail(DDL_E_UNSUPP, "%s: pitch above 2^22 elements", who);
+    const int64_t pitch_dy = rows > 1 ? ld_dy : n, pitch_x = rows > 1 ? ld_x : k;
+    const int64_t span = (rows + 64) * (dw && pitch_x > pitch_dy ? pitch_x : pitch_dy);
+    const bool within = span <= (dtype == DDL_DT_F32 ? kMostSpan / 2 : kMostSpan);
+    if (limited && dw && experts && dtype == DDL_DT_F32 && !within)
+        return fail(DDL_E_UNSUPP, "%s: %lld rows, %lld elements apart, are more than 2^31 bytes", who, static_cast<long long>(rows), static_cast<long long>(pitch_x > pitch_dy ? pitch_x : pitch_dy));
+    int dev = 0;
+    const int cus = compute_units(dev);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool f16 = dtype == DDL_DT_F16;
+    ExpertArgs g{};
+    g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
+    if (dx && rows) {   // rows of n features by w read along its k columns
+        ExpertArgs d = g;
+        d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
+        int rc;
+        if (few_for_all(d)) {
+            rc = run_expert_across(who, d, s);
+        } else if (dtype == DDL_DT_F32) {
+            rc = rows32(who, true, d, s);
+        } else {
+            const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;
+            double us;
+            rc = run_expert_rows16(who, best_for_rows(kCosts16, aligned, rows, experts, k, 2 * n, cus, &us), f16, true, d, dev, s);
+        }
+        if (rc) return rc;
+    }
+    if (dw && experts) {
+        ExpertArgs d = g;
+        d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
+        d.places = d.experts, d.few = -1;
+        if (mostly_few(d)) {
+            d.few = few_rows(d), d.places = d.rows / (d.few + 1);   // so many can have more
+            if (int rc = run_expert_outer(who, d, s)) return rc;
+            if (d.places == 0) return 0;
+        }
+        if (dtype == DDL_DT_F32) return weights32(who, d, within, s);
+        const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
+        return run_expert_weights16(who, best_for_weights(aligned, rows, likely_places(d), n, k, cus), f16, d, dev, s);
+    }
     return 0;
 }
 
@@ -351,55 +404,12 @@ int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w, 
 
 int ddl_expert_linear_backward(const void* dy, const void* x, const void* w, int dtype, const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k,
                                int64_t ld_dy, int64_t ld_x, void* dx, void* dw, void* stream) {
-    using namespace ddl;
-    const char* who = "ddl_expert_linear_backward";
-    if (dtype != DDL_DT_F32 && dtype != DDL_DT_BF16 && dtype != DDL_DT_F16) return fail(DDL_E_ARG, "%s: dtype %d", who, dtype);
-    if (int rc = check_product(who, experts, rows, n, k, dtype == DDL_DT_F32 ? 1 : 8)) return rc;
-    if ((dx && rows) || (dw && experts)) {
-        if (!offsets || (rows && !dy) || (dx && experts && !w) || (dw && rows && !x)) return fail(DDL_E_ARG, "%s: null pointer", who);
-    }
-    if (rows > 1 && (ld_dy < n || (dw && ld_x < k))) return fail(DDL_E_ARG, "%s: pitch below %lld or %lld features", who, static_cast<long long>(n), static_cast<long long>(k));
-    if (ld_dy > 0x3FFFFF || (dw && ld_x > 0x3FFFFF)) return fail(DDL_E_UNSUPP, "%s: pitch above 2^22 elements", who);
-    const int64_t pitch_dy = rows > 1 ? ld_dy : n, pitch_x = rows > 1 ? ld_x : k;
-    const int64_t span = (rows + 64) * (dw && pitch_x > pitch_dy ? pitch_x : pitch_dy);
-    const bool within = span <= (dtype == DDL_DT_F32 ? kMostSpan / 2 : kMostSpan);
-    if (dw && experts && dtype == DDL_DT_F32 && !within)
-        return fail(DDL_E_UNSUPP, "%s: %lld rows, %lld elements apart, are more than 2^31 bytes", who, static_cast<long long>(rows), static_cast<long long>(pitch_x > pitch_dy ? pitch_x : pitch_dy));
-    int dev = 0;
-    const int cus = compute_units(dev);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool f16 = dtype == DDL_DT_F16;
-    ExpertArgs g{};
-    g.offsets = offsets, g.experts = static_cast<int>(experts), g.rows = static_cast<int>(rows), g.out_dtype = dtype, g.cus = cus;
-    if (dx && rows) {   // rows of n features by w read along its k columns
-        ExpertArgs d = g;
-        d.a = dy, d.w = w, d.y = dx, d.n = k, d.k = n, d.lda = pitch_dy, d.ldw = k, d.w_stride = n * k, d.ldy = k;
-        int rc;
-        if (few_for_all(d)) {
-            rc = run_expert_across(who, d, s);
-        } else if (dtype == DDL_DT_F32) {
-            rc = rows32(who, true, d, s);
-        } else {
-            const bool aligned = aligned_to(dy, 16) && aligned_to(w, 16) && pitch_dy % 8 == 0 && n % 8 == 0 && k % 8 == 0;
-            double us;
-            rc = run_expert_rows16(who, best_for_rows(kCosts16, aligned, rows, experts, k, 2 * n, cus, &us), f16, true, d, dev, s);
-        }
-        if (rc) return rc;
-    }
-    if (dw && experts) {
-        ExpertArgs d = g;
-        d.a = dy, d.w = x, d.y = dw, d.n = n, d.k = k, d.lda = pitch_dy, d.ldw = pitch_x;
-        d.places = d.experts, d.few = -1;
-        if (mostly_few(d)) {
-            d.few = few_rows(d), d.places = d.rows / (d.few + 1);   // so many can have more
-            if (int rc = run_expert_outer(who, d, s)) return rc;
-            if (d.places == 0) return 0;
-        }
-        if (dtype == DDL_DT_F32) return weights32(who, d, s);
-        const bool aligned = aligned_to(dy, 16) && aligned_to(x, 16) && pitch_dy % 8 == 0 && pitch_x % 8 == 0 && n % 8 == 0 && k % 8 == 0 && within;
-        return run_expert_weights16(who, best_for_weights(aligned, rows, likely_places(d), n, k, cus), f16, d, dev, s);
-    }
-    return 0;
+    return ddl::product_backward("ddl_expert_linear_backward", true, dy, x, w, dtype, offsets, experts, rows, n, k, ld_dy, ld_x, dx, dw, stream);
+}
+
+int ddl_expert_linear_backward_long(const void* dy, const void* x, const void* w, int dtype, const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k,
+                                    int64_t ld_dy, int64_t ld_x, void* dx, void* dw, void* stream) {
+    return ddl::product_backward("ddl_expert_linear_backward_long", false, dy, x, w, dtype, offsets, experts, rows, n, k, ld_dy, ld_x, dx, dw, stream);
 }
 
 }  // extern "C"

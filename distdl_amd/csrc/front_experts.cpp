@@ -147,9 +147,9 @@ std::optional<Two> expert_linear_backward(const Tensor& dy, const Tensor& x, con
     Tensor dx, dw;
     if (want_input) dx = at::empty(x.sizes(), x.options());
     if (want_weight) dw = at::empty(w.sizes(), w.options());
-    check(ddl_expert_linear_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), float_code(x), offsets.data_ptr<int32_t>(), w.size(0), rows, n, k, n, k, pointer(dx),
+    check(ddl_expert_linear_backward_long(dy.data_ptr(), x.data_ptr(), w.data_ptr(), float_code(x), offsets.data_ptr<int32_t>(), w.size(0), rows, n, k, n, k, pointer(dx),
                                      pointer(dw), current_stream()),
-          "ddl_expert_linear_backward");
+          "ddl_expert_linear_backward_long");
     return Two(want_input ? MaybeTensor(dx) : std::nullopt, want_weight ? MaybeTensor(dw) : std::nullopt);
 }
 

@@ -1656,7 +1656,7 @@ def expert_linear_backward(dy, x, weight, offsets, want_input=True, want_weight=
     dx = torch.empty((rows, k), dtype=x.dtype, device=x.device) if want_input else None
     dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if want_weight else None
     with _on_device_of(x):
-        rc = _lib.load().ddl_expert_linear_backward(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _LN_DTYPES[x.dtype], offsets.data_ptr(), experts, rows, n, k,
+        rc = _lib.load().ddl_expert_linear_backward_long(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _LN_DTYPES[x.dtype], offsets.data_ptr(), experts, rows, n, k,
                                                     _pitch(dy), _pitch(x), _ptr(dx), _ptr(dw), _stream())
-    _lib.check(rc, "ddl_expert_linear_backward")
+    _lib.check(rc, "ddl_expert_linear_backward_long")
     return dx, dw

@@ -842,13 +842,19 @@ int ddl_expert_linear_8bit(const void* x, const float* x_scales, const void* w,
 
 /* The adjoint of ddl_expert_linear: dx[i] = w[e]^T dy[i] (zeros for rows without an expert) and
  * dw[e] = sum over its rows of dy[i] x[i]^T (zeros without rows).  dx or dw may be NULL.
- * Gradients of fp32 weights take rows x pitch of fewer than 2^29 elements (DDL_E_UNSUPP).
+ * Gradients of fp32 weights take rows x pitch of fewer than 2^29 elements (DDL_E_UNSUPP);
+ * ddl_expert_linear_backward_long, which is the same otherwise, takes any number.
  * Nothing is added atomically: equal calls give equal bits. */
 int ddl_expert_linear_backward(const void* dy, const void* x, const void* w,
                                int dtype, const int32_t* offsets,
                                int64_t experts, int64_t rows, int64_t n, int64_t k,
                                int64_t ld_dy, int64_t ld_x, void* dx, void* dw,
                                void* stream);
+int ddl_expert_linear_backward_long(const void* dy, const void* x, const void* w,
+                                    int dtype, const int32_t* offsets,
+                                    int64_t experts, int64_t rows, int64_t n,
+                                    int64_t k, int64_t ld_dy, int64_t ld_x,
+                                    void* dx, void* dw, void* stream);
 
 #ifdef __cplusplus
 }
