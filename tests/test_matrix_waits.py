@@ -1,9 +1,9 @@
 """The built library's own instructions, read back: on every way through a kernel there are the wait states between a matrix instruction and what reads or
-overwrites its result, and between a vector instruction that writes scalar registers and a memory request that takes them.  Neither is waited for by the hardware; the compiler
-fills in what it sees, but it may look at the longer one of two ways that meet, and does not look into assembly.
+overwrites its result, between a vector instruction and a matrix instruction that takes what it writes, and between one that writes scalar registers and a memory request that
+takes them.  None is waited for by the hardware; the compiler fills in what it sees, but it may look at the longer one of two ways that meet, and does not look into assembly.
 
 A wait state is an instruction's slot.  A result needs its matrix instruction's passes (of four cycles) and two more states, of types below 32 bits four more; matrix
-instructions follow each other when the one before has made its passes.  A scalar register needs five."""
+instructions follow each other when the one before has made its passes.  A matrix instruction's operand needs two, a scalar register five."""
 
 import heapq
 import os
@@ -19,7 +19,7 @@ LIBRARY = pathlib.Path(__file__).resolve().parent.parent / "distdl_amd" / "libdi
 OBJDUMP = pathlib.Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "llvm" / "bin" / "llvm-objdump"
 PASSES = {"v_mfma_f32_32x32x2_f32": 16, "v_mfma_f32_16x16x4_f32": 8, "v_mfma_f32_16x16x32_bf16": 4, "v_mfma_f32_16x16x32_f16": 4, "v_mfma_f32_32x32x16_bf16": 8,
           "v_mfma_f32_32x32x16_f16": 8, "v_mfma_f32_16x16x128_f8f6f4": 8, "v_mfma_scale_f32_16x16x128_f8f6f4": 8}
-SCALAR_STATES = 5
+OPERAND_STATES, SCALAR_STATES = 2, 5
 VECTOR = re.compile(r"\b([av])(?:\[(\d+):(\d+)\]|(\d+))(?![\w\[])")
 SCALAR = re.compile(r"\b(s)(?:\[(\d+):(\d+)\]|(\d+))(?![\w\[])")
 LINE = re.compile(r"^\t(\S+)(?: (.*?))?\s*// ([0-9A-F]+):.*?(?:<(\S+?)(?:\+0x([0-9a-f]+))?>)?$")
@@ -96,30 +96,34 @@ class Kernel:
                     heapq.heappush(ways, (states + states_of, at + 1, live, free, lanes))
         return found
 
-    def early_requests(self):
-        """(vector instruction, memory request that takes a scalar register it writes, wait states there)."""
+    def written_late(self, pattern, states_needed, takes, taken):
+        """(vector instruction, instruction that ``takes`` a register it writes, wait states between them) wherever those are too few."""
         found = []
         for last, op in enumerate(self.ops):
-            if not op.startswith(("buffer_", "global_", "flat_")):
-                continue
-            taken, seen = registers(SCALAR, self.args[last]), set()
-            ways = [(0, last, frozenset(taken))] if taken else []
+            registers_taken = registers(pattern, taken(self.args[last])) if takes(op) else ()
+            ways, seen = [(0, last, frozenset(registers_taken))], set()
             while ways:
                 states, at, live = ways.pop()
-                if states >= SCALAR_STATES or not live or (states, at, live) in seen:
+                if states >= states_needed or not live or (states, at, live) in seen:
                     continue
                 seen.add((states, at, live))
-                ways += [(states + 1, source, live) for source in self.sources.get(at, ())] if at != last or states == 0 else []
+                ways += [(states + 1, source, live) for source in self.sources.get(at, ())]
                 at -= 1
                 if at < 0 or self.ops[at] in ("s_branch", "s_endpgm"):
                     continue
-                op, first = self.ops[at], self.args[at].split(",")[0]
-                states_of = int(self.args[at], 0) + 1 if op == "s_nop" else 1
-                written = registers(SCALAR, first) if op.startswith(("v_", "s_")) and not op.startswith(("s_cmp", "s_cbranch", "s_waitcnt", "s_nop", "s_barrier")) else set()
-                if op.startswith("v_") and written & live:
+                op, args = self.ops[at], self.args[at]
+                writes = op.startswith(("v_", "s_")) and not op.startswith(("s_cmp", "s_cbranch", "s_waitcnt", "s_nop", "s_barrier"))
+                written = registers(pattern, args.split(",")[0]) if writes else set()
+                if op.startswith("v_") and not op.startswith("v_mfma") and written & live:
                     found.append((at, last, states))
-                ways.append((states + states_of, at, live - written))
+                ways.append((states + (int(args, 0) + 1 if op == "s_nop" else 1), at, live - written))
         return found
+
+    def early_requests(self):
+        return self.written_late(SCALAR, SCALAR_STATES, lambda op: op.startswith(("buffer_", "global_", "flat_")), lambda args: args)
+
+    def early_products(self):
+        return self.written_late(VECTOR, OPERAND_STATES, lambda op: op.startswith("v_mfma"), lambda args: args.partition(",")[2])
 
 
 def kernels(path):
@@ -142,7 +146,7 @@ def faults(path):
     found, matrix = [], 0
     for kernel in kernels(path):
         matrix += sum(op.startswith("v_mfma") for op in kernel.ops)
-        for first, at, states in kernel.early_readers() + kernel.early_requests():
+        for first, at, states in kernel.early_readers() + kernel.early_requests() + kernel.early_products():
             found.append(f"{kernel.name}: {kernel.ops[first]} {kernel.args[first]} -> {kernel.ops[at]} {kernel.args[at]} after {states}")
     return found, matrix
 
@@ -185,6 +189,9 @@ def test_the_reading_of_ways():
     assert made(product, ("s_cbranch_scc1 1", 3), ("s_nop 9", None), ("s_nop 9", None), reader).early_readers() == [(0, 4, 11)]
     assert made(product, ("v_mfma_f32_32x32x2_f32 a[16:31], v1, v2, a[16:31]", None), ("s_nop 1", None), reader).early_readers() == []
     assert made(product, ("v_mfma_f32_32x32x2_f32 a[0:15], v1, v2, a[0:15]", None), ("s_nop 1", None), reader).early_readers() == [(1, 3, 2)]
+    operand = ("v_perm_b32 v1, v3, v4, v5", None)
+    assert made(operand, product).early_products() == [(0, 1, 0)] and made(operand, ("s_nop 0", None), product).early_products() == [(0, 2, 1)]
+    assert made(operand, ("s_nop 1", None), product).early_products() == [] == made(product, product).early_products()
     request = ("buffer_load_dwordx4 v1, s[4:7], s8 offen lds", None)
     assert made(("v_readfirstlane_b32 s8, v1", None), ("s_nop 2", None), request).early_requests() == [(0, 2, 3)]
     assert made(("v_readfirstlane_b32 s8, v1", None), ("s_nop 4", None), request).early_requests() == []
