@@ -167,8 +167,8 @@ int launch_stream(const char* who, const ExpertArgs& g, hipStream_t s) {
 
 constexpr int64_t kMostSpan = 0x3FFFFFFF;   // elements that a tile's 32-bit byte offsets reach over
 
-// Estimates in microseconds, fits of sweeps over 1 to 64 experts, 512 to 8192 features and 2 to 2048 rows for each, within a tenth for most and a quarter
-// for nearly all.  A round is what the chip holds at once: four workgroups of 64 x 64 tiles for a CU, two of 128 x 128, one of the large
+// Estimates in microseconds, fits of sweeps over 1 to 64 experts, 512 to 8192 features and 2 to 2048 rows for each, which are taken to be spread evenly (choices that all go to
+// one expert were no slower: 4096 rows to 128 of [512, 1024] 25 and 13 us).  A round is what the chip holds at once: four workgroups of 64 x 64 tiles for a CU, two of 128 x 128, one of the large
 // ones, which come in whole rounds.  A round costs its start and its stores, and for each k-tile (128 bytes) some time of its own and some that grows with
 // the CUs' load.  ([8 x 512, 8192] by 3584: 64 x 64 414 us, 128 x 128 282, 128 x 256 225, 256 x 256 184; of 64 rows each 99, 104, 126, 154.)
 struct TileCost {

@@ -4,7 +4,8 @@
 // reads, of some rows, four elements of dy and one vector of x.  Matrix instruction (i, j) takes element i of every lane's four and element j of its vector, so which row
 // and column of the tile it computes is spread over the lanes, and a lane ends up with whole vectors of dw.  (16-bit elements: eight rows' pairs are put into one register first.)
 // No LDS, no barrier: what a tile of expert_linear16.hip or expert_linear32.hip waits for at its start and end takes longer than writing it.  ([8 x 2048, 2048] bf16 of 2 to 32 rows each 29 us by
-// tiles, here 13 to 14 (5 TB/s), of 128 29 and 20; fp32 of 2 to 16 57 and 28, of 32 49 and 41.  With the products on the vector units, bf16 13 for two rows and 37 for 32.)
+// tiles, here 13 to 14 (5 TB/s), of 128 29 and 20; fp32 of 2 to 16 57 and 28, of 32 49 and 41.  With the products on the vector units, bf16 13 for two rows and 37 for 32; quicker for one row
+// and matrices of no whole lines, [16 x 3743, 4476] bf16 90 and here 100, fp32 171 and 264, by tiles 409.)
 // An expert without rows gets its zeros the same way.  Operands of any address and pitch: the last vector of a row and the last rows of a matrix are moved
 // back to end with it, what is written twice is the same.  Every XCD has an eighth of each expert's wavefronts side by side.
 #include "expert_parts.h"
